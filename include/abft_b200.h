@@ -392,6 +392,108 @@ int abft_check_only(const abft_check_args* args, void* stream);
 #define ABFT_NO_ALLOC_SCRATCH_BYTES (4u << 20)
 int abft_check_only_noalloc(const abft_check_args* args, void* stream);
 
+/* ---- Paged key-value cache ------------------------------------------------
+ *
+ * The cache of one decoder layer that the checked linears of a decode step
+ * write to and read from: pages of `page_size` token slots, handed to
+ * sequences through a page table, so that sequences of unlike length share
+ * one pool. No counterpart in the reference, whose model driver keeps one
+ * dense cache per sequence (pytorch/qwen_abft_benchmark.py:130-154).
+ *
+ * Sequence b holds seq_lens[b] tokens INCLUDING those the current step adds.
+ * With cu_seqlens ([batch + 1], non-decreasing, from 0) the packed token rows
+ * [cu_seqlens[b], cu_seqlens[b+1]) are the last tokens of sequence b: row i
+ * of n has position seq_lens[b] - n + i. Rows at or behind cu_seqlens[batch]
+ * belong to no sequence and are left as they were. Position p of sequence b
+ * lives in slot p % page_size of page page_table[b][p / page_size].
+ *
+ * Lengths, table entries and cu_seqlens live on the device, so they are
+ * checked there: a bad value never reads or writes outside the tensors. It
+ * sets a bit of *status (when status is not NULL; bits stay until the caller
+ * clears them) and
+ *   ABFT_PAGED_BAD_PAGE   a table entry outside [0, num_pages): an append
+ *                         skips the token, attention reads the slots as
+ *                         zeros;
+ *   ABFT_PAGED_BAD_LEN    a length below 0 (taken as 0), a length beyond
+ *                         max_pages * page_size (attention: cut there; append:
+ *                         skips the tokens beyond), or more new tokens than
+ *                         the length (append skips those of negative
+ *                         position; attention gives them 0);
+ *   ABFT_PAGED_BAD_ANGLE  a position at or beyond max_positions of the
+ *                         rotation table: append skips the token.
+ * Slots at or beyond a sequence's length are never used: they may hold
+ * anything, NaN included. */
+#define ABFT_PAGED_BAD_PAGE  1u
+#define ABFT_PAGED_BAD_LEN   2u
+#define ABFT_PAGED_BAD_ANGLE 4u
+
+/* A page pool and the sequences in it. */
+typedef struct abft_paged_kv {
+  void* k_pages;              /* [num_pages, kv_heads, page_size, head_dim], dense     */
+  void* v_pages;              /* within a page; the same for values                    */
+  int64_t k_page_stride;      /* elements from page to page, a multiple of 8 of at     */
+  int64_t v_page_stride;      /* least kv_heads * page_size * head_dim                 */
+  const int32_t* page_table;  /* [batch, table_stride], max_pages entries of a row used */
+  int64_t table_stride;
+  const int32_t* seq_lens;    /* [batch]                                               */
+  uint32_t* status;           /* ABFT_PAGED_* bits, or NULL                            */
+  int32_t num_pages;
+  int32_t page_size;          /* 16, 32, 64 or 128                                     */
+  int32_t kv_heads;
+  int32_t head_dim;           /* 64 or 128                                             */
+  int32_t batch;              /* at most 65535                                         */
+  int32_t max_pages;          /* pages a sequence can hold (1 or more when batch > 0)  */
+  int32_t dtype;              /* ABFT_DTYPE_BF16 or ABFT_DTYPE_F16                     */
+  int32_t reserved;
+} abft_paged_kv;
+
+/* Append: rotates the q and k rows by their positions (half-split pairs
+ * (j, j + head_dim/2), fp32, rounded once), writes k and v to their slots and
+ * the rotated q to q_out. */
+typedef struct abft_kv_append_args {
+  abft_paged_kv kv;
+  const void* q;              /* [tokens, heads, head_dim]; strides in elements,       */
+  const void* k;              /* multiples of 8; [tokens, kv_heads, head_dim]          */
+  const void* v;
+  void* q_out;                /* [tokens, heads, head_dim]; may be q itself            */
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t o_token_stride, o_head_stride;
+  const int32_t* cu_seqlens;  /* [batch + 1], or NULL: token b belongs to sequence b   */
+  const float* rope;          /* [max_positions, head_dim / 2, 2] (cos, sin), or NULL: */
+                              /* no rotation                                           */
+  int64_t max_positions;
+  int64_t tokens;             /* == kv.batch when cu_seqlens is NULL                   */
+  int32_t heads;              /* a multiple of kv_heads, at most 64 per kv head; or 0:  */
+  int32_t reserved;           /* no q (q and q_out unused)                             */
+} abft_kv_append_args;
+
+/* Attention over the cache: out = softmax(scale * q k^T) v, statistics and
+ * sums in fp32, per query row over the slots it sees. */
+typedef struct abft_paged_attn_args {
+  abft_paged_kv kv;
+  const void* q;              /* [tokens, heads, head_dim]; strides in elements,       */
+  void* out;                  /* multiples of 8                                        */
+  int64_t q_token_stride, q_head_stride;
+  int64_t o_token_stride, o_head_stride;
+  const int32_t* cu_seqlens;  /* prefill: [batch + 1]; unused by decode                */
+  int64_t tokens;             /* rows of q (decode: kv.batch)                          */
+  int32_t heads;              /* a multiple of kv_heads, at most 64 per kv head        */
+  float scale;
+  void* workspace;            /* device scratch, abft_paged_*_workspace_bytes()        */
+  size_t workspace_bytes;
+  int32_t num_splits;         /* 0 = choose; else pieces each sequence is cut into     */
+  int32_t num_sms;            /* 0 = all SMs of the current device                     */
+} abft_paged_attn_args;
+
+int abft_kv_append(const abft_kv_append_args* args, void* stream);
+
+/* One query row per sequence (its newest token), which sees every slot below
+ * seq_lens[b]; a sequence of length 0 gives a row of zeros. */
+size_t abft_paged_decode_workspace_bytes(const abft_paged_attn_args* args);
+int abft_paged_decode(const abft_paged_attn_args* args, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

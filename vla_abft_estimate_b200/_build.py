@@ -9,6 +9,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -18,14 +19,19 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libabft_b200.so"
 INCLUDE_DIR = REPO_DIR / "include"
 
-SOURCES = ["abft_api.cu"]
-HEADERS = ["ptx.cuh", "gemm_kernel.cuh", "aux_kernels.cuh"]
+OBJ_DIR = LIB_DIR / "obj"
+
+# Each source with the headers it includes; a source is recompiled when one
+# of them is newer than its object.
+SOURCES = {
+    "abft_api.cu": ["ptx.cuh", "gemm_kernel.cuh", "aux_kernels.cuh"],
+    "paged_api.cu": ["ptx.cuh", "paged_index.cuh", "paged_append.cuh", "paged_decode.cuh"],
+}
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
-    "-shared",
 ]
 
 
@@ -36,32 +42,53 @@ def _nvcc() -> str:
     return cand
 
 
-def _inputs() -> list[Path]:
-    return [CSRC_DIR / s for s in SOURCES] + [CSRC_DIR / h for h in HEADERS] + [INCLUDE_DIR / "abft_b200.h"]
+def _inputs(source: str) -> list[Path]:
+    return [CSRC_DIR / source, *[CSRC_DIR / h for h in SOURCES[source]], INCLUDE_DIR / "abft_b200.h"]
+
+
+def _newer(out: Path, inputs: list[Path]) -> bool:
+    """``out`` exists and is not older than any of ``inputs``."""
+    if not out.exists():
+        return False
+    t = out.stat().st_mtime
+    return all(p.stat().st_mtime <= t for p in inputs)
 
 
 def is_stale() -> bool:
-    if not LIB_PATH.exists():
-        return True
-    t = LIB_PATH.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in _inputs())
+    return not all(_newer(LIB_PATH, _inputs(s)) for s in SOURCES)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if it is missing or older than its sources."""
-    if not force and not is_stale():
-        return LIB_PATH
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, f"-I{INCLUDE_DIR}", *[str(CSRC_DIR / s) for s in SOURCES], "-o", str(tmp)]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd))
+def _run(cmd: list[str], verbose: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     if verbose and res.stderr:
         print(res.stderr)
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the library if it is missing or older than its sources (the
+    sources that changed, side by side, then one link)."""
+    if not force and not is_stale():
+        return LIB_PATH
+    OBJ_DIR.mkdir(parents=True, exist_ok=True)
+    jobs = []
+    for src in SOURCES:
+        obj = OBJ_DIR / (Path(src).stem + ".o")
+        if force or not _newer(obj, _inputs(src)):
+            tmp = obj.with_suffix(".o.tmp")
+            jobs.append((tmp, obj, [_nvcc(), *NVCC_FLAGS, f"-I{INCLUDE_DIR}", "-c", str(CSRC_DIR / src), "-o", str(tmp)]))
+    if verbose:
+        for _, _, cmd in jobs:
+            cmd.insert(1, "-Xptxas=-v")
+            print(" ".join(cmd))
+    with ThreadPoolExecutor(max(1, len(jobs))) as pool:
+        list(pool.map(lambda j: _run(j[2], verbose), jobs))
+    for tmp, obj, _ in jobs:
+        os.replace(tmp, obj)
+    tmp = LIB_PATH.with_suffix(".so.tmp")
+    _run([_nvcc(), *NVCC_FLAGS[:2], "-shared", *[str(OBJ_DIR / (Path(s).stem + ".o")) for s in SOURCES],
+          "-o", str(tmp)], verbose)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

@@ -68,9 +68,17 @@ EXPORTED_SYMBOLS = (
     "abft_check_workspace_bytes",
     "abft_check_only",
     "abft_check_only_noalloc",
+    "abft_kv_append",
+    "abft_paged_decode_workspace_bytes",
+    "abft_paged_decode",
 )
 
 NO_ALLOC_SCRATCH_BYTES = 4 << 20
+
+# status bits of the paged cache (abft_paged_kv.status)
+PAGED_BAD_PAGE = 1
+PAGED_BAD_LEN = 2
+PAGED_BAD_ANGLE = 4
 
 
 class AbftError(RuntimeError):
@@ -172,6 +180,77 @@ class CheckArgs(ctypes.Structure):
     ]
 
 
+class PagedKv(ctypes.Structure):
+    """Mirror of ``abft_paged_kv``."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_page_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """Mirror of ``abft_kv_append_args``."""
+
+    _fields_ = [
+        ("kv", PagedKv),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("o_token_stride", ctypes.c_int64),
+        ("o_head_stride", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("rope", ctypes.c_void_p),
+        ("max_positions", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """Mirror of ``abft_paged_attn_args``."""
+
+    _fields_ = [
+        ("kv", PagedKv),
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("o_token_stride", ctypes.c_int64),
+        ("o_head_stride", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("num_splits", ctypes.c_int32),
+        ("num_sms", ctypes.c_int32),
+    ]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -193,6 +272,9 @@ def lib() -> ctypes.CDLL:
     if L.abft_version() != LIB_VERSION:
         raise RuntimeError(f"{path} has ABI version {L.abft_version()}, this binding needs {LIB_VERSION}: "
                            "rebuild it with `python -m vla_abft_estimate_b200._build`")
+    missing = [name for name in EXPORTED_SYMBOLS if not hasattr(L, name)]
+    if missing:
+        raise RuntimeError(f"{path} lacks {', '.join(missing)}: rebuild it with `python -m vla_abft_estimate_b200._build`")
     L.abft_status_string.restype = ctypes.c_char_p
     L.abft_status_string.argtypes = [ctypes.c_int]
     L.abft_report_bytes.restype = sz
@@ -229,6 +311,12 @@ def lib() -> ctypes.CDLL:
     L.abft_check_only.argtypes = [ctypes.POINTER(CheckArgs), vp]
     L.abft_check_only_noalloc.restype = ctypes.c_int
     L.abft_check_only_noalloc.argtypes = [ctypes.POINTER(CheckArgs), vp]
+    L.abft_kv_append.restype = ctypes.c_int
+    L.abft_kv_append.argtypes = [ctypes.POINTER(KvAppendArgs), vp]
+    L.abft_paged_decode_workspace_bytes.restype = sz
+    L.abft_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs)]
+    L.abft_paged_decode.restype = ctypes.c_int
+    L.abft_paged_decode.argtypes = [ctypes.POINTER(PagedAttnArgs), vp]
     _LIB = L
     return L
 

@@ -1,0 +1,287 @@
+// paged_api.cu - the extern "C" entry points of the paged key-value cache:
+// argument validation, workspace layout and launches. Declarations are in
+// include/abft_b200.h.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <mutex>
+
+#include "paged_append.cuh"
+#include "paged_decode.cuh"
+
+using namespace abft;
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+struct DeviceInfo {
+  bool init, ok;
+  int sms;
+  bool smem_set[8];  // by decode_slot()
+};
+DeviceInfo g_paged_dev[kMaxDevices];
+std::mutex g_paged_mu;
+
+int paged_device(int* dev_out, int* sms) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+    cudaGetLastError();
+    return ABFT_ERR_NO_DEVICE;
+  }
+  std::lock_guard<std::mutex> lk(g_paged_mu);
+  DeviceInfo& d = g_paged_dev[dev];
+  if (!d.init) {
+    int major = 0, minor = 0, n = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    cudaGetLastError();
+    d.ok = major == 10 && minor == 0;
+    d.sms = n;
+    d.init = true;
+  }
+  if (!d.ok) return ABFT_ERR_NO_DEVICE;
+  *dev_out = dev;
+  *sms = d.sms;
+  return ABFT_OK;
+}
+
+// Raises a kernel's dynamic shared-memory limit once per device.
+template <typename K>
+int raise_smem(int dev, int slot, K kernel, int bytes) {
+  std::lock_guard<std::mutex> lk(g_paged_mu);
+  bool& set = g_paged_dev[dev].smem_set[slot];
+  if (set) return ABFT_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return ABFT_ERR_CUDA;
+  }
+  set = true;
+  return ABFT_OK;
+}
+
+inline int launch_result() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? ABFT_OK : ABFT_ERR_CUDA;
+}
+
+inline bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+inline bool off8el(int64_t s) { return (s & 7) != 0; }
+
+// Launch with programmatic serialization: the kernel waits
+// (griddepcontrol.wait) before any global access.
+template <typename K, typename P>
+int launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return ABFT_ERR_CUDA;
+  }
+  return launch_result();
+}
+
+int check_kv(const abft_paged_kv& c) {
+  if (c.batch < 0 || c.num_pages < 0 || c.max_pages < 0 || c.kv_heads <= 0) return ABFT_ERR_INVALID_ARG;
+  if (c.dtype != ABFT_DTYPE_BF16 && c.dtype != ABFT_DTYPE_F16)
+    return c.dtype == ABFT_DTYPE_F32 ? ABFT_ERR_UNSUPPORTED : ABFT_ERR_INVALID_ARG;
+  if (c.head_dim != 64 && c.head_dim != 128) return ABFT_ERR_UNSUPPORTED;
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128) return ABFT_ERR_UNSUPPORTED;
+  if (c.batch == 0) return ABFT_OK;
+  if (c.k_pages == nullptr || c.v_pages == nullptr || c.page_table == nullptr || c.seq_lens == nullptr ||
+      c.max_pages == 0 || c.num_pages == 0)
+    return ABFT_ERR_INVALID_ARG;
+  if (c.batch > 65535 || c.kv_heads > 4096) return ABFT_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(c.max_pages) * c.page_size >= (int64_t{1} << 30)) return ABFT_ERR_UNSUPPORTED;
+  if (c.table_stride < (c.batch > 1 ? c.max_pages : 0)) return ABFT_ERR_INVALID_ARG;
+  const int64_t page = static_cast<int64_t>(c.kv_heads) * c.page_size * c.head_dim;
+  if (c.num_pages > 1 && (c.k_page_stride < page || c.v_page_stride < page)) return ABFT_ERR_INVALID_ARG;
+  if (off16(c.k_pages) || off16(c.v_pages) || off8el(c.k_page_stride) || off8el(c.v_page_stride))
+    return ABFT_ERR_ALIGNMENT;
+  return ABFT_OK;
+}
+
+int check_heads(int heads, int kv_heads) {
+  if (heads <= 0 || heads % kv_heads != 0) return ABFT_ERR_INVALID_ARG;
+  return heads / kv_heads > 64 ? ABFT_ERR_UNSUPPORTED : ABFT_OK;
+}
+
+PagedView view_of(const abft_paged_kv& c) {
+  PagedView v;
+  v.k_pages = c.k_pages;
+  v.v_pages = c.v_pages;
+  v.k_page_stride = c.k_page_stride;
+  v.v_page_stride = c.v_page_stride;
+  v.page_table = c.page_table;
+  v.table_stride = c.table_stride;
+  v.seq_lens = c.seq_lens;
+  v.status = c.status;
+  v.num_pages = c.num_pages;
+  v.page_shift = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : c.page_size == 64 ? 6 : 7;
+  v.kv_heads = c.kv_heads;
+  v.batch = c.batch;
+  v.max_pages = c.max_pages;
+  return v;
+}
+
+template <int D, bool F16>
+int launch_append(const AppendParams& p, cudaStream_t s) {
+  return launch(kv_append_kernel<D, F16>, dim3(static_cast<unsigned>(p.tokens)), dim3(kAppendThreads), 0, s, p);
+}
+
+// ---- decode -------------------------------------------------------------------
+// Query heads of a group that one CTA takes: one 8-column product, or two
+// (16) for larger groups; beyond 16, several CTAs read the same keys.
+inline int decode_nt(int group) { return group > 8 ? 2 : 1; }
+
+int attn_check(const abft_paged_attn_args* a, bool decode) {
+  if (a == nullptr) return ABFT_ERR_INVALID_ARG;
+  int rc = check_kv(a->kv);
+  if (rc != ABFT_OK) return rc;
+  if (a->tokens < 0 || a->num_splits < 0 || a->num_sms < 0 || !isfinite(a->scale)) return ABFT_ERR_INVALID_ARG;
+  if ((rc = check_heads(a->heads, a->kv.kv_heads)) != ABFT_OK) return rc;
+  if (decode && a->tokens != a->kv.batch) return ABFT_ERR_INVALID_ARG;
+  if (a->tokens == 0 || a->kv.batch == 0) return ABFT_OK;
+  if (a->q == nullptr || a->out == nullptr || (!decode && a->cu_seqlens == nullptr)) return ABFT_ERR_INVALID_ARG;
+  if (off16(a->q) || off16(a->out) || off8el(a->q_token_stride) || off8el(a->q_head_stride) ||
+      off8el(a->o_token_stride) || off8el(a->o_head_stride))
+    return ABFT_ERR_ALIGNMENT;
+  return ABFT_OK;
+}
+
+int decode_splits(const abft_paged_attn_args* a, int sms) {
+  const int64_t tiles = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
+  if (a->num_splits > 0) return static_cast<int>(a->num_splits < tiles ? a->num_splits : tiles);
+  const int group = a->heads / a->kv.kv_heads;
+  const int chunks = (group + 8 * decode_nt(group) - 1) / (8 * decode_nt(group));
+  const int64_t ctas = static_cast<int64_t>(a->kv.batch) * a->kv.kv_heads * chunks;
+  int64_t n = (2 * sms + ctas - 1) / ctas;
+  const int64_t most = (tiles + 3) / 4;  // a tile for each warp
+  if (n > most) n = most;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+
+size_t split_bytes(const abft_paged_attn_args* a, int splits) {
+  if (splits <= 1) return 0;
+  const size_t rows = static_cast<size_t>(a->kv.batch) * a->heads * splits;
+  return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2));
+}
+
+template <int D, int NT, bool F16>
+int launch_decode(int dev, int slot, const DecodeParams& p, int heads, cudaStream_t s) {
+  using Cfg = DecodeCfg<D, NT>;
+  int rc = raise_smem(dev, slot, paged_decode_kernel<D, NT, F16>, Cfg::kSmemBytes);
+  if (rc != ABFT_OK) return rc;
+  const dim3 grid(p.splits, p.kv.kv_heads * p.head_chunks, p.kv.batch);
+  rc = launch(paged_decode_kernel<D, NT, F16>, grid, dim3(128), Cfg::kSmemBytes, s, p);
+  if (rc != ABFT_OK || p.splits == 1) return rc;
+  JoinParams j;
+  j.seq_lens = p.kv.seq_lens;
+  j.out = p.out;
+  j.ot = p.ot;
+  j.oh = p.oh;
+  j.heads = heads;
+  j.splits = p.splits;
+  j.max_pages = p.kv.max_pages;
+  j.page_shift = p.kv.page_shift;
+  j.part_o = p.part_o;
+  j.part_ml = p.part_ml;
+  return launch(paged_join_kernel<D, F16>, dim3(heads, p.kv.batch), dim3(128), 0, s, j);
+}
+
+}  // namespace
+
+extern "C" {
+
+int abft_kv_append(const abft_kv_append_args* a, void* stream) {
+  if (a == nullptr) return ABFT_ERR_INVALID_ARG;
+  int rc = check_kv(a->kv);
+  if (rc != ABFT_OK) return rc;
+  if (a->tokens < 0 || a->heads < 0 || a->max_positions < 0) return ABFT_ERR_INVALID_ARG;
+  if (a->heads > 0 && (rc = check_heads(a->heads, a->kv.kv_heads)) != ABFT_OK) return rc;
+  if (a->cu_seqlens == nullptr && a->tokens != a->kv.batch) return ABFT_ERR_INVALID_ARG;
+  if (a->tokens == 0 || a->kv.batch == 0) return ABFT_OK;
+  if (a->tokens >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
+  if (a->k == nullptr || a->v == nullptr || (a->heads > 0 && (a->q == nullptr || a->q_out == nullptr)))
+    return ABFT_ERR_INVALID_ARG;
+  if (off16(a->k) || off16(a->v) || off16(a->rope) || off8el(a->k_token_stride) || off8el(a->k_head_stride) ||
+      off8el(a->v_token_stride) || off8el(a->v_head_stride))
+    return ABFT_ERR_ALIGNMENT;
+  if (a->heads > 0 && (off16(a->q) || off16(a->q_out) || off8el(a->q_token_stride) || off8el(a->q_head_stride) ||
+                       off8el(a->o_token_stride) || off8el(a->o_head_stride)))
+    return ABFT_ERR_ALIGNMENT;
+  int dev = 0, sms = 0;
+  if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
+  AppendParams p;
+  p.kv = view_of(a->kv);
+  p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out;
+  p.qt = a->q_token_stride, p.qh = a->q_head_stride;
+  p.kt = a->k_token_stride, p.kh = a->k_head_stride;
+  p.vt = a->v_token_stride, p.vh = a->v_head_stride;
+  p.ot = a->o_token_stride, p.oh = a->o_head_stride;
+  p.cu = a->cu_seqlens;
+  p.rope = a->rope;
+  p.max_positions = a->max_positions;
+  p.tokens = a->tokens;
+  p.heads = a->heads;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
+  if (a->kv.head_dim == 128) return f16 ? launch_append<128, true>(p, s) : launch_append<128, false>(p, s);
+  return f16 ? launch_append<64, true>(p, s) : launch_append<64, false>(p, s);
+}
+
+size_t abft_paged_decode_workspace_bytes(const abft_paged_attn_args* a) {
+  if (attn_check(a, true) != ABFT_OK || a->kv.batch == 0) return 0;
+  int dev = 0, sms = a->num_sms;
+  if (sms == 0 && paged_device(&dev, &sms) != ABFT_OK) sms = 148;
+  return split_bytes(a, decode_splits(a, sms));
+}
+
+int abft_paged_decode(const abft_paged_attn_args* a, void* stream) {
+  int rc = attn_check(a, true);
+  if (rc != ABFT_OK || a->kv.batch == 0) return rc;
+  int dev = 0, sms = 0;
+  if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
+  if (a->num_sms > 0) sms = a->num_sms;
+  DecodeParams p;
+  p.kv = view_of(a->kv);
+  p.q = a->q, p.out = a->out;
+  p.qt = a->q_token_stride, p.qh = a->q_head_stride;
+  p.ot = a->o_token_stride, p.oh = a->o_head_stride;
+  p.group = a->heads / a->kv.kv_heads;
+  const int nt = decode_nt(p.group);
+  p.head_chunks = (p.group + 8 * nt - 1) / (8 * nt);
+  if (static_cast<int64_t>(a->kv.kv_heads) * p.head_chunks > 65535) return ABFT_ERR_UNSUPPORTED;
+  p.splits = decode_splits(a, sms);
+  p.scale_log2 = a->scale * 1.44269504088896340736f;
+  const size_t need = split_bytes(a, p.splits);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
+  if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(
+      p.part_o + static_cast<size_t>(a->kv.batch) * a->heads * p.splits * a->kv.head_dim);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
+  const int slot = (a->kv.head_dim == 128 ? 4 : 0) + (nt == 2 ? 2 : 0) + (f16 ? 1 : 0);
+  switch (slot) {
+    case 0: return launch_decode<64, 1, false>(dev, slot, p, a->heads, s);
+    case 1: return launch_decode<64, 1, true>(dev, slot, p, a->heads, s);
+    case 2: return launch_decode<64, 2, false>(dev, slot, p, a->heads, s);
+    case 3: return launch_decode<64, 2, true>(dev, slot, p, a->heads, s);
+    case 4: return launch_decode<128, 1, false>(dev, slot, p, a->heads, s);
+    case 5: return launch_decode<128, 1, true>(dev, slot, p, a->heads, s);
+    case 6: return launch_decode<128, 2, false>(dev, slot, p, a->heads, s);
+    default: return launch_decode<128, 2, true>(dev, slot, p, a->heads, s);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,148 @@
+// paged_append.cuh - new tokens' keys and values into the paged cache, with
+// the rotation by position applied on the way to q and k.
+//
+// For token t of sequence b at position p, angle pairs (c_j, s_j) = rope[p][j]:
+//   x'[j] = x[j] c_j - x[j + D/2] s_j,   x'[j + D/2] = x[j + D/2] c_j + x[j] s_j
+// in fp32, rounded once to the element type. The rows are read once and
+// written once; there is nothing to reuse, so the kernel is bound by memory
+// traffic (large calls) or by its chain of dependent loads (small ones).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/abft_b200.h"
+#include "paged_index.cuh"
+#include "ptx.cuh"
+
+namespace abft {
+
+// Two packed 16-bit elements <-> two floats.
+template <bool F16>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct AppendParams {
+  PagedView kv;
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t qt, qh, kt, kh, vt, vh, ot, oh;  // token and head strides, elements
+  const int32_t* cu;
+  const float* rope;
+  int64_t max_positions;
+  int64_t tokens;
+  int32_t heads;
+};
+
+// Sequence that owns packed token t: the number of boundaries cu[1..batch]
+// at or below t, counted by a whole warp (independent loads instead of a
+// chain of a binary search; boundaries do not decrease). batch when the row
+// is behind the last sequence.
+__device__ __forceinline__ int owner_of(const int32_t* cu, int batch, int64_t t, int lane) {
+  int n = 0;
+  for (int i = 0; i < batch; i += 32) {
+    const bool below = i + lane < batch && cu[1 + i + lane] <= t;
+    n += __popc(__ballot_sync(0xFFFFFFFFu, below));
+  }
+  return n;
+}
+
+// One thread owns chunk c of a row's pairs: elements [8c, 8c + 8) and their
+// partners [D/2 + 8c, D/2 + 8c + 8). D / 16 threads cover a row, a warp 512 / D
+// rows of one token; the block's warps walk the token's heads (q, then k, then
+// v).
+constexpr int kAppendThreads = 256;
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
+  constexpr int kChunks = D / 16;  // threads per row
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t t = blockIdx.x;
+  const PagedView& kv = p.kv;
+  int b, pos, place = 0, n = 1;
+  if (p.cu != nullptr) {
+    b = owner_of(p.cu, kv.batch, t, lane);
+    if (b >= kv.batch) return;  // behind the last sequence
+    const int begin = p.cu[b];
+    n = p.cu[b + 1] - begin;
+    place = static_cast<int>(t) - begin;
+  } else {
+    b = static_cast<int>(t);
+  }
+  const int len = kv.seq_lens[b];
+  if (p.cu == nullptr && len == 0) return;  // a slot without a sequence
+  const int64_t pos64 = static_cast<int64_t>(len) - n + place;
+  uint32_t bad = 0;
+  if (pos64 < 0 || pos64 >= (static_cast<int64_t>(kv.max_pages) << kv.page_shift)) bad = ABFT_PAGED_BAD_LEN;
+  pos = static_cast<int>(pos64);
+  if (bad == 0 && p.rope != nullptr && pos >= p.max_positions) bad = ABFT_PAGED_BAD_ANGLE;
+  int page = 0;
+  if (bad == 0) {
+    page = kv.page_table[b * kv.table_stride + (pos >> kv.page_shift)];
+    if (page < 0 || page >= kv.num_pages) bad = ABFT_PAGED_BAD_PAGE;
+  }
+  if (bad != 0) {
+    if (threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, bad);
+    return;
+  }
+  const int c = threadIdx.x % kChunks;
+  const int slot = pos & ((1 << kv.page_shift) - 1);
+  constexpr int kShift = D == 128 ? 7 : 6;
+  float cs[16];  // this chunk's (cos, sin) pairs
+  if (p.rope != nullptr) {
+    const float4* r = reinterpret_cast<const float4*>(p.rope + static_cast<int64_t>(pos) * D) + c * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 x = __ldg(r + i);
+      cs[4 * i] = x.x, cs[4 * i + 1] = x.y, cs[4 * i + 2] = x.z, cs[4 * i + 3] = x.w;
+    }
+  }
+  const int rows = p.heads + 2 * kv.kv_heads;
+  for (int r = threadIdx.x / kChunks; r < rows; r += kAppendThreads / kChunks) {
+    const uint16_t* src;
+    uint16_t* dst;
+    bool turn = p.rope != nullptr;
+    if (r < p.heads) {
+      src = static_cast<const uint16_t*>(p.q) + t * p.qt + r * p.qh;
+      dst = static_cast<uint16_t*>(p.q_out) + t * p.ot + r * p.oh;
+    } else if (r < p.heads + kv.kv_heads) {
+      const int h = r - p.heads;
+      src = static_cast<const uint16_t*>(p.k) + t * p.kt + h * p.kh;
+      dst = static_cast<uint16_t*>(kv.k_pages) + paged_offset(page, kv.k_page_stride, h, slot, kv.page_shift, kShift);
+    } else {
+      const int h = r - p.heads - kv.kv_heads;
+      src = static_cast<const uint16_t*>(p.v) + t * p.vt + h * p.vh;
+      dst = static_cast<uint16_t*>(kv.v_pages) + paged_offset(page, kv.v_page_stride, h, slot, kv.page_shift, kShift);
+      turn = false;
+    }
+    uint4 lo = *reinterpret_cast<const uint4*>(src + 8 * c);
+    uint4 hi = *reinterpret_cast<const uint4*>(src + D / 2 + 8 * c);
+    if (turn) {
+      uint32_t* a = reinterpret_cast<uint32_t*>(&lo);
+      uint32_t* z = reinterpret_cast<uint32_t*>(&hi);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = unpack2<F16>(a[i]), y = unpack2<F16>(z[i]);
+        const float c0 = cs[4 * i], s0 = cs[4 * i + 1], c1 = cs[4 * i + 2], s1 = cs[4 * i + 3];
+        a[i] = pack2<F16>(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
+        z[i] = pack2<F16>(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + 8 * c) = lo;
+    *reinterpret_cast<uint4*>(dst + D / 2 + 8 * c) = hi;
+  }
+}
+
+}  // namespace abft

@@ -1,0 +1,263 @@
+"""Paged key-value cache: appending with rotation, and the attention over it.
+
+The cache of one decoder layer, next to the checked linears of a decode step
+(``ops.abft_linear``, ``AbftInjector``): pages of token slots that sequences
+of unlike length share, where a dense cache reserves the longest length for
+each. PyTorch supplies memory and streams, every computation runs in
+libabft_b200.so; tensors are CUDA bf16 or fp16 on an sm_100 device.
+
+    cache = PagedKVCache(k_pages, v_pages, page_table, seq_lens)
+    # each step: seq_lens counts the step's tokens already
+    q = cache.append(q, k, v, rope, cu_seqlens=cu)   # rotate q and k, store k and v
+    o = cache.prefill(q, cu)                         # causal, several tokens per sequence
+    q = cache.append(q, k, v, rope)                  # one token per sequence
+    o = cache.decode(q)
+
+``page_table`` and ``seq_lens`` stay on the device and are read by the
+kernels, so a captured step (``torch.cuda.graph``) replays with the lengths
+and pages of the moment. Bad entries never lead outside the tensors; they set
+bits that ``check_status`` turns into an error. Calls are queued on the
+current stream of the cache's device; results and workspaces are allocated
+there, per call.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _native as N
+
+_DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+
+
+def rope_table(positions: int, head_dim: int, theta: float = 1e6, device=None) -> torch.Tensor:
+    """(cos, sin) of position p and pair j, angle p * theta^(-2j / head_dim):
+    fp32 [positions, head_dim / 2, 2], computed in 64 bits (a 32-bit product
+    of a far position loses the angle's fraction) and rounded once."""
+    if head_dim % 2 or positions < 0:
+        raise ValueError(f"rope_table takes an even head_dim and positions >= 0, got {head_dim} and {positions}")
+    inv = float(theta) ** (-torch.arange(0, head_dim, 2, device=device, dtype=torch.float64) / head_dim)
+    ang = torch.outer(torch.arange(positions, device=device, dtype=torch.float64), inv)
+    return torch.stack((ang.cos(), ang.sin()), dim=-1).float()
+
+
+def _i32(name: str, t: torch.Tensor, dim: int, device: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or t.device != device:
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{name} must be a {dim}-D int32 tensor on {device}, got {got}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit stride in its last dimension")
+
+
+class PagedKVCache:
+    """Pages, page table and lengths of one layer's cache.
+
+    ``k_pages``, ``v_pages``: [num_pages, kv_heads, page_size, head_dim],
+    dense within a page (the page stride is free, so both may be views of one
+    [num_pages, 2, ...] pool), page_size 16, 32, 64 or 128, head_dim 64 or
+    128. ``page_table``: int32 [batch, max_pages]; ``seq_lens``: int32
+    [batch], the tokens of each sequence including the current step's. The
+    object holds references: write new entries into the tensors in place.
+    Sequences may share pages that neither appends to; tokens appended by one
+    call must go to distinct slots. Slots at or behind a sequence's length
+    may hold anything; keys and values below it are taken as finite numbers
+    (a non-finite value of a slot may reach every query of its sequence that
+    ``prefill`` answers in the same call).
+    """
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 seq_lens: torch.Tensor, *, status: Optional[torch.Tensor] = None):
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+            if t.dim() != 4:
+                raise ValueError(f"{name} must be [num_pages, kv_heads, page_size, head_dim], got {tuple(t.shape)}")
+            if t.dtype not in _DTYPES:
+                raise ValueError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+        if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.device != k_pages.device:
+            raise ValueError("k_pages and v_pages must have one shape, type and device")
+        num_pages, kv_heads, page_size, head_dim = k_pages.shape
+        if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}, got "
+                             f"{page_size} and {head_dim}")
+        if kv_heads == 0:
+            raise ValueError("k_pages has no heads")
+        if not k_pages.is_cuda:
+            raise ValueError("k_pages must be a CUDA tensor (the library has no CPU path)")
+        dense = (page_size * head_dim, head_dim, 1)
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            inner = [(s, d) for s, d, n in zip(t.stride()[1:], dense, t.shape[1:]) if n > 1]
+            if any(s != d for s, d in inner) or (num_pages > 1 and (t.stride(0) < kv_heads * dense[0] or t.stride(0) % 8)):
+                raise ValueError(f"{name} must be dense within a page, pages a multiple of 8 elements apart; strides "
+                                 f"{t.stride()} of shape {tuple(t.shape)}")
+        dev = k_pages.device
+        _i32("page_table", page_table, 2, dev)
+        _i32("seq_lens", seq_lens, 1, dev)
+        batch, max_pages = page_table.shape
+        if seq_lens.shape[0] != batch:
+            raise ValueError(f"seq_lens has {seq_lens.shape[0]} entries, page_table {batch} rows")
+        if batch > 1 and page_table.stride(0) < max_pages:
+            raise ValueError("page_table rows must not overlap")
+        if batch and (num_pages == 0 or max_pages == 0):
+            raise ValueError("a cache with sequences needs at least one page and one table column")
+        if status is None:
+            status = torch.zeros(1, dtype=torch.int32, device=dev)
+        else:
+            _i32("status", status, 1, dev)
+        self.k_pages, self.v_pages, self.page_table, self.seq_lens, self.status = k_pages, v_pages, page_table, seq_lens, status
+        self.batch, self.max_pages, self.num_pages = batch, max_pages, num_pages
+        self.kv_heads, self.page_size, self.head_dim = kv_heads, page_size, head_dim
+        self.dtype, self.device = k_pages.dtype, dev
+        kv = N.PagedKv()
+        kv.k_pages, kv.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+        kv.k_page_stride, kv.v_page_stride = k_pages.stride(0), v_pages.stride(0)
+        kv.page_table, kv.table_stride, kv.seq_lens = page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr()
+        kv.status = status.data_ptr()
+        kv.num_pages, kv.page_size, kv.kv_heads, kv.head_dim = num_pages, page_size, kv_heads, head_dim
+        kv.batch, kv.max_pages, kv.dtype = batch, max_pages, _DTYPES[k_pages.dtype]
+        self._kv = kv
+        self._index = dev.index
+        self._splits: dict = {}
+
+    # ---- argument checks ------------------------------------------------------
+    def _rows(self, name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int]) -> torch.Tensor:
+        """``t`` as [tokens, heads, head_dim] rows the kernels can read in
+        place (16-byte pieces), copied when its strides do not allow it."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        shape = t.shape
+        if (t.dtype != self.dtype or t.device != self.device or len(shape) != 3 or shape[2] != self.head_dim
+                or (tokens is not None and shape[0] != tokens) or (heads is not None and shape[1] != heads)):
+            raise ValueError(f"{name} must be a {self.dtype} tensor [{'tokens' if tokens is None else tokens}, "
+                             f"{'heads' if heads is None else heads}, {self.head_dim}] on {self.device}, got {t.dtype} "
+                             f"{tuple(shape)} on {t.device}")
+        s = t.stride()
+        if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+            return t.contiguous()
+        return t
+
+    def _group(self, heads: int) -> None:
+        if heads == 0 or heads % self.kv_heads or heads // self.kv_heads > 64:
+            raise ValueError(f"q has {heads} heads: a multiple of the cache's {self.kv_heads} kv heads, at most 64 "
+                             "for each, is needed")
+
+    def _out(self, name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+        if out is None:
+            return torch.empty(like.shape, dtype=self.dtype, device=self.device)
+        if self._rows(name, out, like.shape[0], like.shape[1]) is not out:
+            raise ValueError(f"{name} must be 16-byte aligned, with strides a multiple of 8 and unit stride in its last "
+                             "dimension")
+        return out
+
+    def _boundaries(self, cu: torch.Tensor) -> None:
+        _i32("cu_seqlens", cu, 1, self.device)
+        if cu.shape[0] != self.batch + 1:
+            raise ValueError(f"cu_seqlens must have {self.batch + 1} entries, got {cu.shape[0]}")
+
+    def _call(self, name: str, fn, args) -> None:
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(self._index))
+        else:
+            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(self._index))
+        if rc != N.ABFT_OK:
+            N.check(name, rc)
+
+    # ---- operators --------------------------------------------------------------
+    def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rope: Optional[torch.Tensor] = None, *,
+               cu_seqlens: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """Stores the new tokens' keys and values and returns the rotated q.
+
+        ``q`` [tokens, heads, head_dim], ``k`` and ``v`` [tokens, kv_heads,
+        head_dim] (any strides; parts of one fused projection are read in
+        place). ``cu_seqlens`` int32 [batch + 1]: rows cu[b] to cu[b + 1] are
+        the last tokens of sequence b, rows behind cu[batch] belong to none;
+        without it row b is the newest token of sequence b, none where
+        seq_lens[b] is 0. ``rope``: fp32 [positions, head_dim / 2, 2]
+        (``rope_table``) rotates q and k by position, in fp32, rounded once;
+        None stores k as it is. ``q_out`` (may be ``q``) receives q; rows of
+        no sequence are left as they were. q None stores k and v only.
+        """
+        k = self._rows("k", k, None, self.kv_heads)
+        tokens = k.shape[0]
+        v = self._rows("v", v, tokens, self.kv_heads)
+        args = N.KvAppendArgs()
+        args.kv = self._kv
+        if cu_seqlens is not None:
+            self._boundaries(cu_seqlens)
+            args.cu_seqlens = cu_seqlens.data_ptr()
+        elif tokens != self.batch:
+            raise ValueError(f"without cu_seqlens k must have one row for each of the {self.batch} sequences, got {tokens}")
+        if rope is not None:
+            if (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1] * 2 != self.head_dim or rope.shape[2] != 2
+                    or rope.device != self.device or not rope.is_contiguous() or rope.data_ptr() % 16):
+                raise ValueError(f"rope must be a contiguous float32 [positions, {self.head_dim // 2}, 2] tensor on "
+                                 f"{self.device}, got {rope.dtype} {tuple(rope.shape)}")
+            args.rope, args.max_positions = rope.data_ptr(), rope.shape[0]
+            if rope.shape[0] == 0:
+                raise ValueError("rope has no positions")
+        if q is not None:
+            self._group(q.shape[1] if q.dim() == 3 else 0)
+            q = self._rows("q", q, tokens, None)
+            q_out = self._out("q_out", q_out, q)
+            args.q, args.q_out, args.heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+            args.q_token_stride, args.q_head_stride, _ = q.stride()
+            args.o_token_stride, args.o_head_stride, _ = q_out.stride()
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        args.k, args.v, args.tokens = k.data_ptr(), v.data_ptr(), tokens
+        args.k_token_stride, args.k_head_stride, _ = k.stride()
+        args.v_token_stride, args.v_head_stride, _ = v.stride()
+        self._call("abft_kv_append", N.lib().abft_kv_append, args)
+        return q_out
+
+    def decode(self, q: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               num_splits: int = 0) -> torch.Tensor:
+        """Attention of each sequence's newest token over its cache: ``q``
+        [batch, heads, head_dim], returns the same shape. ``scale`` defaults
+        to head_dim^-0.5. A sequence of length 0 gives zeros. ``num_splits``:
+        pieces a sequence is cut into (0: chosen from the batch, the heads and
+        the table's width)."""
+        args, out, q = self._attn(q, scale, out, self.batch, num_splits)  # q: alive until the launch is queued
+        L = N.lib()
+        key = ("decode", args.heads, num_splits)
+        need = self._splits.get(key)
+        if need is None:  # depends on sizes alone
+            with torch.cuda.device(self._index):
+                need = self._splits[key] = int(L.abft_paged_decode_workspace_bytes(ctypes.byref(args)))
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        self._call("abft_paged_decode", L.abft_paged_decode, args)
+        return out
+
+    def _attn(self, q, scale, out, tokens, num_splits):
+        self._group(q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0)
+        q = self._rows("q", q, tokens, None)
+        out = self._out("out", out, q)
+        args = N.PagedAttnArgs()
+        args.kv = self._kv
+        args.q, args.out = q.data_ptr(), out.data_ptr()
+        args.tokens, args.heads = q.shape[0], q.shape[1]
+        args.q_token_stride, args.q_head_stride, _ = q.stride()
+        args.o_token_stride, args.o_head_stride, _ = out.stride()
+        args.scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        args.num_splits = int(num_splits)
+        return args, out, q
+
+    def check_status(self) -> None:
+        """Raises ValueError when a call since the last check met a bad page
+        entry, length or position on the device (which it skipped), and
+        clears the record. Synchronises."""
+        bits = int(self.status.cpu()[0])
+        if not bits:
+            return
+        self.status.zero_()
+        said = [text for bit, text in ((N.PAGED_BAD_PAGE, "a page_table entry outside the pool"),
+                                       (N.PAGED_BAD_LEN, "a length below 0, beyond the table or below the new tokens"),
+                                       (N.PAGED_BAD_ANGLE, "a position beyond the rotation table")) if bits & bit]
+        raise ValueError("paged cache: " + "; ".join(said))
