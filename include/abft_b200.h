@@ -420,12 +420,15 @@ int abft_check_only_noalloc(const abft_check_args* args, void* stream);
  *                         the length (append skips those of negative
  *                         position; attention gives them 0);
  *   ABFT_PAGED_BAD_ANGLE  a position at or beyond max_positions of the
- *                         rotation table: append skips the token.
+ *                         rotation table: append skips the token;
+ *   ABFT_PAGED_TIMEOUT    a bounded wait of the prefill kernel gave up: its
+ *                         output is incomplete.
  * Slots at or beyond a sequence's length are never used: they may hold
  * anything, NaN included. */
 #define ABFT_PAGED_BAD_PAGE  1u
 #define ABFT_PAGED_BAD_LEN   2u
 #define ABFT_PAGED_BAD_ANGLE 4u
+#define ABFT_PAGED_TIMEOUT   8u
 
 /* A page pool and the sequences in it. */
 typedef struct abft_paged_kv {
@@ -493,6 +496,14 @@ int abft_kv_append(const abft_kv_append_args* args, void* stream);
  * seq_lens[b]; a sequence of length 0 gives a row of zeros. */
 size_t abft_paged_decode_workspace_bytes(const abft_paged_attn_args* args);
 int abft_paged_decode(const abft_paged_attn_args* args, void* stream);
+
+/* Causal: query row i of the n new tokens of sequence b sees the slots
+ * j <= seq_lens[b] - n + i (none: a row of zeros). Any n from 0 up; rows
+ * behind cu_seqlens[batch] are left as they were. Within a sequence keys and
+ * values are taken as finite: a non-finite value also reaches rows that do
+ * not see it (its weight there is 0, and 0 * inf is not). */
+size_t abft_paged_prefill_workspace_bytes(const abft_paged_attn_args* args);
+int abft_paged_prefill(const abft_paged_attn_args* args, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -251,3 +251,112 @@ def test_decode_bad_entries(cuda_device):
     assert "length" in attempt(lens=-1)
     assert "length" in attempt(lens=49)
     assert "length" in attempt(lens=2147483647)
+
+
+# ---- prefill ------------------------------------------------------------------
+def owners_of(new, total):
+    return [(b, t - n + i + 1) for b, (n, t) in enumerate(zip(new, total)) for i in range(n)]
+
+
+def run_prefill(dev, new, total, heads, kv_heads, d, page, dtype, *, seed=0, splits=0, spread=1.5, joint=False, extra=0,
+                scale=None, pad=0):
+    pool = Pool(total, kv_heads, page, d, dtype, seed=seed, joint=joint, extra_columns=extra)
+    cache = pool.device_cache(dev, PagedKVCache)
+    tokens = sum(new)
+    q = (torch.randn(tokens + pad, heads, d, generator=torch.Generator().manual_seed(seed + 9)) * spread).to(dtype)
+    cu = torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32, device=dev)
+    out = torch.full((tokens + pad, heads, d), 7.0, dtype=dtype, device=dev)
+    got = cache.prefill(q.to(dev), cu, num_splits=splits, scale=scale, out=out)
+    assert got is out
+    cache.check_status()
+    want, tol = attention(pool, q[:tokens], owners_of(new, total), scale)
+    close(got[:tokens], want, tol)
+    assert (out[tokens:] == 7.0).all()
+    return cache, q.to(dev), cu, out
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (28, 4), (5, 5), (16, 2), (9, 1), (17, 1), (64, 1)])
+def test_prefill_head_layouts(cuda_device, heads, kv_heads, d, dtype):
+    run_prefill(cuda_device, [77, 3], [77, 300], heads, kv_heads, d, 16, dtype)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 2, 5])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("new,total", [([1], [1]), ([2], [2]), ([17], [17]), ([1], [513]), ([129, 5], [129, 128]),
+                                       ([16, 16], [128, 144]), ([5, 0, 0, 40], [700, 3, 0, 40]),
+                                       ([255, 256, 257], [255, 256, 257])])
+def test_prefill_lengths(cuda_device, new, total, page, splits):
+    run_prefill(cuda_device, new, [max(n, t) for n, t in zip(new, total)], 7, 1, 128, page, BF16, splits=splits)
+
+
+def test_prefill_longer_and_peaked(cuda_device):
+    run_prefill(cuda_device, [700], [1500], 7, 1, 128, 32, BF16)
+    run_prefill(cuda_device, [300, 20], [700, 2000], 8, 4, 64, 64, F16, spread=30.0)
+    run_prefill(cuda_device, [300, 20], [700, 2000], 8, 4, 64, 64, F16, scale=0.0)
+    run_prefill(cuda_device, [300, 20], [700, 2000], 8, 4, 64, 64, BF16, scale=-0.2)
+
+
+def test_prefill_rows_of_no_sequence_joint_pool_wide_table(cuda_device):
+    run_prefill(cuda_device, [30, 0, 100], [30, 0, 117], 12, 4, 128, 16, F16, joint=True, extra=50, pad=9)
+    run_prefill(cuda_device, [2, 1], [900, 17], 12, 4, 128, 16, F16, joint=True, extra=50, pad=200, splits=3)
+
+
+def test_prefill_rising_maximum(cuda_device):
+    """Scores that rise by far more than 2^8 from step to step: every step rescales."""
+    pool = Pool([900], 1, 16, 64, BF16)
+    held = pool.table[0, :57].long()
+    ramp = torch.arange(57 * 16).view(57, 1, 16, 1) / 900.0
+    pool.k[held] = (ramp * 20 * torch.ones(64)).to(BF16)
+    pool.k[held[-1], :, 4:] = float("nan")
+    cache = pool.device_cache(cuda_device, PagedKVCache)
+    q = torch.full((100, 2, 64), 3.0).to(BF16)
+    want, tol = attention(pool, q, owners_of([100], [900]), 1.0)
+    cu = torch.tensor([0, 100], dtype=torch.int32, device=cuda_device)
+    close(cache.prefill(q.to(cuda_device), cu, scale=1.0), want, tol)
+    want, tol = attention(pool, -q, owners_of([100], [900]), 1.0)  # falling
+    close(cache.prefill(-q.to(cuda_device), cu, scale=1.0), want, tol)
+
+
+def test_prefill_same_bits_twice_other_strides_and_decode(cuda_device):
+    cache, q, cu, got = run_prefill(cuda_device, [90, 1, 33], [900, 1234, 33], 28, 4, 128, 16, BF16)
+    assert torch.equal(cache.prefill(q, cu), got)
+    wide = torch.zeros(124, 28, 256, dtype=BF16, device=cuda_device)
+    wide[:, :, 128:] = q
+    assert torch.equal(cache.prefill(wide[:, :, 128:], cu), got)
+    assert torch.equal(cache.prefill(q.transpose(1, 2).contiguous().transpose(1, 2), cu), got)
+    # the newest tokens again, one per sequence
+    newest = (cu[1:] - 1).long()
+    one = cache.decode(q[newest])
+    assert (one.float() - got[newest].float()).abs().max() <= 2.0 ** -6 * got.float().abs().max()
+
+
+def test_prefill_bad_entries(cuda_device):
+    def attempt(lens=None, entry=None, column=1, new=(20, 25)):
+        pool = Pool([48, 25], 2, 16, 64, BF16)
+        cache = pool.device_cache(cuda_device, PagedKVCache)
+        total = [48, 25]
+        if lens is not None:
+            cache.seq_lens[0] = lens
+            total[0] = max(0, min(48, lens))
+        if entry is not None:
+            cache.page_table[0, column] = entry
+            at = pool.table[0, column].long().item()
+            pool.k[at] = 0
+            pool.v[at] = 0
+        q = torch.randn(sum(new), 4, 64, generator=torch.Generator().manual_seed(3)).to(BF16)
+        cu = torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device=cuda_device)
+        got = cache.prefill(q.to(cuda_device), cu)
+        want, tol = attention(pool, q, owners_of(new, total))
+        close(got, want, tol)
+        with pytest.raises(ValueError) as e:
+            cache.check_status()
+        return str(e.value)
+
+    assert "page_table" in attempt(entry=5000)
+    assert "page_table" in attempt(entry=-2, column=0)
+    assert "length" in attempt(lens=-1)
+    assert "length" in attempt(lens=49)
+    assert "length" in attempt(lens=7)  # fewer than the new tokens: the first 13 see nothing
+    assert "length" in attempt(lens=2147483647)

@@ -13,7 +13,7 @@ from vla_abft_estimate_b200.paged import PagedKVCache, rope_table
 INDEX_PROGRAM = r"""
 #include <cstdio>
 #include <cstdlib>
-#include "paged_index.cuh"
+#include "paged_prefill.cuh"
 using namespace abft;
 static void need(bool ok, const char* what) {
   if (!ok) { std::printf("FAILED %s\n", what); std::exit(1); }
@@ -53,6 +53,23 @@ int main() {
   const int64_t page = int64_t{32} * 128 * 128;
   need(paged_offset(1 << 20, page, 31, 127, 7, 7) == (int64_t{1} << 20) * page + (int64_t{31} * 128 + 127) * 128, "offset");
   need(paged_offset(3, 1000000, 2, 5, 4, 6) == 3000000 + (2 * 16 + 5) * 64, "small offset");
+  // packed rows of a sequence stay within the tensor whatever the boundaries say
+  const int cu[] = {-5, 3, 2, 900, 50, 50, 0x7FFFFFFF, static_cast<int>(0x80000000u), 7};
+  for (int b = 0; b < 8; ++b) {
+    int lo, hi;
+    packed_range(cu, b, 60, &lo, &hi);
+    need(0 <= lo && lo <= hi && hi <= 60, "packed range");
+  }
+  int lo, hi;
+  const int good[] = {0, 4, 4, 60};
+  packed_range(good, 0, 60, &lo, &hi);
+  need(lo == 0 && hi == 4, "packed 0");
+  packed_range(good, 1, 60, &lo, &hi);
+  need(lo == 4 && hi == 4, "packed 1");
+  packed_range(good, 2, 60, &lo, &hi);
+  need(lo == 4 && hi == 60, "packed 2");
+  need(visible_keys(10, 3, 0) == 8 && visible_keys(10, 3, 2) == 10, "visible");
+  need(visible_keys(1, 3, 0) == 0 && visible_keys(1, 3, 1) == 0 && visible_keys(1, 3, 2) == 1, "none visible");
   std::printf("%ld\n", checks);
   return 0;
 }
@@ -73,7 +90,7 @@ def test_index_arithmetic(tmp_path):
     src.write_text(INDEX_PROGRAM)
     exe = tmp_path / "ix"
     subprocess.check_call([_build._nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O2",
-                           f"-I{_build.CSRC_DIR}", str(src), "-o", str(exe)])
+                           f"-I{_build.CSRC_DIR}", f"-I{_build.INCLUDE_DIR}", str(src), "-o", str(exe)])
     out = subprocess.run([str(exe)], capture_output=True, text=True)
     assert out.returncode == 0, out.stdout
     assert int(out.stdout) > 10_000_000
@@ -127,6 +144,9 @@ def test_cache_refusals(field, value, code):
     d.kv, d.q, d.out, d.heads, d.tokens, d.scale = kv, 0x50000, 0x60000, 28, kv.batch, 1.0
     assert L.abft_paged_decode(ctypes.byref(d), None) == code
     assert L.abft_paged_decode_workspace_bytes(ctypes.byref(d)) == 0
+    d.cu_seqlens = 0x70000
+    assert L.abft_paged_prefill(ctypes.byref(d), None) == code
+    assert L.abft_paged_prefill_workspace_bytes(ctypes.byref(d)) == 0
 
 
 def test_append_refusals():
@@ -163,7 +183,7 @@ def test_attention_refusals():
             setattr(a, k, v)
         return fn(ctypes.byref(a), None)
 
-    for fn in (L.abft_paged_decode,):
+    for fn in (L.abft_paged_decode, L.abft_paged_prefill):
         assert fn(None, None) == -1
         for over, code in [({"tokens": -1}, -1), ({"num_splits": -1}, -1), ({"num_sms": -1}, -1),
                            ({"scale": float("inf")}, -1), ({"scale": float("nan")}, -1), ({"heads": 0}, -1),
@@ -174,6 +194,9 @@ def test_attention_refusals():
         if not torch.cuda.is_available():
             assert call(fn) == -6
     assert call(L.abft_paged_decode, tokens=1) == -1  # one row per sequence
+    assert call(L.abft_paged_prefill, cu_seqlens=None) == -1
+    assert call(L.abft_paged_prefill, tokens=0) == 0
+    assert call(L.abft_paged_prefill, tokens=1 << 30) == -3
 
 
 def test_workspace_grows_with_pieces():

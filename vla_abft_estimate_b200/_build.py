@@ -25,7 +25,8 @@ OBJ_DIR = LIB_DIR / "obj"
 # of them is newer than its object.
 SOURCES = {
     "abft_api.cu": ["ptx.cuh", "gemm_kernel.cuh", "aux_kernels.cuh"],
-    "paged_api.cu": ["ptx.cuh", "paged_index.cuh", "paged_append.cuh", "paged_decode.cuh"],
+    "paged_api.cu": ["ptx.cuh", "paged_index.cuh", "paged_append.cuh", "paged_decode.cuh",
+                     "paged_prefill.cuh"],
 }
 
 NVCC_FLAGS = [

@@ -71,6 +71,8 @@ EXPORTED_SYMBOLS = (
     "abft_kv_append",
     "abft_paged_decode_workspace_bytes",
     "abft_paged_decode",
+    "abft_paged_prefill_workspace_bytes",
+    "abft_paged_prefill",
 )
 
 NO_ALLOC_SCRATCH_BYTES = 4 << 20
@@ -79,6 +81,7 @@ NO_ALLOC_SCRATCH_BYTES = 4 << 20
 PAGED_BAD_PAGE = 1
 PAGED_BAD_LEN = 2
 PAGED_BAD_ANGLE = 4
+PAGED_TIMEOUT = 8
 
 
 class AbftError(RuntimeError):
@@ -317,6 +320,10 @@ def lib() -> ctypes.CDLL:
     L.abft_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs)]
     L.abft_paged_decode.restype = ctypes.c_int
     L.abft_paged_decode.argtypes = [ctypes.POINTER(PagedAttnArgs), vp]
+    L.abft_paged_prefill_workspace_bytes.restype = sz
+    L.abft_paged_prefill_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs)]
+    L.abft_paged_prefill.restype = ctypes.c_int
+    L.abft_paged_prefill.argtypes = [ctypes.POINTER(PagedAttnArgs), vp]
     _LIB = L
     return L
 

@@ -9,6 +9,7 @@
 
 #include "paged_append.cuh"
 #include "paged_decode.cuh"
+#include "paged_prefill.cuh"
 
 using namespace abft;
 
@@ -18,7 +19,7 @@ constexpr int kMaxDevices = 64;
 struct DeviceInfo {
   bool init, ok;
   int sms;
-  bool smem_set[8];  // by decode_slot()
+  bool smem_set[12];  // decode instances 0-7, prefill instances 8-11
 };
 DeviceInfo g_paged_dev[kMaxDevices];
 std::mutex g_paged_mu;
@@ -71,8 +72,8 @@ inline bool off8el(int64_t s) { return (s & 7) != 0; }
 
 // Launch with programmatic serialization: the kernel waits
 // (griddepcontrol.wait) before any global access.
-template <typename K, typename P>
-int launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const P& p) {
+template <typename K, typename... P>
+int launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const P&... p) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -83,7 +84,7 @@ int launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const P
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, p...) != cudaSuccess) {
     cudaGetLastError();
     return ABFT_ERR_CUDA;
   }
@@ -151,6 +152,8 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
   if ((rc = check_heads(a->heads, a->kv.kv_heads)) != ABFT_OK) return rc;
   if (decode && a->tokens != a->kv.batch) return ABFT_ERR_INVALID_ARG;
   if (a->tokens == 0 || a->kv.batch == 0) return ABFT_OK;
+  // Grids (blocks x kv heads, rows x heads for the join) stay below 2^31.
+  if (a->tokens >= (int64_t{1} << 30) / a->heads) return ABFT_ERR_UNSUPPORTED;
   if (a->q == nullptr || a->out == nullptr || (!decode && a->cu_seqlens == nullptr)) return ABFT_ERR_INVALID_ARG;
   if (off16(a->q) || off16(a->out) || off8el(a->q_token_stride) || off8el(a->q_head_stride) ||
       off8el(a->o_token_stride) || off8el(a->o_head_stride))
@@ -196,6 +199,91 @@ int launch_decode(int dev, int slot, const DecodeParams& p, int heads, cudaStrea
   j.part_o = p.part_o;
   j.part_ml = p.part_ml;
   return launch(paged_join_kernel<D, F16>, dim3(heads, p.kv.batch), dim3(128), 0, s, j);
+}
+
+// ---- prefill ------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn tile_encoder() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+    else
+      cudaGetLastError();
+  });
+  return fn;
+}
+
+// Map of a page pool: [page][64-column block][head and slot][64 columns];
+// a box is one page's slots of one head and column block, 128-byte swizzled.
+int page_map(CUtensorMap* m, const abft_paged_kv& c, const void* pages, int64_t stride) {
+  EncodeTiledFn enc = tile_encoder();
+  if (enc == nullptr) return ABFT_ERR_DRIVER;
+  const int64_t dense = static_cast<int64_t>(c.kv_heads) * c.page_size * c.head_dim;
+  if (c.num_pages <= 1) stride = dense;
+  cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(c.kv_heads) * c.page_size, static_cast<cuuint64_t>(c.head_dim / 64),
+                        static_cast<cuuint64_t>(c.num_pages)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.head_dim) * 2, 128, static_cast<cuuint64_t>(stride) * 2};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(c.page_size), 1, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type =
+      c.dtype == ABFT_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = enc(m, type, 4, const_cast<void*>(pages), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ABFT_OK : ABFT_ERR_ALIGNMENT;
+}
+
+int64_t prefill_blocks(const abft_paged_attn_args* a) {
+  const int tile_tokens = kPreRows / (a->heads / a->kv.kv_heads);
+  return a->tokens / (2 * tile_tokens) + a->kv.batch;
+}
+
+// Pieces a block's keys are cut into: while the blocks alone would leave SMs
+// idle, as many as fill them once.
+int prefill_splits(const abft_paged_attn_args* a, int sms) {
+  const int64_t steps = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kPreKeys - 1) / kPreKeys;
+  int64_t n = a->num_splits > 0 ? a->num_splits : sms / (prefill_blocks(a) * a->kv.kv_heads);
+  if (n > steps) n = steps;
+  if (n > 65535) n = 65535;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+
+size_t prefill_bytes(const abft_paged_attn_args* a, int splits) {
+  if (splits <= 1) return 0;
+  const size_t rows = static_cast<size_t>(a->tokens) * a->heads * splits;
+  return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2));
+}
+
+template <int D, bool F16>
+int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                   const PrefillParams& p, cudaStream_t s) {
+  using Cfg = PrefillCfg<D>;
+  int rc = raise_smem(dev, slot, paged_prefill_kernel<D, F16>, Cfg::kSmemBytes);
+  if (rc != ABFT_OK) return rc;
+  rc = launch(paged_prefill_kernel<D, F16>, dim3(static_cast<unsigned>(p.blocks) * p.kv.kv_heads, p.splits),
+              dim3(kPreThreads), Cfg::kSmemBytes, s, tm_k, tm_v, p);
+  if (rc != ABFT_OK || p.splits == 1) return rc;
+  PrefillJoinParams j;
+  j.kv = p.kv;
+  j.cu = p.cu;
+  j.out = p.out;
+  j.ot = p.ot;
+  j.oh = p.oh;
+  j.tokens = p.tokens;
+  j.heads = a->heads;
+  j.splits = p.splits;
+  j.tile_tokens = p.tile_tokens;
+  j.part_o = p.part_o;
+  j.part_ml = p.part_ml;
+  return launch(paged_prefill_join_kernel<D, F16>, dim3(static_cast<unsigned>(p.tokens) * a->heads), dim3(128), 0, s, j);
 }
 
 }  // namespace
@@ -282,6 +370,51 @@ int abft_paged_decode(const abft_paged_attn_args* a, void* stream) {
     case 6: return launch_decode<128, 2, false>(dev, slot, p, a->heads, s);
     default: return launch_decode<128, 2, true>(dev, slot, p, a->heads, s);
   }
+}
+
+size_t abft_paged_prefill_workspace_bytes(const abft_paged_attn_args* a) {
+  if (attn_check(a, false) != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return 0;
+  int dev = 0, sms = a->num_sms;
+  if (sms == 0 && paged_device(&dev, &sms) != ABFT_OK) sms = 148;
+  return prefill_bytes(a, prefill_splits(a, sms));
+}
+
+int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
+  int rc = attn_check(a, false);
+  if (rc != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return rc;
+  int dev = 0, sms = 0;
+  if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
+  if (a->num_sms > 0) sms = a->num_sms;
+  PrefillParams p;
+  p.kv = view_of(a->kv);
+  p.q = a->q, p.out = a->out;
+  p.qt = a->q_token_stride, p.qh = a->q_head_stride;
+  p.ot = a->o_token_stride, p.oh = a->o_head_stride;
+  p.cu = a->cu_seqlens;
+  p.tokens = static_cast<int32_t>(a->tokens);
+  p.group = a->heads / a->kv.kv_heads;
+  p.tile_tokens = kPreRows / p.group;
+  p.splits = prefill_splits(a, sms);
+  p.blocks = static_cast<int32_t>(prefill_blocks(a));
+  const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
+  p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
+  p.flip = a->scale < 0.f ? 0x80008000u : 0u;
+  const size_t need = prefill_bytes(a, p.splits);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
+  if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(
+      p.part_o + static_cast<size_t>(a->tokens) * a->heads * p.splits * a->kv.head_dim);
+  CUtensorMap tm_k, tm_v;
+  if ((rc = page_map(&tm_k, a->kv, a->kv.k_pages, a->kv.k_page_stride)) != ABFT_OK) return rc;
+  if ((rc = page_map(&tm_v, a->kv, a->kv.v_pages, a->kv.v_page_stride)) != ABFT_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
+  if (a->kv.head_dim == 128)
+    return f16 ? launch_prefill<128, true>(dev, 11, a, tm_k, tm_v, p, s)
+               : launch_prefill<128, false>(dev, 10, a, tm_k, tm_v, p, s);
+  return f16 ? launch_prefill<64, true>(dev, 9, a, tm_k, tm_v, p, s)
+             : launch_prefill<64, false>(dev, 8, a, tm_k, tm_v, p, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,607 @@
+// paged_prefill.cuh - causal attention of prompt chunks over the paged cache.
+//
+// Query row i of sequence b (n new tokens of L in all) sees the slots
+// j <= L - n + i:   o = sum_j softmax_j(scale q . k_j) v_j.
+//
+// Bound: 4 d flops per visible (query, key) pair against 2 bytes of K and V
+// per key and 128-row tile: a chunk of some hundred tokens is bound by the
+// tensor cores and by the exponentials (one per pair: 16 a clock and SM,
+// as long as the 4 d = 512 flops of the pair take at 8192 a clock), a short
+// one by reading the cache.
+//
+// One CTA takes two tiles of 128 query rows of one kv head. A tile's rows are
+// (token, query head of the group) pairs, so that a group shares each key and
+// a short chunk fills its rows. Per 128 keys:
+//   S = Q K^T   tcgen05.mma, both operands in shared memory, S in TMEM
+//   P = 2^(x - m) by one thread per row (no exchange between lanes): S is read
+//       from TMEM, P goes back over it as 16-bit operand
+//   O += P V    tcgen05.mma with P from TMEM, V as N-major operand
+// The two tiles alternate: while the tensor core works on one, the other's
+// rows are exponentiated. O stays in TMEM; it is rescaled only when a row's
+// maximum has risen by more than 2^8 since the last rescaling (P and the sum
+// l then still fit their formats, and the quotient is unchanged), which after
+// the first tiles of a row hardly happens.
+//
+// Warps: 0-3 and 4-7 the rows of tile 0 and 1 (TMEM lane quadrant = warp % 4),
+// 8 TMA loads of pages into a ring of tiles, 9 the MMA issuer.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged_decode.cuh"
+#include "paged_index.cuh"
+#include "ptx.cuh"
+
+namespace abft {
+
+constexpr int kPreRows = 128;   // query rows of a tile
+constexpr int kPreKeys = 128;   // keys of a step
+constexpr int kPreThreads = 320;
+
+template <int D>
+struct PrefillCfg {
+  static constexpr int kHalves = D / 64;                     // 128-byte wide column blocks of a row
+  static constexpr int kTileBytes = kPreKeys * D * 2;        // a K, V or Q tile
+  static constexpr int kBlockBytes = kPreKeys * 128;         // one column block of it
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kOffRing = 2 * kTileBytes;            // after the two Q tiles
+  static constexpr int kOffBar = kOffRing + kSlots * kTileBytes;
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 1;  // full, empty, qfull, sfull, pfull, ofull, drain
+  static constexpr int kOffMisc = kOffBar + kBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 64 + 1024;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static_assert(kSmemBytes > 232448 / 2, "one CTA per SM: each takes all of TMEM");
+  // TMEM columns: S of both tiles (P over its first half), then O of both.
+  static constexpr int kTmemCols = 512;
+  static constexpr int kColO = 256;
+};
+
+struct PrefillParams {
+  PagedView kv;
+  const void* q;
+  void* out;
+  int64_t qt, qh, ot, oh;  // token and head strides, elements
+  const int32_t* cu;
+  int32_t tokens;          // rows of q
+  int32_t group;           // query heads per kv head
+  int32_t tile_tokens;     // tokens of one tile: 128 / group
+  int32_t blocks;          // CTAs per kv head and split: tokens / (2 tile_tokens) + batch at most
+  int32_t splits;
+  float scale_log2;        // |scale| * log2(e), never 0
+  uint32_t flip;           // sign bits of a packed pair when scale < 0: applied to q
+  float* part_o;           // [tokens * heads][splits][head_dim]
+  float2* part_ml;         // [tokens * heads][splits]
+};
+
+// A sequence's share of the packed rows, safe for any cu: begin <= end <= tokens.
+__host__ __device__ __forceinline__ void packed_range(const int32_t* cu, int b, int tokens, int* begin, int* end) {
+  const int lo = cu[b], hi = cu[b + 1];
+  *begin = lo < 0 ? 0 : (lo > tokens ? tokens : lo);
+  *end = hi < *begin ? *begin : (hi > tokens ? tokens : hi);
+}
+
+// Keys that local token i of n sees in a sequence of length len.
+__host__ __device__ __forceinline__ int visible_keys(int len, int n, int i) {
+  const int v = len - n + i + 1;
+  return v > 0 ? v : 0;
+}
+
+// Block `index` of the packed sequences, each cut into blocks of `per`
+// tokens; called by one warp. Heavier blocks (later tokens) of a sequence
+// come first. Returns false behind the last block.
+__device__ __forceinline__ bool find_block(const int32_t* cu, int batch, int tokens, int per, int index, int lane,
+                                           int* seq, int* block) {
+  int before = 0;
+  for (int i = 0; i < batch; i += 32) {
+    int mine = 0;
+    if (i + lane < batch) {
+      int lo, hi;
+      packed_range(cu, i + lane, tokens, &lo, &hi);
+      mine = (hi - lo + per - 1) / per;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > index);
+    if (past != 0) {
+      const int src = __ffs(past) - 1;
+      const int first = before + __shfl_sync(0xFFFFFFFFu, upto - mine, src);
+      const int count = __shfl_sync(0xFFFFFFFFu, mine, src);
+      const int at = count - 1 - (index - first);
+      if (at < 0 || at >= count) return false;  // boundaries that do not rise
+      *seq = i + src;
+      *block = at;
+      return true;
+    }
+    before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+  }
+  return false;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint64_t* bar, int32_t x, int32_t y, int32_t z,
+                                            int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// D += A B with A (16-bit pairs, one row per lane) in TMEM.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Descriptor of a [keys x D] tile as N-major B operand (its keys are the
+// MMA's K dimension): 128-byte swizzled rows, 64 columns per block, `block`
+// bytes from one column block to the next (leading offset), 1024 from 8 keys
+// to the next 8 (stride offset).
+__device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t saddr, uint32_t block) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(block >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+constexpr uint32_t kIdescBNMajor = 1u << 16;
+
+// mbar_wait that goes on after an abort: for what is still in flight.
+__device__ __forceinline__ void mbar_wait_bounded(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (global_timer_ns() - t0 > kWaitTimeoutNs) return;
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kPreThreads, 1)
+    paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                         const PrefillParams p) {
+  using Cfg = PrefillCfg<D>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
+  uint64_t* empty = full + Cfg::kSlots;
+  uint64_t* qfull = empty + Cfg::kSlots;
+  uint64_t* sfull = qfull + 2;
+  uint64_t* pfull = sfull + 2;
+  uint64_t* ofull = pfull + 2;
+  uint64_t* drain = ofull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* where = reinterpret_cast<volatile int*>(tmem_slot + 2);  // sequence (-1: none), block
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedView& kv = p.kv;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Cfg::kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&qfull[t], kPreRows);
+      mbar_init(&sfull[t], 1);
+      mbar_init(&pfull[t], kPreRows);
+      mbar_init(&ofull[t], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  griddep_wait();
+  griddep_launch();
+  const int hk = blockIdx.x % kv.kv_heads;
+  const int index = blockIdx.x / kv.kv_heads;
+  const int split = blockIdx.y;
+  if (warp == 0) {
+    int seq = -1, block = 0;
+    find_block(p.cu, kv.batch, p.tokens, 2 * p.tile_tokens, index, lane, &seq, &block);
+    if (lane == 0) {
+      where[0] = seq;
+      where[1] = block;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int seq = where[0], block = where[1];
+
+  if (seq >= 0) {
+    int row0, row_end;
+    packed_range(p.cu, seq, p.tokens, &row0, &row_end);
+    const int n = row_end - row0;
+    bool bad_len;
+    const int len = paged_clamp_len(kv.seq_lens[seq], kv.max_pages, kv.page_shift, &bad_len);
+    if ((bad_len || len < n) && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
+    // First token and steps (of 128 keys) of each tile; a tile behind the
+    // chunk's end has none.
+    const int tok0 = block * 2 * p.tile_tokens;
+    int steps[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int first = tok0 + t * p.tile_tokens;
+      const int last = min(first + p.tile_tokens, n) - 1;
+      steps[t] = last >= first ? (visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys : 0;
+    }
+    int j0, j1;
+    split_tiles(max(steps[0], steps[1]), p.splits, split, &j0, &j1);
+    const int end[2] = {max(j0, min(j1, steps[0])), max(j0, min(j1, steps[1]))};
+    const int total = 2 * (j1 - j0);  // ring loads: K and V of each step
+
+    if (warp < 8) {
+      // ---------------------------------------------------------- softmax rows
+      const int t = warp >> 2;
+      const int r = threadIdx.x & 127;
+      const int first = tok0 + t * p.tile_tokens;
+      const int here = max(0, min(p.tile_tokens, n - first)) * p.group;  // rows in use
+      // Q tile into shared memory, in the swizzled layout of a TMA box.
+      if (end[t] > j0) {
+        uint8_t* dst = smem + t * Cfg::kTileBytes;
+        constexpr int kCpr = D / 8;
+#pragma unroll 4
+        for (int i = r; i < kPreRows * kCpr; i += kPreRows) {
+          const int row = i / kCpr, c = i % kCpr;
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (row < here) {
+            const int tok = row / p.group, g = row - tok * p.group;
+            x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (row0 + first + tok) * p.qt +
+                                                (hk * p.group + g) * p.qh + c * 8);
+            x.x ^= p.flip, x.y ^= p.flip, x.z ^= p.flip, x.w ^= p.flip;
+          }
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * Cfg::kBlockBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&qfull[t]);
+      }
+      const int tok = r / p.group;
+      const bool live = r < here;
+      const int vis = live ? visible_keys(len, n, first + tok) : 0;
+      const int vis_min = visible_keys(len, n, first);  // of the tile's first token
+      const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+      const uint32_t ts = lanes + t * 128, to = lanes + Cfg::kColO + t * D;
+      float m = -INFINITY, l = 0.f;  // m: maximum that P refers to (raw scores)
+      bool ok = true;
+      for (int j = j0; j < end[t]; ++j) {
+        if (!mbar_wait(&sfull[t], (j - j0) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + c * 32, s[c]);
+        tmem_ld_wait();
+        if (vis_min < (j + 1) * kPreKeys) {
+          const int lim = vis - j * kPreKeys;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= lim) s[c][i] = 0xFF800000u;  // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+        }
+        const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        const bool raise = (mn - m) * p.scale_log2 > 8.f;  // also from m = -inf; false for -inf, -inf
+        if (j == j0) {
+          m = mn;
+        } else if (__any_sync(0xFFFFFFFFu, raise)) {
+          const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * p.scale_log2);
+          m = mn;
+          l *= f;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(to + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_32x32b_x32(to + c * 32, o);
+          }
+          tmem_st_wait();
+        }
+        const float shift = m == -INFINITY ? 0.f : -m * p.scale_log2;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float x = exp2_approx(fmaf(__uint_as_float(s[2 * h + c][i]), p.scale_log2, shift));
+              const float y = exp2_approx(fmaf(__uint_as_float(s[2 * h + c][i + 1]), p.scale_log2, shift));
+              sum[(i >> 1) & 3] += x + y;
+              pk[c * 16 + (i >> 1)] = pack2<F16>(x, y);
+            }
+          tmem_st_32x32b_x32(ts + h * 32, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&pfull[t]);
+      }
+      if (ok && end[t] > j0) {
+        ok = mbar_wait(&ofull[t], 0, abort_flag);
+        tc_fence_after();
+      }
+      if (ok && (p.splits == 1 || j0 < j1)) {
+        const int head = hk * p.group + (r - tok * p.group);
+        const int64_t row = row0 + first + tok;
+        const bool any = end[t] > j0;
+        if (p.splits == 1) {
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            if (any) {
+              tmem_ld_32x32b_x32(to + c * 32, o);
+              tmem_ld_wait();
+            }
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (any && l != 0.f) {
+                  x.x = pack2<F16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+                  x.y = pack2<F16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                  x.z = pack2<F16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                  x.w = pack2<F16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                }
+                *reinterpret_cast<uint4*>(dst + c * 32 + i) = x;
+              }
+            }
+          }
+        } else {
+          const int64_t at = (row * (kv.kv_heads * p.group) + head) * p.splits + split;
+          if (live) p.part_ml[at] = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
+          if (any) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(to + c * 32, o);
+              tmem_ld_wait();
+              if (live) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                  *reinterpret_cast<uint4*>(p.part_o + at * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+    } else if (warp == 8) {
+      // ---------------------------------------------------------- page loads
+      const int32_t* table = kv.page_table + seq * kv.table_stride;
+      const int page = 1 << kv.page_shift;
+      const int piece = lane / Cfg::kHalves, half = lane % Cfg::kHalves;  // page of the step, column block
+      const int per_step = kPreKeys >> kv.page_shift;
+      const int held = (len + page - 1) >> kv.page_shift;  // pages of the sequence
+      auto entry = [&](int j) {
+        const int at = j * per_step + piece;
+        return piece < per_step && at < held ? table[at] : 0;
+      };
+      int next = j0 < j1 ? entry(j0) : 0;
+      int issued = 0;
+      bool ok = true;
+      for (int j = j0; j < j1 && ok; ++j) {
+        const int id = next;
+        if (j + 1 < j1) next = entry(j + 1);
+        const int pieces = min(per_step, held - j * per_step);
+        const bool mine = piece < pieces;
+        if (mine && half == 0 && (id < 0 || id >= kv.num_pages) && kv.status != nullptr)
+          atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int it = 2 * (j - j0) + x;
+          const int slot = it % Cfg::kSlots;
+          if (it >= Cfg::kSlots && !mbar_wait(&empty[slot], (it / Cfg::kSlots - 1) & 1, abort_flag)) ok = false;
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(pieces * page * D * 2));
+          __syncwarp();
+          if (mine) {
+            // A bad id lies outside the map's page dimension and loads zeros.
+            const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes + half * Cfg::kBlockBytes) +
+                                 piece * page * 128;
+            tma_load_4d(dst, x == 0 ? &tm_k : &tm_v, &full[slot], 0, hk << kv.page_shift, half, id);
+          }
+          ++issued;
+        }
+      }
+      // Copies in flight have landed before shared memory goes (all have, but
+      // after an abort).
+      for (int it = max(0, issued - Cfg::kSlots); it < issued; ++it)
+        mbar_wait_bounded(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1);
+    } else {
+      // ---------------------------------------------------------- MMA issuer
+      constexpr uint32_t fmt = F16 ? 0u : 1u;
+      constexpr uint32_t idesc_s = umma_idesc(kPreRows, kPreKeys, fmt);
+      constexpr uint32_t idesc_o = umma_idesc(kPreRows, D, fmt) | kIdescBNMajor;
+      const uint32_t ring = smem_u32(smem + Cfg::kOffRing);
+      bool ok = true;
+      auto ready = [&](int it) {
+        ok = ok && mbar_wait(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1, abort_flag);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        tc_fence_after();
+        return ok;
+      };
+      auto scores = [&](int t, int it) {
+        if (lane == 0) {
+          const uint32_t a = smem_u32(smem + t * Cfg::kTileBytes), b = ring + (it % Cfg::kSlots) * Cfg::kTileBytes;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = (k / 4) * Cfg::kBlockBytes + (k % 4) * 32;
+            umma_bf16_ss(tmem + t * 128, sw128_kmajor_desc(a + off), sw128_kmajor_desc(b + off), idesc_s, k > 0);
+          }
+          umma_commit(&sfull[t]);
+        }
+        __syncwarp();
+      };
+      auto release = [&](int it) {  // the slot is loaded again: once the MMAs so far have read it
+        if (lane == 0 && it + Cfg::kSlots < total) umma_commit(&empty[it % Cfg::kSlots]);
+        __syncwarp();
+      };
+      for (int t = 0; t < 2; ++t)
+        if (end[t] > j0) ok = ok && mbar_wait(&qfull[t], 0, abort_flag);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (ok && j0 < j1 && ready(0)) {
+        for (int t = 0; t < 2; ++t)
+          if (end[t] > j0) scores(t, 0);
+        release(0);
+      }
+      for (int j = j0; j < j1 && ok; ++j) {
+        const int iv = 2 * (j - j0) + 1, ik = iv + 1;
+        if (!ready(iv)) break;
+        const uint32_t vb = ring + (iv % Cfg::kSlots) * Cfg::kTileBytes;
+        // Weights of slots behind the length are 0, but the slots may hold
+        // anything (a page's last owner, NaN): only whole groups of 16 keys
+        // that the sequence reaches are multiplied, the rest of the last
+        // group is cleared.
+        const int valid = min(kPreKeys, len - j * kPreKeys);
+        const int groups = (valid + 15) / 16;
+        if (valid & 15) {
+          uint8_t* v = smem + Cfg::kOffRing + (iv % Cfg::kSlots) * Cfg::kTileBytes;
+          for (int i = valid * (D / 8) + lane; i < groups * 16 * (D / 8); i += 32) {
+            const int row = i / (D / 8), c = i % (D / 8);  // every piece of the row: its order does not matter
+            *reinterpret_cast<uint4*>(v + (c >> 3) * Cfg::kBlockBytes + row * 128 + ((c & 7) << 4)) =
+                make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        bool loaded = false;
+        for (int t = 0; t < 2; ++t) {
+          if (j < end[t]) {
+            ok = ok && mbar_wait(&pfull[t], (j - j0) & 1, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+              for (int k = 0; k < groups; ++k)
+                umma_f16_ts(tmem + Cfg::kColO + t * D, tmem + t * 128 + k * 8,
+                            sw128_nmajor_desc(vb + k * 2048, Cfg::kBlockBytes), idesc_o, (j > j0) | (k > 0));
+              if (j + 1 == end[t]) umma_commit(&ofull[t]);
+            }
+            __syncwarp();
+          }
+          if (j + 1 < end[t]) {
+            if (!loaded && !ready(ik)) break;
+            loaded = true;
+            scores(t, ik);
+          }
+        }
+        if (!ok) break;
+        release(iv);
+        if (loaded) release(ik);
+      }
+      if (lane == 0) {  // nothing still writes TMEM when it is freed
+        umma_commit(drain);
+        mbar_wait_bounded(drain, 0);
+      }
+      __syncwarp();
+    }
+    if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, Cfg::kTmemCols);
+}
+
+// Joins the pieces of each (packed row, head): grid (heads, tokens).
+struct PrefillJoinParams {
+  PagedView kv;
+  const int32_t* cu;
+  void* out;
+  int64_t ot, oh;
+  int32_t tokens, heads, splits, tile_tokens;
+  const float* part_o;
+  const float2* part_ml;
+};
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PrefillJoinParams p) {
+  constexpr int kPer = D / 32;
+  __shared__ float so[4][D];
+  __shared__ float2 sml[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch();
+  const int row = blockIdx.x / p.heads, h = blockIdx.x - row * p.heads;
+  const int b = owner_of(p.cu, p.kv.batch, row, lane);
+  if (b >= p.kv.batch) return;  // behind the last sequence
+  int row0, row_end;
+  packed_range(p.cu, b, p.tokens, &row0, &row_end);
+  if (row < row0 || row >= row_end) return;
+  const int n = row_end - row0;
+  bool bad;
+  const int len = paged_clamp_len(p.kv.seq_lens[b], p.kv.max_pages, p.kv.page_shift, &bad);
+  // Pieces of the row's block, as its CTAs cut them.
+  const int per = 2 * p.tile_tokens;
+  const int last = min(((row - row0) / per + 1) * per, n) - 1;
+  const int count = split_count((visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys, p.splits);
+  const int64_t at = (static_cast<int64_t>(row) * p.heads + h) * p.splits;
+  float m = -INFINITY, l = 0.f, o[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+  for (int s = warp; s < count; s += 4) {
+    const float2 ml = p.part_ml[at + s];
+    if (ml.y == 0.f) continue;  // the row saw nothing there: its sums were not written
+    const float* src = p.part_o + (at + s) * D + lane * kPer;
+    const float mn = fmaxf(m, ml.x);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    const float f0 = exp2_approx(m - ms), f1 = exp2_approx(ml.x - ms);
+    m = mn;
+    l = l * f0 + ml.y * f1;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = o[i] * f0 + src[i] * f1;
+  }
+  if (lane == 0) sml[warp] = make_float2(m, l);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = o[i];
+  __syncthreads();
+  if (threadIdx.x < D / 2) {
+    const int d = threadIdx.x * 2;
+    const float top = fmaxf(fmaxf(sml[0].x, sml[1].x), fmaxf(sml[2].x, sml[3].x));
+    const float ms = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2_approx(sml[w].x - ms);
+      sum += sml[w].y * f;
+      x += so[w][d] * f;
+      y += so[w][d + 1] * f;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+    uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + h * p.oh + d;
+    *reinterpret_cast<uint32_t*>(dst) = pack2<F16>(x * inv, y * inv);
+  }
+}
+
+}  // namespace abft

@@ -121,7 +121,7 @@ class PagedKVCache:
         kv.batch, kv.max_pages, kv.dtype = batch, max_pages, _DTYPES[k_pages.dtype]
         self._kv = kv
         self._index = dev.index
-        self._splits: dict = {}
+        self._sizes: dict = {}  # workspace bytes by call sizes
 
     # ---- argument checks ------------------------------------------------------
     def _rows(self, name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int]) -> torch.Tensor:
@@ -222,17 +222,35 @@ class PagedKVCache:
         to head_dim^-0.5. A sequence of length 0 gives zeros. ``num_splits``:
         pieces a sequence is cut into (0: chosen from the batch, the heads and
         the table's width)."""
-        args, out, q = self._attn(q, scale, out, self.batch, num_splits)  # q: alive until the launch is queued
+        return self._attention("abft_paged_decode", q, scale, out, self.batch, num_splits, None)
+
+    def prefill(self, q: torch.Tensor, cu_seqlens: torch.Tensor, *, scale: Optional[float] = None,
+                out: Optional[torch.Tensor] = None, num_splits: int = 0) -> torch.Tensor:
+        """Causal attention of the newest tokens of each sequence over its
+        cache: rows cu[b] to cu[b + 1] of ``q`` [tokens, heads, head_dim] are
+        the last tokens of sequence b (``append`` has stored their keys), and
+        row i of n sees the slots up to seq_lens[b] - n + i. Chunks of any
+        length, 0 and 1 included; rows behind cu[batch] are left as they were
+        in ``out`` (undefined without one). ``num_splits`` as for decode."""
+        self._boundaries(cu_seqlens)
+        return self._attention("abft_paged_prefill", q, scale, out, None, num_splits, cu_seqlens)
+
+    def _attention(self, name, q, scale, out, tokens, num_splits, cu):
+        args, out, q = self._attn(q, scale, out, tokens, num_splits)  # q: alive until the launch is queued
+        if cu is not None:
+            args.cu_seqlens = cu.data_ptr()
         L = N.lib()
-        key = ("decode", args.heads, num_splits)
-        need = self._splits.get(key)
+        key = (name, args.tokens, args.heads, num_splits)
+        need = self._sizes.get(key)
         if need is None:  # depends on sizes alone
+            if len(self._sizes) >= 256:
+                self._sizes.clear()
             with torch.cuda.device(self._index):
-                need = self._splits[key] = int(L.abft_paged_decode_workspace_bytes(ctypes.byref(args)))
+                need = self._sizes[key] = int(getattr(L, name + "_workspace_bytes")(ctypes.byref(args)))
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        self._call("abft_paged_decode", L.abft_paged_decode, args)
+        self._call(name, getattr(L, name), args)
         return out
 
     def _attn(self, q, scale, out, tokens, num_splits):
@@ -259,5 +277,6 @@ class PagedKVCache:
         self.status.zero_()
         said = [text for bit, text in ((N.PAGED_BAD_PAGE, "a page_table entry outside the pool"),
                                        (N.PAGED_BAD_LEN, "a length below 0, beyond the table or below the new tokens"),
-                                       (N.PAGED_BAD_ANGLE, "a position beyond the rotation table")) if bits & bit]
+                                       (N.PAGED_BAD_ANGLE, "a position beyond the rotation table"),
+                                       (N.PAGED_TIMEOUT, "a bounded device wait gave up")) if bits & bit]
         raise ValueError("paged cache: " + "; ".join(said))
