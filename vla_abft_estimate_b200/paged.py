@@ -23,7 +23,7 @@ there, per call.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -51,6 +51,28 @@ def _i32(name: str, t: torch.Tensor, dim: int, device: torch.device) -> None:
         raise ValueError(f"{name} must be a {dim}-D int32 tensor on {device}, got {got}")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have unit stride in its last dimension")
+
+
+def _signature(t: Optional[torch.Tensor]):
+    """All a call checks of a tensor, its address apart."""
+    if t is None:
+        return None
+    try:
+        return t.shape, t.stride(), t.dtype, t.device, t.requires_grad and torch.is_grad_enabled()
+    except AttributeError:
+        raise TypeError(f"expected a torch.Tensor, got {type(t).__name__}") from None
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a dense copy of it when it does not start on 16 bytes."""
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() & 15 else t
+
+
+def _address(name: str, t: torch.Tensor) -> int:
+    p = t.data_ptr()
+    if p & 15:
+        raise ValueError(f"{name} must be 16-byte aligned")
+    return p
 
 
 class PagedKVCache:
@@ -121,37 +143,54 @@ class PagedKVCache:
         kv.batch, kv.max_pages, kv.dtype = batch, max_pages, _DTYPES[k_pages.dtype]
         self._kv = kv
         self._index = dev.index
-        self._sizes: dict = {}  # workspace bytes by call sizes
+        self._plans: dict = {}
 
     # ---- argument checks ------------------------------------------------------
-    def _rows(self, name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int]) -> torch.Tensor:
-        """``t`` as [tokens, heads, head_dim] rows the kernels can read in
-        place (16-byte pieces), copied when its strides do not allow it."""
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+    # A call's sizes, strides, types and devices are checked once and kept as
+    # a filled argument struct under that signature; a later call with the
+    # same signature only sets its addresses.
+    def _plan(self, key: tuple, make):
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = make()
+            if len(self._plans) >= 256:  # callers whose packed lengths never repeat
+                self._plans.clear()
+            self._plans[key] = plan
+        return plan
+
+    def _rows(self, name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int]) -> Tuple[int, int]:
+        """Checks [tokens, heads, head_dim] rows; returns the token and head
+        strides the kernels read or write them with: their own, or dense ones
+        when the call has to work on a copy (``_in_place`` is false)."""
         shape = t.shape
         if (t.dtype != self.dtype or t.device != self.device or len(shape) != 3 or shape[2] != self.head_dim
                 or (tokens is not None and shape[0] != tokens) or (heads is not None and shape[1] != heads)):
             raise ValueError(f"{name} must be a {self.dtype} tensor [{'tokens' if tokens is None else tokens}, "
                              f"{'heads' if heads is None else heads}, {self.head_dim}] on {self.device}, got {t.dtype} "
                              f"{tuple(shape)} on {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient, which the paged cache operators do not give: call them under "
+                             "torch.no_grad()")
+        return t.stride()[:2] if self._in_place(t) else (shape[1] * shape[2], shape[2])
+
+    @staticmethod
+    def _in_place(t: torch.Tensor) -> bool:
+        """The strides let the kernels read rows in 16-byte pieces."""
         s = t.stride()
-        if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
-            return t.contiguous()
-        return t
+        return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0
 
     def _group(self, heads: int) -> None:
         if heads == 0 or heads % self.kv_heads or heads // self.kv_heads > 64:
             raise ValueError(f"q has {heads} heads: a multiple of the cache's {self.kv_heads} kv heads, at most 64 "
                              "for each, is needed")
 
-    def _out(self, name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
-        if out is None:
-            return torch.empty(like.shape, dtype=self.dtype, device=self.device)
-        if self._rows(name, out, like.shape[0], like.shape[1]) is not out:
-            raise ValueError(f"{name} must be 16-byte aligned, with strides a multiple of 8 and unit stride in its last "
-                             "dimension")
-        return out
+    def _result(self, name: str, out: torch.Tensor, like: torch.Tensor) -> Tuple[int, int]:
+        strides = self._rows(name, out, like.shape[0], like.shape[1])
+        if not self._in_place(out):
+            raise ValueError(f"{name} must have strides a multiple of 8 and unit stride in its last dimension")
+        if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+            raise ValueError(f"{name} must not repeat memory")
+        return strides
 
     def _boundaries(self, cu: torch.Tensor) -> None:
         _i32("cu_seqlens", cu, 1, self.device)
@@ -173,47 +212,68 @@ class PagedKVCache:
         """Stores the new tokens' keys and values and returns the rotated q.
 
         ``q`` [tokens, heads, head_dim], ``k`` and ``v`` [tokens, kv_heads,
-        head_dim] (any strides; parts of one fused projection are read in
-        place). ``cu_seqlens`` int32 [batch + 1]: rows cu[b] to cu[b + 1] are
-        the last tokens of sequence b, rows behind cu[batch] belong to none;
-        without it row b is the newest token of sequence b, none where
-        seq_lens[b] is 0. ``rope``: fp32 [positions, head_dim / 2, 2]
-        (``rope_table``) rotates q and k by position, in fp32, rounded once;
-        None stores k as it is. ``q_out`` (may be ``q``) receives q; rows of
-        no sequence are left as they were. q None stores k and v only.
+        head_dim] (parts of one fused projection are read in place; rows that
+        are not 16-byte aligned are copied first). ``cu_seqlens`` int32
+        [batch + 1]: rows cu[b] to cu[b + 1] are the last tokens of sequence
+        b, rows behind cu[batch] belong to none; without it row b is the
+        newest token of sequence b, none where seq_lens[b] is 0. ``rope``:
+        fp32 [positions, head_dim / 2, 2] (``rope_table``) rotates q and k by
+        position, in fp32, rounded once; None stores k as it is. ``q_out``
+        (may be ``q``, but not overlap it otherwise) receives q; rows of no
+        sequence are left as they were (undefined without ``q_out``). q None
+        stores k and v only.
         """
-        k = self._rows("k", k, None, self.kv_heads)
-        tokens = k.shape[0]
-        v = self._rows("v", v, tokens, self.kv_heads)
+        key = (_signature(q), _signature(k), _signature(v), _signature(rope), _signature(cu_seqlens), _signature(q_out))
+        template, copies = self._plan(key, lambda: self._plan_append(q, k, v, rope, cu_seqlens, q_out))
+        args = N.KvAppendArgs.from_buffer_copy(template)
+        if copies:
+            q, k, v = (t if t is None or self._in_place(t) else t.contiguous() for t in (q, k, v))
+        kp, vp = k.data_ptr(), v.data_ptr()
+        if (kp | vp) & 15:
+            k, v = _aligned(k), _aligned(v)
+            kp, vp = k.data_ptr(), v.data_ptr()
+            return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
+        args.k, args.v = kp, vp
+        if q is not None:
+            qp = q.data_ptr()
+            if qp & 15:
+                return self.append(_aligned(q), k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
+            if q_out is None:
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            args.q, args.q_out = qp, _address("q_out", q_out)
+        if rope is not None:
+            args.rope = _address("rope", rope)
+        if cu_seqlens is not None:
+            args.cu_seqlens = cu_seqlens.data_ptr()
+        self._call("abft_kv_append", N.lib().abft_kv_append, args)
+        return q_out
+
+    def _plan_append(self, q, k, v, rope, cu_seqlens, q_out):
         args = N.KvAppendArgs()
         args.kv = self._kv
+        args.k_token_stride, args.k_head_stride = self._rows("k", k, None, self.kv_heads)
+        tokens = k.shape[0]
+        args.tokens = tokens
+        args.v_token_stride, args.v_head_stride = self._rows("v", v, tokens, self.kv_heads)
         if cu_seqlens is not None:
             self._boundaries(cu_seqlens)
-            args.cu_seqlens = cu_seqlens.data_ptr()
         elif tokens != self.batch:
             raise ValueError(f"without cu_seqlens k must have one row for each of the {self.batch} sequences, got {tokens}")
         if rope is not None:
             if (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1] * 2 != self.head_dim or rope.shape[2] != 2
-                    or rope.device != self.device or not rope.is_contiguous() or rope.data_ptr() % 16):
+                    or rope.device != self.device or not rope.is_contiguous() or rope.shape[0] == 0):
                 raise ValueError(f"rope must be a contiguous float32 [positions, {self.head_dim // 2}, 2] tensor on "
                                  f"{self.device}, got {rope.dtype} {tuple(rope.shape)}")
-            args.rope, args.max_positions = rope.data_ptr(), rope.shape[0]
-            if rope.shape[0] == 0:
-                raise ValueError("rope has no positions")
+            args.max_positions = rope.shape[0]
         if q is not None:
             self._group(q.shape[1] if q.dim() == 3 else 0)
-            q = self._rows("q", q, tokens, None)
-            q_out = self._out("q_out", q_out, q)
-            args.q, args.q_out, args.heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-            args.q_token_stride, args.q_head_stride, _ = q.stride()
-            args.o_token_stride, args.o_head_stride, _ = q_out.stride()
+            args.q_token_stride, args.q_head_stride = self._rows("q", q, tokens, None)
+            args.heads = q.shape[1]
+            args.o_token_stride, args.o_head_stride = (
+                (q.shape[1] * self.head_dim, self.head_dim) if q_out is None else self._result("q_out", q_out, q))
         elif q_out is not None:
             raise ValueError("q_out without q")
-        args.k, args.v, args.tokens = k.data_ptr(), v.data_ptr(), tokens
-        args.k_token_stride, args.k_head_stride, _ = k.stride()
-        args.v_token_stride, args.v_head_stride, _ = v.stride()
-        self._call("abft_kv_append", N.lib().abft_kv_append, args)
-        return q_out
+        return bytes(args), not all(t is None or self._in_place(t) for t in (q, k, v))
 
     def decode(self, q: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                num_splits: int = 0) -> torch.Tensor:
@@ -222,7 +282,7 @@ class PagedKVCache:
         to head_dim^-0.5. A sequence of length 0 gives zeros. ``num_splits``:
         pieces a sequence is cut into (0: chosen from the batch, the heads and
         the table's width)."""
-        return self._attention("abft_paged_decode", q, scale, out, self.batch, num_splits, None)
+        return self._attention("abft_paged_decode", q, None, scale, out, num_splits)
 
     def prefill(self, q: torch.Tensor, cu_seqlens: torch.Tensor, *, scale: Optional[float] = None,
                 out: Optional[torch.Tensor] = None, num_splits: int = 0) -> torch.Tensor:
@@ -232,40 +292,54 @@ class PagedKVCache:
         row i of n sees the slots up to seq_lens[b] - n + i. Chunks of any
         length, 0 and 1 included; rows behind cu[batch] are left as they were
         in ``out`` (undefined without one). ``num_splits`` as for decode."""
-        self._boundaries(cu_seqlens)
-        return self._attention("abft_paged_prefill", q, scale, out, None, num_splits, cu_seqlens)
+        return self._attention("abft_paged_prefill", q, cu_seqlens, scale, out, num_splits)
 
-    def _attention(self, name, q, scale, out, tokens, num_splits, cu):
-        args, out, q = self._attn(q, scale, out, tokens, num_splits)  # q: alive until the launch is queued
+    def _attention(self, name, q, cu, scale, out, num_splits):
+        key = (name, _signature(q), _signature(cu), scale, _signature(out), num_splits)
+        template, copies, space = self._plan(key, lambda: self._plan_attention(name, q, cu, scale, out, num_splits))
+        args = N.PagedAttnArgs.from_buffer_copy(template)
+        if copies:
+            q = q.contiguous()
+        qp = q.data_ptr()
+        if qp & 15:
+            q = _aligned(q)
+            return self._attention(name, q, cu, scale, out, num_splits)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        args.q, args.out = qp, _address("out", out)
         if cu is not None:
             args.cu_seqlens = cu.data_ptr()
-        L = N.lib()
-        key = (name, args.tokens, args.heads, num_splits)
-        need = self._sizes.get(key)
-        if need is None:  # depends on sizes alone
-            if len(self._sizes) >= 256:
-                self._sizes.clear()
-            with torch.cuda.device(self._index):
-                need = self._sizes[key] = int(getattr(L, name + "_workspace_bytes")(ctypes.byref(args)))
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        self._call(name, getattr(L, name), args)
+        if space is not None:
+            ws = torch.empty_like(space)  # of this call alone: calls of other threads or graphs have their own
+            args.workspace = ws.data_ptr()
+        self._call(name, getattr(N.lib(), name), args)
         return out
 
-    def _attn(self, q, scale, out, tokens, num_splits):
-        self._group(q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0)
-        q = self._rows("q", q, tokens, None)
-        out = self._out("out", out, q)
+    def _plan_attention(self, name, q, cu, scale, out, num_splits):
+        decode = name == "abft_paged_decode"
+        if not decode:
+            self._boundaries(cu)
+        self._group(q.shape[1] if q.dim() == 3 else 0)
         args = N.PagedAttnArgs()
         args.kv = self._kv
-        args.q, args.out = q.data_ptr(), out.data_ptr()
+        args.q_token_stride, args.q_head_stride = self._rows("q", q, self.batch if decode else None, None)
+        args.o_token_stride, args.o_head_stride = (
+            (q.shape[1] * self.head_dim, self.head_dim) if out is None else self._result("out", out, q))
         args.tokens, args.heads = q.shape[0], q.shape[1]
-        args.q_token_stride, args.q_head_stride, _ = q.stride()
-        args.o_token_stride, args.o_head_stride, _ = out.stride()
         args.scale = self.head_dim ** -0.5 if scale is None else float(scale)
         args.num_splits = int(num_splits)
-        return args, out, q
+        space = None
+        if q.shape[0] and self.batch:
+            # placeholder addresses: sizes decide how much scratch the call needs
+            args.q = args.out = args.cu_seqlens = 1 << 20
+            with torch.cuda.device(self._index):
+                need = int(getattr(N.lib(), name + "_workspace_bytes")(ctypes.byref(args)))
+            args.q = args.out = args.cu_seqlens = None
+            if need:
+                args.workspace_bytes = need
+                # one byte seen as `need` of them: empty_like gives that many
+                space = torch.empty(1, dtype=torch.uint8, device=self.device).expand(need)
+        return bytes(args), not self._in_place(q), space
 
     def check_status(self) -> None:
         """Raises ValueError when a call since the last check met a bad page
