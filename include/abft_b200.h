@@ -484,10 +484,11 @@ typedef struct abft_paged_attn_args {
   int64_t tokens;             /* rows of q (decode: kv.batch)                          */
   int32_t heads;              /* a multiple of kv_heads, at most 64 per kv head        */
   float scale;
-  void* workspace;            /* device scratch, abft_paged_*_workspace_bytes()        */
-  size_t workspace_bytes;
-  int32_t num_splits;         /* 0 = choose; else pieces each sequence is cut into     */
-  int32_t num_sms;            /* 0 = all SMs of the current device                     */
+  void* workspace;            /* device scratch of this call, any content:             */
+  size_t workspace_bytes;     /* abft_paged_*_workspace_bytes()                        */
+  int32_t num_splits;         /* prefill: pieces the keys of a block of query rows are */
+                              /* cut into, 0 = choose; decode: not used                */
+  int32_t num_sms;            /* SMs to plan for, 0 = all of the current device        */
 } abft_paged_attn_args;
 
 int abft_kv_append(const abft_kv_append_args* args, void* stream);

@@ -153,12 +153,12 @@ def test_append_skips_bad_entries(cuda_device):
 
 
 # ---- decode -------------------------------------------------------------------
-def run_decode(dev, lens, heads, kv_heads, d, page, dtype, *, seed=0, splits=0, spread=1.5, joint=False, extra=0,
+def run_decode(dev, lens, heads, kv_heads, d, page, dtype, *, seed=0, sms=0, spread=1.5, joint=False, extra=0,
                scale=None):
     pool = Pool(lens, kv_heads, page, d, dtype, seed=seed, joint=joint, extra_columns=extra)
     cache = pool.device_cache(dev, PagedKVCache)
     q = (torch.randn(len(lens), heads, d, generator=torch.Generator().manual_seed(seed + 9)) * spread).to(dtype)
-    got = cache.decode(q.to(dev), num_splits=splits, scale=scale)
+    got = cache.decode(q.to(dev), num_sms=sms, scale=scale)
     cache.check_status()
     want, tol = attention(pool, q, list(enumerate(lens)), scale)
     close(got, want, tol)
@@ -172,11 +172,20 @@ def test_decode_head_layouts(cuda_device, heads, kv_heads, d, dtype):
     run_decode(cuda_device, [77, 300], heads, kv_heads, d, 16, dtype)
 
 
-@pytest.mark.parametrize("splits", [0, 1, 2, 3, 7, 1000])
+@pytest.mark.parametrize("sms", [0, 1, 2, 3, 7, 1000])
 @pytest.mark.parametrize("page", [16, 128])
 @pytest.mark.parametrize("lens", [[1], [2], [15, 16, 17], [31, 32, 33], [0, 1, 127, 128, 129, 0], [1000, 3, 513]])
-def test_decode_lengths_and_splits(cuda_device, lens, page, splits):
-    run_decode(cuda_device, lens, 7, 1, 128, page, BF16, splits=splits)
+def test_decode_lengths_and_shares(cuda_device, lens, page, sms):
+    """Shares of any size: segments within a warp, across warps and across CTAs."""
+    run_decode(cuda_device, lens, 7, 1, 128, page, BF16, sms=sms)
+
+
+@pytest.mark.parametrize("sms", [1, 5, 0])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (36, 3), (40, 2)])
+def test_decode_many_sequences(cuda_device, heads, kv_heads, sms):
+    """More sequences than a warp scans at once, empty ones among them."""
+    run_decode(cuda_device, [(i * 53) % 170 if i % 7 else 0 for i in range(75)], heads, kv_heads, 64, 32, F16, sms=sms)
+    run_decode(cuda_device, [0] * 40 + [333] + [0] * 40, heads, kv_heads, 128, 16, BF16, sms=sms)
 
 
 def test_decode_long_and_peaked(cuda_device):

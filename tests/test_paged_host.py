@@ -41,6 +41,19 @@ int main() {
       need(at == tiles, "cover");
       need(filled == split_count(tiles, splits), "count");
     }
+  // shares cover the tiles in order, differ by one at most, and share_of inverts them
+  for (int total : {0, 1, 3, 4, 591, 592, 5000})
+    for (int shares : {1, 2, 4, 12, 592}) {
+      need(share_start(total, shares, 0) == 0 && share_start(total, shares, shares) == total, "share ends");
+      for (int w = 0; w < shares; ++w) {
+        const int a = share_start(total, shares, w), e = share_start(total, shares, w + 1);
+        need(a <= e && e - a >= total / shares && e - a <= total / shares + 1, "share size");
+        for (int u = a; u < e; ++u) need(share_of(total, shares, u) == w, "share_of");
+      }
+    }
+  const int huge = 0x7FFFFFF0;
+  need(share_of(huge, 592, share_start(huge, 592, 300)) == 300, "large shares");
+  need(share_start(huge, 592, 592) == huge && share_of(huge, 592, huge - 1) == 591, "large share ends");
   // lengths are cut to the table
   bool bad;
   need(paged_clamp_len(0, 3, 4, &bad) == 0 && !bad, "0");
@@ -194,18 +207,28 @@ def test_attention_refusals():
         if not torch.cuda.is_available():
             assert call(fn) == -6
     assert call(L.abft_paged_decode, tokens=1) == -1  # one row per sequence
+    kv = _kv()
+    kv.max_pages = kv.table_stride = 1 << 26
+    kv.batch = 16
+    assert call(L.abft_paged_decode, kv=kv, tokens=16) == -3  # 2^31 tiles
     assert call(L.abft_paged_prefill, cu_seqlens=None) == -1
     assert call(L.abft_paged_prefill, tokens=0) == 0
     assert call(L.abft_paged_prefill, tokens=1 << 30) == -3
 
 
-def test_workspace_grows_with_pieces():
+def test_workspace_sizes():
     a = N.PagedAttnArgs()
     a.kv, a.q, a.out, a.tokens, a.heads, a.scale, a.num_sms = _kv(), 0x50000, 0x60000, 2, 28, 0.1, 148
+    a.cu_seqlens = 0x70000
+    # decode: 2 sequences x 4 kv heads x 2 tiles of 32 slots = 16 tiles for 4 CTAs' warps
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 4 * (2 * 8 * (128 * 4 + 8) + 16)
+    a.num_sms = 3
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 3 * (2 * 8 * (128 * 4 + 8) + 16)
     a.num_splits = 1
-    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 0
-    a.num_splits = 2  # two pieces of 48 slots: 2 tiles
-    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) >= 2 * 28 * 2 * (128 * 4 + 8)
+    assert N.lib().abft_paged_prefill_workspace_bytes(ctypes.byref(a)) == 0
+    a.kv.max_pages = a.kv.table_stride = 64  # 8 steps of 128 slots
+    a.num_splits = 2
+    assert N.lib().abft_paged_prefill_workspace_bytes(ctypes.byref(a)) == 2 * 28 * 2 * (128 * 4 + 8)
 
 
 def test_python_refusals_without_gpu():

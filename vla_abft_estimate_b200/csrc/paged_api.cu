@@ -144,6 +144,14 @@ int launch_append(const AppendParams& p, cudaStream_t s) {
 // (16) for larger groups; beyond 16, several CTAs read the same keys.
 inline int decode_nt(int group) { return group > 8 ? 2 : 1; }
 
+// Tiles of a full cache.
+int64_t decode_tiles(const abft_paged_attn_args* a) {
+  const int64_t tiles = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
+  const int group = a->heads / a->kv.kv_heads;
+  const int chunks = (group + 8 * decode_nt(group) - 1) / (8 * decode_nt(group));
+  return tiles * a->kv.batch * a->kv.kv_heads * chunks;
+}
+
 int attn_check(const abft_paged_attn_args* a, bool decode) {
   if (a == nullptr) return ABFT_ERR_INVALID_ARG;
   int rc = check_kv(a->kv);
@@ -152,6 +160,9 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
   if ((rc = check_heads(a->heads, a->kv.kv_heads)) != ABFT_OK) return rc;
   if (decode && a->tokens != a->kv.batch) return ABFT_ERR_INVALID_ARG;
   if (a->tokens == 0 || a->kv.batch == 0) return ABFT_OK;
+  // The list of tiles (32 slots of a kv head and up to 8 or 16 of its query
+  // heads) is counted in 32 bits.
+  if (decode && decode_tiles(a) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
   // Grids (blocks x kv heads, rows x heads for the join) stay below 2^31.
   if (a->tokens >= (int64_t{1} << 30) / a->heads) return ABFT_ERR_UNSUPPORTED;
   if (a->q == nullptr || a->out == nullptr || (!decode && a->cu_seqlens == nullptr)) return ABFT_ERR_INVALID_ARG;
@@ -161,44 +172,37 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
   return ABFT_OK;
 }
 
-int decode_splits(const abft_paged_attn_args* a, int sms) {
-  const int64_t tiles = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
-  if (a->num_splits > 0) return static_cast<int>(a->num_splits < tiles ? a->num_splits : tiles);
-  const int group = a->heads / a->kv.kv_heads;
-  const int chunks = (group + 8 * decode_nt(group) - 1) / (8 * decode_nt(group));
-  const int64_t ctas = static_cast<int64_t>(a->kv.batch) * a->kv.kv_heads * chunks;
-  int64_t n = (2 * sms + ctas - 1) / ctas;
-  const int64_t most = (tiles + 3) / 4;  // a tile for each warp
-  if (n > most) n = most;
-  return static_cast<int>(n < 1 ? 1 : n);
+// CTAs of a decode launch: one per SM, fewer when the cache cannot hold a tile
+// for each of their warps.
+int decode_grid(const abft_paged_attn_args* a, int sms) {
+  const int64_t ctas = (decode_tiles(a) + kDecWarps - 1) / kDecWarps;
+  return static_cast<int>(ctas < sms ? ctas : sms);
 }
 
-size_t split_bytes(const abft_paged_attn_args* a, int splits) {
-  if (splits <= 1) return 0;
-  const size_t rows = static_cast<size_t>(a->kv.batch) * a->heads * splits;
-  return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2));
+// Scratch: two pieces of 8 or 16 heads and one spill record per CTA.
+size_t decode_bytes(const abft_paged_attn_args* a, int grid) {
+  const size_t rows = static_cast<size_t>(grid) * 2 * 8 * decode_nt(a->heads / a->kv.kv_heads);
+  return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2)) + grid * sizeof(int4);
 }
 
 template <int D, int NT, bool F16>
-int launch_decode(int dev, int slot, const DecodeParams& p, int heads, cudaStream_t s) {
+int launch_decode(int dev, int slot, const DecodeParams& p, int grid, cudaStream_t s) {
   using Cfg = DecodeCfg<D, NT>;
   int rc = raise_smem(dev, slot, paged_decode_kernel<D, NT, F16>, Cfg::kSmemBytes);
   if (rc != ABFT_OK) return rc;
-  const dim3 grid(p.splits, p.kv.kv_heads * p.head_chunks, p.kv.batch);
-  rc = launch(paged_decode_kernel<D, NT, F16>, grid, dim3(128), Cfg::kSmemBytes, s, p);
-  if (rc != ABFT_OK || p.splits == 1) return rc;
+  rc = launch(paged_decode_kernel<D, NT, F16>, dim3(grid), dim3(kDecThreads), Cfg::kSmemBytes, s, p);
+  if (rc != ABFT_OK) return rc;
   JoinParams j;
-  j.seq_lens = p.kv.seq_lens;
   j.out = p.out;
   j.ot = p.ot;
   j.oh = p.oh;
-  j.heads = heads;
-  j.splits = p.splits;
-  j.max_pages = p.kv.max_pages;
-  j.page_shift = p.kv.page_shift;
+  j.group = p.group;
+  j.head_chunks = p.head_chunks;
   j.part_o = p.part_o;
   j.part_ml = p.part_ml;
-  return launch(paged_join_kernel<D, F16>, dim3(heads, p.kv.batch), dim3(128), 0, s, j);
+  j.spill = p.spill;
+  const int heads = p.group < Cfg::kHeads ? p.group : Cfg::kHeads;
+  return launch(paged_join_kernel<D, NT, F16>, dim3(grid, heads), dim3(32 * kJoinWarps), 0, s, j);
 }
 
 // ---- prefill ------------------------------------------------------------------
@@ -331,7 +335,7 @@ size_t abft_paged_decode_workspace_bytes(const abft_paged_attn_args* a) {
   if (attn_check(a, true) != ABFT_OK || a->kv.batch == 0) return 0;
   int dev = 0, sms = a->num_sms;
   if (sms == 0 && paged_device(&dev, &sms) != ABFT_OK) sms = 148;
-  return split_bytes(a, decode_splits(a, sms));
+  return decode_bytes(a, decode_grid(a, sms));
 }
 
 int abft_paged_decode(const abft_paged_attn_args* a, void* stream) {
@@ -348,27 +352,26 @@ int abft_paged_decode(const abft_paged_attn_args* a, void* stream) {
   p.group = a->heads / a->kv.kv_heads;
   const int nt = decode_nt(p.group);
   p.head_chunks = (p.group + 8 * nt - 1) / (8 * nt);
-  if (static_cast<int64_t>(a->kv.kv_heads) * p.head_chunks > 65535) return ABFT_ERR_UNSUPPORTED;
-  p.splits = decode_splits(a, sms);
   p.scale_log2 = a->scale * 1.44269504088896340736f;
-  const size_t need = split_bytes(a, p.splits);
-  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
-  if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
+  const int grid = decode_grid(a, sms);
+  if (a->workspace == nullptr || a->workspace_bytes < decode_bytes(a, grid)) return ABFT_ERR_WORKSPACE;
+  if (off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
+  const size_t rows = static_cast<size_t>(grid) * 2 * 8 * nt;
   p.part_o = static_cast<float*>(a->workspace);
-  p.part_ml = reinterpret_cast<float2*>(
-      p.part_o + static_cast<size_t>(a->kv.batch) * a->heads * p.splits * a->kv.head_dim);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * a->kv.head_dim);
+  p.spill = reinterpret_cast<int4*>(p.part_ml + rows);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
   const int slot = (a->kv.head_dim == 128 ? 4 : 0) + (nt == 2 ? 2 : 0) + (f16 ? 1 : 0);
   switch (slot) {
-    case 0: return launch_decode<64, 1, false>(dev, slot, p, a->heads, s);
-    case 1: return launch_decode<64, 1, true>(dev, slot, p, a->heads, s);
-    case 2: return launch_decode<64, 2, false>(dev, slot, p, a->heads, s);
-    case 3: return launch_decode<64, 2, true>(dev, slot, p, a->heads, s);
-    case 4: return launch_decode<128, 1, false>(dev, slot, p, a->heads, s);
-    case 5: return launch_decode<128, 1, true>(dev, slot, p, a->heads, s);
-    case 6: return launch_decode<128, 2, false>(dev, slot, p, a->heads, s);
-    default: return launch_decode<128, 2, true>(dev, slot, p, a->heads, s);
+    case 0: return launch_decode<64, 1, false>(dev, slot, p, grid, s);
+    case 1: return launch_decode<64, 1, true>(dev, slot, p, grid, s);
+    case 2: return launch_decode<64, 2, false>(dev, slot, p, grid, s);
+    case 3: return launch_decode<64, 2, true>(dev, slot, p, grid, s);
+    case 4: return launch_decode<128, 1, false>(dev, slot, p, grid, s);
+    case 5: return launch_decode<128, 1, true>(dev, slot, p, grid, s);
+    case 6: return launch_decode<128, 2, false>(dev, slot, p, grid, s);
+    default: return launch_decode<128, 2, true>(dev, slot, p, grid, s);
   }
 }
 

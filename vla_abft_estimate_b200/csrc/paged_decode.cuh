@@ -22,6 +22,16 @@
 // P is rounded to 16 bits for the product, as hi + lo (two products), so
 // that the output's own rounding stays the only one that counts: the second
 // product hides behind the loads.
+//
+// Work is one list of 32-key tiles over all (sequence, kv head) segments, cut
+// into equal shares for the warps of one CTA per SM: lengths of any mix keep
+// every SM reading to the end. A warp's ring of loads runs on across segment
+// boundaries. A segment inside one warp's share is finished by that warp;
+// pieces of a segment that crosses warps are joined in shared memory, those of
+// one that crosses CTAs by a second, small kernel, in a fixed order. (Joined
+// instead by the last CTA to arrive, an atomic counter's choice, 37 pieces of
+// 8 heads took one SM 12 us; spread over one block per head, launch included,
+// 3 us.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -89,100 +99,168 @@ struct DecodeParams {
   void* out;
   int64_t qt, qh, ot, oh;  // token and head strides, elements
   int32_t group;           // query heads per kv head
-  int32_t head_chunks;     // CTAs that share a kv head's query heads
-  int32_t splits;
+  int32_t head_chunks;     // segments that share a kv head's query heads
   float scale_log2;        // scale * log2(e)
-  float* part_o;           // [batch * heads][splits][head_dim]
-  float2* part_ml;         // [batch * heads][splits] (m, l)
+  float* part_o;           // [grid][2][heads of a segment][head_dim]: pieces of segments that cross CTAs
+  float2* part_ml;         // [grid][2][heads of a segment] (m, l)
+  int4* spill;             // [grid] the segment that starts in this CTA and ends in a later one: (sequence, kv head
+                           // and chunk, pieces, -), pieces 0 when there is none
 };
 
 constexpr int kDecTile = 32;  // keys of one warp step
+constexpr int kDecWarps = 4;
+constexpr int kDecThreads = 32 * kDecWarps;
 
 template <int D, int NT>
 struct DecodeCfg {
-  static constexpr int kWarps = 4;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = D == 128 ? 3 : 6;
   static constexpr int kRowBytes = D * 2;
   static constexpr int kHalfBytes = kDecTile * kRowBytes;  // keys of a stage; as much again for values
   static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kJoinPitch = D + 4;  // floats of one head's row when the warps join
-  static constexpr int kRingBytes = kWarps * kWarpBytes;
-  static constexpr int kJoinBytes = kWarps * kHeads * (kJoinPitch + 2) * 4;
-  static constexpr int kSmemBytes = (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes);
+  // A piece of a segment: kHeads rows of unnormalised sums (padded against
+  // bank conflicts) and (m, l) of each.
+  static constexpr int kPitch = D + 4;
+  static constexpr int kPieceBytes = kHeads * (kPitch + 2) * 4;
+  static_assert(kPieceBytes <= kWarpBytes, "a warp's last piece takes the place of its ring");
+  static constexpr int kOffFirst = kDecWarps * kWarpBytes;  // the warps' first pieces
+  static constexpr int kSmemBytes = kOffFirst + kDecWarps * kPieceBytes;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
-// Grid: (splits, kv_heads * head_chunks, batch). A warp owns every fourth
-// 32-key tile of its CTA's piece, with a private ring of cp.async stages:
-// no block-wide barrier before the warps join.
+// A position in the list of tiles.
+struct TileIter {
+  int left;        // tiles of the share still to come, this one included
+  int b, y;        // sequence; kv head and chunk
+  int tile, tiles; // tile within the segment, and the segment's tiles
+  int len;
+};
+
+__device__ __forceinline__ int tiles_of(const PagedView& kv, int b, int* len, bool* bad) {
+  *len = paged_clamp_len(kv.seq_lens[b], kv.max_pages, kv.page_shift, bad);
+  return (*len + kDecTile - 1) / kDecTile;
+}
+
+// The next tile; only called while left > 1.
+__device__ __forceinline__ void advance(TileIter& it, const PagedView& kv, int rows) {
+  --it.left;
+  if (++it.tile < it.tiles) return;
+  if (it.y + 1 < rows) {
+    it.tile = 0;
+    ++it.y;
+    return;
+  }
+  if (it.b + 1 >= kv.batch) return;
+  it.tile = it.y = 0;
+  bool bad;
+  do {
+    ++it.b;
+    it.tiles = tiles_of(kv, it.b, &it.len, &bad);
+  } while (it.tiles == 0 && it.b + 1 < kv.batch);
+}
+
 template <int D, int NT, bool F16>
-__global__ void __launch_bounds__(128) paged_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const DecodeParams p) {
   using Cfg = DecodeCfg<D, NT>;
   extern __shared__ __align__(128) unsigned char smem[];
+  // Pieces of segments that cross the warp's share: the first began in an
+  // earlier share (0: there is none, 1: the segment ends in this share, 2: it
+  // goes on), the last begins here and goes on (0, 2).
+  __shared__ int s_first[kDecWarps], s_last[kDecWarps];
+  __shared__ int s_seg[kDecWarps][2][2];   // (sequence, kv head and chunk) of first and last
+  __shared__ int s_end[kDecWarps];         // the last's segment: its final tile in the list
   constexpr int kShift = D == 128 ? 7 : 6;
   constexpr int kCpr = D / 8;  // 16-byte pieces of a row
   constexpr int kMt = D / 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, tq = lane & 3;
   const PagedView& kv = p.kv;
-  const int b = blockIdx.z, split = blockIdx.x;
-  const int hk = blockIdx.y / p.head_chunks, hc = blockIdx.y - hk * p.head_chunks;
-  const int heads = kv.kv_heads * p.group;
-  const int head0 = hk * p.group + hc * Cfg::kHeads;
-  const int nheads = min(Cfg::kHeads, p.group - hc * Cfg::kHeads);
+  const int rows = kv.kv_heads * p.head_chunks;  // segments of a sequence
 
   griddep_wait();
   griddep_launch();
-  bool bad_len;
-  const int len = paged_clamp_len(kv.seq_lens[b], kv.max_pages, kv.page_shift, &bad_len);
-  if (bad_len && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
-  const int tiles = (len + kDecTile - 1) / kDecTile;
-  int t0, t1;
-  split_tiles(tiles, p.splits, split, &t0, &t1);
-  if (t0 >= t1 && (p.splits > 1 || tiles > 0)) return;
 
-  // Q^T fragments: column g = head, rows = head dimension.
-  uint32_t qf[NT][D / 16][2];
+  // ---- this warp's share ------------------------------------------------------
+  int len0 = 0, tiles0 = 0;  // this lane's sequence of the first 32
+  int sum = 0;
+  for (int b = lane; b < kv.batch; b += 32) {
+    int len;
+    bool bad;
+    const int tiles = tiles_of(kv, b, &len, &bad);
+    if (b == lane) len0 = len, tiles0 = tiles;
+    sum += tiles;
+    if (bad && blockIdx.x == 0 && warp == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
+  }
+  sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+  const int total = sum * rows;  // the host keeps it below 2^31
+  const int shares = gridDim.x * kDecWarps;
+  const int share = blockIdx.x * kDecWarps + warp;
+  const int u0 = share_start(total, shares, share), u1 = share_start(total, shares, share + 1);
+
+  TileIter head;
+  head.left = u1 - u0;
+  head.b = head.y = head.tile = head.tiles = head.len = 0;
+  if (head.left > 0) {  // the sequence that holds tile u0
+    int before = 0;
+    for (int i = 0; i < kv.batch; i += 32) {
+      int mine = tiles0, len = len0;
+      bool bad;
+      if (i > 0) mine = i + lane < kv.batch ? tiles_of(kv, i + lane, &len, &bad) : 0;
+      int upto = mine;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int h = nt * 8 + g;
-    const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.qt + (head0 + h) * p.qh;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        qf[nt][ks][i] = h < nheads ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + i * 8 + tq * 2) : 0u;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, (before + upto) * rows > u0);
+      if (past != 0) {
+        const int src = __ffs(past) - 1;
+        head.b = i + src;
+        head.tiles = __shfl_sync(0xFFFFFFFFu, mine, src);
+        head.len = __shfl_sync(0xFFFFFFFFu, len, src);
+        const int in = u0 - (before + __shfl_sync(0xFFFFFFFFu, upto - mine, src)) * rows;
+        head.y = in / head.tiles;
+        head.tile = in - head.y * head.tiles;
+        break;
+      }
+      before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
   }
 
   const uint32_t ring = smem_u32(smem) + warp * Cfg::kWarpBytes;
-  const int32_t* table = kv.page_table + b * kv.table_stride;
   const uint16_t* kbase = static_cast<const uint16_t*>(kv.k_pages);
   const uint16_t* vbase = static_cast<const uint16_t*>(kv.v_pages);
 
-  // Table entries of the two 16-key halves of tile t (-1: nothing to read).
-  auto entries = [&](int t, int (&pg)[2]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int key = t * kDecTile + i * 16;
-      pg[i] = (t < t1 && key < len) ? table[key >> kv.page_shift] : -1;
-    }
+  // Lane i holds the table entry of 16 keys, the i-th from tile `held` on: one
+  // load serves 16 tiles, and the next 16 are asked for ahead of their use.
+  int entry = 0, entry_next = 0, held = 0;
+  auto look_up = [&](const TileIter& it, int tile) {
+    const int key = tile * kDecTile + lane * 16;
+    return key < it.len ? kv.page_table[it.b * kv.table_stride + (key >> kv.page_shift)] : 0;
   };
-  auto issue = [&](int t, int stage, const int (&pg)[2]) {
+  auto entries = [&](const TileIter& it) {  // of a segment that begins
+    held = it.tile;
+    entry = look_up(it, held);
+    entry_next = look_up(it, held + 16);
+  };
+  auto issue = [&](const TileIter& it, int stage) {
     constexpr int kRowsPerOp = 32 / kCpr;  // rows one warp-wide copy covers
     const int sub = lane / kCpr, c = lane % kCpr;
+    const int hk = p.head_chunks == 1 ? it.y : it.y / p.head_chunks;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int key0 = t * kDecTile + i * 16;
-      bool ok = pg[i] >= 0 && pg[i] < kv.num_pages;
-      if (!ok && t < t1 && key0 < len && lane == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
+      const int key0 = it.tile * kDecTile + i * 16;
+      const int page = __shfl_sync(0xFFFFFFFFu, entry, 2 * (it.tile - held) + i);
+      const bool ok = page >= 0 && page < kv.num_pages;
+      if (!ok && lane == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
       const int slot = key0 & ((1 << kv.page_shift) - 1);
-      const int64_t ko = ok ? paged_offset(pg[i], kv.k_page_stride, hk, slot, kv.page_shift, kShift) : 0;
-      const int64_t vo = ok ? paged_offset(pg[i], kv.v_page_stride, hk, slot, kv.page_shift, kShift) : 0;
+      const int64_t ko = ok ? paged_offset(page, kv.k_page_stride, hk, slot, kv.page_shift, kShift) : 0;
+      const int64_t vo = ok ? paged_offset(page, kv.v_page_stride, hk, slot, kv.page_shift, kShift) : 0;
 #pragma unroll
       for (int j = 0; j < 16 / kRowsPerOp; ++j) {
         const int r = j * kRowsPerOp + sub;  // row within the half
-        const uint32_t bytes = (ok && key0 + r < len) ? 16u : 0u;
+        const uint32_t bytes = (ok && key0 + r < it.len) ? 16u : 0u;
         const int row = bytes ? r : 0;
         const uint32_t dst = ring + stage * Cfg::kStageBytes + (i * 16 + r) * Cfg::kRowBytes + ((c ^ (r & 7)) << 4);
         cp_async16(dst, kbase + ko + row * D + c * 8, bytes);
@@ -193,230 +271,358 @@ __global__ void __launch_bounds__(128) paged_decode_kernel(const DecodeParams p)
 
   float o[kMt][NT][4];
   float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-    for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[mt][nt][i] = 0.f;
-  }
-
-  int pg[2];
-  const int first = t0 + warp;
-#pragma unroll
-  for (int s = 0; s < Cfg::kStages - 1; ++s) {
-    const int t = first + s * Cfg::kWarps;
-    entries(t, pg);
-    if (t < t1) issue(t, s, pg);
-    cp_async_commit();
-  }
-  entries(first + (Cfg::kStages - 1) * Cfg::kWarps, pg);
-
-  int stage = 0;
-  for (int t = first; t < t1; t += Cfg::kWarps) {
-    cp_async_wait<Cfg::kStages - 2>();
-    __syncwarp();
-    // Refill the stage that the previous step emptied.
-    {
-      const int tn = t + (Cfg::kStages - 1) * Cfg::kWarps;
-      int sn = stage + Cfg::kStages - 1;
-      if (sn >= Cfg::kStages) sn -= Cfg::kStages;
-      if (tn < t1) issue(tn, sn, pg);
-      cp_async_commit();
-      entries(tn + Cfg::kWarps, pg);
-    }
-    const uint32_t ks_base = ring + stage * Cfg::kStageBytes;
-    const uint32_t vs_base = ks_base + Cfg::kHalfBytes;
-
-    float s[2][NT][4];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[mt][nt][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int r = mt * 16 + (lane & 15);
-        const int c = ks * 2 + (lane >> 4);
-        uint32_t a[4];
-        ldsm_x4(a, ks_base + r * Cfg::kRowBytes + ((c ^ (r & 7)) << 4));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(s[mt][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
-      }
-    }
-
-    // Scores in units of log2(e); keys behind the length drop out.
-    const int key_g = t * kDecTile + g;
-    const bool ragged = t * kDecTile + kDecTile > len;
-    float scale[NT][2];
+  uint32_t qf[NT][D / 16][2];  // Q^T fragments: column g = head, rows = head dimension
+  auto begin_segment = [&](const TileIter& it) {
+    const int hk = it.y / p.head_chunks, hc = it.y - hk * p.head_chunks;
+    const int nheads = min(Cfg::kHeads, p.group - hc * Cfg::kHeads);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + g;
+      const uint16_t* src =
+          static_cast<const uint16_t*>(p.q) + it.b * p.qt + (hk * p.group + hc * Cfg::kHeads + h) * p.qh;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          qf[nt][ks][i] = h < nheads ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + i * 8 + tq * 2) : 0u;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[mt][nt][i] = 0.f;
+    }
+  };
+  // Sums of l over the lanes that hold other keys of the same head.
+  auto fold_l = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float& x = s[mt][nt][half * 2 + e];
-            x *= p.scale_log2;
-            if (ragged && key_g + mt * 16 + half * 8 >= len) x = -INFINITY;
-            top = fmaxf(top, x);
-          }
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-        const float mn = fmaxf(m[nt][e], top);
-        const float ms = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: weights 0, not NaN
-        scale[nt][e] = exp2_approx(m[nt][e] - ms);
-        m[nt][e] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float& x = s[mt][nt][half * 2 + e];
-            x = exp2_approx(x - ms);
-            sum += x;
-          }
-        l[nt][e] = l[nt][e] * scale[nt][e] + sum;
+        l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], 4);
+        l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], 8);
+        l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], 16);
       }
+  };
+  auto store_piece = [&](unsigned char* at) {
+    float* row = reinterpret_cast<float*>(at);
+    float2* ml = reinterpret_cast<float2*>(row + Cfg::kHeads * Cfg::kPitch);
 #pragma unroll
-      for (int mt = 0; mt < kMt; ++mt) {
-        o[mt][nt][0] *= scale[nt][0];
-        o[mt][nt][1] *= scale[nt][1];
-        o[mt][nt][2] *= scale[nt][0];
-        o[mt][nt][3] *= scale[nt][1];
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = nt * 8 + tq * 2 + e;
+        if (g == 0) ml[h] = make_float2(m[nt][e], l[nt][e]);
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) {
+          row[h * Cfg::kPitch + mt * 16 + g] = o[mt][nt][e];
+          row[h * Cfg::kPitch + mt * 16 + g + 8] = o[mt][nt][2 + e];
+        }
+      }
+  };
+
+  TileIter cur = head;  // consumer; `head` runs kStages - 1 tiles ahead
+  if (lane == 0) s_first[warp] = s_last[warp] = 0;
+  if (cur.left > 0) {
+    entries(head);
+    begin_segment(cur);
+    bool from_before = cur.tile > 0;  // the segment began in an earlier share
+    int ahead = head.left;            // tiles not yet issued
+    int stage = 0;
+    auto fill = [&](int sn) {
+      if (ahead > 0) {
+        issue(head, sn);
+        if (--ahead > 0) {
+          advance(head, kv, rows);
+          if (head.tile == 0) {
+            entries(head);
+          } else if (head.tile - held == 16) {
+            held += 16;
+            entry = entry_next;
+            entry_next = look_up(head, held + 16);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll 1
+    for (int s = 0; s < Cfg::kStages - 1; ++s) fill(s);
+    while (true) {
+      cp_async_wait<Cfg::kStages - 2>();
+      __syncwarp();
+      // Refill the stage that the previous step emptied.
+      fill(stage == 0 ? Cfg::kStages - 1 : stage - 1);
+      const uint32_t ks_base = ring + stage * Cfg::kStageBytes;
+      const uint32_t vs_base = ks_base + Cfg::kHalfBytes;
+
+      float s[2][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[mt][nt][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const int r = mt * 16 + (lane & 15);
+          const int c = ks * 2 + (lane >> 4);
+          uint32_t a[4];
+          ldsm_x4(a, ks_base + r * Cfg::kRowBytes + ((c ^ (r & 7)) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(s[mt][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+        }
+      }
+
+      // Scores in units of log2(e); keys behind the length drop out.
+      const int key_g = cur.tile * kDecTile + g;
+      const bool ragged = cur.tile * kDecTile + kDecTile > cur.len;
+      float scale[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float& x = s[mt][nt][half * 2 + e];
+              x *= p.scale_log2;
+              if (ragged && key_g + mt * 16 + half * 8 >= cur.len) x = -INFINITY;
+              top = fmaxf(top, x);
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+          const float mn = fmaxf(m[nt][e], top);
+          const float ms = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: weights 0, not NaN
+          scale[nt][e] = exp2_approx(m[nt][e] - ms);
+          m[nt][e] = mn;
+          float sum_p = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float& x = s[mt][nt][half * 2 + e];
+              x = exp2_approx(x - ms);
+              sum_p += x;
+            }
+          l[nt][e] = l[nt][e] * scale[nt][e] + sum_p;
+        }
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) {
+          o[mt][nt][0] *= scale[nt][0];
+          o[mt][nt][1] *= scale[nt][1];
+          o[mt][nt][2] *= scale[nt][0];
+          o[mt][nt][3] *= scale[nt][1];
+        }
+      }
+
+      // P^T fragments (column = head), hi and lo terms, by 16 keys.
+      uint32_t ph[2][NT][2], pl[2][NT][2];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float x = s[kk][nt][half * 2], y = s[kk][nt][half * 2 + 1];
+            const uint32_t hi = pack2<F16>(x, y);
+            const float2 back = unpack2<F16>(hi);
+            ph[kk][nt][half] = movm_t(hi);
+            pl[kk][nt][half] = movm_t(pack2<F16>(x - back.x, y - back.y));
+          }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) {
+          const int r = kk * 16 + (lane & 7) + ((lane >> 4) << 3);
+          const int c = mt * 2 + ((lane >> 3) & 1);
+          uint32_t a[4];
+          ldsm_x4_t(a, vs_base + r * Cfg::kRowBytes + ((c ^ (r & 7)) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_16816<F16>(o[mt][nt], a, ph[kk][nt][0], ph[kk][nt][1]);
+            mma_16816<F16>(o[mt][nt], a, pl[kk][nt][0], pl[kk][nt][1]);
+          }
+        }
+      __syncwarp();  // every lane has read the stage before it is refilled
+      if (++stage == Cfg::kStages) stage = 0;
+
+      const bool ends = cur.tile + 1 == cur.tiles, stops = cur.left == 1;
+      if (ends || stops) {
+        fold_l();
+        if (from_before) {
+          store_piece(smem + Cfg::kOffFirst + warp * Cfg::kPieceBytes);
+          if (lane == 0) {
+            s_first[warp] = ends ? 1 : 2;
+            s_seg[warp][0][0] = cur.b;
+            s_seg[warp][0][1] = cur.y;
+          }
+        } else if (!ends) {
+          cp_async_wait<0>();
+          __syncwarp();
+          store_piece(smem + warp * Cfg::kWarpBytes);
+          if (lane == 0) {
+            s_last[warp] = 2;
+            s_seg[warp][1][0] = cur.b;
+            s_seg[warp][1][1] = cur.y;
+            s_end[warp] = u1 - cur.left + (cur.tiles - 1 - cur.tile);
+          }
+        } else {  // the whole segment: its rows are done
+          const int hk = cur.y / p.head_chunks, hc = cur.y - hk * p.head_chunks;
+          const int nheads = min(Cfg::kHeads, p.group - hc * Cfg::kHeads);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float inv[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              inv[e] = l[nt][e] > 0.f ? 1.f / l[nt][e] : (l[nt][e] == 0.f ? 0.f : l[nt][e]);
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + cur.b * p.ot +
+                            (hk * p.group + hc * Cfg::kHeads + nt * 8 + g) * p.oh + tq * 2;
+#pragma unroll
+            for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                // (element g; heads 2tq, 2tq + 1) to (head g; elements 2tq, 2tq + 1)
+                const uint32_t x =
+                    movm_t(pack2<F16>(o[mt][nt][half * 2] * inv[0], o[mt][nt][half * 2 + 1] * inv[1]));
+                if (nt * 8 + g < nheads) *reinterpret_cast<uint32_t*>(dst + mt * 16 + half * 8) = x;
+              }
+          }
+        }
+        if (stops) break;
+      }
+      advance(cur, kv, rows);
+      if (ends) {
+        begin_segment(cur);
+        from_before = false;
       }
     }
-
-    // P^T fragments (column = head), hi and lo terms, by 16 keys.
-    uint32_t ph[2][NT][2], pl[2][NT][2];
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float x = s[kk][nt][half * 2], y = s[kk][nt][half * 2 + 1];
-          const uint32_t hi = pack2<F16>(x, y);
-          const float2 back = unpack2<F16>(hi);
-          ph[kk][nt][half] = movm_t(hi);
-          pl[kk][nt][half] = movm_t(pack2<F16>(x - back.x, y - back.y));
-        }
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int mt = 0; mt < kMt; ++mt) {
-        const int r = kk * 16 + (lane & 7) + ((lane >> 4) << 3);
-        const int c = mt * 2 + ((lane >> 3) & 1);
-        uint32_t a[4];
-        ldsm_x4_t(a, vs_base + r * Cfg::kRowBytes + ((c ^ (r & 7)) << 4));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_16816<F16>(o[mt][nt], a, ph[kk][nt][0], ph[kk][nt][1]);
-          mma_16816<F16>(o[mt][nt], a, pl[kk][nt][0], pl[kk][nt][1]);
-        }
-      }
-    __syncwarp();  // every lane has read the stage before it is refilled
-    if (++stage == Cfg::kStages) stage = 0;
   }
   cp_async_wait<0>();
-  __syncthreads();  // the rings become the join area
+  // Sequences without tokens: rows of zeros.
+  for (int b = blockIdx.x; b < kv.batch; b += gridDim.x) {
+    int len;
+    bool bad;
+    if (tiles_of(kv, b, &len, &bad) == 0)
+      for (int i = threadIdx.x; i < kv.kv_heads * p.group * kCpr; i += kDecThreads)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + b * p.ot + (i / kCpr) * p.oh + (i % kCpr) * 8) =
+            make_uint4(0u, 0u, 0u, 0u);
+  }
+  __syncthreads();
 
-  float* jo = reinterpret_cast<float*>(smem);                       // [warp][head][pitch]
-  float2* jml = reinterpret_cast<float2*>(jo + Cfg::kWarps * Cfg::kHeads * Cfg::kJoinPitch);  // [warp][head]
+  // ---- pieces that cross warps ------------------------------------------------
+  // A chain is a last piece and the first pieces of the following warps as far
+  // as the segment goes; the chain before warp 0 lacks its start (in an earlier
+  // CTA). One warp takes a head, a lane D / 32 of its elements.
+  constexpr int kPer = D / 32;
+  auto write_row = [&](int b, int y, int h, const float (&x)[kPer], float l_sum) {
+    const float inv = l_sum > 0.f ? 1.f / l_sum : (l_sum == 0.f ? 0.f : l_sum);
+    const int hk = y / p.head_chunks, hc = y - hk * p.head_chunks;
+    uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.ot + (hk * p.group + hc * Cfg::kHeads + h) * p.oh + lane * kPer;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack2<F16>(x[i] * inv, x[i + 1] * inv);
+  };
+  int over = -1;  // warp whose last piece goes on in the next CTA
+  for (int w = -1; w < kDecWarps; ++w) {
+    if (w < 0 ? s_first[0] == 0 : s_last[w] == 0) continue;
+    int to = w + 1;
+    bool on = true;
+    while (to < kDecWarps && on) on = s_first[to++] == 2;
+    const int b = w < 0 ? s_seg[0][0][0] : s_seg[w][1][0], y = w < 0 ? s_seg[0][0][1] : s_seg[w][1][1];
+    const int nheads = min(Cfg::kHeads, p.group - (y % p.head_chunks) * Cfg::kHeads);
+    const bool whole = w >= 0 && !on;
+    if (w >= 0 && on) over = w;
+    const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (w < 0 ? 0 : 1)) * Cfg::kHeads;
+    for (int h = warp; h < nheads; h += kDecWarps) {
+      auto piece = [&](int k) {
+        return reinterpret_cast<const float*>(k == w ? smem + w * Cfg::kWarpBytes
+                                                     : smem + Cfg::kOffFirst + k * Cfg::kPieceBytes);
+      };
+      const int k0 = max(w, 0);
+      float top = -INFINITY, l_sum = 0.f, x[kPer];
+      for (int k = k0; k < to; ++k)
+        top = fmaxf(top, reinterpret_cast<const float2*>(piece(k) + Cfg::kHeads * Cfg::kPitch)[h].x);
+      const float ms = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float sum = l[nt][e];
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
-      const int h = nt * 8 + tq * 2 + e;
-      if (g == 0) jml[warp * Cfg::kHeads + h] = make_float2(m[nt][e], sum);
-      float* row = jo + (warp * Cfg::kHeads + h) * Cfg::kJoinPitch;
+      for (int i = 0; i < kPer; ++i) x[i] = 0.f;
+      for (int k = k0; k < to; ++k) {
+        const float2 ml = reinterpret_cast<const float2*>(piece(k) + Cfg::kHeads * Cfg::kPitch)[h];
+        const float* row = piece(k) + h * Cfg::kPitch + lane * kPer;
+        const float f = exp2_approx(ml.x - ms);
+        l_sum += ml.y * f;
 #pragma unroll
-      for (int mt = 0; mt < kMt; ++mt) {
-        row[mt * 16 + g] = o[mt][nt][e];
-        row[mt * 16 + g + 8] = o[mt][nt][2 + e];
+        for (int i = 0; i < kPer; ++i) x[i] += row[i] * f;
+      }
+      if (whole) {
+        write_row(b, y, h, x, l_sum);
+      } else {
+        float* dst = p.part_o + (slot + h) * D + lane * kPer;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(x[i], x[i + 1]);
+        if (lane == 0) p.part_ml[slot + h] = make_float2(top, l_sum);
       }
     }
-  __syncthreads();
-  // Two elements per thread and step.
-  for (int i = threadIdx.x; i < nheads * (D / 2); i += 128) {
-    const int h = i / (D / 2), d = (i % (D / 2)) * 2;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < Cfg::kWarps; ++w) top = fmaxf(top, jml[w * Cfg::kHeads + h].x);
-    const float ms = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-    for (int w = 0; w < Cfg::kWarps; ++w) {
-      const float2 ml = jml[w * Cfg::kHeads + h];
-      const float f = exp2_approx(ml.x - ms);
-      sum += ml.y * f;
-      const float2 v = *reinterpret_cast<const float2*>(jo + (w * Cfg::kHeads + h) * Cfg::kJoinPitch + d);
-      x += v.x * f;
-      y += v.y * f;
-    }
-    if (p.splits == 1) {
-      const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-      uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.ot + (head0 + h) * p.oh + d;
-      *reinterpret_cast<uint32_t*>(dst) = pack2<F16>(x * inv, y * inv);
-    } else {
-      const int64_t row = (static_cast<int64_t>(b) * heads + head0 + h) * p.splits + split;
-      *reinterpret_cast<float2*>(p.part_o + row * D + d) = make_float2(x, y);
-      if (d == 0) p.part_ml[row] = make_float2(top, sum);
-    }
+  }
+  if (threadIdx.x == 0) {
+    int4 spill = make_int4(0, 0, 0, 0);
+    if (over >= 0)
+      spill = make_int4(s_seg[over][1][0], s_seg[over][1][1],
+                        share_of(total, shares, s_end[over]) / kDecWarps - static_cast<int>(blockIdx.x) + 1, 0);
+    p.spill[blockIdx.x] = spill;
   }
 }
 
-// Joins the pieces of each (sequence, head): grid (heads, batch), one warp
-// per fourth of the pieces, four head-dimension elements (two for D = 64) per
-// lane.
+// Joins the segments that cross CTAs: block (c, h) takes head h of the
+// segment that starts in CTA c and ends in a later one; its pieces are CTA
+// c's second slot and the following CTAs' first ones. Each warp takes every
+// eighth piece.
 struct JoinParams {
-  const int32_t* seq_lens;
   void* out;
   int64_t ot, oh;
-  int32_t heads, splits, max_pages, page_shift;
+  int32_t group, head_chunks;
   const float* part_o;
   const float2* part_ml;
+  const int4* spill;
 };
+constexpr int kJoinWarps = 8;
 
-template <int D, bool F16>
-__global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
+template <int D, int NT, bool F16>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const JoinParams p) {
+  constexpr int kHeads = DecodeCfg<D, NT>::kHeads;
   constexpr int kPer = D / 32;
-  __shared__ float so[4][D];
-  __shared__ float2 sml[4];
+  __shared__ float so[kJoinWarps][D];
+  __shared__ float2 sml[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x, b = blockIdx.y;
+  const int c = blockIdx.x, h = blockIdx.y;
   griddep_wait();
   griddep_launch();
-  bool bad;
-  const int len = paged_clamp_len(p.seq_lens[b], p.max_pages, p.page_shift, &bad);
-  const int count = split_count((len + kDecTile - 1) / kDecTile, p.splits);
-  const int64_t row0 = (static_cast<int64_t>(b) * p.heads + h) * p.splits;
+  const int4 seg = p.spill[c];
+  if (seg.z == 0) return;
+  const int hk = seg.y / p.head_chunks, hc = seg.y - hk * p.head_chunks;
+  if (hc * kHeads + h >= p.group) return;
   float m = -INFINITY, l = 0.f, o[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) o[i] = 0.f;
 #pragma unroll 4
-  for (int s = warp; s < count; s += 4) {
-    const float2 ml = p.part_ml[row0 + s];
-    const float* src = p.part_o + (row0 + s) * D + lane * kPer;
+  for (int s = warp; s < seg.z; s += kJoinWarps) {
+    const int64_t at = (static_cast<int64_t>(c + s) * 2 + (s == 0 ? 1 : 0)) * kHeads + h;
+    const float2 ml = p.part_ml[at];
+    const float2* src = reinterpret_cast<const float2*>(p.part_o + at * D + lane * kPer);
     const float mn = fmaxf(m, ml.x);
     const float ms = mn == -INFINITY ? 0.f : mn;
     const float f0 = exp2_approx(m - ms), f1 = exp2_approx(ml.x - ms);
     m = mn;
     l = l * f0 + ml.y * f1;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = o[i] * f0 + src[i] * f1;
+    for (int i = 0; i < kPer / 2; ++i) {
+      const float2 v = src[i];
+      o[2 * i] = o[2 * i] * f0 + v.x * f1;
+      o[2 * i + 1] = o[2 * i + 1] * f0 + v.y * f1;
+    }
   }
   if (lane == 0) sml[warp] = make_float2(m, l);
 #pragma unroll
@@ -424,19 +630,21 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
   __syncthreads();
   if (threadIdx.x < D / 2) {
     const int d = threadIdx.x * 2;
-    const float top = fmaxf(fmaxf(sml[0].x, sml[1].x), fmaxf(sml[2].x, sml[3].x));
+    float top = sml[0].x;
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) top = fmaxf(top, sml[w].x);
     const float ms = top == -INFINITY ? 0.f : top;
     float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kJoinWarps; ++w) {
       const float f = exp2_approx(sml[w].x - ms);
       sum += sml[w].y * f;
       x += so[w][d] * f;
       y += so[w][d + 1] * f;
     }
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-    uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.ot + h * p.oh + d;
-    *reinterpret_cast<uint32_t*>(dst) = pack2<F16>(x * inv, y * inv);
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + seg.x * p.ot +
+                                 (hk * p.group + hc * kHeads + h) * p.oh + d) = pack2<F16>(x * inv, y * inv);
   }
 }
 

@@ -54,4 +54,17 @@ __host__ __device__ __forceinline__ int split_count(int tiles, int splits) {
   return (tiles + per - 1) / per;
 }
 
+// `total` tiles dealt to `shares` equal shares (they differ by one tile at
+// most): the first tile of share w ...
+__host__ __device__ __forceinline__ int share_start(int total, int shares, int w) {
+  const int base = total / shares, rest = total - base * shares;
+  return w * base + (w < rest ? w : rest);
+}
+// ... and the share that holds tile u < total.
+__host__ __device__ __forceinline__ int share_of(int total, int shares, int u) {
+  const int base = total / shares, rest = total - base * shares;
+  const int cut = rest * (base + 1);
+  return u < cut ? u / (base + 1) : rest + (u - cut) / base;
+}
+
 }  // namespace abft

@@ -23,6 +23,7 @@ there, per call.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -198,11 +199,7 @@ class PagedKVCache:
             raise ValueError(f"cu_seqlens must have {self.batch + 1} entries, got {cu.shape[0]}")
 
     def _call(self, name: str, fn, args) -> None:
-        if torch._C._cuda_getDevice() != self._index:
-            with torch.cuda.device(self._index):
-                rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(self._index))
-        else:
-            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(self._index))
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(self._index))
         if rc != N.ABFT_OK:
             N.check(name, rc)
 
@@ -223,6 +220,9 @@ class PagedKVCache:
         sequence are left as they were (undefined without ``q_out``). q None
         stores k and v only.
         """
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
         key = (_signature(q), _signature(k), _signature(v), _signature(rope), _signature(cu_seqlens), _signature(q_out))
         template, copies = self._plan(key, lambda: self._plan_append(q, k, v, rope, cu_seqlens, q_out))
         args = N.KvAppendArgs.from_buffer_copy(template)
@@ -276,13 +276,12 @@ class PagedKVCache:
         return bytes(args), not all(t is None or self._in_place(t) for t in (q, k, v))
 
     def decode(self, q: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-               num_splits: int = 0) -> torch.Tensor:
+               num_sms: int = 0) -> torch.Tensor:
         """Attention of each sequence's newest token over its cache: ``q``
         [batch, heads, head_dim], returns the same shape. ``scale`` defaults
-        to head_dim^-0.5. A sequence of length 0 gives zeros. ``num_splits``:
-        pieces a sequence is cut into (0: chosen from the batch, the heads and
-        the table's width)."""
-        return self._attention("abft_paged_decode", q, None, scale, out, num_splits)
+        to head_dim^-0.5. A sequence of length 0 gives zeros. ``num_sms``:
+        SMs the caches are shared out to (0: all)."""
+        return self._attention("abft_paged_decode", q, None, scale, out, 0, num_sms)
 
     def prefill(self, q: torch.Tensor, cu_seqlens: torch.Tensor, *, scale: Optional[float] = None,
                 out: Optional[torch.Tensor] = None, num_splits: int = 0) -> torch.Tensor:
@@ -291,19 +290,24 @@ class PagedKVCache:
         the last tokens of sequence b (``append`` has stored their keys), and
         row i of n sees the slots up to seq_lens[b] - n + i. Chunks of any
         length, 0 and 1 included; rows behind cu[batch] are left as they were
-        in ``out`` (undefined without one). ``num_splits`` as for decode."""
-        return self._attention("abft_paged_prefill", q, cu_seqlens, scale, out, num_splits)
+        in ``out`` (undefined without one). ``num_splits``: pieces the keys of
+        a block of query rows are cut into (0: chosen from the rows, the heads
+        and the table's width)."""
+        return self._attention("abft_paged_prefill", q, cu_seqlens, scale, out, num_splits, 0)
 
-    def _attention(self, name, q, cu, scale, out, num_splits):
-        key = (name, _signature(q), _signature(cu), scale, _signature(out), num_splits)
-        template, copies, space = self._plan(key, lambda: self._plan_attention(name, q, cu, scale, out, num_splits))
+    def _attention(self, name, q, cu, scale, out, num_splits, num_sms):
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                return self._attention(name, q, cu, scale, out, num_splits, num_sms)
+        key = (name, _signature(q), _signature(cu), scale, _signature(out), num_splits, num_sms)
+        template, copies, space = self._plan(key, lambda: self._plan_attention(name, q, cu, scale, out, num_splits, num_sms))
         args = N.PagedAttnArgs.from_buffer_copy(template)
         if copies:
             q = q.contiguous()
         qp = q.data_ptr()
         if qp & 15:
             q = _aligned(q)
-            return self._attention(name, q, cu, scale, out, num_splits)
+            return self._attention(name, q, cu, scale, out, num_splits, num_sms)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         args.q, args.out = qp, _address("out", out)
@@ -315,7 +319,7 @@ class PagedKVCache:
         self._call(name, getattr(N.lib(), name), args)
         return out
 
-    def _plan_attention(self, name, q, cu, scale, out, num_splits):
+    def _plan_attention(self, name, q, cu, scale, out, num_splits, num_sms):
         decode = name == "abft_paged_decode"
         if not decode:
             self._boundaries(cu)
@@ -327,18 +331,19 @@ class PagedKVCache:
             (q.shape[1] * self.head_dim, self.head_dim) if out is None else self._result("out", out, q))
         args.tokens, args.heads = q.shape[0], q.shape[1]
         args.scale = self.head_dim ** -0.5 if scale is None else float(scale)
-        args.num_splits = int(num_splits)
+        args.num_splits, args.num_sms = int(num_splits), int(num_sms)
+        if args.num_splits < 0 or args.num_sms < 0 or not math.isfinite(args.scale):
+            raise ValueError(f"scale must be finite, num_splits and num_sms at least 0, got {scale}, {num_splits}, {num_sms}")
         space = None
         if q.shape[0] and self.batch:
             # placeholder addresses: sizes decide how much scratch the call needs
             args.q = args.out = args.cu_seqlens = 1 << 20
-            with torch.cuda.device(self._index):
-                need = int(getattr(N.lib(), name + "_workspace_bytes")(ctypes.byref(args)))
+            need = int(getattr(N.lib(), name + "_workspace_bytes")(ctypes.byref(args)))
             args.q = args.out = args.cu_seqlens = None
             if need:
                 args.workspace_bytes = need
                 # one byte seen as `need` of them: empty_like gives that many
-                space = torch.empty(1, dtype=torch.uint8, device=self.device).expand(need)
+                space = self.status.view(torch.uint8)[:1].expand(need)
         return bytes(args), not self._in_place(q), space
 
     def check_status(self) -> None:
