@@ -83,6 +83,9 @@ int main() {
   need(lo == 4 && hi == 60, "packed 2");
   need(visible_keys(10, 3, 0) == 8 && visible_keys(10, 3, 2) == 10, "visible");
   need(visible_keys(1, 3, 0) == 0 && visible_keys(1, 3, 1) == 0 && visible_keys(1, 3, 2) == 1, "none visible");
+  for (int group = 1; group <= 64; ++group)
+    for (int row = 0; row < 128; ++row)
+      need(row_token(row, (65536u + group - 1) / group) == row / group, "row token");
   std::printf("%ld\n", checks);
   return 0;
 }

@@ -251,10 +251,14 @@ int64_t prefill_blocks(const abft_paged_attn_args* a) {
 }
 
 // Pieces a block's keys are cut into: while the blocks alone would leave SMs
-// idle, as many as fill them once.
+// idle, as many as fill them about twice, of four steps at least.
 int prefill_splits(const abft_paged_attn_args* a, int sms) {
   const int64_t steps = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kPreKeys - 1) / kPreKeys;
-  int64_t n = a->num_splits > 0 ? a->num_splits : sms / (prefill_blocks(a) * a->kv.kv_heads);
+  int64_t n = a->num_splits;
+  if (n == 0) {
+    n = 2 * sms / (prefill_blocks(a) * a->kv.kv_heads);
+    if (n > steps / 4) n = steps / 4;
+  }
   if (n > steps) n = steps;
   if (n > 65535) n = 65535;
   return static_cast<int>(n < 1 ? 1 : n);
@@ -401,7 +405,8 @@ int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
   p.blocks = static_cast<int32_t>(prefill_blocks(a));
   const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
   p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
-  p.flip = a->scale < 0.f ? 0x80008000u : 0u;
+  p.negate = a->scale < 0.f;
+  p.group_inv = (65536u + p.group - 1) / p.group;
   const size_t need = prefill_bytes(a, p.splits);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
   if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;

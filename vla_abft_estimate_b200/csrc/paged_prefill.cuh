@@ -23,7 +23,8 @@
 // the first tiles of a row hardly happens.
 //
 // Warps: 0-3 and 4-7 the rows of tile 0 and 1 (TMEM lane quadrant = warp % 4),
-// 8 TMA loads of pages into a ring of tiles, 9 the MMA issuer.
+// 8 TMA loads of pages into a ring of tiles, 9 the MMA issuer, 10 and 11 idle
+// (registers move between groups of four warps).
 #pragma once
 
 #include <cuda.h>
@@ -38,7 +39,11 @@ namespace abft {
 
 constexpr int kPreRows = 128;   // query rows of a tile
 constexpr int kPreKeys = 128;   // keys of a step
-constexpr int kPreThreads = 320;
+constexpr int kPreThreads = 384;
+// Registers: 384 threads launch with at most 168 each (64,512 in all); the
+// rows' warps hold a whole row of S and take 216, the others keep 72:
+// 256 * 216 + 128 * 72 = 64,512.
+constexpr int kPreRegsRows = 216, kPreRegsOther = 72;
 
 template <int D>
 struct PrefillCfg {
@@ -70,7 +75,8 @@ struct PrefillParams {
   int32_t blocks;          // CTAs per kv head and split: tokens / (2 tile_tokens) + batch at most
   int32_t splits;
   float scale_log2;        // |scale| * log2(e), never 0
-  uint32_t flip;           // sign bits of a packed pair when scale < 0: applied to q
+  int32_t negate;          // scale < 0
+  uint32_t group_inv;      // ceil(2^16 / group): row_token()
   float* part_o;           // [tokens * heads][splits][head_dim]
   float2* part_ml;         // [tokens * heads][splits]
 };
@@ -80,6 +86,12 @@ __host__ __device__ __forceinline__ void packed_range(const int32_t* cu, int b, 
   const int lo = cu[b], hi = cu[b + 1];
   *begin = lo < 0 ? 0 : (lo > tokens ? tokens : lo);
   *end = hi < *begin ? *begin : (hi > tokens ? tokens : hi);
+}
+
+// row / group for a row of a tile: exact for rows below 128 and groups up to 64
+// (the product overshoots the quotient by less than 128 / 2^16 < 1 / 64).
+__host__ __device__ __forceinline__ int row_token(int row, uint32_t group_inv) {
+  return static_cast<int>((static_cast<uint32_t>(row) * group_inv) >> 16);
 }
 
 // Keys that local token i of n sees in a sequence of length len.
@@ -130,6 +142,27 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint6
           "r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // D += A B with A (16-bit pairs, one row per lane) in TMEM.
@@ -249,30 +282,31 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 
     if (warp < 8) {
       // ---------------------------------------------------------- softmax rows
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsRows));
       const int t = warp >> 2;
       const int r = threadIdx.x & 127;
       const int first = tok0 + t * p.tile_tokens;
       const int here = max(0, min(p.tile_tokens, n - first)) * p.group;  // rows in use
       // Q tile into shared memory, in the swizzled layout of a TMA box.
       if (end[t] > j0) {
-        uint8_t* dst = smem + t * Cfg::kTileBytes;
+        const uint32_t dst = smem_u32(smem + t * Cfg::kTileBytes);
         constexpr int kCpr = D / 8;
-#pragma unroll 4
-        for (int i = r; i < kPreRows * kCpr; i += kPreRows) {
-          const int row = i / kCpr, c = i % kCpr;
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (row < here) {
-            const int tok = row / p.group, g = row - tok * p.group;
-            x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (row0 + first + tok) * p.qt +
-                                                (hk * p.group + g) * p.qh + c * 8);
-            x.x ^= p.flip, x.y ^= p.flip, x.z ^= p.flip, x.w ^= p.flip;
-          }
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * Cfg::kBlockBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x;
+        const int c = r % kCpr;
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (row0 + first) * p.qt + hk * p.group * p.qh + c * 8;
+#pragma unroll
+        for (int i = 0; i < kCpr; ++i) {
+          const int row = i * (kPreRows / kCpr) + r / kCpr;
+          const bool in = row < here;
+          const int tok = in ? row_token(row, p.group_inv) : 0, g = in ? row - tok * p.group : 0;
+          cp_async16(dst + (c >> 3) * Cfg::kBlockBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                     src + tok * p.qt + g * p.qh, in ? 16u : 0u);
         }
+        cp_async_commit();
+        cp_async_wait<0>();
         fence_proxy_async_smem();
         mbar_arrive(&qfull[t]);
       }
-      const int tok = r / p.group;
+      const int tok = row_token(r, p.group_inv);
       const bool live = r < here;
       const int vis = live ? visible_keys(len, n, first + tok) : 0;
       const int vis_min = visible_keys(len, n, first);  // of the tile's first token
@@ -290,6 +324,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + c * 32, s[c]);
         tmem_ld_wait();
+        if (p.negate) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[c][i] ^= 0x80000000u;
+        }
         if (vis_min < (j + 1) * kPreKeys) {
           const int lim = vis - j * kPreKeys;
 #pragma unroll
@@ -301,11 +341,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          mx[c] = -INFINITY;
+          mx[c] = max3(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]), __uint_as_float(s[c][2]));
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+          for (int i = 3; i < 31; i += 2) mx[c] = max3(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+          mx[c] = fmaxf(mx[c], __uint_as_float(s[c][31]));
         }
-        const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        const float mn = fmaxf(m, max3(mx[0], mx[1], fmaxf(mx[2], mx[3])));
         const bool raise = (mn - m) * p.scale_log2 > 8.f;  // also from m = -inf; false for -inf, -inf
         if (j == j0) {
           m = mn;
@@ -325,7 +366,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           tmem_st_wait();
         }
         const float shift = m == -INFINITY ? 0.f : -m * p.scale_log2;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t pk[32];
@@ -333,14 +375,16 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float x = exp2_approx(fmaf(__uint_as_float(s[2 * h + c][i]), p.scale_log2, shift));
-              const float y = exp2_approx(fmaf(__uint_as_float(s[2 * h + c][i + 1]), p.scale_log2, shift));
-              sum[(i >> 1) & 3] += x + y;
-              pk[c * 16 + (i >> 1)] = pack2<F16>(x, y);
+              float2 x = fma2(make_float2(__uint_as_float(s[2 * h + c][i]), __uint_as_float(s[2 * h + c][i + 1])),
+                              scale2, shift2);
+              x.x = exp2_approx(x.x);
+              x.y = exp2_approx(x.y);
+              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
+              pk[c * 16 + (i >> 1)] = pack2<F16>(x.x, x.y);
             }
           tmem_st_32x32b_x32(ts + h * 32, pk);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&pfull[t]);
@@ -396,136 +440,139 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
       }
       tc_fence_before();
-    } else if (warp == 8) {
-      // ---------------------------------------------------------- page loads
-      const int32_t* table = kv.page_table + seq * kv.table_stride;
-      const int page = 1 << kv.page_shift;
-      const int piece = lane / Cfg::kHalves, half = lane % Cfg::kHalves;  // page of the step, column block
-      const int per_step = kPreKeys >> kv.page_shift;
-      const int held = (len + page - 1) >> kv.page_shift;  // pages of the sequence
-      auto entry = [&](int j) {
-        const int at = j * per_step + piece;
-        return piece < per_step && at < held ? table[at] : 0;
-      };
-      int next = j0 < j1 ? entry(j0) : 0;
-      int issued = 0;
-      bool ok = true;
-      for (int j = j0; j < j1 && ok; ++j) {
-        const int id = next;
-        if (j + 1 < j1) next = entry(j + 1);
-        const int pieces = min(per_step, held - j * per_step);
-        const bool mine = piece < pieces;
-        if (mine && half == 0 && (id < 0 || id >= kv.num_pages) && kv.status != nullptr)
-          atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int it = 2 * (j - j0) + x;
-          const int slot = it % Cfg::kSlots;
-          if (it >= Cfg::kSlots && !mbar_wait(&empty[slot], (it / Cfg::kSlots - 1) & 1, abort_flag)) ok = false;
-          ok = __all_sync(0xFFFFFFFFu, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(pieces * page * D * 2));
-          __syncwarp();
-          if (mine) {
-            // A bad id lies outside the map's page dimension and loads zeros.
-            const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes + half * Cfg::kBlockBytes) +
-                                 piece * page * 128;
-            tma_load_4d(dst, x == 0 ? &tm_k : &tm_v, &full[slot], 0, hk << kv.page_shift, half, id);
-          }
-          ++issued;
-        }
-      }
-      // Copies in flight have landed before shared memory goes (all have, but
-      // after an abort).
-      for (int it = max(0, issued - Cfg::kSlots); it < issued; ++it)
-        mbar_wait_bounded(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1);
     } else {
-      // ---------------------------------------------------------- MMA issuer
-      constexpr uint32_t fmt = F16 ? 0u : 1u;
-      constexpr uint32_t idesc_s = umma_idesc(kPreRows, kPreKeys, fmt);
-      constexpr uint32_t idesc_o = umma_idesc(kPreRows, D, fmt) | kIdescBNMajor;
-      const uint32_t ring = smem_u32(smem + Cfg::kOffRing);
-      bool ok = true;
-      auto ready = [&](int it) {
-        ok = ok && mbar_wait(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1, abort_flag);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        tc_fence_after();
-        return ok;
-      };
-      auto scores = [&](int t, int it) {
-        if (lane == 0) {
-          const uint32_t a = smem_u32(smem + t * Cfg::kTileBytes), b = ring + (it % Cfg::kSlots) * Cfg::kTileBytes;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k / 4) * Cfg::kBlockBytes + (k % 4) * 32;
-            umma_bf16_ss(tmem + t * 128, sw128_kmajor_desc(a + off), sw128_kmajor_desc(b + off), idesc_s, k > 0);
-          }
-          umma_commit(&sfull[t]);
-        }
-        __syncwarp();
-      };
-      auto release = [&](int it) {  // the slot is loaded again: once the MMAs so far have read it
-        if (lane == 0 && it + Cfg::kSlots < total) umma_commit(&empty[it % Cfg::kSlots]);
-        __syncwarp();
-      };
-      for (int t = 0; t < 2; ++t)
-        if (end[t] > j0) ok = ok && mbar_wait(&qfull[t], 0, abort_flag);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (ok && j0 < j1 && ready(0)) {
-        for (int t = 0; t < 2; ++t)
-          if (end[t] > j0) scores(t, 0);
-        release(0);
-      }
-      for (int j = j0; j < j1 && ok; ++j) {
-        const int iv = 2 * (j - j0) + 1, ik = iv + 1;
-        if (!ready(iv)) break;
-        const uint32_t vb = ring + (iv % Cfg::kSlots) * Cfg::kTileBytes;
-        // Weights of slots behind the length are 0, but the slots may hold
-        // anything (a page's last owner, NaN): only whole groups of 16 keys
-        // that the sequence reaches are multiplied, the rest of the last
-        // group is cleared.
-        const int valid = min(kPreKeys, len - j * kPreKeys);
-        const int groups = (valid + 15) / 16;
-        if (valid & 15) {
-          uint8_t* v = smem + Cfg::kOffRing + (iv % Cfg::kSlots) * Cfg::kTileBytes;
-          for (int i = valid * (D / 8) + lane; i < groups * 16 * (D / 8); i += 32) {
-            const int row = i / (D / 8), c = i % (D / 8);  // every piece of the row: its order does not matter
-            *reinterpret_cast<uint4*>(v + (c >> 3) * Cfg::kBlockBytes + row * 128 + ((c & 7) << 4)) =
-                make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        bool loaded = false;
-        for (int t = 0; t < 2; ++t) {
-          if (j < end[t]) {
-            ok = ok && mbar_wait(&pfull[t], (j - j0) & 1, abort_flag);
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsOther));
+      if (warp == 8) {
+        // ---------------------------------------------------------- page loads
+        const int32_t* table = kv.page_table + seq * kv.table_stride;
+        const int page = 1 << kv.page_shift;
+        const int piece = lane / Cfg::kHalves, half = lane % Cfg::kHalves;  // page of the step, column block
+        const int per_step = kPreKeys >> kv.page_shift;
+        const int held = (len + page - 1) >> kv.page_shift;  // pages of the sequence
+        auto entry = [&](int j) {
+          const int at = j * per_step + piece;
+          return piece < per_step && at < held ? table[at] : 0;
+        };
+        int next = j0 < j1 ? entry(j0) : 0;
+        int issued = 0;
+        bool ok = true;
+        for (int j = j0; j < j1 && ok; ++j) {
+          const int id = next;
+          if (j + 1 < j1) next = entry(j + 1);
+          const int pieces = min(per_step, held - j * per_step);
+          const bool mine = piece < pieces;
+          if (mine && half == 0 && (id < 0 || id >= kv.num_pages) && kv.status != nullptr)
+            atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
+  #pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int it = 2 * (j - j0) + x;
+            const int slot = it % Cfg::kSlots;
+            if (it >= Cfg::kSlots && !mbar_wait(&empty[slot], (it / Cfg::kSlots - 1) & 1, abort_flag)) ok = false;
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
-            tc_fence_after();
-            if (lane == 0) {
-              for (int k = 0; k < groups; ++k)
-                umma_f16_ts(tmem + Cfg::kColO + t * D, tmem + t * 128 + k * 8,
-                            sw128_nmajor_desc(vb + k * 2048, Cfg::kBlockBytes), idesc_o, (j > j0) | (k > 0));
-              if (j + 1 == end[t]) umma_commit(&ofull[t]);
-            }
+            if (lane == 0) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(pieces * page * D * 2));
             __syncwarp();
-          }
-          if (j + 1 < end[t]) {
-            if (!loaded && !ready(ik)) break;
-            loaded = true;
-            scores(t, ik);
+            if (mine) {
+              // A bad id lies outside the map's page dimension and loads zeros.
+              const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes + half * Cfg::kBlockBytes) +
+                                   piece * page * 128;
+              tma_load_4d(dst, x == 0 ? &tm_k : &tm_v, &full[slot], 0, hk << kv.page_shift, half, id);
+            }
+            ++issued;
           }
         }
-        if (!ok) break;
-        release(iv);
-        if (loaded) release(ik);
+        // Copies in flight have landed before shared memory goes (all have, but
+        // after an abort).
+        for (int it = max(0, issued - Cfg::kSlots); it < issued; ++it)
+          mbar_wait_bounded(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1);
+      } else if (warp == 9) {
+        // ---------------------------------------------------------- MMA issuer
+        constexpr uint32_t fmt = F16 ? 0u : 1u;
+        constexpr uint32_t idesc_s = umma_idesc(kPreRows, kPreKeys, fmt);
+        constexpr uint32_t idesc_o = umma_idesc(kPreRows, D, fmt) | kIdescBNMajor;
+        const uint32_t ring = smem_u32(smem + Cfg::kOffRing);
+        bool ok = true;
+        auto ready = [&](int it) {
+          ok = ok && mbar_wait(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1, abort_flag);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          tc_fence_after();
+          return ok;
+        };
+        auto scores = [&](int t, int it) {
+          if (lane == 0) {
+            const uint32_t a = smem_u32(smem + t * Cfg::kTileBytes), b = ring + (it % Cfg::kSlots) * Cfg::kTileBytes;
+  #pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = (k / 4) * Cfg::kBlockBytes + (k % 4) * 32;
+              umma_bf16_ss(tmem + t * 128, sw128_kmajor_desc(a + off), sw128_kmajor_desc(b + off), idesc_s, k > 0);
+            }
+            umma_commit(&sfull[t]);
+          }
+          __syncwarp();
+        };
+        auto release = [&](int it) {  // the slot is loaded again: once the MMAs so far have read it
+          if (lane == 0 && it + Cfg::kSlots < total) umma_commit(&empty[it % Cfg::kSlots]);
+          __syncwarp();
+        };
+        for (int t = 0; t < 2; ++t)
+          if (end[t] > j0) ok = ok && mbar_wait(&qfull[t], 0, abort_flag);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (ok && j0 < j1 && ready(0)) {
+          for (int t = 0; t < 2; ++t)
+            if (end[t] > j0) scores(t, 0);
+          release(0);
+        }
+        for (int j = j0; j < j1 && ok; ++j) {
+          const int iv = 2 * (j - j0) + 1, ik = iv + 1;
+          if (!ready(iv)) break;
+          const uint32_t vb = ring + (iv % Cfg::kSlots) * Cfg::kTileBytes;
+          // Weights of slots behind the length are 0, but the slots may hold
+          // anything (a page's last owner, NaN): only whole groups of 16 keys
+          // that the sequence reaches are multiplied, the rest of the last
+          // group is cleared.
+          const int valid = min(kPreKeys, len - j * kPreKeys);
+          const int groups = (valid + 15) / 16;
+          if (valid & 15) {
+            uint8_t* v = smem + Cfg::kOffRing + (iv % Cfg::kSlots) * Cfg::kTileBytes;
+            for (int i = valid * (D / 8) + lane; i < groups * 16 * (D / 8); i += 32) {
+              const int row = i / (D / 8), c = i % (D / 8);  // every piece of the row: its order does not matter
+              *reinterpret_cast<uint4*>(v + (c >> 3) * Cfg::kBlockBytes + row * 128 + ((c & 7) << 4)) =
+                  make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          bool loaded = false;
+          for (int t = 0; t < 2; ++t) {
+            if (j < end[t]) {
+              ok = ok && mbar_wait(&pfull[t], (j - j0) & 1, abort_flag);
+              ok = __all_sync(0xFFFFFFFFu, ok);
+              if (!ok) break;
+              tc_fence_after();
+              if (lane == 0) {
+                for (int k = 0; k < groups; ++k)
+                  umma_f16_ts(tmem + Cfg::kColO + t * D, tmem + t * 128 + k * 8,
+                              sw128_nmajor_desc(vb + k * 2048, Cfg::kBlockBytes), idesc_o, (j > j0) | (k > 0));
+                if (j + 1 == end[t]) umma_commit(&ofull[t]);
+              }
+              __syncwarp();
+            }
+            if (j + 1 < end[t]) {
+              if (!loaded && !ready(ik)) break;
+              loaded = true;
+              scores(t, ik);
+            }
+          }
+          if (!ok) break;
+          release(iv);
+          if (loaded) release(ik);
+        }
+        if (lane == 0) {  // nothing still writes TMEM when it is freed
+          umma_commit(drain);
+          mbar_wait_bounded(drain, 0);
+        }
+        __syncwarp();
       }
-      if (lane == 0) {  // nothing still writes TMEM when it is freed
-        umma_commit(drain);
-        mbar_wait_bounded(drain, 0);
-      }
-      __syncwarp();
     }
     if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   }
