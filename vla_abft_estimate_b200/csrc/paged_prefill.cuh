@@ -144,6 +144,17 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint6
       : "memory");
 }
 
+// One lane of a converged warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -278,7 +289,6 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     int j0, j1;
     split_tiles(max(steps[0], steps[1]), p.splits, split, &j0, &j1);
     const int end[2] = {max(j0, min(j1, steps[0])), max(j0, min(j1, steps[1]))};
-    const int total = 2 * (j1 - j0);  // ring loads: K and V of each step
 
     if (warp < 8) {
       // ---------------------------------------------------------- softmax rows
@@ -487,53 +497,74 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           mbar_wait_bounded(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1);
       } else if (warp == 9) {
         // ---------------------------------------------------------- MMA issuer
+        // Control values through a shuffle and one elected lane: the compiler
+        // then keeps descriptors in uniform registers. (With values it could
+        // not prove uniform each MMA cost 130 clocks to issue, twice its run
+        // time.)
         constexpr uint32_t fmt = F16 ? 0u : 1u;
         constexpr uint32_t idesc_s = umma_idesc(kPreRows, kPreKeys, fmt);
         constexpr uint32_t idesc_o = umma_idesc(kPreRows, D, fmt) | kIdescBNMajor;
-        const uint32_t ring = smem_u32(smem + Cfg::kOffRing);
+        const int first_j = __shfl_sync(0xFFFFFFFFu, j0, 0), last_j = __shfl_sync(0xFFFFFFFFu, j1, 0);
+        const int stop[2] = {__shfl_sync(0xFFFFFFFFu, end[0], 0), __shfl_sync(0xFFFFFFFFu, end[1], 0)};
+        const int length = __shfl_sync(0xFFFFFFFFu, len, 0);
+        const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+        const uint32_t q_base = __shfl_sync(0xFFFFFFFFu, smem_u32(smem), 0);
+        const uint64_t desc_q = sw128_kmajor_desc(q_base), desc_k = sw128_kmajor_desc(q_base + Cfg::kOffRing);
+        const uint64_t desc_v = sw128_nmajor_desc(q_base + Cfg::kOffRing, Cfg::kBlockBytes);
+        const int loads = 2 * (last_j - first_j);
         bool ok = true;
-        auto ready = [&](int it) {
-          ok = ok && mbar_wait(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1, abort_flag);
-          ok = __all_sync(0xFFFFFFFFu, ok);
+        // Ring positions of the next K and V tile: slot and phase.
+        int slot = 0, phase = 0;
+        auto ready = [&](int at, int ph) {
+          ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&full[at], ph, abort_flag));
           tc_fence_after();
           return ok;
         };
-        auto scores = [&](int t, int it) {
-          if (lane == 0) {
-            const uint32_t a = smem_u32(smem + t * Cfg::kTileBytes), b = ring + (it % Cfg::kSlots) * Cfg::kTileBytes;
-  #pragma unroll
+        auto scores = [&](int t, int at) {
+          if (elect_one()) {
+            const uint64_t dq = desc_q + t * (Cfg::kTileBytes >> 4), dk = desc_k + at * (Cfg::kTileBytes >> 4);
+#pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint32_t off = (k / 4) * Cfg::kBlockBytes + (k % 4) * 32;
-              umma_bf16_ss(tmem + t * 128, sw128_kmajor_desc(a + off), sw128_kmajor_desc(b + off), idesc_s, k > 0);
+              const int off = ((k / 4) * Cfg::kBlockBytes + (k % 4) * 32) >> 4;
+              umma_bf16_ss(tm + t * 128, dq + off, dk + off, idesc_s, k > 0);
             }
             umma_commit(&sfull[t]);
           }
           __syncwarp();
         };
-        auto release = [&](int it) {  // the slot is loaded again: once the MMAs so far have read it
-          if (lane == 0 && it + Cfg::kSlots < total) umma_commit(&empty[it % Cfg::kSlots]);
+        auto release = [&](int it, int at) {  // the slot is loaded again: once the MMAs so far have read it
+          if (it + Cfg::kSlots < loads && elect_one()) umma_commit(&empty[at]);
           __syncwarp();
         };
+        auto step_ring = [&]() {
+          if (++slot == Cfg::kSlots) {
+            slot = 0;
+            phase ^= 1;
+          }
+        };
         for (int t = 0; t < 2; ++t)
-          if (end[t] > j0) ok = ok && mbar_wait(&qfull[t], 0, abort_flag);
+          if (stop[t] > first_j) ok = ok && mbar_wait(&qfull[t], 0, abort_flag);
         ok = __all_sync(0xFFFFFFFFu, ok);
-        if (ok && j0 < j1 && ready(0)) {
+        if (ok && first_j < last_j && ready(0, 0)) {
+#pragma unroll
           for (int t = 0; t < 2; ++t)
-            if (end[t] > j0) scores(t, 0);
-          release(0);
+            if (stop[t] > first_j) scores(t, 0);
+          release(0, 0);
+          step_ring();
         }
-        for (int j = j0; j < j1 && ok; ++j) {
-          const int iv = 2 * (j - j0) + 1, ik = iv + 1;
-          if (!ready(iv)) break;
-          const uint32_t vb = ring + (iv % Cfg::kSlots) * Cfg::kTileBytes;
+        for (int j = first_j; j < last_j && ok; ++j) {
+          const int iv = 2 * (j - first_j) + 1;
+          const int vs = slot;
+          if (!ready(vs, phase)) break;
+          step_ring();
           // Weights of slots behind the length are 0, but the slots may hold
           // anything (a page's last owner, NaN): only whole groups of 16 keys
           // that the sequence reaches are multiplied, the rest of the last
           // group is cleared.
-          const int valid = min(kPreKeys, len - j * kPreKeys);
+          const int valid = min(kPreKeys, length - j * kPreKeys);
           const int groups = (valid + 15) / 16;
           if (valid & 15) {
-            uint8_t* v = smem + Cfg::kOffRing + (iv % Cfg::kSlots) * Cfg::kTileBytes;
+            uint8_t* v = smem + Cfg::kOffRing + vs * Cfg::kTileBytes;
             for (int i = valid * (D / 8) + lane; i < groups * 16 * (D / 8); i += 32) {
               const int row = i / (D / 8), c = i % (D / 8);  // every piece of the row: its order does not matter
               *reinterpret_cast<uint4*>(v + (c >> 3) * Cfg::kBlockBytes + row * 128 + ((c & 7) << 4)) =
@@ -543,35 +574,44 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             __syncwarp();
           }
           bool loaded = false;
+#pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (j < end[t]) {
-              ok = ok && mbar_wait(&pfull[t], (j - j0) & 1, abort_flag);
-              ok = __all_sync(0xFFFFFFFFu, ok);
-              if (!ok) break;
-              tc_fence_after();
-              if (lane == 0) {
-                for (int k = 0; k < groups; ++k)
-                  umma_f16_ts(tmem + Cfg::kColO + t * D, tmem + t * 128 + k * 8,
-                              sw128_nmajor_desc(vb + k * 2048, Cfg::kBlockBytes), idesc_o, (j > j0) | (k > 0));
-                if (j + 1 == end[t]) umma_commit(&ofull[t]);
+            if (j < stop[t] && ok) {
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(&pfull[t], (j - first_j) & 1, abort_flag));
+              if (ok) {
+                tc_fence_after();
+                if (elect_one()) {
+                  const uint64_t dv = desc_v + vs * (Cfg::kTileBytes >> 4);
+                  const uint32_t d = tm + Cfg::kColO + t * D, a = tm + t * 128;
+                  umma_f16_ts(d, a, dv, idesc_o, j > first_j);
+                  if (groups == kPreKeys / 16) {
+#pragma unroll
+                    for (int k = 1; k < kPreKeys / 16; ++k) umma_f16_ts(d, a + k * 8, dv + k * (2048 >> 4), idesc_o, 1);
+                  } else {
+                    for (int k = 1; k < groups; ++k) umma_f16_ts(d, a + k * 8, dv + k * (2048 >> 4), idesc_o, 1);
+                  }
+                  if (j + 1 == stop[t]) umma_commit(&ofull[t]);
+                }
+                __syncwarp();
               }
-              __syncwarp();
             }
-            if (j + 1 < end[t]) {
-              if (!loaded && !ready(ik)) break;
+            if (j + 1 < stop[t] && ok) {
+              if (!loaded) ready(slot, phase);
               loaded = true;
-              scores(t, ik);
+              if (ok) scores(t, slot);
             }
           }
           if (!ok) break;
-          release(iv);
-          if (loaded) release(ik);
+          release(iv, vs);
+          if (loaded) {
+            release(iv + 1, slot);
+            step_ring();
+          }
         }
-        if (lane == 0) {  // nothing still writes TMEM when it is freed
-          umma_commit(drain);
-          mbar_wait_bounded(drain, 0);
-        }
+        // Nothing still writes TMEM when it is freed.
+        if (elect_one()) umma_commit(drain);
         __syncwarp();
+        mbar_wait_bounded(drain, 0);
       }
     }
     if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
