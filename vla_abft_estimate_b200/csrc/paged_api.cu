@@ -225,43 +225,58 @@ EncodeTiledFn tile_encoder() {
   return fn;
 }
 
-// Map of a page pool: [page][64-column block][head and slot][64 columns];
-// a box is one page's slots of one head and column block, 128-byte swizzled.
+// Map of a page pool: [page][group of 8 slots of a head][64-column block][slot
+// of the group][64 columns]; a box is one page's slots of one head, whole rows,
+// 128-byte swizzled.
 int page_map(CUtensorMap* m, const abft_paged_kv& c, const void* pages, int64_t stride) {
   EncodeTiledFn enc = tile_encoder();
   if (enc == nullptr) return ABFT_ERR_DRIVER;
   const int64_t dense = static_cast<int64_t>(c.kv_heads) * c.page_size * c.head_dim;
   if (c.num_pages <= 1) stride = dense;
-  cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(c.kv_heads) * c.page_size, static_cast<cuuint64_t>(c.head_dim / 64),
-                        static_cast<cuuint64_t>(c.num_pages)};
-  cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.head_dim) * 2, 128, static_cast<cuuint64_t>(stride) * 2};
-  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(c.page_size), 1, 1};
-  cuuint32_t es[4] = {1, 1, 1, 1};
+  const cuuint64_t row = static_cast<cuuint64_t>(c.head_dim) * 2;
+  cuuint64_t dims[5] = {64, 8, static_cast<cuuint64_t>(c.head_dim / 64),
+                        static_cast<cuuint64_t>(c.kv_heads) * c.page_size / 8, static_cast<cuuint64_t>(c.num_pages)};
+  cuuint64_t strides[4] = {row, 128, 8 * row, static_cast<cuuint64_t>(stride) * 2};
+  cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(c.head_dim / 64), static_cast<cuuint32_t>(c.page_size / 8), 1};
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
   const CUtensorMapDataType type =
       c.dtype == ABFT_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUresult r = enc(m, type, 4, const_cast<void*>(pages), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUresult r = enc(m, type, 5, const_cast<void*>(pages), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? ABFT_OK : ABFT_ERR_ALIGNMENT;
 }
 
-int64_t prefill_blocks(const abft_paged_attn_args* a) {
-  const int tile_tokens = kPreRows / (a->heads / a->kv.kv_heads);
-  return a->tokens / (2 * tile_tokens) + a->kv.batch;
-}
+// How a prefill call is cut: items of one or two tiles of query rows and one
+// kv head, their keys in pieces of `piece` steps.
+struct PrefillPlan {
+  int tile_tokens, block_tokens, splits, piece;
+  int64_t items;  // blocks of the grid
+};
 
-// Pieces a block's keys are cut into: while the blocks alone would leave SMs
-// idle, as many as fill them about twice, of four steps at least.
-int prefill_splits(const abft_paged_attn_args* a, int sms) {
+PrefillPlan prefill_plan(const abft_paged_attn_args* a, int sms) {
+  PrefillPlan r;
+  r.tile_tokens = kPreRows / (a->heads / a->kv.kv_heads);
+  // Two tiles an item keep the tensor core at work on one while the other's
+  // rows are exponentiated; a call that has an SM for each tile takes one.
+  r.block_tokens = 2 * r.tile_tokens;
+  const auto blocks = [&](int per) { return (a->tokens / per + a->kv.batch) * a->kv.kv_heads; };
+  if (blocks(r.tile_tokens) <= sms) r.block_tokens = r.tile_tokens;
+  const int64_t base = blocks(r.block_tokens);
   const int64_t steps = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kPreKeys - 1) / kPreKeys;
+  // Pieces: while the items alone would leave SMs idle, as many as fill them
+  // twice, of four steps at least.
   int64_t n = a->num_splits;
   if (n == 0) {
-    n = 2 * sms / (prefill_blocks(a) * a->kv.kv_heads);
+    n = 2 * sms / base;
     if (n > steps / 4) n = steps / 4;
   }
   if (n > steps) n = steps;
-  if (n > 65535) n = 65535;
-  return static_cast<int>(n < 1 ? 1 : n);
+  if (n < 1) n = 1;
+  r.piece = static_cast<int>((steps + n - 1) / n);
+  r.splits = static_cast<int>((steps + r.piece - 1) / r.piece);
+  r.items = base * r.splits;
+  return r;
 }
 
 size_t prefill_bytes(const abft_paged_attn_args* a, int splits) {
@@ -272,12 +287,12 @@ size_t prefill_bytes(const abft_paged_attn_args* a, int splits) {
 
 template <int D, bool F16>
 int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
-                   const PrefillParams& p, cudaStream_t s) {
+                   const PrefillParams& p, int64_t items, cudaStream_t s) {
   using Cfg = PrefillCfg<D>;
   int rc = raise_smem(dev, slot, paged_prefill_kernel<D, F16>, Cfg::kSmemBytes);
   if (rc != ABFT_OK) return rc;
-  rc = launch(paged_prefill_kernel<D, F16>, dim3(static_cast<unsigned>(p.blocks) * p.kv.kv_heads, p.splits),
-              dim3(kPreThreads), Cfg::kSmemBytes, s, tm_k, tm_v, p);
+  rc = launch(paged_prefill_kernel<D, F16>, dim3(static_cast<unsigned>(items)), dim3(kPreThreads), Cfg::kSmemBytes, s,
+              tm_k, tm_v, p);
   if (rc != ABFT_OK || p.splits == 1) return rc;
   PrefillJoinParams j;
   j.kv = p.kv;
@@ -288,7 +303,8 @@ int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUten
   j.tokens = p.tokens;
   j.heads = a->heads;
   j.splits = p.splits;
-  j.tile_tokens = p.tile_tokens;
+  j.piece = p.piece;
+  j.block_tokens = p.block_tokens;
   j.part_o = p.part_o;
   j.part_ml = p.part_ml;
   return launch(paged_prefill_join_kernel<D, F16>, dim3(static_cast<unsigned>(p.tokens) * a->heads), dim3(128), 0, s, j);
@@ -383,7 +399,7 @@ size_t abft_paged_prefill_workspace_bytes(const abft_paged_attn_args* a) {
   if (attn_check(a, false) != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return 0;
   int dev = 0, sms = a->num_sms;
   if (sms == 0 && paged_device(&dev, &sms) != ABFT_OK) sms = 148;
-  return prefill_bytes(a, prefill_splits(a, sms));
+  return prefill_bytes(a, prefill_plan(a, sms).splits);
 }
 
 int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
@@ -400,9 +416,12 @@ int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
   p.cu = a->cu_seqlens;
   p.tokens = static_cast<int32_t>(a->tokens);
   p.group = a->heads / a->kv.kv_heads;
-  p.tile_tokens = kPreRows / p.group;
-  p.splits = prefill_splits(a, sms);
-  p.blocks = static_cast<int32_t>(prefill_blocks(a));
+  const PrefillPlan plan = prefill_plan(a, sms);
+  if (plan.items >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
+  p.tile_tokens = plan.tile_tokens;
+  p.block_tokens = plan.block_tokens;
+  p.splits = plan.splits;
+  p.piece = plan.piece;
   const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
   p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
   p.negate = a->scale < 0.f;
@@ -419,10 +438,10 @@ int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
   if (a->kv.head_dim == 128)
-    return f16 ? launch_prefill<128, true>(dev, 11, a, tm_k, tm_v, p, s)
-               : launch_prefill<128, false>(dev, 10, a, tm_k, tm_v, p, s);
-  return f16 ? launch_prefill<64, true>(dev, 9, a, tm_k, tm_v, p, s)
-             : launch_prefill<64, false>(dev, 8, a, tm_k, tm_v, p, s);
+    return f16 ? launch_prefill<128, true>(dev, 11, a, tm_k, tm_v, p, plan.items, s)
+               : launch_prefill<128, false>(dev, 10, a, tm_k, tm_v, p, plan.items, s);
+  return f16 ? launch_prefill<64, true>(dev, 9, a, tm_k, tm_v, p, plan.items, s)
+             : launch_prefill<64, false>(dev, 8, a, tm_k, tm_v, p, plan.items, s);
 }
 
 }  // extern "C"

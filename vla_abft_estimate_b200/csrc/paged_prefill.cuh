@@ -41,21 +41,25 @@ constexpr int kPreRows = 128;   // query rows of a tile
 constexpr int kPreKeys = 128;   // keys of a step
 constexpr int kPreThreads = 384;
 // Registers: 384 threads launch with at most 168 each (64,512 in all); the
-// rows' warps hold a whole row of S and take 216, the others keep 72:
-// 256 * 216 + 128 * 72 = 64,512.
-constexpr int kPreRegsRows = 216, kPreRegsOther = 72;
+// rows' warps hold a whole row of S and take 200, the others keep 104:
+// 256 * 200 + 128 * 104 = 64,512. (The issuer's loop in local memory for want
+// of registers doubles the kernel's time.)
+constexpr int kPreRegsRows = 200, kPreRegsOther = 104;
 
 template <int D>
 struct PrefillCfg {
-  static constexpr int kHalves = D / 64;                     // 128-byte wide column blocks of a row
   static constexpr int kTileBytes = kPreKeys * D * 2;        // a K, V or Q tile
-  static constexpr int kBlockBytes = kPreKeys * 128;         // one column block of it
+  static constexpr int kBlockBytes = kPreRows * 128;         // one 64-column block of a Q tile
+  static constexpr int kGroupBytes = 8 * D * 2;              // 8 keys of a ring tile
   static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kOffRing = 2 * kTileBytes;            // after the two Q tiles
   static constexpr int kOffBar = kOffRing + kSlots * kTileBytes;
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 1;  // full, empty, qfull, sfull, pfull, ofull, drain
+  // full, empty, qfull, sfull, pfull, ofull, item full and empty, work, drain
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 4 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
-  static constexpr int kSmemBytes = kOffMisc + 64 + 1024;
+  static constexpr int kOffItems = kOffMisc + 16;  // two items and the launch-control answer
+  static constexpr int kSmemBytes = kOffItems + 2 * 48 + 16 + 1024;
+  static_assert(kBars % 2 == 0, "the answer is 16-byte aligned");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
   static_assert(kSmemBytes > 232448 / 2, "one CTA per SM: each takes all of TMEM");
   // TMEM columns: S of both tiles (P over its first half), then O of both.
@@ -72,8 +76,9 @@ struct PrefillParams {
   int32_t tokens;          // rows of q
   int32_t group;           // query heads per kv head
   int32_t tile_tokens;     // tokens of one tile: 128 / group
-  int32_t blocks;          // CTAs per kv head and split: tokens / (2 tile_tokens) + batch at most
-  int32_t splits;
+  int32_t block_tokens;    // tokens of an item: one tile's or two's
+  int32_t splits;          // pieces of an item's keys at most: blocks of the grid for it
+  int32_t piece;           // steps of a piece
   float scale_log2;        // |scale| * log2(e), never 0
   int32_t negate;          // scale < 0
   uint32_t group_inv;      // ceil(2^16 / group): row_token()
@@ -135,12 +140,12 @@ __device__ __forceinline__ bool find_block(const int32_t* cu, int batch, int tok
   return false;
 }
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint64_t* bar, int32_t x, int32_t y, int32_t z,
-                                            int32_t w) {
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* map, uint64_t* bar, int32_t x, int32_t y, int32_t z,
+                                            int32_t w, int32_t v) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
-          "r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
       : "memory");
 }
 
@@ -170,9 +175,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
 }
+// The largest of three, NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -187,15 +193,18 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       : "memory");
 }
 
-// Descriptor of a [keys x D] tile as N-major B operand (its keys are the
-// MMA's K dimension): 128-byte swizzled rows, 64 columns per block, `block`
-// bytes from one column block to the next (leading offset), 1024 from 8 keys
-// to the next 8 (stride offset).
-__device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t saddr, uint32_t block) {
+// Descriptors of a ring tile: groups of 8 keys, each group D / 64 blocks of
+// 8 x 128 bytes (128-byte swizzle), one per 64 elements of the head dimension:
+// the order in which one TMA box brings a whole page. As K-major operand (Q
+// K^T) a group follows the last after D * 16 bytes, and a block of 64 elements
+// starts 1024 bytes after the last one; as N-major operand (P V, the keys are
+// the MMA's K dimension) the leading offset is the blocks' distance and the
+// stride offset the groups'.
+__device__ __forceinline__ uint64_t ring_desc(uint32_t saddr, uint32_t leading, uint32_t group) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(block >> 4) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(leading >> 4) << 16;
+  d |= static_cast<uint64_t>(group >> 4) << 32;
   d |= static_cast<uint64_t>(1u) << 46;
   d |= static_cast<uint64_t>(2u) << 61;
   return d;
@@ -207,6 +216,45 @@ __device__ __forceinline__ void mbar_wait_bounded(uint64_t* bar, uint32_t parity
   const uint64_t t0 = global_timer_ns();
   while (!mbar_try_wait(bar, parity))
     if (global_timer_ns() - t0 > kWaitTimeoutNs) return;
+}
+
+// One work item.
+struct __align__(16) PrefillItem {
+  int32_t valid;    // 0: no more work
+  int32_t hk;       // kv head
+  int32_t split;    // piece
+  int32_t seq, len; // sequence, its keys
+  int32_t row0, n;  // its first packed row and its rows
+  int32_t tok0;     // first token of the item within them
+  int32_t j0, j1;   // steps of the piece
+  int32_t end0, end1;  // steps of the tiles within it (j0: none)
+};
+static_assert(sizeof(PrefillItem) == 48, "items' place in shared memory");
+
+// Asks for a block of the grid that has not started; the answer (16 bytes)
+// completes a phase of `bar`.
+__device__ __forceinline__ void ask_for_work(void* answer, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The block taken over, or -1 when all have started.
+__device__ __forceinline__ int work_answer(const void* answer) {
+  uint32_t x = 0, ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      ".reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}\n"
+      : "=r"(x), "=r"(ok)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok ? static_cast<int>(x) : -1;
 }
 
 template <int D, bool F16>
@@ -222,10 +270,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   uint64_t* sfull = qfull + 2;
   uint64_t* pfull = sfull + 2;
   uint64_t* ofull = pfull + 2;
-  uint64_t* drain = ofull + 2;
+  uint64_t* item_full = ofull + 2;
+  uint64_t* item_empty = item_full + 2;
+  uint64_t* work = item_empty + 2;
+  uint64_t* drain = work + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* where = reinterpret_cast<volatile int*>(tmem_slot + 2);  // sequence (-1: none), block
+  PrefillItem* items = reinterpret_cast<PrefillItem*>(smem + Cfg::kOffItems);
+  void* answer = items + 2;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedView& kv = p.kv;
@@ -239,7 +291,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       mbar_init(&sfull[t], 1);
       mbar_init(&pfull[t], kPreRows);
       mbar_init(&ofull[t], 1);
+      mbar_init(&item_full[t], 1);
+      mbar_init(&item_empty[t], 10);  // a lane of each row warp, the loader's and the issuer's
     }
+    mbar_init(work, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -250,82 +305,90 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish();
   }
-  griddep_wait();
-  griddep_launch();
-  const int hk = blockIdx.x % kv.kv_heads;
-  const int index = blockIdx.x / kv.kv_heads;
-  const int split = blockIdx.y;
-  if (warp == 0) {
-    int seq = -1, block = 0;
-    find_block(p.cu, kv.batch, p.tokens, 2 * p.tile_tokens, index, lane, &seq, &block);
-    if (lane == 0) {
-      where[0] = seq;
-      where[1] = block;
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int seq = where[0], block = where[1];
+  griddep_wait();
 
-  if (seq >= 0) {
-    int row0, row_end;
-    packed_range(p.cu, seq, p.tokens, &row0, &row_end);
-    const int n = row_end - row0;
-    bool bad_len;
-    const int len = paged_clamp_len(kv.seq_lens[seq], kv.max_pages, kv.page_shift, &bad_len);
-    if ((bad_len || len < n) && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
-    // First token and steps (of 128 keys) of each tile; a tile behind the
-    // chunk's end has none.
-    const int tok0 = block * 2 * p.tile_tokens;
-    int steps[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int first = tok0 + t * p.tile_tokens;
-      const int last = min(first + p.tile_tokens, n) - 1;
-      steps[t] = last >= first ? (visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys : 0;
+  // The i-th item of this CTA, copied out of its slot.
+  auto get_item = [&](int i, PrefillItem* x) {
+    const bool got = __all_sync(0xFFFFFFFFu, mbar_wait(&item_full[i & 1], (i >> 1) & 1, abort_flag));
+    if (!got) {
+      x->valid = 0;
+      return false;
     }
-    int j0, j1;
-    split_tiles(max(steps[0], steps[1]), p.splits, split, &j0, &j1);
-    const int end[2] = {max(j0, min(j1, steps[0])), max(j0, min(j1, steps[1]))};
+    *x = items[i & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[i & 1]);
+    return x->valid != 0;
+  };
 
-    if (warp < 8) {
-      // ---------------------------------------------------------- softmax rows
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsRows));
-      const int t = warp >> 2;
-      const int r = threadIdx.x & 127;
-      const int first = tok0 + t * p.tile_tokens;
-      const int here = max(0, min(p.tile_tokens, n - first)) * p.group;  // rows in use
-      // Q tile into shared memory, in the swizzled layout of a TMA box.
-      if (end[t] > j0) {
-        const uint32_t dst = smem_u32(smem + t * Cfg::kTileBytes);
-        constexpr int kCpr = D / 8;
-        const int c = r % kCpr;
-        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (row0 + first) * p.qt + hk * p.group * p.qh + c * 8;
-#pragma unroll
-        for (int i = 0; i < kCpr; ++i) {
-          const int row = i * (kPreRows / kCpr) + r / kCpr;
-          const bool in = row < here;
-          const int tok = in ? row_token(row, p.group_inv) : 0, g = in ? row - tok * p.group : 0;
-          cp_async16(dst + (c >> 3) * Cfg::kBlockBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
-                     src + tok * p.qt + g * p.qh, in ? 16u : 0u);
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        fence_proxy_async_smem();
-        mbar_arrive(&qfull[t]);
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsRows));
+    const int t = warp >> 2;
+    // The thread's row, hidden from the compiler: what follows from it outside
+    // the steps is computed where it is used instead of being kept in
+    // registers across them.
+    auto row_of_thread = []() {
+      int r = threadIdx.x & 127;
+      asm volatile("" : "+r"(r));
+      return r;
+    };
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t ts = lanes + t * 128, to = lanes + Cfg::kColO + t * D;
+    // Items stay in their slots while the rows work on them and are read
+    // there: a row of S leaves few registers.
+    auto wait_item = [&](int i) {
+      return __all_sync(0xFFFFFFFFu, mbar_wait(&item_full[i & 1], (i >> 1) & 1, abort_flag)) &&
+             items[i & 1].valid != 0;
+    };
+    auto steps_end = [&](const PrefillItem& x) { return t == 0 ? x.end0 : x.end1; };
+    // Q tile into shared memory, in the swizzled layout of a TMA box.
+    auto load_q = [&](const PrefillItem& x) {
+      int r = row_of_thread();
+      const int first = x.tok0 + t * p.tile_tokens;
+      const int here = max(0, min(p.tile_tokens, x.n - first)) * p.group;
+      const uint32_t dst = smem_u32(smem + t * Cfg::kTileBytes);
+      constexpr int kCpr = D / 8;
+      const int c = r % kCpr;
+      const uint16_t* src =
+          static_cast<const uint16_t*>(p.q) + (x.row0 + first) * p.qt + x.hk * p.group * p.qh + c * 8;
+#pragma unroll 4
+      for (int i = 0; i < kCpr; ++i) {
+        const int row = i * (kPreRows / kCpr) + r / kCpr;
+        const bool in = row < here;
+        const int qtok = in ? row_token(row, p.group_inv) : 0, g = in ? row - qtok * p.group : 0;
+        cp_async16(dst + (c >> 3) * Cfg::kBlockBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                   src + qtok * p.qt + g * p.qh, in ? 16u : 0u);
       }
-      const int tok = row_token(r, p.group_inv);
-      const bool live = r < here;
-      const int vis = live ? visible_keys(len, n, first + tok) : 0;
-      const int vis_min = visible_keys(len, n, first);  // of the tile's first token
-      const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-      const uint32_t ts = lanes + t * 128, to = lanes + Cfg::kColO + t * D;
-      float m = -INFINITY, l = 0.f;  // m: maximum that P refers to (raw scores)
-      bool ok = true;
-      for (int j = j0; j < end[t]; ++j) {
-        if (!mbar_wait(&sfull[t], (j - j0) & 1, abort_flag)) {
+      cp_async_commit();
+    };
+    auto send_q = [&]() {
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      mbar_arrive(&qfull[t]);
+    };
+    bool ok = wait_item(0);
+    int count = 0, used = 0;  // steps and items of this tile so far
+    if (ok && steps_end(items[0]) > items[0].j0) {
+      load_q(items[0]);
+      send_q();
+    }
+    for (int i = 0; ok; ++i) {
+      const PrefillItem& x = items[i & 1];
+      const int end = steps_end(x), j0 = x.j0;
+      int vis, vis_min;  // keys seen by the row (0: not in use) and by the tile's first token
+      {
+        const int first = x.tok0 + t * p.tile_tokens, r = row_of_thread();
+        const bool live = r < max(0, min(p.tile_tokens, x.n - first)) * p.group;
+        vis = live ? visible_keys(x.len, x.n, first + row_token(r, p.group_inv)) : 0;
+        vis_min = visible_keys(x.len, x.n, first);
+      }
+      float m = -INFINITY, l = 0.f;                         // m: maximum that P refers to (raw scores)
+      for (int j = j0; j < end; ++j, ++count) {
+        if (!mbar_wait(&sfull[t], count & 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -338,42 +401,44 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[c][i] ^= 0x80000000u;
+            for (int k = 0; k < 32; ++k) s[c][k] ^= 0x80000000u;
         }
         if (vis_min < (j + 1) * kPreKeys) {
           const int lim = vis - j * kPreKeys;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= lim) s[c][i] = 0xFF800000u;  // -inf
+            for (int k = 0; k < 32; ++k)
+              if (c * 32 + k >= lim) s[c][k] = 0xFF800000u;  // -inf
         }
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           mx[c] = max3(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]), __uint_as_float(s[c][2]));
 #pragma unroll
-          for (int i = 3; i < 31; i += 2) mx[c] = max3(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-          mx[c] = fmaxf(mx[c], __uint_as_float(s[c][31]));
+          for (int k = 3; k < 31; k += 2) mx[c] = max3(mx[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+          mx[c] = max3(mx[c], __uint_as_float(s[c][31]), m);
         }
-        const float mn = fmaxf(m, max3(mx[0], mx[1], fmaxf(mx[2], mx[3])));
-        const bool raise = (mn - m) * p.scale_log2 > 8.f;  // also from m = -inf; false for -inf, -inf
-        if (j == j0) {
-          m = mn;
-        } else if (__any_sync(0xFFFFFFFFu, raise)) {
+        float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);  // NaN if a score is
+        // Also true from m = -inf and for NaN, but not while all is -inf.
+        const bool raise = !((mn - m) * p.scale_log2 <= 8.f) && mn != -INFINITY;
+        if (j == j0 || __any_sync(0xFFFFFFFFu, raise)) {
+          if (mn == INFINITY) mn = __int_as_float(0x7FC00000);  // inf - inf: the row is NaN
           const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * p.scale_log2);
           m = mn;
-          l *= f;
+          if (j > j0) {
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(to + c * 32, o);
+              tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(to + c * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st_32x32b_x32(to + c * 32, o);
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st_32x32b_x32(to + c * 32, o);
+            }
+            tmem_st_wait();
           }
-          tmem_st_wait();
         }
         const float shift = m == -INFINITY ? 0.f : -m * p.scale_log2;
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
@@ -384,13 +449,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 x = fma2(make_float2(__uint_as_float(s[2 * h + c][i]), __uint_as_float(s[2 * h + c][i + 1])),
+            for (int k = 0; k < 32; k += 2) {
+              float2 y = fma2(make_float2(__uint_as_float(s[2 * h + c][k]), __uint_as_float(s[2 * h + c][k + 1])),
                               scale2, shift2);
-              x.x = exp2_approx(x.x);
-              x.y = exp2_approx(x.y);
-              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
-              pk[c * 16 + (i >> 1)] = pack2<F16>(x.x, x.y);
+              y.x = exp2_approx(y.x);
+              y.y = exp2_approx(y.y);
+              sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], y);
+              pk[c * 16 + (k >> 1)] = pack2<F16>(y.x, y.y);
             }
           tmem_st_32x32b_x32(ts + h * 32, pk);
         }
@@ -399,161 +464,175 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         tc_fence_before();
         mbar_arrive(&pfull[t]);
       }
-      if (ok && end[t] > j0) {
-        ok = mbar_wait(&ofull[t], 0, abort_flag);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      // The next item's Q comes while the last product runs (all of this
+      // item's Q K^T are done: the rows have seen the last scores).
+      const bool next = wait_item(i + 1);
+      const bool more = next && steps_end(items[(i + 1) & 1]) > items[(i + 1) & 1].j0;
+      if (more) load_q(items[(i + 1) & 1]);
+      const bool any = end > j0;
+      if (any) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[t], used & 1, abort_flag));
         tc_fence_after();
+        ++used;
       }
-      if (ok && (p.splits == 1 || j0 < j1)) {
-        const int head = hk * p.group + (r - tok * p.group);
-        const int64_t row = row0 + first + tok;
-        const bool any = end[t] > j0;
-        if (p.splits == 1) {
-          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-          uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
+      if (more) send_q();
+      if (!ok) break;
+      const int first = x.tok0 + t * p.tile_tokens, r = row_of_thread();
+      const int tok = row_token(r, p.group_inv);
+      const bool live = r < max(0, min(p.tile_tokens, x.n - first)) * p.group;
+      const int head = x.hk * p.group + (r - tok * p.group);
+      const int64_t row = x.row0 + first + tok;
+      if (any) {
+        // The row's sums, in 32-column pieces.
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const int64_t at = (row * (kv.kv_heads * p.group) + head) * p.splits + x.split;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
+        float* part = p.part_o + at * D;
+        if (p.splits > 1 && live) p.part_ml[at] = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(to + c, o);
+          tmem_ld_wait();
+          if (!live) continue;
+          if (p.splits > 1) {
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            if (any) {
-              tmem_ld_32x32b_x32(to + c * 32, o);
-              tmem_ld_wait();
-            }
-            if (live) {
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(part + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          } else {
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) {
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (any && l != 0.f) {
-                  x.x = pack2<F16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-                  x.y = pack2<F16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                  x.z = pack2<F16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-                  x.w = pack2<F16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-                }
-                *reinterpret_cast<uint4*>(dst + c * 32 + i) = x;
-              }
-            }
-          }
-        } else {
-          const int64_t at = (row * (kv.kv_heads * p.group) + head) * p.splits + split;
-          if (live) p.part_ml[at] = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
-          if (any) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(to + c * 32, o);
-              tmem_ld_wait();
-              if (live) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                  *reinterpret_cast<uint4*>(p.part_o + at * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-              }
+            for (int k = 0; k < 32; k += 8) {
+              uint4 y;
+              y.x = pack2<F16>(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+              y.y = pack2<F16>(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+              y.z = pack2<F16>(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
+              y.w = pack2<F16>(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + c + k) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : y;
             }
           }
         }
+      } else if (live && p.splits == 1) {
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
+        for (int k = 0; k < D; k += 8) *reinterpret_cast<uint4*>(dst + k) = make_uint4(0u, 0u, 0u, 0u);
+      } else if (live) {
+        p.part_ml[(row * (kv.kv_heads * p.group) + head) * p.splits + x.split] = make_float2(-INFINITY, 0.f);
       }
-      tc_fence_before();
-    } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsOther));
-      if (warp == 8) {
-        // ---------------------------------------------------------- page loads
-        const int32_t* table = kv.page_table + seq * kv.table_stride;
-        const int page = 1 << kv.page_shift;
-        const int piece = lane / Cfg::kHalves, half = lane % Cfg::kHalves;  // page of the step, column block
-        const int per_step = kPreKeys >> kv.page_shift;
-        const int held = (len + page - 1) >> kv.page_shift;  // pages of the sequence
-        auto entry = [&](int j) {
-          const int at = j * per_step + piece;
-          return piece < per_step && at < held ? table[at] : 0;
+      tc_fence_before();  // O is read before the next item's first P is announced
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[i & 1]);
+      ok = next;
+    }
+    tc_fence_before();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsOther));
+    if (warp == 8) {
+      // ---------------------------------------------------------- page loads
+      const int page = 1 << kv.page_shift;
+      const int per_step = kPreKeys >> kv.page_shift;
+      int issued = 0;  // tiles so far: slot and phase of the ring
+      PrefillItem x;
+      bool ok = true;
+      for (int i = 0; ok && get_item(i, &x); ++i) {
+        const int32_t* table = kv.page_table + x.seq * kv.table_stride;
+        const int held = (x.len + page - 1) >> kv.page_shift;  // pages of the sequence
+        auto entry = [&](int j) {  // a lane per page of the step
+          const int at = j * per_step + lane;
+          return lane < per_step && at < held ? table[at] : 0;
         };
-        int next = j0 < j1 ? entry(j0) : 0;
-        int issued = 0;
-        bool ok = true;
-        for (int j = j0; j < j1 && ok; ++j) {
+        int next = x.j0 < x.j1 ? entry(x.j0) : 0;
+        for (int j = x.j0; j < x.j1 && ok; ++j) {
           const int id = next;
-          if (j + 1 < j1) next = entry(j + 1);
+          if (j + 1 < x.j1) next = entry(j + 1);
           const int pieces = min(per_step, held - j * per_step);
-          const bool mine = piece < pieces;
-          if (mine && half == 0 && (id < 0 || id >= kv.num_pages) && kv.status != nullptr)
-            atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
-  #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int it = 2 * (j - j0) + x;
-            const int slot = it % Cfg::kSlots;
-            if (it >= Cfg::kSlots && !mbar_wait(&empty[slot], (it / Cfg::kSlots - 1) & 1, abort_flag)) ok = false;
+          const bool mine = lane < pieces;
+          if (mine && (id < 0 || id >= kv.num_pages) && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int slot = issued % Cfg::kSlots;
+            if (issued >= Cfg::kSlots && !mbar_wait(&empty[slot], (issued / Cfg::kSlots - 1) & 1, abort_flag)) ok = false;
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(pieces * page * D * 2));
             __syncwarp();
             if (mine) {
               // A bad id lies outside the map's page dimension and loads zeros.
-              const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes + half * Cfg::kBlockBytes) +
-                                   piece * page * 128;
-              tma_load_4d(dst, x == 0 ? &tm_k : &tm_v, &full[slot], 0, hk << kv.page_shift, half, id);
+              const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes) + lane * page * D * 2;
+              tma_load_5d(dst, k == 0 ? &tm_k : &tm_v, &full[slot], 0, 0, 0, x.hk << (kv.page_shift - 3), id);
             }
             ++issued;
           }
         }
-        // Copies in flight have landed before shared memory goes (all have, but
-        // after an abort).
-        for (int it = max(0, issued - Cfg::kSlots); it < issued; ++it)
-          mbar_wait_bounded(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1);
-      } else if (warp == 9) {
-        // ---------------------------------------------------------- MMA issuer
-        // Control values through a shuffle and one elected lane: the compiler
-        // then keeps descriptors in uniform registers. (With values it could
-        // not prove uniform each MMA cost 130 clocks to issue, twice its run
-        // time.)
-        constexpr uint32_t fmt = F16 ? 0u : 1u;
-        constexpr uint32_t idesc_s = umma_idesc(kPreRows, kPreKeys, fmt);
-        constexpr uint32_t idesc_o = umma_idesc(kPreRows, D, fmt) | kIdescBNMajor;
-        const int first_j = __shfl_sync(0xFFFFFFFFu, j0, 0), last_j = __shfl_sync(0xFFFFFFFFu, j1, 0);
-        const int stop[2] = {__shfl_sync(0xFFFFFFFFu, end[0], 0), __shfl_sync(0xFFFFFFFFu, end[1], 0)};
-        const int length = __shfl_sync(0xFFFFFFFFu, len, 0);
-        const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-        const uint32_t q_base = __shfl_sync(0xFFFFFFFFu, smem_u32(smem), 0);
-        const uint64_t desc_q = sw128_kmajor_desc(q_base), desc_k = sw128_kmajor_desc(q_base + Cfg::kOffRing);
-        const uint64_t desc_v = sw128_nmajor_desc(q_base + Cfg::kOffRing, Cfg::kBlockBytes);
-        const int loads = 2 * (last_j - first_j);
-        bool ok = true;
-        // Ring positions of the next K and V tile: slot and phase.
-        int slot = 0, phase = 0;
-        auto ready = [&](int at, int ph) {
-          ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&full[at], ph, abort_flag));
-          tc_fence_after();
-          return ok;
-        };
-        auto scores = [&](int t, int at) {
-          if (elect_one()) {
-            const uint64_t dq = desc_q + t * (Cfg::kTileBytes >> 4), dk = desc_k + at * (Cfg::kTileBytes >> 4);
+      }
+      // Copies in flight have landed before shared memory goes (all have, but
+      // after an abort).
+      for (int it = max(0, issued - Cfg::kSlots); it < issued; ++it)
+        mbar_wait_bounded(&full[it % Cfg::kSlots], (it / Cfg::kSlots) & 1);
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- MMA issuer
+      // Control values through a shuffle and one elected lane: the compiler
+      // then keeps descriptors in uniform registers. (With values it could
+      // not prove uniform each MMA cost 130 clocks to issue, twice its run
+      // time.)
+      constexpr uint32_t fmt = F16 ? 0u : 1u;
+      constexpr uint32_t idesc_s = umma_idesc(kPreRows, kPreKeys, fmt);
+      constexpr uint32_t idesc_o = umma_idesc(kPreRows, D, fmt) | kIdescBNMajor;
+      const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+      const uint32_t q_base = __shfl_sync(0xFFFFFFFFu, smem_u32(smem), 0);
+      const uint64_t desc_q = sw128_kmajor_desc(q_base);
+      const uint64_t desc_k = ring_desc(q_base + Cfg::kOffRing, 16, Cfg::kGroupBytes);
+      const uint64_t desc_v = ring_desc(q_base + Cfg::kOffRing, 1024, Cfg::kGroupBytes);
+      bool ok = true;
+      int slot = 0, phase = 0;     // of the next tile in the ring
+      int pcount[2] = {0, 0};      // steps of each tile so far
+      int qcount[2] = {0, 0};      // items of each tile so far
+      auto ready = [&](int at, int ph) {
+        ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&full[at], ph, abort_flag));
+        tc_fence_after();
+        return ok;
+      };
+      auto scores = [&](int t, int at) {
+        if (elect_one()) {
+          const uint64_t dq = desc_q + t * (Cfg::kTileBytes >> 4), dk = desc_k + at * (Cfg::kTileBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const int off = ((k / 4) * Cfg::kBlockBytes + (k % 4) * 32) >> 4;
-              umma_bf16_ss(tm + t * 128, dq + off, dk + off, idesc_s, k > 0);
-            }
-            umma_commit(&sfull[t]);
+          for (int k = 0; k < D / 16; ++k) {
+            umma_bf16_ss(tm + t * 128, dq + (((k / 4) * Cfg::kBlockBytes + (k % 4) * 32) >> 4),
+                         dk + (((k / 4) * 1024 + (k % 4) * 32) >> 4), idesc_s, k > 0);
           }
-          __syncwarp();
-        };
-        auto release = [&](int it, int at) {  // the slot is loaded again: once the MMAs so far have read it
-          if (it + Cfg::kSlots < loads && elect_one()) umma_commit(&empty[at]);
-          __syncwarp();
-        };
-        auto step_ring = [&]() {
-          if (++slot == Cfg::kSlots) {
-            slot = 0;
-            phase ^= 1;
-          }
-        };
-        for (int t = 0; t < 2; ++t)
-          if (stop[t] > first_j) ok = ok && mbar_wait(&qfull[t], 0, abort_flag);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (ok && first_j < last_j && ready(0, 0)) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (stop[t] > first_j) scores(t, 0);
-          release(0, 0);
-          step_ring();
+          umma_commit(&sfull[t]);
         }
+        __syncwarp();
+      };
+      auto release = [&](int at) {  // once the MMAs so far have read the slot
+        if (elect_one()) umma_commit(&empty[at]);
+        __syncwarp();
+      };
+      auto step_ring = [&]() {
+        if (++slot == Cfg::kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      PrefillItem x;
+      for (int i = 0; ok && get_item(i, &x); ++i) {
+        const int first_j = __shfl_sync(0xFFFFFFFFu, x.j0, 0), last_j = __shfl_sync(0xFFFFFFFFu, x.j1, 0);
+        const int stop[2] = {__shfl_sync(0xFFFFFFFFu, x.end0, 0), __shfl_sync(0xFFFFFFFFu, x.end1, 0)};
+        const int length = __shfl_sync(0xFFFFFFFFu, x.len, 0);
+        if (first_j >= last_j) continue;
+        if (!ready(slot, phase)) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (stop[t] > first_j && ok) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&qfull[t], qcount[t] & 1, abort_flag));
+            ++qcount[t];
+            tc_fence_after();
+            if (ok) scores(t, slot);
+          }
+        if (!ok) break;
+        release(slot);
+        step_ring();
         for (int j = first_j; j < last_j && ok; ++j) {
-          const int iv = 2 * (j - first_j) + 1;
           const int vs = slot;
           if (!ready(vs, phase)) break;
           step_ring();
@@ -565,10 +644,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           const int groups = (valid + 15) / 16;
           if (valid & 15) {
             uint8_t* v = smem + Cfg::kOffRing + vs * Cfg::kTileBytes;
-            for (int i = valid * (D / 8) + lane; i < groups * 16 * (D / 8); i += 32) {
-              const int row = i / (D / 8), c = i % (D / 8);  // every piece of the row: its order does not matter
-              *reinterpret_cast<uint4*>(v + (c >> 3) * Cfg::kBlockBytes + row * 128 + ((c & 7) << 4)) =
-                  make_uint4(0u, 0u, 0u, 0u);
+            for (int k = valid * (D / 8) + lane; k < groups * 16 * (D / 8); k += 32) {
+              const int row = k / (D / 8), c = k % (D / 8);  // every piece of the row: its order does not matter
+              *reinterpret_cast<uint4*>(v + (row >> 3) * Cfg::kGroupBytes + (c >> 3) * 1024 + (row & 7) * 128 +
+                                        ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -577,7 +656,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (j < stop[t] && ok) {
-              ok = __all_sync(0xFFFFFFFFu, mbar_wait(&pfull[t], (j - first_j) & 1, abort_flag));
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(&pfull[t], pcount[t] & 1, abort_flag));
+              ++pcount[t];
               if (ok) {
                 tc_fence_after();
                 if (elect_one()) {
@@ -586,9 +666,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                   umma_f16_ts(d, a, dv, idesc_o, j > first_j);
                   if (groups == kPreKeys / 16) {
 #pragma unroll
-                    for (int k = 1; k < kPreKeys / 16; ++k) umma_f16_ts(d, a + k * 8, dv + k * (2048 >> 4), idesc_o, 1);
+                    for (int k = 1; k < kPreKeys / 16; ++k)
+                      umma_f16_ts(d, a + k * 8, dv + k * (2 * Cfg::kGroupBytes >> 4), idesc_o, 1);
                   } else {
-                    for (int k = 1; k < groups; ++k) umma_f16_ts(d, a + k * 8, dv + k * (2048 >> 4), idesc_o, 1);
+                    for (int k = 1; k < groups; ++k)
+                      umma_f16_ts(d, a + k * 8, dv + k * (2 * Cfg::kGroupBytes >> 4), idesc_o, 1);
                   }
                   if (j + 1 == stop[t]) umma_commit(&ofull[t]);
                 }
@@ -602,20 +684,84 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             }
           }
           if (!ok) break;
-          release(iv, vs);
+          release(vs);
           if (loaded) {
-            release(iv + 1, slot);
+            release(slot);
             step_ring();
           }
         }
-        // Nothing still writes TMEM when it is freed.
-        if (elect_one()) umma_commit(drain);
+      }
+      // Nothing still writes TMEM when it is freed.
+      if (elect_one()) umma_commit(drain);
+      __syncwarp();
+      mbar_wait_bounded(drain, 0);
+    } else if (warp == 10) {
+      // ---------------------------------------------------------- work
+      int index = blockIdx.x, published = 0, asked = 0;
+      bool ok = true;
+      while (ok) {
+        PrefillItem x;
+        x.valid = 0;
+        bool publish = index < 0;
+        if (index >= 0) {
+          // Ask for the next block before looking at this one.
+          if (lane == 0) ask_for_work(answer, work);
+          const int rest = index / p.splits;
+          x.split = index - rest * p.splits;
+          x.hk = rest % kv.kv_heads;
+          int seq = 0, block = 0;
+          if (find_block(p.cu, kv.batch, p.tokens, p.block_tokens, rest / kv.kv_heads, lane, &seq, &block)) {
+            int row_end;
+            packed_range(p.cu, seq, p.tokens, &x.row0, &row_end);
+            x.n = row_end - x.row0;
+            bool bad_len;
+            x.seq = seq;
+            x.len = paged_clamp_len(kv.seq_lens[seq], kv.max_pages, kv.page_shift, &bad_len);
+            if ((bad_len || x.len < x.n) && lane == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
+            // Steps of each tile (a tile behind the rows' end has none) and of
+            // this piece.
+            x.tok0 = block * p.block_tokens;
+            int steps[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int first = x.tok0 + t * p.tile_tokens;
+              const int last = min(min(first + p.tile_tokens, x.n), x.tok0 + p.block_tokens) - 1;
+              steps[t] = last >= first ? (visible_keys(x.len, x.n, last) + kPreKeys - 1) / kPreKeys : 0;
+            }
+            const int most = max(steps[0], steps[1]);
+            x.j0 = min(x.split * p.piece, most);
+            x.j1 = min(x.j0 + p.piece, most);
+            x.end0 = max(x.j0, min(x.j1, steps[0]));
+            x.end1 = max(x.j0, min(x.j1, steps[1]));
+            // Without keys the rows still get their zeros when no join follows.
+            publish = x.j0 < x.j1 || p.splits == 1;
+            x.valid = 1;
+          }
+        }
+        if (publish) {
+          const int at = published & 1;
+          if (published >= 2) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&item_empty[at], ((published >> 1) - 1) & 1, abort_flag));
+          if (ok && lane == 0) {
+            items[at] = x;
+            mbar_arrive(&item_full[at]);
+          }
+          ++published;
+        }
+        if (index < 0) break;
+        const bool told = __all_sync(0xFFFFFFFFu, mbar_wait(work, asked & 1, abort_flag));
+        ++asked;
+        if (!told) {
+          mbar_wait_bounded(work, (asked - 1) & 1);  // the answer is not written after shared memory goes
+          ok = false;
+          break;
+        }
+        index = work_answer(answer);
+        fence_proxy_async_smem();  // read before the next answer is written there
         __syncwarp();
-        mbar_wait_bounded(drain, 0);
       }
     }
-    if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   }
+  if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   __syncthreads();
   tc_fence_after();
   if (warp == 9) tmem_dealloc(tmem, Cfg::kTmemCols);
@@ -627,7 +773,7 @@ struct PrefillJoinParams {
   const int32_t* cu;
   void* out;
   int64_t ot, oh;
-  int32_t tokens, heads, splits, tile_tokens;
+  int32_t tokens, heads, splits, piece, block_tokens;
   const float* part_o;
   const float2* part_ml;
 };
@@ -649,10 +795,9 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PrefillJo
   const int n = row_end - row0;
   bool bad;
   const int len = paged_clamp_len(p.kv.seq_lens[b], p.kv.max_pages, p.kv.page_shift, &bad);
-  // Pieces of the row's block, as its CTAs cut them.
-  const int per = 2 * p.tile_tokens;
-  const int last = min(((row - row0) / per + 1) * per, n) - 1;
-  const int count = split_count((visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys, p.splits);
+  // Pieces of the row's item.
+  const int last = min(((row - row0) / p.block_tokens + 1) * p.block_tokens, n) - 1;
+  const int count = ((visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys + p.piece - 1) / p.piece;
   const int64_t at = (static_cast<int64_t>(row) * p.heads + h) * p.splits;
   float m = -INFINITY, l = 0.f, o[kPer];
 #pragma unroll
