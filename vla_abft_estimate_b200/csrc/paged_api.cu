@@ -264,11 +264,18 @@ PrefillPlan prefill_plan(const abft_paged_attn_args* a, int sms) {
   if (blocks(r.tile_tokens) <= sms) r.block_tokens = r.tile_tokens;
   const int64_t base = blocks(r.block_tokens);
   const int64_t steps = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kPreKeys - 1) / kPreKeys;
-  // Pieces: while the items alone would leave SMs idle, as many as fill them
-  // twice, of four steps at least.
+  // Pieces, of four steps at least: as many as give each SM one item, counted
+  // without the blocks that only ragged chunks have, and twice as many for
+  // several sequences, whose lengths may differ. (One sequence, 64 tokens on
+  // 16,384: 1 piece 214 us, 8 pieces 41, 16 51; 512 tokens on 8,192, 116 items:
+  // 1 piece 118, 2 pieces 129, for the sums that go through memory. Nine
+  // sequences of 5 tokens on up to 7,777: 4 pieces 35, 8 pieces 25; four on
+  // 32,768 each: 4 pieces 118, 8 pieces 124.)
   int64_t n = a->num_splits;
   if (n == 0) {
-    n = 2 * sms / base;
+    int64_t least = (a->tokens + r.block_tokens - 1) / r.block_tokens;
+    if (least < a->kv.batch) least = a->kv.batch;
+    n = (a->kv.batch > 1 ? 2 : 1) * sms / (least * a->kv.kv_heads);
     if (n > steps / 4) n = steps / 4;
   }
   if (n > steps) n = steps;
@@ -307,7 +314,9 @@ int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUten
   j.block_tokens = p.block_tokens;
   j.part_o = p.part_o;
   j.part_ml = p.part_ml;
-  return launch(paged_prefill_join_kernel<D, F16>, dim3(static_cast<unsigned>(p.tokens) * a->heads), dim3(128), 0, s, j);
+  const unsigned rows = static_cast<unsigned>(p.tokens) * a->heads;
+  return launch(paged_prefill_join_kernel<D, F16>, dim3((rows + kPreJoinWarps - 1) / kPreJoinWarps),
+                dim3(32 * kPreJoinWarps), 0, s, j);
 }
 
 }  // namespace
@@ -422,6 +431,7 @@ int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
   p.block_tokens = plan.block_tokens;
   p.splits = plan.splits;
   p.piece = plan.piece;
+  p.items = static_cast<int32_t>(plan.items / plan.splits);
   const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
   p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
   p.negate = a->scale < 0.f;

@@ -54,8 +54,9 @@ struct PrefillCfg {
   static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kOffRing = 2 * kTileBytes;            // after the two Q tiles
   static constexpr int kOffBar = kOffRing + kSlots * kTileBytes;
-  // full, empty, qfull, sfull, pfull, ofull, item full and empty, work, drain
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 4 + 1 + 1;
+  // full, empty, qfull, sfull, pfull, ofull, item full and empty, work, loaded,
+  // drain, (even number)
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 4 + 1 + 1 + 2;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kOffItems = kOffMisc + 16;  // two items and the launch-control answer
   static constexpr int kSmemBytes = kOffItems + 2 * 48 + 16 + 1024;
@@ -79,6 +80,7 @@ struct PrefillParams {
   int32_t block_tokens;    // tokens of an item: one tile's or two's
   int32_t splits;          // pieces of an item's keys at most: blocks of the grid for it
   int32_t piece;           // steps of a piece
+  int32_t items;           // blocks of the grid for one piece of every item
   float scale_log2;        // |scale| * log2(e), never 0
   int32_t negate;          // scale < 0
   uint32_t group_inv;      // ceil(2^16 / group): row_token()
@@ -273,7 +275,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   uint64_t* item_full = ofull + 2;
   uint64_t* item_empty = item_full + 2;
   uint64_t* work = item_empty + 2;
-  uint64_t* drain = work + 1;
+  uint64_t* loaded_all = work + 1;
+  uint64_t* drain = loaded_all + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PrefillItem* items = reinterpret_cast<PrefillItem*>(smem + Cfg::kOffItems);
@@ -295,6 +298,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       mbar_init(&item_empty[t], 10);  // a lane of each row warp, the loader's and the issuer's
     }
     mbar_init(work, 1);
+    mbar_init(loaded_all, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -564,6 +568,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             ++issued;
           }
         }
+        if (lane == 0) mbar_arrive(loaded_all);
       }
       // Copies in flight have landed before shared memory goes (all have, but
       // after an abort).
@@ -704,10 +709,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         x.valid = 0;
         bool publish = index < 0;
         if (index >= 0) {
-          // Ask for the next block before looking at this one.
-          if (lane == 0) ask_for_work(answer, work);
-          const int rest = index / p.splits;
-          x.split = index - rest * p.splits;
+          // First pieces first: every item has one, few have the last.
+          x.split = index / p.items;
+          const int rest = index - x.split * p.items;
           x.hk = rest % kv.kv_heads;
           int seq = 0, block = 0;
           if (find_block(p.cu, kv.batch, p.tokens, p.block_tokens, rest / kv.kv_heads, lane, &seq, &block)) {
@@ -746,8 +750,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             mbar_arrive(&item_full[at]);
           }
           ++published;
+          // The next block is asked for when this item's last tile has been
+          // loaded: early enough to find it meanwhile, too late to take one
+          // that an idle SM could start.
+          if (index >= 0 && ok)
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(loaded_all, (published - 1) & 1, abort_flag));
         }
-        if (index < 0) break;
+        if (index < 0 || !ok) break;
+        if (lane == 0) ask_for_work(answer, work);
+        __syncwarp();
         const bool told = __all_sync(0xFFFFFFFFu, mbar_wait(work, asked & 1, abort_flag));
         ++asked;
         if (!told) {
@@ -767,7 +778,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   if (warp == 9) tmem_dealloc(tmem, Cfg::kTmemCols);
 }
 
-// Joins the pieces of each (packed row, head): grid (heads, tokens).
+// Joins the pieces of each (packed row, head): one warp per row and head,
+// D / 32 elements per lane, the pieces in their order.
 struct PrefillJoinParams {
   PagedView kv;
   const int32_t* cu;
@@ -777,16 +789,16 @@ struct PrefillJoinParams {
   const float* part_o;
   const float2* part_ml;
 };
+constexpr int kPreJoinWarps = 8;
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PrefillJoinParams p) {
+__global__ void __launch_bounds__(32 * kPreJoinWarps) paged_prefill_join_kernel(const PrefillJoinParams p) {
   constexpr int kPer = D / 32;
-  __shared__ float so[4][D];
-  __shared__ float2 sml[4];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   griddep_wait();
-  griddep_launch();
-  const int row = blockIdx.x / p.heads, h = blockIdx.x - row * p.heads;
+  const int index = blockIdx.x * kPreJoinWarps + (threadIdx.x >> 5);
+  const int row = index / p.heads, h = index - row * p.heads;
+  if (row >= p.tokens) return;
   const int b = owner_of(p.cu, p.kv.batch, row, lane);
   if (b >= p.kv.batch) return;  // behind the last sequence
   int row0, row_end;
@@ -799,41 +811,43 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PrefillJo
   const int last = min(((row - row0) / p.block_tokens + 1) * p.block_tokens, n) - 1;
   const int count = ((visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys + p.piece - 1) / p.piece;
   const int64_t at = (static_cast<int64_t>(row) * p.heads + h) * p.splits;
-  float m = -INFINITY, l = 0.f, o[kPer];
+  // The maximum of all pieces first, then sums that do not wait for each other.
+  float top = -INFINITY;
+  for (int s = lane; s < count; s += 32) {
+    const float2 ml = p.part_ml[at + s];
+    if (ml.y != 0.f) top = fmaxf(top, ml.x);
+  }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, i));
+  const float ms = top == -INFINITY ? 0.f : top;
+  float l = 0.f, o[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  for (int s = warp; s < count; s += 4) {
-    const float2 ml = p.part_ml[at + s];
-    if (ml.y == 0.f) continue;  // the row saw nothing there: its sums were not written
-    const float* src = p.part_o + (at + s) * D + lane * kPer;
-    const float mn = fmaxf(m, ml.x);
-    const float ms = mn == -INFINITY ? 0.f : mn;
-    const float f0 = exp2_approx(m - ms), f1 = exp2_approx(ml.x - ms);
-    m = mn;
-    l = l * f0 + ml.y * f1;
+  for (int s0 = 0; s0 < count; s0 += 32) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (s0 + lane < count) ml = p.part_ml[at + s0 + lane];
+    const float f = ml.y == 0.f ? 0.f : exp2_approx(ml.x - ms);
+    l += ml.y * f;
+    const float2* src = reinterpret_cast<const float2*>(p.part_o + (at + s0) * D + lane * kPer);
+    const int most = min(32, count - s0);
+#pragma unroll 8
+    for (int s = 0; s < most; ++s) {
+      const float fs = __shfl_sync(0xFFFFFFFFu, f, s);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = o[i] * f0 + src[i] * f1;
-  }
-  if (lane == 0) sml[warp] = make_float2(m, l);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = o[i];
-  __syncthreads();
-  if (threadIdx.x < D / 2) {
-    const int d = threadIdx.x * 2;
-    const float top = fmaxf(fmaxf(sml[0].x, sml[1].x), fmaxf(sml[2].x, sml[3].x));
-    const float ms = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2_approx(sml[w].x - ms);
-      sum += sml[w].y * f;
-      x += so[w][d] * f;
-      y += so[w][d + 1] * f;
+      for (int i = 0; i < kPer / 2; ++i) {
+        float2 v = src[s * (D / 2) + i];
+        if (fs == 0.f) v = make_float2(0.f, 0.f);  // the row saw nothing there: its sums were not written
+        o[2 * i] += v.x * fs;
+        o[2 * i + 1] += v.y * fs;
+      }
     }
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-    uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + h * p.oh + d;
-    *reinterpret_cast<uint32_t*>(dst) = pack2<F16>(x * inv, y * inv);
   }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, i);
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + h * p.oh + lane * kPer;
+#pragma unroll
+  for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack2<F16>(o[i] * inv, o[i + 1] * inv);
 }
 
 }  // namespace abft
