@@ -25,6 +25,33 @@ QWEN2_7B = dict(hidden=3584, inter=18944, layers=28, heads=28, kv_heads=4, head_
                 rope_theta=1000000.0, eps=1e-6)
 
 
+class PagedCaches:
+    """The paged caches of a decoder's layers: one page pool per layer, one
+    page table and one array of lengths for all of them, and the rotation
+    table. ``layers``: a ``paged.PagedKVCache`` per layer; ``table`` int32
+    [batch, pages]; ``lens`` int32 [batch], the tokens of each sequence
+    including the ones of the next call."""
+
+    def __init__(self, layers, table, lens, rope):
+        self.layers, self.table, self.lens, self.rope = layers, table, lens, rope
+
+    @classmethod
+    def allocate(cls, layers, batch, t_max, page_size, kv_heads, head_dim, theta, dtype, device):
+        """Pools that hold t_max tokens of each sequence; sequence b starts
+        with pages b, b + batch, ... and length 0."""
+        import torch
+
+        from .paged import PagedKVCache, rope_table
+
+        per = -(-t_max // page_size)
+        table = torch.arange(per * batch, dtype=torch.int32, device=device).view(per, batch).t().contiguous()
+        lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        pools = [torch.zeros(per * batch, 2, kv_heads, page_size, head_dim, dtype=dtype, device=device)
+                 for _ in range(layers)]
+        return cls([PagedKVCache(p[:, 0], p[:, 1], table, lens) for p in pools], table, lens,
+                   rope_table(t_max, head_dim, theta, device))
+
+
 def build_qwen2(cfg, device, seed=0, dtype=None):
     """Qwen2-style decoder: RMSNorm, fused QKV (with bias) + RoPE + GQA
     attention (SDPA), SwiGLU MLP with fused gate+up, tied-free lm_head.
@@ -33,6 +60,12 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
     a 0-d device tensor ``pos`` keeps every shape fixed (attention over the
     whole cache, later positions masked), so a decode step can be captured
     in a CUDA graph and replayed as ``pos`` advances.
+    ``model.forward_paged(ids, caches, cu_seqlens)`` runs a batch of sequences
+    over ``model.new_paged_caches(...)``: rotation, cache writes and attention
+    by the library's paged operators (head_dim 64 or 128, CUDA). ids are the
+    packed new tokens; cu_seqlens bounds each sequence's (prompts and chunks
+    of any length), or is None for one token per sequence.
+    ``caches.lens`` counts the new tokens already: advance it first.
     ``dtype``: bfloat16 (default) or float16, the reference driver's
     ``--dtype`` (qwen_abft_benchmark.py:26)."""
     import torch
@@ -88,6 +121,16 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
             g, u = self.gate_up(self.ln2(x)).chunk(2, dim=-1)
             return x + self.down(F.silu(g) * u)
 
+        def forward_paged(self, x, rope, cache, cu_seqlens):
+            nh, nkv, hd = cfg["heads"], cfg["kv_heads"], cfg["head_dim"]
+            t = x.shape[0]
+            q, k, v = self.qkv(self.ln1(x)).split([nh * hd, nkv * hd, nkv * hd], dim=-1)
+            q = cache.append(q.view(t, nh, hd), k.view(t, nkv, hd), v.view(t, nkv, hd), rope, cu_seqlens=cu_seqlens)
+            a = cache.decode(q) if cu_seqlens is None else cache.prefill(q, cu_seqlens)
+            x = x + self.o(a.view(t, nh * hd))
+            g, u = self.gate_up(self.ln2(x)).chunk(2, dim=-1)
+            return x + self.down(F.silu(g) * u)
+
     class Model(nn.Module):
         def __init__(self):
             super().__init__()
@@ -113,6 +156,16 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
         def new_caches(self, t_max):
             return [torch.zeros(2, cfg["kv_heads"], t_max, cfg["head_dim"], dtype=dt,
                                 device=self.embed.weight.device) for _ in range(cfg["layers"])]
+
+        def forward_paged(self, ids, caches, cu_seqlens=None):
+            x = self.embed(ids)
+            for layer, cache in zip(self.layers, caches.layers):
+                x = layer.forward_paged(x, caches.rope, cache, cu_seqlens)
+            return self.lm_head(self.norm(x))
+
+        def new_paged_caches(self, batch, t_max, page_size=16):
+            return PagedCaches.allocate(len(self.layers), batch, t_max, page_size, cfg["kv_heads"], cfg["head_dim"],
+                                        cfg["rope_theta"], dt, self.embed.weight.device)
 
     dt = torch.bfloat16 if dtype is None else dtype
     torch.manual_seed(seed)
