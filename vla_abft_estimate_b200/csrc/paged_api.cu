@@ -135,8 +135,12 @@ PagedView view_of(const abft_paged_kv& c) {
 }
 
 template <int D, bool F16>
-int launch_append(const AppendParams& p, cudaStream_t s) {
-  return launch(kv_append_kernel<D, F16>, dim3(static_cast<unsigned>(p.tokens)), dim3(kAppendThreads), 0, s, p);
+int launch_append(AppendParams p, int sms, cudaStream_t s) {
+  // Halve the warps of a token while a full set of the SMs' blocks is left.
+  p.warps_shift = 3;
+  while (p.warps_shift > 0 && (p.tokens << (p.warps_shift - 1)) >= int64_t{16} * sms) --p.warps_shift;
+  const int64_t blocks = ((p.tokens << p.warps_shift) + kAppendWarps - 1) / kAppendWarps;
+  return launch(kv_append_kernel<D, F16>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, s, p);
 }
 
 // ---- decode -------------------------------------------------------------------
@@ -356,8 +360,8 @@ int abft_kv_append(const abft_kv_append_args* a, void* stream) {
   p.heads = a->heads;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
-  if (a->kv.head_dim == 128) return f16 ? launch_append<128, true>(p, s) : launch_append<128, false>(p, s);
-  return f16 ? launch_append<64, true>(p, s) : launch_append<64, false>(p, s);
+  if (a->kv.head_dim == 128) return f16 ? launch_append<128, true>(p, sms, s) : launch_append<128, false>(p, sms, s);
+  return f16 ? launch_append<64, true>(p, sms, s) : launch_append<64, false>(p, sms, s);
 }
 
 size_t abft_paged_decode_workspace_bytes(const abft_paged_attn_args* a) {

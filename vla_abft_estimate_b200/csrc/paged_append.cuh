@@ -43,6 +43,7 @@ struct AppendParams {
   int64_t max_positions;
   int64_t tokens;
   int32_t heads;
+  int32_t warps_shift;  // log2 of the warps that share a token
 };
 
 // Sequence that owns packed token t: the number of boundaries cu[1..batch]
@@ -60,16 +61,23 @@ __device__ __forceinline__ int owner_of(const int32_t* cu, int batch, int64_t t,
 
 // One thread owns chunk c of a row's pairs: elements [8c, 8c + 8) and their
 // partners [D/2 + 8c, D/2 + 8c + 8). D / 16 threads cover a row, a warp 512 / D
-// rows of one token; the block's warps walk the token's heads (q, then k, then
-// v).
-constexpr int kAppendThreads = 256;
+// rows of one token. `warps` warps share a token's rows (q's heads, then k's,
+// then v's): one when there are tokens enough to fill the SMs, so that the
+// angles are read once per token and lane, eight when there are few and the
+// chain of dependent loads is what counts.
+constexpr int kAppendWarps = 8;
+constexpr int kAppendThreads = 32 * kAppendWarps;
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
   constexpr int kChunks = D / 16;  // threads per row
   griddep_wait();
+  constexpr int kRows = 32 / kChunks;  // rows a warp covers at once
   const int lane = threadIdx.x & 31;
-  const int64_t t = blockIdx.x;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
+  const int64_t t = w >> p.warps_shift;
+  const int sub = static_cast<int>(w) & ((1 << p.warps_shift) - 1);
+  if (t >= p.tokens) return;
   const PagedView& kv = p.kv;
   int b, pos, place = 0, n = 1;
   if (p.cu != nullptr) {
@@ -94,10 +102,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
     if (page < 0 || page >= kv.num_pages) bad = ABFT_PAGED_BAD_PAGE;
   }
   if (bad != 0) {
-    if (threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, bad);
+    if (lane == 0 && sub == 0 && kv.status != nullptr) atomicOr(kv.status, bad);
     return;
   }
-  const int c = threadIdx.x % kChunks;
+  const int c = lane % kChunks;
   const int slot = pos & ((1 << kv.page_shift) - 1);
   constexpr int kShift = D == 128 ? 7 : 6;
   float cs[16];  // this chunk's (cos, sin) pairs
@@ -110,7 +118,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
     }
   }
   const int rows = p.heads + 2 * kv.kv_heads;
-  for (int r = threadIdx.x / kChunks; r < rows; r += kAppendThreads / kChunks) {
+#pragma unroll 3
+  for (int r = sub * kRows + lane / kChunks; r < rows; r += kRows << p.warps_shift) {
     const uint16_t* src;
     uint16_t* dst;
     bool turn = p.rope != nullptr;
