@@ -257,3 +257,19 @@ def test_rope_table_is_exact_far_out():
         rope_table(4, 7)
     with pytest.raises(ValueError):
         rope_table(-1, 8)
+
+
+def test_host_extension_takes_only_its_struct_and_passes_on_the_rest():
+    from vla_abft_estimate_b200.paged import _host
+
+    Calls = _host().Calls
+    with pytest.raises(ValueError):
+        Calls(bytes(ctypes.sizeof(N.PagedKv) - 8), 0, 0, 0, 0, 0, 0)
+    with pytest.raises(TypeError):
+        Calls(bytes(ctypes.sizeof(N.PagedKv)), 0)
+    c = Calls(bytes(_kv()), 0, 0, 0, 0, 0, 0)
+    t = torch.zeros(2, 4, 128, dtype=torch.bfloat16)
+    assert c.append(t, t, t, None, None, None) is None
+    assert c.append(t) is None
+    assert c.attend(False, t, None, None, None, 0, 0) is None
+    assert c.attend(True, 3, None, "x", None, 0, 0) is None

@@ -1,7 +1,8 @@
-"""Build libabft_b200.so in-tree with nvcc for sm_100a.
+"""Build libabft_b200.so in-tree with nvcc for sm_100a, and _paged_host.so,
+the extension that takes Python calls of the paged cache to it.
 
-The shared library lands in ``vla_abft_estimate_b200/_lib/`` next to the
-package so that it travels with the source tree; nothing is installed into
+Both land in ``vla_abft_estimate_b200/_lib/`` next to the
+package so that they travel with the source tree; nothing is installed into
 site-packages and nothing is JIT-compiled at import time.
 """
 from __future__ import annotations
@@ -17,6 +18,8 @@ REPO_DIR = PKG_DIR.parent
 CSRC_DIR = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libabft_b200.so"
+HOST_PATH = LIB_DIR / "_paged_host.so"
+HOST_SOURCE = CSRC_DIR / "paged_host.cpp"
 INCLUDE_DIR = REPO_DIR / "include"
 
 OBJ_DIR = LIB_DIR / "obj"
@@ -55,14 +58,34 @@ def _newer(out: Path, inputs: list[Path]) -> bool:
     return all(p.stat().st_mtime <= t for p in inputs)
 
 
+def _host_stale() -> bool:
+    return not _newer(HOST_PATH, [HOST_SOURCE, INCLUDE_DIR / "abft_b200.h"])
+
+
 def is_stale() -> bool:
-    return not all(_newer(LIB_PATH, _inputs(s)) for s in SOURCES)
+    return _host_stale() or not all(_newer(LIB_PATH, _inputs(s)) for s in SOURCES)
+
+
+def _host_cmd(out: Path) -> list[str]:
+    """g++ on the extension, against the headers and libraries of the torch
+    that is installed (it reads torch tensors without Python's attributes)."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    includes = [INCLUDE_DIR, root / "include", root / "include/torch/csrc/api/include", cuda / "include",
+                sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[f"-I{i}" for i in includes], str(HOST_SOURCE), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+            "-lc10", "-lc10_cuda", "-o", str(out)]
 
 
 def _run(cmd: list[str], verbose: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     if verbose and res.stderr:
         print(res.stderr)
 
@@ -83,10 +106,15 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         for _, _, cmd in jobs:
             cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd))
+    if force or _host_stale():
+        tmp = HOST_PATH.with_suffix(".so.tmp")
+        jobs.append((tmp, HOST_PATH, _host_cmd(tmp)))
     with ThreadPoolExecutor(max(1, len(jobs))) as pool:
         list(pool.map(lambda j: _run(j[2], verbose), jobs))
     for tmp, obj, _ in jobs:
         os.replace(tmp, obj)
+    if not force and all(_newer(LIB_PATH, _inputs(s)) for s in SOURCES):
+        return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
     _run([_nvcc(), *NVCC_FLAGS[:2], "-shared", *[str(OBJ_DIR / (Path(s).stem + ".o")) for s in SOURCES],
           "-o", str(tmp)], verbose)

@@ -23,11 +23,13 @@ there, per call.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import math
-from typing import Optional, Tuple
+from typing import Optional
 
 import torch
 
+from . import _build
 from . import _native as N
 
 _DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
@@ -54,26 +56,20 @@ def _i32(name: str, t: torch.Tensor, dim: int, device: torch.device) -> None:
         raise ValueError(f"{name} must have unit stride in its last dimension")
 
 
-def _signature(t: Optional[torch.Tensor]):
-    """All a call checks of a tensor, its address apart."""
-    if t is None:
-        return None
-    try:
-        return t.shape, t.stride(), t.dtype, t.device, t.requires_grad and torch.is_grad_enabled()
-    except AttributeError:
-        raise TypeError(f"expected a torch.Tensor, got {type(t).__name__}") from None
+_HOST = None
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a dense copy of it when it does not start on 16 bytes."""
-    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() & 15 else t
-
-
-def _address(name: str, t: torch.Tensor) -> int:
-    p = t.data_ptr()
-    if p & 15:
-        raise ValueError(f"{name} must be 16-byte aligned")
-    return p
+def _host():
+    """The extension of csrc/paged_host.cpp, built next to the library."""
+    global _HOST
+    if _HOST is None:
+        path = _build.HOST_PATH
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m vla_abft_estimate_b200._build`")
+        spec = importlib.util.spec_from_file_location("_paged_host", path)
+        _HOST = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_HOST)
+    return _HOST
 
 
 class PagedKVCache:
@@ -144,25 +140,21 @@ class PagedKVCache:
         kv.batch, kv.max_pages, kv.dtype = batch, max_pages, _DTYPES[k_pages.dtype]
         self._kv = kv
         self._index = dev.index
-        self._plans: dict = {}
+        L = N.lib()
+        entry = [ctypes.cast(getattr(L, name), ctypes.c_void_p).value
+                 for name in ("abft_kv_append", "abft_paged_decode", "abft_paged_decode_workspace_bytes",
+                              "abft_paged_prefill", "abft_paged_prefill_workspace_bytes")]
+        self._fast = _host().Calls(bytes(kv), dev.index, *entry)
 
     # ---- argument checks ------------------------------------------------------
-    # A call's sizes, strides, types and devices are checked once and kept as
-    # a filled argument struct under that signature; a later call with the
-    # same signature only sets its addresses.
-    def _plan(self, key: tuple, make):
-        plan = self._plans.get(key)
-        if plan is None:
-            plan = make()
-            if len(self._plans) >= 256:  # callers whose packed lengths never repeat
-                self._plans.clear()
-            self._plans[key] = plan
-        return plan
-
-    def _rows(self, name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int]) -> Tuple[int, int]:
-        """Checks [tokens, heads, head_dim] rows; returns the token and head
-        strides the kernels read or write them with: their own, or dense ones
-        when the call has to work on a copy (``_in_place`` is false)."""
+    # A call whose arguments are all in order goes to the library through
+    # _paged_host (csrc/paged_host.cpp), which returns None for any other; the
+    # checks below then copy what has to be copied or say what is wrong.
+    def _rows(self, name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int]) -> torch.Tensor:
+        """Checks [tokens, heads, head_dim] rows; returns them as the kernels
+        can read them (16-byte pieces): themselves, or a dense copy."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
         shape = t.shape
         if (t.dtype != self.dtype or t.device != self.device or len(shape) != 3 or shape[2] != self.head_dim
                 or (tokens is not None and shape[0] != tokens) or (heads is not None and shape[1] != heads)):
@@ -172,36 +164,38 @@ class PagedKVCache:
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient, which the paged cache operators do not give: call them under "
                              "torch.no_grad()")
-        return t.stride()[:2] if self._in_place(t) else (shape[1] * shape[2], shape[2])
+        if not self._in_place(t):
+            return t.clone(memory_format=torch.contiguous_format)
+        return t
 
     @staticmethod
     def _in_place(t: torch.Tensor) -> bool:
-        """The strides let the kernels read rows in 16-byte pieces."""
         s = t.stride()
-        return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0
+        return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0
 
     def _group(self, heads: int) -> None:
         if heads == 0 or heads % self.kv_heads or heads // self.kv_heads > 64:
             raise ValueError(f"q has {heads} heads: a multiple of the cache's {self.kv_heads} kv heads, at most 64 "
                              "for each, is needed")
 
-    def _result(self, name: str, out: torch.Tensor, like: torch.Tensor) -> Tuple[int, int]:
-        strides = self._rows(name, out, like.shape[0], like.shape[1])
-        if not self._in_place(out):
-            raise ValueError(f"{name} must have strides a multiple of 8 and unit stride in its last dimension")
+    def _result(self, name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+        if out is None:
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
+        if self._rows(name, out, like.shape[0], like.shape[1]) is not out:
+            raise ValueError(f"{name} must be 16-byte aligned, with strides a multiple of 8 and unit stride in its last "
+                             "dimension")
         if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
             raise ValueError(f"{name} must not repeat memory")
-        return strides
+        return out
 
     def _boundaries(self, cu: torch.Tensor) -> None:
         _i32("cu_seqlens", cu, 1, self.device)
         if cu.shape[0] != self.batch + 1:
             raise ValueError(f"cu_seqlens must have {self.batch + 1} entries, got {cu.shape[0]}")
 
-    def _call(self, name: str, fn, args) -> None:
-        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(self._index))
-        if rc != N.ABFT_OK:
-            N.check(name, rc)
+    def _call(self, name: str, args) -> None:
+        stream = torch._C._cuda_getCurrentRawStream(self._index)
+        N.check(name, getattr(N.lib(), name)(ctypes.byref(args), stream))
 
     # ---- operators --------------------------------------------------------------
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rope: Optional[torch.Tensor] = None, *,
@@ -220,60 +214,43 @@ class PagedKVCache:
         sequence are left as they were (undefined without ``q_out``). q None
         stores k and v only.
         """
+        done = self._fast.append(q, k, v, rope, cu_seqlens, q_out)
+        if done is not None:
+            return done if type(done) is not int else N.check("abft_kv_append", done)
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
                 return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
-        key = (_signature(q), _signature(k), _signature(v), _signature(rope), _signature(cu_seqlens), _signature(q_out))
-        template, copies = self._plan(key, lambda: self._plan_append(q, k, v, rope, cu_seqlens, q_out))
-        args = N.KvAppendArgs.from_buffer_copy(template)
-        if copies:
-            q, k, v = (t if t is None or self._in_place(t) else t.contiguous() for t in (q, k, v))
-        kp, vp = k.data_ptr(), v.data_ptr()
-        if (kp | vp) & 15:
-            k, v = _aligned(k), _aligned(v)
-            kp, vp = k.data_ptr(), v.data_ptr()
-            return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
-        args.k, args.v = kp, vp
-        if q is not None:
-            qp = q.data_ptr()
-            if qp & 15:
-                return self.append(_aligned(q), k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
-            if q_out is None:
-                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            args.q, args.q_out = qp, _address("q_out", q_out)
-        if rope is not None:
-            args.rope = _address("rope", rope)
-        if cu_seqlens is not None:
-            args.cu_seqlens = cu_seqlens.data_ptr()
-        self._call("abft_kv_append", N.lib().abft_kv_append, args)
-        return q_out
-
-    def _plan_append(self, q, k, v, rope, cu_seqlens, q_out):
         args = N.KvAppendArgs()
         args.kv = self._kv
-        args.k_token_stride, args.k_head_stride = self._rows("k", k, None, self.kv_heads)
+        k = self._rows("k", k, None, self.kv_heads)
         tokens = k.shape[0]
-        args.tokens = tokens
-        args.v_token_stride, args.v_head_stride = self._rows("v", v, tokens, self.kv_heads)
+        v = self._rows("v", v, tokens, self.kv_heads)
         if cu_seqlens is not None:
             self._boundaries(cu_seqlens)
+            args.cu_seqlens = cu_seqlens.data_ptr()
         elif tokens != self.batch:
             raise ValueError(f"without cu_seqlens k must have one row for each of the {self.batch} sequences, got {tokens}")
         if rope is not None:
-            if (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1] * 2 != self.head_dim or rope.shape[2] != 2
-                    or rope.device != self.device or not rope.is_contiguous() or rope.shape[0] == 0):
-                raise ValueError(f"rope must be a contiguous float32 [positions, {self.head_dim // 2}, 2] tensor on "
-                                 f"{self.device}, got {rope.dtype} {tuple(rope.shape)}")
-            args.max_positions = rope.shape[0]
+            if (not isinstance(rope, torch.Tensor) or rope.dtype != torch.float32 or rope.dim() != 3
+                    or rope.shape[1] * 2 != self.head_dim or rope.shape[2] != 2 or rope.device != self.device
+                    or not rope.is_contiguous() or rope.shape[0] == 0 or rope.data_ptr() % 16):
+                raise ValueError(f"rope must be a contiguous, 16-byte aligned float32 [positions, {self.head_dim // 2}, 2] "
+                                 f"tensor on {self.device}")
+            args.rope, args.max_positions = rope.data_ptr(), rope.shape[0]
         if q is not None:
-            self._group(q.shape[1] if q.dim() == 3 else 0)
-            args.q_token_stride, args.q_head_stride = self._rows("q", q, tokens, None)
-            args.heads = q.shape[1]
-            args.o_token_stride, args.o_head_stride = (
-                (q.shape[1] * self.head_dim, self.head_dim) if q_out is None else self._result("q_out", q_out, q))
+            self._group(q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0)
+            q = self._rows("q", q, tokens, None)
+            q_out = self._result("q_out", q_out, q)
+            args.q, args.q_out, args.heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+            args.q_token_stride, args.q_head_stride, _ = q.stride()
+            args.o_token_stride, args.o_head_stride, _ = q_out.stride()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        return bytes(args), not all(t is None or self._in_place(t) for t in (q, k, v))
+        args.k, args.v, args.tokens = k.data_ptr(), v.data_ptr(), tokens
+        args.k_token_stride, args.k_head_stride, _ = k.stride()
+        args.v_token_stride, args.v_head_stride, _ = v.stride()
+        self._call("abft_kv_append", args)
+        return q_out
 
     def decode(self, q: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                num_sms: int = 0) -> torch.Tensor:
@@ -281,7 +258,7 @@ class PagedKVCache:
         [batch, heads, head_dim], returns the same shape. ``scale`` defaults
         to head_dim^-0.5. A sequence of length 0 gives zeros. ``num_sms``:
         SMs the caches are shared out to (0: all)."""
-        return self._attention("abft_paged_decode", q, None, scale, out, 0, num_sms)
+        return self._attention(False, q, None, scale, out, 0, num_sms)
 
     def prefill(self, q: torch.Tensor, cu_seqlens: torch.Tensor, *, scale: Optional[float] = None,
                 out: Optional[torch.Tensor] = None, num_splits: int = 0) -> torch.Tensor:
@@ -293,58 +270,39 @@ class PagedKVCache:
         in ``out`` (undefined without one). ``num_splits``: pieces the keys of
         a block of query rows are cut into (0: chosen from the rows, the heads
         and the table's width)."""
-        return self._attention("abft_paged_prefill", q, cu_seqlens, scale, out, num_splits, 0)
+        return self._attention(True, q, cu_seqlens, scale, out, num_splits, 0)
 
-    def _attention(self, name, q, cu, scale, out, num_splits, num_sms):
+    def _attention(self, prefill, q, cu, scale, out, num_splits, num_sms):
+        done = self._fast.attend(prefill, q, cu, scale, out, num_splits, num_sms)
+        name = "abft_paged_prefill" if prefill else "abft_paged_decode"
+        if done is not None:
+            return done if type(done) is not int else N.check(name, done)
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
-                return self._attention(name, q, cu, scale, out, num_splits, num_sms)
-        key = (name, _signature(q), _signature(cu), scale, _signature(out), num_splits, num_sms)
-        template, copies, space = self._plan(key, lambda: self._plan_attention(name, q, cu, scale, out, num_splits, num_sms))
-        args = N.PagedAttnArgs.from_buffer_copy(template)
-        if copies:
-            q = q.contiguous()
-        qp = q.data_ptr()
-        if qp & 15:
-            q = _aligned(q)
-            return self._attention(name, q, cu, scale, out, num_splits, num_sms)
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        args.q, args.out = qp, _address("out", out)
-        if cu is not None:
-            args.cu_seqlens = cu.data_ptr()
-        if space is not None:
-            ws = torch.empty_like(space)  # of this call alone: calls of other threads or graphs have their own
-            args.workspace = ws.data_ptr()
-        self._call(name, getattr(N.lib(), name), args)
-        return out
-
-    def _plan_attention(self, name, q, cu, scale, out, num_splits, num_sms):
-        decode = name == "abft_paged_decode"
-        if not decode:
-            self._boundaries(cu)
-        self._group(q.shape[1] if q.dim() == 3 else 0)
+                return self._attention(prefill, q, cu, scale, out, num_splits, num_sms)
         args = N.PagedAttnArgs()
         args.kv = self._kv
-        args.q_token_stride, args.q_head_stride = self._rows("q", q, self.batch if decode else None, None)
-        args.o_token_stride, args.o_head_stride = (
-            (q.shape[1] * self.head_dim, self.head_dim) if out is None else self._result("out", out, q))
-        args.tokens, args.heads = q.shape[0], q.shape[1]
+        if prefill:
+            self._boundaries(cu)
+            args.cu_seqlens = cu.data_ptr()
+        if not isinstance(q, torch.Tensor):
+            raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
+        self._group(q.shape[1] if q.dim() == 3 else 0)
+        q = self._rows("q", q, None if prefill else self.batch, None)
+        out = self._result("out", out, q)
+        args.q, args.out, args.tokens, args.heads = q.data_ptr(), out.data_ptr(), q.shape[0], q.shape[1]
+        args.q_token_stride, args.q_head_stride, _ = q.stride()
+        args.o_token_stride, args.o_head_stride, _ = out.stride()
         args.scale = self.head_dim ** -0.5 if scale is None else float(scale)
-        args.num_splits, args.num_sms = int(num_splits), int(num_sms)
-        if args.num_splits < 0 or args.num_sms < 0 or not math.isfinite(args.scale):
+        if int(num_splits) < 0 or int(num_sms) < 0 or not math.isfinite(args.scale):
             raise ValueError(f"scale must be finite, num_splits and num_sms at least 0, got {scale}, {num_splits}, {num_sms}")
-        space = None
-        if q.shape[0] and self.batch:
-            # placeholder addresses: sizes decide how much scratch the call needs
-            args.q = args.out = args.cu_seqlens = 1 << 20
-            need = int(getattr(N.lib(), name + "_workspace_bytes")(ctypes.byref(args)))
-            args.q = args.out = args.cu_seqlens = None
-            if need:
-                args.workspace_bytes = need
-                # one byte seen as `need` of them: empty_like gives that many
-                space = self.status.view(torch.uint8)[:1].expand(need)
-        return bytes(args), not self._in_place(q), space
+        args.num_splits, args.num_sms = int(num_splits), int(num_sms)
+        need = int(getattr(N.lib(), name + "_workspace_bytes")(ctypes.byref(args)))
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)  # of this call alone
+            args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        self._call(name, args)
+        return out
 
     def check_status(self) -> None:
         """Raises ValueError when a call since the last check met a bad page
