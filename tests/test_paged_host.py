@@ -223,10 +223,17 @@ def test_workspace_sizes():
     a = N.PagedAttnArgs()
     a.kv, a.q, a.out, a.tokens, a.heads, a.scale, a.num_sms = _kv(), 0x50000, 0x60000, 2, 28, 0.1, 148
     a.cu_seqlens = 0x70000
-    # decode: 2 sequences x 4 kv heads x 2 tiles of 32 slots = 16 tiles for 4 CTAs' warps
-    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 4 * (2 * 8 * (128 * 4 + 8) + 16)
+    # decode: 2 sequences x 4 kv heads, 8 segments of 2 tiles of 32 slots: a CTA each and no scratch
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 0
+    cta = 2 * 8 * (128 * 4 + 8) + 16  # two pieces of 8 heads and a record
     a.num_sms = 3
-    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 3 * (2 * 8 * (128 * 4 + 8) + 16)
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 3 * cta
+    a.num_sms = 148
+    a.kv.max_pages = a.kv.table_stride = 64  # 32 tiles each: shared out over 144 SMs, 18 for each segment
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 64 * cta  # 256 tiles for 64 CTAs' warps
+    a.kv.max_pages = a.kv.table_stride = 640
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 144 * cta
+    a.kv.max_pages = a.kv.table_stride = 3
     a.num_splits = 1
     assert N.lib().abft_paged_prefill_workspace_bytes(ctypes.byref(a)) == 0
     a.kv.max_pages = a.kv.table_stride = 64  # 8 steps of 128 slots

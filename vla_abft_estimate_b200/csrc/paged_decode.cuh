@@ -28,7 +28,9 @@
 // every SM reading to the end. A warp's ring of loads runs on across segment
 // boundaries. A segment inside one warp's share is finished by that warp;
 // pieces of a segment that crosses warps are joined in shared memory, those of
-// one that crosses CTAs by a second, small kernel, in a fixed order. (Joined
+// one that crosses CTAs by a second, small kernel, in a fixed order. A cache
+// too small to be worth sharing out gets a CTA per segment instead: nothing
+// crosses CTAs, and one launch does. (Joined
 // instead by the last CTA to arrive, an atomic counter's choice, 37 pieces of
 // 8 heads took one SM 12 us; spread over one block per head, launch included,
 // 3 us.)
@@ -100,6 +102,7 @@ struct DecodeParams {
   int64_t qt, qh, ot, oh;  // token and head strides, elements
   int32_t group;           // query heads per kv head
   int32_t head_chunks;     // segments that share a kv head's query heads
+  int32_t by_segment;      // a CTA per segment; no pieces in memory, no second kernel
   float scale_log2;        // scale * log2(e)
   float* part_o;           // [grid][2][heads of a segment][head_dim]: pieces of segments that cross CTAs
   float2* part_ml;         // [grid][2][heads of a segment] (m, l)
@@ -182,49 +185,63 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
   griddep_launch();
 
   // ---- this warp's share ------------------------------------------------------
-  int len0 = 0, tiles0 = 0;  // this lane's sequence of the first 32
-  int sum = 0;
-  for (int b = lane; b < kv.batch; b += 32) {
-    int len;
-    bool bad;
-    const int tiles = tiles_of(kv, b, &len, &bad);
-    if (b == lane) len0 = len, tiles0 = tiles;
-    sum += tiles;
-    if (bad && blockIdx.x == 0 && warp == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
-  }
-  sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-  const int total = sum * rows;  // the host keeps it below 2^31
-  const int shares = gridDim.x * kDecWarps;
-  const int share = blockIdx.x * kDecWarps + warp;
-  const int u0 = share_start(total, shares, share), u1 = share_start(total, shares, share + 1);
-
   TileIter head;
-  head.left = u1 - u0;
-  head.b = head.y = head.tile = head.tiles = head.len = 0;
-  if (head.left > 0) {  // the sequence that holds tile u0
-    int before = 0;
-    for (int i = 0; i < kv.batch; i += 32) {
-      int mine = tiles0, len = len0;
+  int total, shares, u0, u1;
+  if (p.by_segment) {  // the list is one segment, its shares this CTA's warps'
+    head.b = blockIdx.x / rows;
+    head.y = blockIdx.x - head.b * rows;
+    bool bad;
+    total = head.tiles = tiles_of(kv, head.b, &head.len, &bad);
+    if (bad && head.y == 0 && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
+    shares = kDecWarps;
+    u0 = head.tile = share_start(total, shares, warp);
+    u1 = share_start(total, shares, warp + 1);
+    head.left = u1 - u0;
+  } else {
+    int len0 = 0, tiles0 = 0;  // this lane's sequence of the first 32
+    int sum = 0;
+    for (int b = lane; b < kv.batch; b += 32) {
+      int len;
       bool bad;
-      if (i > 0) mine = i + lane < kv.batch ? tiles_of(kv, i + lane, &len, &bad) : 0;
-      int upto = mine;
+      const int tiles = tiles_of(kv, b, &len, &bad);
+      if (b == lane) len0 = len, tiles0 = tiles;
+      sum += tiles;
+      if (bad && blockIdx.x == 0 && warp == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
+    }
+    sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+    total = sum * rows;  // the host keeps it below 2^31
+    shares = gridDim.x * kDecWarps;
+    const int share = blockIdx.x * kDecWarps + warp;
+    u0 = share_start(total, shares, share);
+    u1 = share_start(total, shares, share + 1);
+
+    head.left = u1 - u0;
+    head.b = head.y = head.tile = head.tiles = head.len = 0;
+    if (head.left > 0) {  // the sequence that holds tile u0
+      int before = 0;
+      for (int i = 0; i < kv.batch; i += 32) {
+        int mine = tiles0, len = len0;
+        bool bad;
+        if (i > 0) mine = i + lane < kv.batch ? tiles_of(kv, i + lane, &len, &bad) : 0;
+        int upto = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += x;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, (before + upto) * rows > u0);
+        if (past != 0) {
+          const int src = __ffs(past) - 1;
+          head.b = i + src;
+          head.tiles = __shfl_sync(0xFFFFFFFFu, mine, src);
+          head.len = __shfl_sync(0xFFFFFFFFu, len, src);
+          const int in = u0 - (before + __shfl_sync(0xFFFFFFFFu, upto - mine, src)) * rows;
+          head.y = in / head.tiles;
+          head.tile = in - head.y * head.tiles;
+          break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
       }
-      const uint32_t past = __ballot_sync(0xFFFFFFFFu, (before + upto) * rows > u0);
-      if (past != 0) {
-        const int src = __ffs(past) - 1;
-        head.b = i + src;
-        head.tiles = __shfl_sync(0xFFFFFFFFu, mine, src);
-        head.len = __shfl_sync(0xFFFFFFFFu, len, src);
-        const int in = u0 - (before + __shfl_sync(0xFFFFFFFFu, upto - mine, src)) * rows;
-        head.y = in / head.tiles;
-        head.tile = in - head.y * head.tiles;
-        break;
-      }
-      before += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
   }
 
@@ -517,56 +534,72 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
   // ---- pieces that cross warps ------------------------------------------------
   // A chain is a last piece and the first pieces of the following warps as far
   // as the segment goes; the chain before warp 0 lacks its start (in an earlier
-  // CTA). One warp takes a head, a lane D / 32 of its elements.
-  constexpr int kPer = D / 32;
-  auto write_row = [&](int b, int y, int h, const float (&x)[kPer], float l_sum) {
-    const float inv = l_sum > 0.f ? 1.f / l_sum : (l_sum == 0.f ? 0.f : l_sum);
-    const int hk = y / p.head_chunks, hc = y - hk * p.head_chunks;
-    uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.ot + (hk * p.group + hc * Cfg::kHeads + h) * p.oh + lane * kPer;
-#pragma unroll
-    for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack2<F16>(x[i] * inv, x[i + 1] * inv);
-  };
+  // CTA). 16 threads take a head, each D / 16 of its elements, and read all
+  // pieces at once.
   int over = -1;  // warp whose last piece goes on in the next CTA
+#pragma unroll 1
   for (int w = -1; w < kDecWarps; ++w) {
     if (w < 0 ? s_first[0] == 0 : s_last[w] == 0) continue;
     int to = w + 1;
     bool on = true;
     while (to < kDecWarps && on) on = s_first[to++] == 2;
     const int b = w < 0 ? s_seg[0][0][0] : s_seg[w][1][0], y = w < 0 ? s_seg[0][0][1] : s_seg[w][1][1];
-    const int nheads = min(Cfg::kHeads, p.group - (y % p.head_chunks) * Cfg::kHeads);
+    const int hk = y / p.head_chunks, hc = y - hk * p.head_chunks;
+    const int nheads = min(Cfg::kHeads, p.group - hc * Cfg::kHeads);
     const bool whole = w >= 0 && !on;
     if (w >= 0 && on) over = w;
     const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (w < 0 ? 0 : 1)) * Cfg::kHeads;
-    for (int h = warp; h < nheads; h += kDecWarps) {
-      auto piece = [&](int k) {
-        return reinterpret_cast<const float*>(k == w ? smem + w * Cfg::kWarpBytes
-                                                     : smem + Cfg::kOffFirst + k * Cfg::kPieceBytes);
-      };
-      const int k0 = max(w, 0);
-      float top = -INFINITY, l_sum = 0.f, x[kPer];
-      for (int k = k0; k < to; ++k)
-        top = fmaxf(top, reinterpret_cast<const float2*>(piece(k) + Cfg::kHeads * Cfg::kPitch)[h].x);
+    constexpr int kPer = D / 16;
+    const int d = (threadIdx.x & 15) * kPer;
+#pragma unroll 1
+    for (int h = threadIdx.x >> 4; h < nheads; h += kDecThreads / 16) {
+      const float* at[kDecWarps + 1];  // the last piece of warp w, the first pieces of warps w + 1 .. to - 1
+      float2 ml[kDecWarps + 1];
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k <= kDecWarps; ++k) {
+        const bool used = k == 0 ? w >= 0 : (k - 1 > w && k - 1 < to);
+        at[k] = reinterpret_cast<const float*>(k == 0 ? smem + max(w, 0) * Cfg::kWarpBytes
+                                                      : smem + Cfg::kOffFirst + (k - 1) * Cfg::kPieceBytes);
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (used) ml[k] = reinterpret_cast<const float2*>(at[k] + Cfg::kHeads * Cfg::kPitch)[h];
+        if (!used) at[k] = nullptr;
+        top = fmaxf(top, ml[k].x);
+      }
       const float ms = top == -INFINITY ? 0.f : top;
+      float l_sum = 0.f, x[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) x[i] = 0.f;
-      for (int k = k0; k < to; ++k) {
-        const float2 ml = reinterpret_cast<const float2*>(piece(k) + Cfg::kHeads * Cfg::kPitch)[h];
-        const float* row = piece(k) + h * Cfg::kPitch + lane * kPer;
-        const float f = exp2_approx(ml.x - ms);
-        l_sum += ml.y * f;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] += row[i] * f;
+      for (int k = 0; k <= kDecWarps; ++k) {
+        if (at[k] == nullptr) continue;
+        const float f = exp2_approx(ml[k].x - ms);
+        l_sum += ml[k].y * f;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(at[k] + h * Cfg::kPitch + d + i);
+          x[i] += v.x * f;
+          x[i + 1] += v.y * f;
+          x[i + 2] += v.z * f;
+          x[i + 3] += v.w * f;
+        }
       }
       if (whole) {
-        write_row(b, y, h, x, l_sum);
-      } else {
-        float* dst = p.part_o + (slot + h) * D + lane * kPer;
+        const float inv = l_sum > 0.f ? 1.f / l_sum : (l_sum == 0.f ? 0.f : l_sum);
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.ot + (hk * p.group + hc * Cfg::kHeads + h) * p.oh + d;
 #pragma unroll
-        for (int i = 0; i < kPer; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(x[i], x[i + 1]);
-        if (lane == 0) p.part_ml[slot + h] = make_float2(top, l_sum);
+        for (int i = 0; i < kPer; i += 4)
+          *reinterpret_cast<uint2*>(dst + i) =
+              make_uint2(pack2<F16>(x[i] * inv, x[i + 1] * inv), pack2<F16>(x[i + 2] * inv, x[i + 3] * inv));
+      } else {
+        float* dst = p.part_o + (slot + h) * D + d;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        if (d == 0) p.part_ml[slot + h] = make_float2(top, l_sum);
       }
     }
   }
+  if (p.by_segment) return;
   if (threadIdx.x == 0) {
     int4 spill = make_int4(0, 0, 0, 0);
     if (over >= 0)
@@ -607,21 +640,39 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const JoinP
   float m = -INFINITY, l = 0.f, o[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-#pragma unroll 4
-  for (int s = warp; s < seg.z; s += kJoinWarps) {
-    const int64_t at = (static_cast<int64_t>(c + s) * 2 + (s == 0 ? 1 : 0)) * kHeads + h;
-    const float2 ml = p.part_ml[at];
-    const float2* src = reinterpret_cast<const float2*>(p.part_o + at * D + lane * kPer);
-    const float mn = fmaxf(m, ml.x);
-    const float ms = mn == -INFINITY ? 0.f : mn;
-    const float f0 = exp2_approx(m - ms), f1 = exp2_approx(ml.x - ms);
-    m = mn;
-    l = l * f0 + ml.y * f1;
+  // Five pieces at a time, all asked for before the first is used.
+  constexpr int kAtOnce = 5;
+#pragma unroll 1
+  for (int s0 = warp; s0 < seg.z; s0 += kAtOnce * kJoinWarps) {
+    float2 ml[kAtOnce], v[kAtOnce][kPer / 2];
 #pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) {
-      const float2 v = src[i];
-      o[2 * i] = o[2 * i] * f0 + v.x * f1;
-      o[2 * i + 1] = o[2 * i + 1] * f0 + v.y * f1;
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int s = s0 + k * kJoinWarps;
+      const int64_t at = (static_cast<int64_t>(c + s) * 2 + (s == 0 ? 1 : 0)) * kHeads + h;
+      const bool in = s < seg.z;
+      ml[k] = in ? p.part_ml[at] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i)
+        v[k][i] = in ? reinterpret_cast<const float2*>(p.part_o + at * D + lane * kPer)[i] : make_float2(0.f, 0.f);
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, ml[k].x);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    const float f0 = exp2_approx(m - ms);
+    m = mn;
+    l *= f0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] *= f0;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float f = exp2_approx(ml[k].x - ms);
+      l += ml[k].y * f;
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i) {
+        o[2 * i] += v[k][i].x * f;
+        o[2 * i + 1] += v[k][i].y * f;
+      }
     }
   }
   if (lane == 0) sml[warp] = make_float2(m, l);
