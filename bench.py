@@ -83,6 +83,8 @@ def parse_args():
                     help="qwen2-7b: prefill-512 tokens/s and decode of a random-init Qwen2-7B-shaped decoder; "
                          "cogact: one CogACT-style VLA forward (ViT-L + SigLIP + Llama-2-7B + DiT-B, 10 "
                          "denoising steps); every linear ABFT-protected (one JSON line)")
+    ap.add_argument("--paged-batch", type=int, default=0, metavar="N",
+                    help="--model qwen2-7b: also the decode step of N sequences over the paged key-value caches")
     ap.add_argument("--profile-case", choices=["off", "check", "both"], default=None,
                     help="only run two rounds of the fused GEMM (unchecked then checked for 'both') "
                          "on randn inputs, for an ncu capture")
@@ -446,7 +448,7 @@ def _nvtx_range(enabled, name):
     return rng()
 
 
-def qwen_prefill_point(reps, warmup, decode_steps=0, cpu_seconds=0.0, dtype="bf16", nvtx=False):
+def qwen_prefill_point(reps, warmup, decode_steps=0, cpu_seconds=0.0, dtype="bf16", nvtx=False, paged_batch=0):
     """a Qwen2-7B-shaped decoder prefill of 512 tokens
     (batch 1, random init N(0, 0.02), random token ids) with every nn.Linear
     through AbftInjector's fused path (reports deferred to one read per
@@ -457,7 +459,8 @@ def qwen_prefill_point(reps, warmup, decode_steps=0, cpu_seconds=0.0, dtype="bf1
     random faults (probability 0.05 per linear, +1.0 on the fp32
     accumulator) and, with ``decode_steps``, single-token decode steps after
     the prefill. ``dtype`` "f16" builds the model in fp16 (the reference
-    driver's --dtype float16)."""
+    driver's --dtype float16). ``paged_batch``: with decode steps, also the
+    decode step of that many sequences over the paged caches."""
     import contextlib
 
     import torch
@@ -642,6 +645,51 @@ def qwen_prefill_point(reps, warmup, decode_steps=0, cpu_seconds=0.0, dtype="bf1
                     "abft: every step's reports read and recorded before the next replay; abft_overlapped_reports: "
                     "recorded one step late from pinned copies queued behind each replay (record(overlap=True)), "
                     "the host work under the next replay; abft_reports_after_last_step: device cost alone"}
+        if paged_batch:
+            def paged_decode(inj):
+                """A decode step of ``paged_batch`` sequences over the paged
+                caches, after their 512-token prompts, as a CUDA graph that
+                advances the lengths."""
+                caches = model.new_paged_caches(paged_batch, tokens + decode_steps + 8)
+                nxt = ids[-1:].repeat(paged_batch)
+                ctx = inj if inj is not None else contextlib.nullcontext()
+                with torch.inference_mode(), ctx:
+                    caches.lens.fill_(tokens)
+                    cu = torch.arange(0, tokens * paged_batch + 1, tokens, dtype=torch.int32, device=dev)
+                    model.forward_paged(ids.repeat(paged_batch), caches, cu)
+                    caches.lens.add_(1)
+                    s = torch.cuda.Stream()
+                    s.wait_stream(torch.cuda.current_stream())
+                    with torch.cuda.stream(s):
+                        model.forward_paged(nxt, caches)
+                    torch.cuda.current_stream().wait_stream(s)
+                    g = torch.cuda.CUDAGraph()
+                    with (inj.capture(g) if inj is not None else torch.cuda.graph(g)) as checks:
+                        model.forward_paged(nxt, caches)
+                        caches.lens.add_(1)
+                    for _ in range(3):
+                        g.replay()
+                    caches.lens.fill_(tokens + 1)
+                    torch.cuda.synchronize()
+                    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                    e0.record()
+                    for _ in range(decode_steps):
+                        g.replay()
+                    e1.record()
+                    if inj is not None:
+                        checks.record()
+                    torch.cuda.synchronize()
+                    for c in caches.layers:
+                        c.check_status()
+                del g
+                return e0.elapsed_time(e1) / decode_steps
+
+            p_torch, p_off, p_chk = paged_decode(None), paged_decode(inj_off), paged_decode(inj_chk)
+            res["paged_decode_graph_ms_per_step"] = {
+                "sequences": paged_batch, "torch_linears": p_torch, "unchecked": p_off, "abft": p_chk,
+                "tokens_per_s_abft": paged_batch / p_chk * 1e3,
+                "note": "append with rotation and paged decode attention in every layer, one CUDA graph per step; "
+                        "abft: reports recorded after the timed steps"}
     if cpu_seconds > 0:
         res["cpu_baseline"] = cpu_model_baseline(cfg, tokens, cpu_seconds)
     linear_flops = 0.0
@@ -1252,7 +1300,7 @@ def run_model(args):
     reps = max(args.steps, 3) if args.steps < 300 else 10
     warmup = max(args.warmup, 2)
     res = qwen_prefill_point(reps, warmup, decode_steps=32, cpu_seconds=0.0 if args.no_cpu_baseline else 20.0,
-                             dtype=args.dtype, nvtx=args.nvtx_enable)
+                             dtype=args.dtype, nvtx=args.nvtx_enable, paged_batch=args.paged_batch)
     cfg = QWEN2_7B
     line = {
         "metric": "Qwen2-7B prefill-512 tokens/s (every linear ABFT-protected)",
