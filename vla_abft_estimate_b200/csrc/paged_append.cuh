@@ -117,40 +117,56 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
       cs[4 * i] = x.x, cs[4 * i + 1] = x.y, cs[4 * i + 2] = x.z, cs[4 * i + 3] = x.w;
     }
   }
+  // kBatch rows are asked for before the first is written (q_out may be q, so
+  // the compiler must not move a load over a store; each thread reads and
+  // writes its own elements only). 10,240 tokens of 36 heads of 128: batches of
+  // 1 / 2 / 3 / 5: 38.0 / 35.6 / 33.3 / 34.8 us, 5.8 TB/s at 3.
+  constexpr int kBatch = 3;
   const int rows = p.heads + 2 * kv.kv_heads;
-#pragma unroll 3
-  for (int r = sub * kRows + lane / kChunks; r < rows; r += kRows << p.warps_shift) {
-    const uint16_t* src;
-    uint16_t* dst;
-    bool turn = p.rope != nullptr;
-    if (r < p.heads) {
-      src = static_cast<const uint16_t*>(p.q) + t * p.qt + r * p.qh;
-      dst = static_cast<uint16_t*>(p.q_out) + t * p.ot + r * p.oh;
-    } else if (r < p.heads + kv.kv_heads) {
-      const int h = r - p.heads;
-      src = static_cast<const uint16_t*>(p.k) + t * p.kt + h * p.kh;
-      dst = static_cast<uint16_t*>(kv.k_pages) + paged_offset(page, kv.k_page_stride, h, slot, kv.page_shift, kShift);
-    } else {
-      const int h = r - p.heads - kv.kv_heads;
-      src = static_cast<const uint16_t*>(p.v) + t * p.vt + h * p.vh;
-      dst = static_cast<uint16_t*>(kv.v_pages) + paged_offset(page, kv.v_page_stride, h, slot, kv.page_shift, kShift);
-      turn = false;
-    }
-    uint4 lo = *reinterpret_cast<const uint4*>(src + 8 * c);
-    uint4 hi = *reinterpret_cast<const uint4*>(src + D / 2 + 8 * c);
-    if (turn) {
-      uint32_t* a = reinterpret_cast<uint32_t*>(&lo);
-      uint32_t* z = reinterpret_cast<uint32_t*>(&hi);
+  const int step = kRows << p.warps_shift;
+  for (int r0 = sub * kRows + lane / kChunks; r0 < rows; r0 += kBatch * step) {
+    uint4 lo[kBatch], hi[kBatch];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x = unpack2<F16>(a[i]), y = unpack2<F16>(z[i]);
-        const float c0 = cs[4 * i], s0 = cs[4 * i + 1], c1 = cs[4 * i + 2], s1 = cs[4 * i + 3];
-        a[i] = pack2<F16>(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
-        z[i] = pack2<F16>(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
-      }
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = r0 + k * step;
+      if (r >= rows) break;
+      const uint16_t* src;
+      if (r < p.heads)
+        src = static_cast<const uint16_t*>(p.q) + t * p.qt + r * p.qh;
+      else if (r < p.heads + kv.kv_heads)
+        src = static_cast<const uint16_t*>(p.k) + t * p.kt + (r - p.heads) * p.kh;
+      else
+        src = static_cast<const uint16_t*>(p.v) + t * p.vt + (r - p.heads - kv.kv_heads) * p.vh;
+      lo[k] = *reinterpret_cast<const uint4*>(src + 8 * c);
+      hi[k] = *reinterpret_cast<const uint4*>(src + D / 2 + 8 * c);
     }
-    *reinterpret_cast<uint4*>(dst + 8 * c) = lo;
-    *reinterpret_cast<uint4*>(dst + D / 2 + 8 * c) = hi;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = r0 + k * step;
+      if (r >= rows) break;
+      uint16_t* dst;
+      if (r < p.heads)
+        dst = static_cast<uint16_t*>(p.q_out) + t * p.ot + r * p.oh;
+      else if (r < p.heads + kv.kv_heads)
+        dst = static_cast<uint16_t*>(kv.k_pages) +
+              paged_offset(page, kv.k_page_stride, r - p.heads, slot, kv.page_shift, kShift);
+      else
+        dst = static_cast<uint16_t*>(kv.v_pages) +
+              paged_offset(page, kv.v_page_stride, r - p.heads - kv.kv_heads, slot, kv.page_shift, kShift);
+      if (p.rope != nullptr && r < p.heads + kv.kv_heads) {
+        uint32_t* a = reinterpret_cast<uint32_t*>(&lo[k]);
+        uint32_t* z = reinterpret_cast<uint32_t*>(&hi[k]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack2<F16>(a[i]), y = unpack2<F16>(z[i]);
+          const float c0 = cs[4 * i], s0 = cs[4 * i + 1], c1 = cs[4 * i + 2], s1 = cs[4 * i + 3];
+          a[i] = pack2<F16>(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
+          z[i] = pack2<F16>(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + 8 * c) = lo[k];
+      *reinterpret_cast<uint4*>(dst + D / 2 + 8 * c) = hi[k];
+    }
   }
 }
 
