@@ -148,12 +148,15 @@ int launch_append(AppendParams p, int sms, cudaStream_t s) {
 // (16) for larger groups; beyond 16, several CTAs read the same keys.
 inline int decode_nt(int group) { return group > 8 ? 2 : 1; }
 
-// Tiles of a full cache.
-int64_t decode_tiles(const abft_paged_attn_args* a) {
-  const int64_t tiles = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
+// Segments (sequence, kv head, chunk of its query heads) and the tiles of one
+// in a full cache.
+int64_t decode_segments(const abft_paged_attn_args* a) {
   const int group = a->heads / a->kv.kv_heads;
   const int chunks = (group + 8 * decode_nt(group) - 1) / (8 * decode_nt(group));
-  return tiles * a->kv.batch * a->kv.kv_heads * chunks;
+  return static_cast<int64_t>(a->kv.batch) * a->kv.kv_heads * chunks;
+}
+int64_t decode_segment_tiles(const abft_paged_attn_args* a) {
+  return (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
 }
 
 int attn_check(const abft_paged_attn_args* a, bool decode) {
@@ -164,9 +167,8 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
   if ((rc = check_heads(a->heads, a->kv.kv_heads)) != ABFT_OK) return rc;
   if (decode && a->tokens != a->kv.batch) return ABFT_ERR_INVALID_ARG;
   if (a->tokens == 0 || a->kv.batch == 0) return ABFT_OK;
-  // The list of tiles (32 slots of a kv head and up to 8 or 16 of its query
-  // heads) is counted in 32 bits.
-  if (decode && decode_tiles(a) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
+  // The list of tiles is counted in 32 bits.
+  if (decode && decode_segments(a) * decode_segment_tiles(a) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
   // Grids (blocks x kv heads, rows x heads for the join) stay below 2^31.
   if (a->tokens >= (int64_t{1} << 30) / a->heads) return ABFT_ERR_UNSUPPORTED;
   if (a->q == nullptr || a->out == nullptr || (!decode && a->cu_seqlens == nullptr)) return ABFT_ERR_INVALID_ARG;
@@ -183,9 +185,8 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
 // 1,280 slots: 9.2 / 17.3 against 11.7 / 21.8. Longer ones are shared out all
 // the same, since lengths may differ by more than that.
 bool decode_by_segment(const abft_paged_attn_args* a, int sms) {
-  const int64_t tiles = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
-  const int64_t segments = decode_tiles(a) / tiles;
-  return segments <= sms && tiles <= (2 * segments >= sms ? 40 : 12);
+  const int64_t segments = decode_segments(a), slots = static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size;
+  return segments <= sms && slots <= (2 * segments >= sms ? 1280 : 384);
 }
 
 // CTAs of a decode launch: one per segment, or one per SM, fewer when the
@@ -195,10 +196,9 @@ bool decode_by_segment(const abft_paged_attn_args* a, int sms) {
 // CTAs 160 us, 148 170; of 2,048: 44 and 48), others lose nothing, since four
 // fifths of the SMs already read at full speed (120 CTAs: 168 and 49).
 int decode_grid(const abft_paged_attn_args* a, int sms) {
-  const int64_t tiles = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
-  const int64_t segments = decode_tiles(a) / tiles;
+  const int64_t segments = decode_segments(a);
   if (decode_by_segment(a, sms)) return static_cast<int>(segments);
-  const int64_t ctas = (decode_tiles(a) + kDecWarps - 1) / kDecWarps;
+  const int64_t ctas = (segments * decode_segment_tiles(a) + kDecWarps - 1) / kDecWarps;
   if (ctas <= sms) return static_cast<int>(ctas);
   for (int g = sms; 5 * g >= 4 * sms; --g)
     if (segments % g == 0 || g % segments == 0) return g;
@@ -218,7 +218,7 @@ int launch_decode(int dev, int slot, const DecodeParams& p, int grid, cudaStream
   using Cfg = DecodeCfg<D, NT>;
   int rc = raise_smem(dev, slot, paged_decode_kernel<D, NT, F16>, Cfg::kSmemBytes);
   if (rc != ABFT_OK) return rc;
-  rc = launch(paged_decode_kernel<D, NT, F16>, dim3(grid), dim3(kDecThreads), Cfg::kSmemBytes, s, p);
+  rc = launch(paged_decode_kernel<D, NT, F16>, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmemBytes, s, p);
   if (rc != ABFT_OK || p.by_segment) return rc;
   JoinParams j;
   j.out = p.out;

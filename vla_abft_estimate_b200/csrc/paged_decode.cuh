@@ -110,15 +110,20 @@ struct DecodeParams {
                            // and chunk, pieces, -), pieces 0 when there is none
 };
 
-constexpr int kDecTile = 32;  // keys of one warp step
+// Warps of a CTA and keys of a warp's step. (Eight warps on 16 keys: as fast,
+// 128 segments of 2,048 slots 26.1 against 24.6 us, the long list 50.6 against
+// 49.5: one SM takes in some 62 GB/s however many warps ask.)
 constexpr int kDecWarps = 4;
-constexpr int kDecThreads = 32 * kDecWarps;
+constexpr int kDecTile = 32;
 
 template <int D, int NT>
 struct DecodeCfg {
+  static constexpr int kWarps = kDecWarps, kThreads = 32 * kWarps;
+  static constexpr int kTile = kDecTile;
+  static constexpr int kM = kTile / 16;  // 16-key row blocks of a step
   static constexpr int kStages = D == 128 ? 3 : 6;
   static constexpr int kRowBytes = D * 2;
-  static constexpr int kHalfBytes = kDecTile * kRowBytes;  // keys of a stage; as much again for values
+  static constexpr int kHalfBytes = kTile * kRowBytes;  // keys of a stage; as much again for values
   static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kHeads = 8 * NT;
@@ -127,8 +132,8 @@ struct DecodeCfg {
   static constexpr int kPitch = D + 4;
   static constexpr int kPieceBytes = kHeads * (kPitch + 2) * 4;
   static_assert(kPieceBytes <= kWarpBytes, "a warp's last piece takes the place of its ring");
-  static constexpr int kOffFirst = kDecWarps * kWarpBytes;  // the warps' first pieces
-  static constexpr int kSmemBytes = kOffFirst + kDecWarps * kPieceBytes;
+  static constexpr int kOffFirst = kWarps * kWarpBytes;  // the warps' first pieces
+  static constexpr int kSmemBytes = kOffFirst + kWarps * kPieceBytes;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
@@ -140,12 +145,14 @@ struct TileIter {
   int len;
 };
 
+template <int kTile>
 __device__ __forceinline__ int tiles_of(const PagedView& kv, int b, int* len, bool* bad) {
   *len = paged_clamp_len(kv.seq_lens[b], kv.max_pages, kv.page_shift, bad);
-  return (*len + kDecTile - 1) / kDecTile;
+  return (*len + kTile - 1) / kTile;
 }
 
 // The next tile; only called while left > 1.
+template <int kTile>
 __device__ __forceinline__ void advance(TileIter& it, const PagedView& kv, int rows) {
   --it.left;
   if (++it.tile < it.tiles) return;
@@ -159,20 +166,21 @@ __device__ __forceinline__ void advance(TileIter& it, const PagedView& kv, int r
   bool bad;
   do {
     ++it.b;
-    it.tiles = tiles_of(kv, it.b, &it.len, &bad);
+    it.tiles = tiles_of<kTile>(kv, it.b, &it.len, &bad);
   } while (it.tiles == 0 && it.b + 1 < kv.batch);
 }
 
 template <int D, int NT, bool F16>
-__global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const DecodeParams p) {
   using Cfg = DecodeCfg<D, NT>;
+  constexpr int kTile = Cfg::kTile, kWarps = Cfg::kWarps, kM = Cfg::kM;
   extern __shared__ __align__(128) unsigned char smem[];
   // Pieces of segments that cross the warp's share: the first began in an
   // earlier share (0: there is none, 1: the segment ends in this share, 2: it
   // goes on), the last begins here and goes on (0, 2).
-  __shared__ int s_first[kDecWarps], s_last[kDecWarps];
-  __shared__ int s_seg[kDecWarps][2][2];   // (sequence, kv head and chunk) of first and last
-  __shared__ int s_end[kDecWarps];         // the last's segment: its final tile in the list
+  __shared__ int s_first[kWarps], s_last[kWarps];
+  __shared__ int s_seg[kWarps][2][2];   // (sequence, kv head and chunk) of first and last
+  __shared__ int s_end[kWarps];         // the last's segment: its final tile in the list
   constexpr int kShift = D == 128 ? 7 : 6;
   constexpr int kCpr = D / 8;  // 16-byte pieces of a row
   constexpr int kMt = D / 16;
@@ -191,9 +199,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
     head.b = blockIdx.x / rows;
     head.y = blockIdx.x - head.b * rows;
     bool bad;
-    total = head.tiles = tiles_of(kv, head.b, &head.len, &bad);
+    total = head.tiles = tiles_of<kTile>(kv, head.b, &head.len, &bad);
     if (bad && head.y == 0 && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
-    shares = kDecWarps;
+    shares = kWarps;
     u0 = head.tile = share_start(total, shares, warp);
     u1 = share_start(total, shares, warp + 1);
     head.left = u1 - u0;
@@ -203,15 +211,15 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
     for (int b = lane; b < kv.batch; b += 32) {
       int len;
       bool bad;
-      const int tiles = tiles_of(kv, b, &len, &bad);
+      const int tiles = tiles_of<kTile>(kv, b, &len, &bad);
       if (b == lane) len0 = len, tiles0 = tiles;
       sum += tiles;
       if (bad && blockIdx.x == 0 && warp == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
     }
     sum = __reduce_add_sync(0xFFFFFFFFu, sum);
     total = sum * rows;  // the host keeps it below 2^31
-    shares = gridDim.x * kDecWarps;
-    const int share = blockIdx.x * kDecWarps + warp;
+    shares = gridDim.x * kWarps;
+    const int share = blockIdx.x * kWarps + warp;
     u0 = share_start(total, shares, share);
     u1 = share_start(total, shares, share + 1);
 
@@ -222,7 +230,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
       for (int i = 0; i < kv.batch; i += 32) {
         int mine = tiles0, len = len0;
         bool bad;
-        if (i > 0) mine = i + lane < kv.batch ? tiles_of(kv, i + lane, &len, &bad) : 0;
+        if (i > 0) mine = i + lane < kv.batch ? tiles_of<kTile>(kv, i + lane, &len, &bad) : 0;
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -250,25 +258,26 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
   const uint16_t* vbase = static_cast<const uint16_t*>(kv.v_pages);
 
   // Lane i holds the table entry of 16 keys, the i-th from tile `held` on: one
-  // load serves 16 tiles, and the next 16 are asked for ahead of their use.
+  // load serves 512 keys, and the next 512 are asked for ahead of their use.
+  constexpr int kHeld = 32 / kM;  // tiles of a load
   int entry = 0, entry_next = 0, held = 0;
   auto look_up = [&](const TileIter& it, int tile) {
-    const int key = tile * kDecTile + lane * 16;
+    const int key = tile * kTile + lane * 16;
     return key < it.len ? kv.page_table[it.b * kv.table_stride + (key >> kv.page_shift)] : 0;
   };
   auto entries = [&](const TileIter& it) {  // of a segment that begins
     held = it.tile;
     entry = look_up(it, held);
-    entry_next = look_up(it, held + 16);
+    entry_next = look_up(it, held + kHeld);
   };
   auto issue = [&](const TileIter& it, int stage) {
     constexpr int kRowsPerOp = 32 / kCpr;  // rows one warp-wide copy covers
     const int sub = lane / kCpr, c = lane % kCpr;
     const int hk = p.head_chunks == 1 ? it.y : it.y / p.head_chunks;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int key0 = it.tile * kDecTile + i * 16;
-      const int page = __shfl_sync(0xFFFFFFFFu, entry, 2 * (it.tile - held) + i);
+    for (int i = 0; i < kM; ++i) {
+      const int key0 = it.tile * kTile + i * 16;
+      const int page = __shfl_sync(0xFFFFFFFFu, entry, kM * (it.tile - held) + i);
       const bool ok = page >= 0 && page < kv.num_pages;
       if (!ok && lane == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
       const int slot = key0 & ((1 << kv.page_shift) - 1);
@@ -289,7 +298,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
   float o[kMt][NT][4];
   float m[NT][2], l[NT][2];
   uint32_t qf[NT][D / 16][2];  // Q^T fragments: column g = head, rows = head dimension
-  auto begin_segment = [&](const TileIter& it) {
+  auto load_q = [&](const TileIter& it, uint32_t (&to)[NT][D / 16][2]) {
     const int hk = it.y / p.head_chunks, hc = it.y - hk * p.head_chunks;
     const int nheads = min(Cfg::kHeads, p.group - hc * Cfg::kHeads);
 #pragma unroll
@@ -301,7 +310,12 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
       for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          qf[nt][ks][i] = h < nheads ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + i * 8 + tq * 2) : 0u;
+          to[nt][ks][i] = h < nheads ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + i * 8 + tq * 2) : 0u;
+    }
+  };
+  auto begin_segment = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
@@ -342,7 +356,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
   if (lane == 0) s_first[warp] = s_last[warp] = 0;
   if (cur.left > 0) {
     entries(head);
-    begin_segment(cur);
+    load_q(cur, qf);
+    begin_segment();
     bool from_before = cur.tile > 0;  // the segment began in an earlier share
     int ahead = head.left;            // tiles not yet issued
     int stage = 0;
@@ -350,13 +365,13 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
       if (ahead > 0) {
         issue(head, sn);
         if (--ahead > 0) {
-          advance(head, kv, rows);
+          advance<kTile>(head, kv, rows);
           if (head.tile == 0) {
             entries(head);
-          } else if (head.tile - held == 16) {
-            held += 16;
+          } else if (head.tile - held == kHeld) {
+            held += kHeld;
             entry = entry_next;
-            entry_next = look_up(head, held + 16);
+            entry_next = look_up(head, held + kHeld);
           }
         }
       }
@@ -369,12 +384,20 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
       __syncwarp();
       // Refill the stage that the previous step emptied.
       fill(stage == 0 ? Cfg::kStages - 1 : stage - 1);
+      // The next segment's query rows are asked for under this one's last step.
+      const bool ends = cur.tile + 1 == cur.tiles, stops = cur.left == 1;
+      uint32_t qn[NT][D / 16][2];
+      TileIter next = cur;
+      if (!stops) {
+        advance<kTile>(next, kv, rows);
+        if (ends) load_q(next, qn);
+      }
       const uint32_t ks_base = ring + stage * Cfg::kStageBytes;
       const uint32_t vs_base = ks_base + Cfg::kHalfBytes;
 
-      float s[2][NT][4];
+      float s[kM][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < kM; ++mt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -382,7 +405,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < kM; ++mt) {
           const int r = mt * 16 + (lane & 15);
           const int c = ks * 2 + (lane >> 4);
           uint32_t a[4];
@@ -393,8 +416,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
       }
 
       // Scores in units of log2(e); keys behind the length drop out.
-      const int key_g = cur.tile * kDecTile + g;
-      const bool ragged = cur.tile * kDecTile + kDecTile > cur.len;
+      const int key_g = cur.tile * kTile + g;
+      const bool ragged = cur.tile * kTile + kTile > cur.len;
       float scale[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -402,7 +425,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
         for (int e = 0; e < 2; ++e) {
           float top = -INFINITY;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < kM; ++mt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               float& x = s[mt][nt][half * 2 + e];
@@ -419,7 +442,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
           m[nt][e] = mn;
           float sum_p = 0.f;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < kM; ++mt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               float& x = s[mt][nt][half * 2 + e];
@@ -438,9 +461,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
       }
 
       // P^T fragments (column = head), hi and lo terms, by 16 keys.
-      uint32_t ph[2][NT][2], pl[2][NT][2];
+      uint32_t ph[kM][NT][2], pl[kM][NT][2];
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+      for (int kk = 0; kk < kM; ++kk)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -452,7 +475,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
             pl[kk][nt][half] = movm_t(pack2<F16>(x - back.x, y - back.y));
           }
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+      for (int kk = 0; kk < kM; ++kk)
 #pragma unroll
         for (int mt = 0; mt < kMt; ++mt) {
           const int r = kk * 16 + (lane & 7) + ((lane >> 4) << 3);
@@ -468,7 +491,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
       __syncwarp();  // every lane has read the stage before it is refilled
       if (++stage == Cfg::kStages) stage = 0;
 
-      const bool ends = cur.tile + 1 == cur.tiles, stops = cur.left == 1;
       if (ends || stops) {
         fold_l();
         if (from_before) {
@@ -512,9 +534,13 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
         }
         if (stops) break;
       }
-      advance(cur, kv, rows);
+      cur = next;
       if (ends) {
-        begin_segment(cur);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) qf[nt][ks][0] = qn[nt][ks][0], qf[nt][ks][1] = qn[nt][ks][1];
+        begin_segment();
         from_before = false;
       }
     }
@@ -524,8 +550,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
   for (int b = blockIdx.x; b < kv.batch; b += gridDim.x) {
     int len;
     bool bad;
-    if (tiles_of(kv, b, &len, &bad) == 0)
-      for (int i = threadIdx.x; i < kv.kv_heads * p.group * kCpr; i += kDecThreads)
+    if (tiles_of<kTile>(kv, b, &len, &bad) == 0)
+      for (int i = threadIdx.x; i < kv.kv_heads * p.group * kCpr; i += Cfg::kThreads)
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + b * p.ot + (i / kCpr) * p.oh + (i % kCpr) * 8) =
             make_uint4(0u, 0u, 0u, 0u);
   }
@@ -538,11 +564,11 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
   // pieces at once.
   int over = -1;  // warp whose last piece goes on in the next CTA
 #pragma unroll 1
-  for (int w = -1; w < kDecWarps; ++w) {
+  for (int w = -1; w < kWarps; ++w) {
     if (w < 0 ? s_first[0] == 0 : s_last[w] == 0) continue;
     int to = w + 1;
     bool on = true;
-    while (to < kDecWarps && on) on = s_first[to++] == 2;
+    while (to < kWarps && on) on = s_first[to++] == 2;
     const int b = w < 0 ? s_seg[0][0][0] : s_seg[w][1][0], y = w < 0 ? s_seg[0][0][1] : s_seg[w][1][1];
     const int hk = y / p.head_chunks, hc = y - hk * p.head_chunks;
     const int nheads = min(Cfg::kHeads, p.group - hc * Cfg::kHeads);
@@ -552,12 +578,12 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
     constexpr int kPer = D / 16;
     const int d = (threadIdx.x & 15) * kPer;
 #pragma unroll 1
-    for (int h = threadIdx.x >> 4; h < nheads; h += kDecThreads / 16) {
-      const float* at[kDecWarps + 1];  // the last piece of warp w, the first pieces of warps w + 1 .. to - 1
-      float2 ml[kDecWarps + 1];
+    for (int h = threadIdx.x >> 4; h < nheads; h += Cfg::kThreads / 16) {
+      const float* at[kWarps + 1];  // the last piece of warp w, the first pieces of warps w + 1 .. to - 1
+      float2 ml[kWarps + 1];
       float top = -INFINITY;
 #pragma unroll
-      for (int k = 0; k <= kDecWarps; ++k) {
+      for (int k = 0; k <= kWarps; ++k) {
         const bool used = k == 0 ? w >= 0 : (k - 1 > w && k - 1 < to);
         at[k] = reinterpret_cast<const float*>(k == 0 ? smem + max(w, 0) * Cfg::kWarpBytes
                                                       : smem + Cfg::kOffFirst + (k - 1) * Cfg::kPieceBytes);
@@ -571,7 +597,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
 #pragma unroll
       for (int i = 0; i < kPer; ++i) x[i] = 0.f;
 #pragma unroll
-      for (int k = 0; k <= kDecWarps; ++k) {
+      for (int k = 0; k <= kWarps; ++k) {
         if (at[k] == nullptr) continue;
         const float f = exp2_approx(ml[k].x - ms);
         l_sum += ml[k].y * f;
@@ -604,7 +630,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) paged_decode_kernel(const Deco
     int4 spill = make_int4(0, 0, 0, 0);
     if (over >= 0)
       spill = make_int4(s_seg[over][1][0], s_seg[over][1][1],
-                        share_of(total, shares, s_end[over]) / kDecWarps - static_cast<int>(blockIdx.x) + 1, 0);
+                        share_of(total, shares, s_end[over]) / kWarps - static_cast<int>(blockIdx.x) + 1, 0);
     p.spill[blockIdx.x] = spill;
   }
 }
