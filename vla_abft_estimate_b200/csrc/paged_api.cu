@@ -294,7 +294,7 @@ PrefillPlan prefill_plan(const abft_paged_attn_args* a, int sms) {
   const int64_t steps = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kPreKeys - 1) / kPreKeys;
   // Pieces, of four steps at least: as many as give each SM one item, counted
   // without the blocks that only ragged chunks have, and twice as many for
-  // several sequences, whose lengths may differ. (One sequence, 64 tokens on
+  // several sequences, whose lengths may differ, if one each is not enough. (One sequence, 64 tokens on
   // 16,384: 1 piece 214 us, 8 pieces 41, 16 51; 512 tokens on 8,192, 116 items:
   // 1 piece 118, 2 pieces 129, for the sums that go through memory. Nine
   // sequences of 5 tokens on up to 7,777: 4 pieces 35, 8 pieces 25; four on
@@ -303,7 +303,8 @@ PrefillPlan prefill_plan(const abft_paged_attn_args* a, int sms) {
   if (n == 0) {
     int64_t least = (a->tokens + r.block_tokens - 1) / r.block_tokens;
     if (least < a->kv.batch) least = a->kv.batch;
-    n = (a->kv.batch > 1 ? 2 : 1) * sms / (least * a->kv.kv_heads);
+    n = sms / (least * a->kv.kv_heads);
+    if (n > 1 && a->kv.batch > 1) n *= 2;
     if (n > steps / 4) n = steps / 4;
   }
   if (n > steps) n = steps;

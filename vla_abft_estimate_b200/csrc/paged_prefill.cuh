@@ -109,14 +109,16 @@ __host__ __device__ __forceinline__ int visible_keys(int len, int n, int i) {
 
 // Block `index` of the packed sequences, each cut into blocks of `per`
 // tokens; called by one warp. Heavier blocks (later tokens) of a sequence
-// come first. Returns false behind the last block.
-__device__ __forceinline__ bool find_block(const int32_t* cu, int batch, int tokens, int per, int index, int lane,
-                                           int* seq, int* block) {
+// come first. Boundaries and lengths are asked for together; *begin, *count
+// and *len are the sequence's packed rows and raw length. Returns false behind
+// the last block.
+__device__ __forceinline__ bool find_block(const PagedView& kv, const int32_t* cu, int tokens, int per, int index, int lane,
+                                           int* seq, int* block, int* begin, int* count, int* len) {
   int before = 0;
-  for (int i = 0; i < batch; i += 32) {
-    int mine = 0;
-    if (i + lane < batch) {
-      int lo, hi;
+  for (int i = 0; i < kv.batch; i += 32) {
+    int mine = 0, lo = 0, hi = 0, length = 0;
+    if (i + lane < kv.batch) {
+      length = kv.seq_lens[i + lane];
       packed_range(cu, i + lane, tokens, &lo, &hi);
       mine = (hi - lo + per - 1) / per;
     }
@@ -130,11 +132,14 @@ __device__ __forceinline__ bool find_block(const int32_t* cu, int batch, int tok
     if (past != 0) {
       const int src = __ffs(past) - 1;
       const int first = before + __shfl_sync(0xFFFFFFFFu, upto - mine, src);
-      const int count = __shfl_sync(0xFFFFFFFFu, mine, src);
-      const int at = count - 1 - (index - first);
-      if (at < 0 || at >= count) return false;  // boundaries that do not rise
+      const int blocks = __shfl_sync(0xFFFFFFFFu, mine, src);
+      const int at = blocks - 1 - (index - first);
+      if (at < 0 || at >= blocks) return false;  // boundaries that do not rise
       *seq = i + src;
       *block = at;
+      *begin = __shfl_sync(0xFFFFFFFFu, lo, src);
+      *count = __shfl_sync(0xFFFFFFFFu, hi - lo, src);
+      *len = __shfl_sync(0xFFFFFFFFu, length, src);
       return true;
     }
     before += __shfl_sync(0xFFFFFFFFu, upto, 31);
@@ -471,17 +476,20 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       // The next item's Q comes while the last product runs (all of this
-      // item's Q K^T are done: the rows have seen the last scores).
-      const bool next = wait_item(i + 1);
-      const bool more = next && steps_end(items[(i + 1) & 1]) > items[(i + 1) & 1].j0;
-      if (more) load_q(items[(i + 1) & 1]);
+      // item's Q K^T are done: the rows have seen the last scores), if the item
+      // is there already.
+      const PrefillItem& y = items[(i + 1) & 1];
+      const bool early = __all_sync(0xFFFFFFFFu, mbar_try_wait(&item_full[(i + 1) & 1], ((i + 1) >> 1) & 1));
+      bool next = early && y.valid != 0;
+      const bool soon = next && steps_end(y) > y.j0;
+      if (soon) load_q(y);
       const bool any = end > j0;
       if (any) {
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[t], used & 1, abort_flag));
         tc_fence_after();
         ++used;
       }
-      if (more) send_q();
+      if (soon) send_q();
       if (!ok) break;
       const int first = x.tok0 + t * p.tile_tokens, r = row_of_thread();
       const int tok = row_token(r, p.group_inv);
@@ -526,6 +534,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       tc_fence_before();  // O is read before the next item's first P is announced
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[i & 1]);
+      if (!early) {
+        next = wait_item(i + 1);
+        if (next && steps_end(y) > y.j0) {
+          load_q(y);
+          send_q();
+        }
+      }
       ok = next;
     }
     tc_fence_before();
@@ -713,14 +728,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           x.split = index / p.items;
           const int rest = index - x.split * p.items;
           x.hk = rest % kv.kv_heads;
-          int seq = 0, block = 0;
-          if (find_block(p.cu, kv.batch, p.tokens, p.block_tokens, rest / kv.kv_heads, lane, &seq, &block)) {
-            int row_end;
-            packed_range(p.cu, seq, p.tokens, &x.row0, &row_end);
-            x.n = row_end - x.row0;
+          int seq = 0, block = 0, raw_len = 0;
+          if (find_block(kv, p.cu, p.tokens, p.block_tokens, rest / kv.kv_heads, lane, &seq, &block, &x.row0, &x.n,
+                         &raw_len)) {
             bool bad_len;
             x.seq = seq;
-            x.len = paged_clamp_len(kv.seq_lens[seq], kv.max_pages, kv.page_shift, &bad_len);
+            x.len = paged_clamp_len(raw_len, kv.max_pages, kv.page_shift, &bad_len);
             if ((bad_len || x.len < x.n) && lane == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
             // Steps of each tile (a tile behind the rows' end has none) and of
             // this piece.
