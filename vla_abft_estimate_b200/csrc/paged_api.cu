@@ -19,7 +19,7 @@ constexpr int kMaxDevices = 64;
 struct DeviceInfo {
   bool init, ok;
   int sms;
-  bool smem_set[12];  // decode instances 0-7, prefill instances 8-11
+  bool smem_set[16];  // decode instances 0-7, prefill instances 8-15
 };
 DeviceInfo g_paged_dev[kMaxDevices];
 std::mutex g_paged_mu;
@@ -321,13 +321,13 @@ size_t prefill_bytes(const abft_paged_attn_args* a, int splits) {
   return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2));
 }
 
-template <int D, bool F16>
+template <int D, bool F16, bool kShared>
 int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                    const PrefillParams& p, int64_t items, cudaStream_t s) {
   using Cfg = PrefillCfg<D>;
-  int rc = raise_smem(dev, slot, paged_prefill_kernel<D, F16>, Cfg::kSmemBytes);
+  int rc = raise_smem(dev, slot, paged_prefill_kernel<D, F16, kShared>, Cfg::kSmemBytes);
   if (rc != ABFT_OK) return rc;
-  rc = launch(paged_prefill_kernel<D, F16>, dim3(static_cast<unsigned>(items)), dim3(kPreThreads), Cfg::kSmemBytes, s,
+  rc = launch(paged_prefill_kernel<D, F16, kShared>, dim3(static_cast<unsigned>(items)), dim3(kPreThreads), Cfg::kSmemBytes, s,
               tm_k, tm_v, p);
   if (rc != ABFT_OK || p.splits == 1) return rc;
   PrefillJoinParams j;
@@ -478,11 +478,19 @@ int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
   if ((rc = page_map(&tm_v, a->kv, a->kv.v_pages, a->kv.v_page_stride)) != ABFT_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
-  if (a->kv.head_dim == 128)
-    return f16 ? launch_prefill<128, true>(dev, 11, a, tm_k, tm_v, p, plan.items, s)
-               : launch_prefill<128, false>(dev, 10, a, tm_k, tm_v, p, plan.items, s);
-  return f16 ? launch_prefill<64, true>(dev, 9, a, tm_k, tm_v, p, plan.items, s)
-             : launch_prefill<64, false>(dev, 8, a, tm_k, tm_v, p, plan.items, s);
+  const bool shared = plan.block_tokens == plan.tile_tokens;
+  const int slot = 8 + (a->kv.head_dim == 128 ? 4 : 0) + (f16 ? 2 : 0) + (shared ? 1 : 0);
+  const int64_t items = plan.items;
+  switch (slot - 8) {
+    case 0: return launch_prefill<64, false, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 1: return launch_prefill<64, false, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 2: return launch_prefill<64, true, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 3: return launch_prefill<64, true, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 4: return launch_prefill<128, false, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 5: return launch_prefill<128, false, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 6: return launch_prefill<128, true, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    default: return launch_prefill<128, true, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+  }
 }
 
 }  // extern "C"

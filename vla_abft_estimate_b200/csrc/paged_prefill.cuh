@@ -22,9 +22,19 @@
 // l then still fit their formats, and the quotient is unchanged), which after
 // the first tiles of a row hardly happens.
 //
+// A call with few rows takes one tile an item, and both groups of row warps
+// work on it, on every other step each ("shared" below), with an O of their
+// own; the two are added at the end (512 tokens on 8,192 slots: 118 us with one
+// group at work, 86 with both, the rate at which an SM takes in K and V).
+//
+// The grid has a block for every work item (one or two tiles, kv head, piece of
+// the keys); a resident CTA takes over the items of blocks that have not
+// started (cluster launch control), so that the next item's loads, Q K^T and
+// set-up run under the last one's end, and items without work cost no launch.
+//
 // Warps: 0-3 and 4-7 the rows of tile 0 and 1 (TMEM lane quadrant = warp % 4),
-// 8 TMA loads of pages into a ring of tiles, 9 the MMA issuer, 10 and 11 idle
-// (registers move between groups of four warps).
+// 8 TMA loads of pages into a ring of tiles, 9 the MMA issuer, 10 finds the
+// work, 11 idle (registers move between groups of four warps).
 #pragma once
 
 #include <cuda.h>
@@ -55,8 +65,8 @@ struct PrefillCfg {
   static constexpr int kOffRing = 2 * kTileBytes;            // after the two Q tiles
   static constexpr int kOffBar = kOffRing + kSlots * kTileBytes;
   // full, empty, qfull, sfull, pfull, ofull, item full and empty, work, loaded,
-  // drain, (even number)
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 4 + 1 + 1 + 2;
+  // both, drain, one unused (an even number)
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 4 + 1 + 1 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kOffItems = kOffMisc + 16;  // two items and the launch-control answer
   static constexpr int kSmemBytes = kOffItems + 2 * 48 + 16 + 1024;
@@ -264,7 +274,9 @@ __device__ __forceinline__ int work_answer(const void* answer) {
   return ok ? static_cast<int>(x) : -1;
 }
 
-template <int D, bool F16>
+// kShared: one tile an item, its steps shared by both groups of row warps. (A
+// template argument: asked at run time it cost the two-tile form 2.5%.)
+template <int D, bool F16, bool kShared>
 __global__ void __launch_bounds__(kPreThreads, 1)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                          const PrefillParams p) {
@@ -281,7 +293,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   uint64_t* item_empty = item_full + 2;
   uint64_t* work = item_empty + 2;
   uint64_t* loaded_all = work + 1;
-  uint64_t* drain = loaded_all + 1;
+  uint64_t* both = loaded_all + 1;  // shared items: all row warps have come this far
+  uint64_t* drain = both + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PrefillItem* items = reinterpret_cast<PrefillItem*>(smem + Cfg::kOffItems);
@@ -304,6 +317,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     }
     mbar_init(work, 1);
     mbar_init(loaded_all, 1);
+    mbar_init(both, 2 * kPreRows);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -347,6 +361,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     };
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t ts = lanes + t * 128, to = lanes + Cfg::kColO + t * D;
+    const int tile = kShared ? 0 : t;                            // whose rows these are
+    const int lag = kShared ? t : 0, stride = kShared ? 2 : 1;  // this group's steps: j0 + lag, by stride
+    int met = 0;  // times the groups have waited for each other
+    auto meet = [&]() {
+      mbar_arrive(both);
+      const bool all = __all_sync(0xFFFFFFFFu, mbar_wait(both, met & 1, abort_flag));
+      ++met;
+      return all;
+    };
     // Items stay in their slots while the rows work on them and are read
     // there: a row of S leaves few registers.
     auto wait_item = [&](int i) {
@@ -354,10 +377,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
              items[i & 1].valid != 0;
     };
     auto steps_end = [&](const PrefillItem& x) { return t == 0 ? x.end0 : x.end1; };
+    auto has_q = [&](const PrefillItem& x) { return steps_end(x) > x.j0 && (t == 0 || !kShared); };
     // Q tile into shared memory, in the swizzled layout of a TMA box.
     auto load_q = [&](const PrefillItem& x) {
       int r = row_of_thread();
-      const int first = x.tok0 + t * p.tile_tokens;
+      const int first = x.tok0 + tile * p.tile_tokens;
       const int here = max(0, min(p.tile_tokens, x.n - first)) * p.group;
       const uint32_t dst = smem_u32(smem + t * Cfg::kTileBytes);
       constexpr int kCpr = D / 8;
@@ -381,7 +405,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     };
     bool ok = wait_item(0);
     int count = 0, used = 0;  // steps and items of this tile so far
-    if (ok && steps_end(items[0]) > items[0].j0) {
+    if (ok && has_q(items[0])) {
       load_q(items[0]);
       send_q();
     }
@@ -390,13 +414,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const int end = steps_end(x), j0 = x.j0;
       int vis, vis_min;  // keys seen by the row (0: not in use) and by the tile's first token
       {
-        const int first = x.tok0 + t * p.tile_tokens, r = row_of_thread();
+        const int first = x.tok0 + tile * p.tile_tokens, r = row_of_thread();
         const bool live = r < max(0, min(p.tile_tokens, x.n - first)) * p.group;
         vis = live ? visible_keys(x.len, x.n, first + row_token(r, p.group_inv)) : 0;
         vis_min = visible_keys(x.len, x.n, first);
       }
       float m = -INFINITY, l = 0.f;                         // m: maximum that P refers to (raw scores)
-      for (int j = j0; j < end; ++j, ++count) {
+      const int begin = j0 + lag;
+      for (int j = begin; j < end; j += stride, ++count) {
         if (!mbar_wait(&sfull[t], count & 1, abort_flag)) {
           ok = false;
           break;
@@ -431,11 +456,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);  // NaN if a score is
         // Also true from m = -inf and for NaN, but not while all is -inf.
         const bool raise = !((mn - m) * p.scale_log2 <= 8.f) && mn != -INFINITY;
-        if (j == j0 || __any_sync(0xFFFFFFFFu, raise)) {
+        if (j == begin || __any_sync(0xFFFFFFFFu, raise)) {
           if (mn == INFINITY) mn = __int_as_float(0x7FC00000);  // inf - inf: the row is NaN
           const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * p.scale_log2);
           m = mn;
-          if (j > j0) {
+          if (j > begin) {
             l *= f;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -476,67 +501,116 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       // The next item's Q comes while the last product runs (all of this
-      // item's Q K^T are done: the rows have seen the last scores), if the item
-      // is there already.
+      // item's Q K^T are done: the rows have seen the last scores; of a shared
+      // item they have when both groups' last product is done), if the item is
+      // there already.
       const PrefillItem& y = items[(i + 1) & 1];
       const bool early = __all_sync(0xFFFFFFFFu, mbar_try_wait(&item_full[(i + 1) & 1], ((i + 1) >> 1) & 1));
       bool next = early && y.valid != 0;
-      const bool soon = next && steps_end(y) > y.j0;
-      if (soon) load_q(y);
-      const bool any = end > j0;
+      const bool soon = next && has_q(y);
+      if (soon && !kShared) load_q(y);
+      const bool any = end > begin;
       if (any) {
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[t], used & 1, abort_flag));
         tc_fence_after();
         ++used;
       }
-      if (soon) send_q();
+      if (soon && !kShared) send_q();
       if (!ok) break;
-      const int first = x.tok0 + t * p.tile_tokens, r = row_of_thread();
+      const int first = x.tok0 + tile * p.tile_tokens, r = row_of_thread();
       const int tok = row_token(r, p.group_inv);
       const bool live = r < max(0, min(p.tile_tokens, x.n - first)) * p.group;
       const int head = x.hk * p.group + (r - tok * p.group);
       const int64_t row = x.row0 + first + tok;
-      if (any) {
-        // The row's sums, in 32-column pieces.
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const int64_t at = (row * (kv.kv_heads * p.group) + head) * p.splits + x.split;
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
-        float* part = p.part_o + at * D;
-        if (p.splits > 1 && live) p.part_ml[at] = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
+      const int64_t at = (row * (kv.kv_heads * p.group) + head) * p.splits + x.split;
+      uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
+      if (kShared ? end == j0 : !any) {  // no keys
+        if (live && (t == 0 || !kShared)) {
+          if (p.splits == 1)
+            for (int k = 0; k < D; k += 8) *reinterpret_cast<uint4*>(dst + k) = make_uint4(0u, 0u, 0u, 0u);
+          else
+            p.part_ml[at] = make_float2(-INFINITY, 0.f);
+        }
+        if (soon && kShared) {
+          load_q(y);
+          send_q();
+        }
+      } else {
+        // Factors of the sums in TMEM: for a tile of its own 1 / l, or 1 when
+        // pieces are joined later; for a shared one those of both groups' (m,
+        // l), exchanged through the second Q tile's place, and each group takes
+        // half the columns.
+        int c0 = 0, c1 = D;
+        float f0 = 1.f, f1 = 0.f;  // of O 0 (or the tile's own O), of O 1
+        if (kShared) {
+          float2* swap = reinterpret_cast<float2*>(smem + Cfg::kTileBytes);
+          swap[t * kPreRows + r] = make_float2(m, l);
+          tc_fence_before();
+          ok = meet();
+          if (!ok) break;
+          tc_fence_after();
+          if (soon) load_q(y);
+          const float2 a = swap[r], z = swap[kPreRows + r];
+          m = fmaxf(a.x, z.x);
+          f0 = a.x == -INFINITY ? 0.f : exp2_approx((a.x - m) * p.scale_log2);
+          f1 = z.x == -INFINITY ? 0.f : exp2_approx((z.x - m) * p.scale_log2);
+          l = a.y * f0 + z.y * f1;
+          c0 = t * (D / 2);
+          c1 = c0 + D / 2;
+        }
+        if (p.splits > 1) {
+          if (live && c0 == 0) p.part_ml[at] = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
+        } else {
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          f0 *= inv;
+          f1 *= inv;
+        }
+        const bool add = kShared && end > j0 + 1;  // the second group had a step
+        const uint32_t from = kShared ? lanes + Cfg::kColO : to;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = c0; c < c1; c += 32) {
           uint32_t o[32];
-          tmem_ld_32x32b_x32(to + c, o);
+          tmem_ld_32x32b_x32(from + c, o);
           tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f0);
+          if (add) {
+            uint32_t z[32];
+            tmem_ld_32x32b_x32(from + D + c, z);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(z[k]), f1, __uint_as_float(o[k])));
+          }
           if (!live) continue;
           if (p.splits > 1) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<uint4*>(part + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              *reinterpret_cast<uint4*>(p.part_o + at * D + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           } else {
 #pragma unroll
             for (int k = 0; k < 32; k += 8) {
-              uint4 y;
-              y.x = pack2<F16>(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
-              y.y = pack2<F16>(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
-              y.z = pack2<F16>(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
-              y.w = pack2<F16>(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + c + k) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : y;
+              uint4 w;
+              w.x = pack2<F16>(__uint_as_float(o[k]), __uint_as_float(o[k + 1]));
+              w.y = pack2<F16>(__uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+              w.z = pack2<F16>(__uint_as_float(o[k + 4]), __uint_as_float(o[k + 5]));
+              w.w = pack2<F16>(__uint_as_float(o[k + 6]), __uint_as_float(o[k + 7]));
+              *reinterpret_cast<uint4*>(dst + c + k) = l == 0.f ? make_uint4(0u, 0u, 0u, 0u) : w;
             }
           }
         }
-      } else if (live && p.splits == 1) {
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
-        for (int k = 0; k < D; k += 8) *reinterpret_cast<uint4*>(dst + k) = make_uint4(0u, 0u, 0u, 0u);
-      } else if (live) {
-        p.part_ml[(row * (kv.kv_heads * p.group) + head) * p.splits + x.split] = make_float2(-INFINITY, 0.f);
+        if (kShared) {
+          if (soon) send_q();
+          tc_fence_before();
+          ok = meet();  // both O are read before either is written again
+          if (!ok) break;
+        }
       }
       tc_fence_before();  // O is read before the next item's first P is announced
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[i & 1]);
       if (!early) {
         next = wait_item(i + 1);
-        if (next && steps_end(y) > y.j0) {
+        if (next && has_q(y)) {
           load_q(y);
           send_q();
         }
@@ -560,28 +634,38 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           const int at = j * per_step + lane;
           return lane < per_step && at < held ? table[at] : 0;
         };
-        int next = x.j0 < x.j1 ? entry(x.j0) : 0;
-        for (int j = x.j0; j < x.j1 && ok; ++j) {
-          const int id = next;
-          if (j + 1 < x.j1) next = entry(j + 1);
+        // Keys come `lead` steps before the values: K of the first steps, then
+        // V and the next K in turn, as the issuer uses them.
+        const int lead = kShared ? 2 : 1;
+        int ids[3];  // table entries of steps j, j + 1, j + 2
+#pragma unroll
+        for (int k = 0; k < 3; ++k) ids[k] = x.j0 + k < x.j1 ? entry(x.j0 + k) : 0;
+        auto load = [&](int j, int id, bool values) {
           const int pieces = min(per_step, held - j * per_step);
           const bool mine = lane < pieces;
-          if (mine && (id < 0 || id >= kv.num_pages) && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int slot = issued % Cfg::kSlots;
-            if (issued >= Cfg::kSlots && !mbar_wait(&empty[slot], (issued / Cfg::kSlots - 1) & 1, abort_flag)) ok = false;
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(pieces * page * D * 2));
-            __syncwarp();
-            if (mine) {
-              // A bad id lies outside the map's page dimension and loads zeros.
-              const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes) + lane * page * D * 2;
-              tma_load_5d(dst, k == 0 ? &tm_k : &tm_v, &full[slot], 0, 0, 0, x.hk << (kv.page_shift - 3), id);
-            }
-            ++issued;
+          if (!values && mine && (id < 0 || id >= kv.num_pages) && kv.status != nullptr)
+            atomicOr(kv.status, ABFT_PAGED_BAD_PAGE);
+          const int slot = issued % Cfg::kSlots;
+          if (issued >= Cfg::kSlots && !mbar_wait(&empty[slot], (issued / Cfg::kSlots - 1) & 1, abort_flag)) ok = false;
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) return;
+          if (lane == 0) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(pieces * page * D * 2));
+          __syncwarp();
+          if (mine) {
+            // A bad id lies outside the map's page dimension and loads zeros.
+            const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes) + lane * page * D * 2;
+            tma_load_5d(dst, values ? &tm_v : &tm_k, &full[slot], 0, 0, 0, x.hk << (kv.page_shift - 3), id);
           }
+          ++issued;
+        };
+        if (x.j0 < x.j1) load(x.j0, ids[0], false);
+        if (lead == 2 && x.j0 + 1 < x.j1 && ok) load(x.j0 + 1, ids[1], false);
+        for (int j = x.j0; j < x.j1 && ok; ++j) {
+          load(j, ids[0], true);
+          if (j + lead < x.j1 && ok) load(j + lead, lead == 2 ? ids[2] : ids[1], false);
+          ids[0] = ids[1];
+          ids[1] = ids[2];
+          ids[2] = j + 3 < x.j1 ? entry(j + 3) : 0;
         }
         if (lane == 0) mbar_arrive(loaded_all);
       }
@@ -612,9 +696,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         tc_fence_after();
         return ok;
       };
+      const int lead = kShared ? 2 : 1;  // steps between a group's own
       auto scores = [&](int t, int at) {
         if (elect_one()) {
-          const uint64_t dq = desc_q + t * (Cfg::kTileBytes >> 4), dk = desc_k + at * (Cfg::kTileBytes >> 4);
+          const uint64_t dq = desc_q + (kShared ? 0 : t) * (Cfg::kTileBytes >> 4), dk = desc_k + at * (Cfg::kTileBytes >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             umma_bf16_ss(tm + t * 128, dq + (((k / 4) * Cfg::kBlockBytes + (k % 4) * 32) >> 4),
@@ -640,10 +725,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         const int stop[2] = {__shfl_sync(0xFFFFFFFFu, x.end0, 0), __shfl_sync(0xFFFFFFFFu, x.end1, 0)};
         const int length = __shfl_sync(0xFFFFFFFFu, x.len, 0);
         if (first_j >= last_j) continue;
+        // The first scores of each tile (of a shared item: of its first two
+        // steps).
         if (!ready(slot, phase)) break;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (stop[t] > first_j && ok) {
+          if (stop[t] > first_j && (t == 0 || !kShared) && ok) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(&qfull[t], qcount[t] & 1, abort_flag));
             ++qcount[t];
             tc_fence_after();
@@ -652,6 +739,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (!ok) break;
         release(slot);
         step_ring();
+        if (kShared && first_j + 1 < last_j) {
+          if (!ready(slot, phase)) break;
+          scores(1, slot);
+          release(slot);
+          step_ring();
+        }
         for (int j = first_j; j < last_j && ok; ++j) {
           const int vs = slot;
           if (!ready(vs, phase)) break;
@@ -675,6 +768,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           bool loaded = false;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
+            if (kShared && t != ((j - first_j) & 1)) continue;
             if (j < stop[t] && ok) {
               ok = __all_sync(0xFFFFFFFFu, mbar_wait(&pfull[t], pcount[t] & 1, abort_flag));
               ++pcount[t];
@@ -683,7 +777,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 if (elect_one()) {
                   const uint64_t dv = desc_v + vs * (Cfg::kTileBytes >> 4);
                   const uint32_t d = tm + Cfg::kColO + t * D, a = tm + t * 128;
-                  umma_f16_ts(d, a, dv, idesc_o, j > first_j);
+                  umma_f16_ts(d, a, dv, idesc_o, j >= first_j + lead);
                   if (groups == kPreKeys / 16) {
 #pragma unroll
                     for (int k = 1; k < kPreKeys / 16; ++k)
@@ -692,12 +786,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                     for (int k = 1; k < groups; ++k)
                       umma_f16_ts(d, a + k * 8, dv + k * (2 * Cfg::kGroupBytes >> 4), idesc_o, 1);
                   }
-                  if (j + 1 == stop[t]) umma_commit(&ofull[t]);
+                  if (j + lead >= stop[t]) umma_commit(&ofull[t]);
                 }
                 __syncwarp();
               }
             }
-            if (j + 1 < stop[t] && ok) {
+            if (j + lead < stop[t] && ok) {
               if (!loaded) ready(slot, phase);
               loaded = true;
               if (ok) scores(t, slot);
@@ -749,7 +843,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             x.j0 = min(x.split * p.piece, most);
             x.j1 = min(x.j0 + p.piece, most);
             x.end0 = max(x.j0, min(x.j1, steps[0]));
-            x.end1 = max(x.j0, min(x.j1, steps[1]));
+            x.end1 = kShared ? x.end0 : max(x.j0, min(x.j1, steps[1]));
             // Without keys the rows still get their zeros when no join follows.
             publish = x.j0 < x.j1 || p.splits == 1;
             x.valid = 1;
