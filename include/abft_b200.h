@@ -488,7 +488,7 @@ typedef struct abft_paged_attn_args {
   size_t workspace_bytes;     /* abft_paged_*_workspace_bytes()                        */
   int32_t num_splits;         /* prefill: pieces the keys of a block of query rows are */
                               /* cut into, 0 = choose; decode: not used                */
-  int32_t num_sms;            /* SMs to plan for, 0 = all of the current device        */
+  int32_t num_sms;            /* SMs to plan for (at most 4096), 0 = all the device's  */
 } abft_paged_attn_args;
 
 int abft_kv_append(const abft_kv_append_args* args, void* stream);

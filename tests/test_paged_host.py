@@ -201,7 +201,7 @@ def test_attention_refusals():
 
     for fn in (L.abft_paged_decode, L.abft_paged_prefill):
         assert fn(None, None) == -1
-        for over, code in [({"tokens": -1}, -1), ({"num_splits": -1}, -1), ({"num_sms": -1}, -1),
+        for over, code in [({"tokens": -1}, -1), ({"num_splits": -1}, -1), ({"num_sms": -1}, -1), ({"num_sms": 5000}, -3),
                            ({"scale": float("inf")}, -1), ({"scale": float("nan")}, -1), ({"heads": 0}, -1),
                            ({"heads": 27}, -1), ({"heads": 4 * 65}, -3), ({"q": None}, -1), ({"out": None}, -1),
                            ({"q": 0x50008}, -2), ({"out": 0x60004}, -2), ({"q_token_stride": 4}, -2),

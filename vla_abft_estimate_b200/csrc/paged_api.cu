@@ -159,11 +159,14 @@ int64_t decode_segment_tiles(const abft_paged_attn_args* a) {
   return (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kDecTile - 1) / kDecTile;
 }
 
+constexpr int kMostSms = 4096;  // more than any device has: scratch grows with it
+
 int attn_check(const abft_paged_attn_args* a, bool decode) {
   if (a == nullptr) return ABFT_ERR_INVALID_ARG;
   int rc = check_kv(a->kv);
   if (rc != ABFT_OK) return rc;
   if (a->tokens < 0 || a->num_splits < 0 || a->num_sms < 0 || !isfinite(a->scale)) return ABFT_ERR_INVALID_ARG;
+  if (a->num_sms > kMostSms) return ABFT_ERR_UNSUPPORTED;
   if ((rc = check_heads(a->heads, a->kv.kv_heads)) != ABFT_OK) return rc;
   if (decode && a->tokens != a->kv.batch) return ABFT_ERR_INVALID_ARG;
   if (a->tokens == 0 || a->kv.batch == 0) return ABFT_OK;
@@ -294,11 +297,11 @@ PrefillPlan prefill_plan(const abft_paged_attn_args* a, int sms) {
   const int64_t steps = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kPreKeys - 1) / kPreKeys;
   // Pieces, of four steps at least: as many as give each SM one item, counted
   // without the blocks that only ragged chunks have, and twice as many for
-  // several sequences, whose lengths may differ, if one each is not enough. (One sequence, 64 tokens on
-  // 16,384: 1 piece 214 us, 8 pieces 41, 16 51; 512 tokens on 8,192, 116 items:
-  // 1 piece 118, 2 pieces 129, for the sums that go through memory. Nine
-  // sequences of 5 tokens on up to 7,777: 4 pieces 35, 8 pieces 25; four on
-  // 32,768 each: 4 pieces 118, 8 pieces 124.)
+  // several sequences, whose lengths may differ, if one each is not enough.
+  // (One sequence, 64 tokens on 16,384 slots: 1 piece 159 us, 8 pieces 34, 16
+  // 44; 512 tokens on 8,192, 116 items: 1 piece 86, 2 pieces 100, for the sums
+  // that go through memory. Nine sequences of 5 tokens on up to 7,777: 4 pieces
+  // 29, 8 pieces 21; four of 16 on 32,768 each: 4 pieces 101, 8 pieces 103.)
   int64_t n = a->num_splits;
   if (n == 0) {
     int64_t least = (a->tokens + r.block_tokens - 1) / r.block_tokens;

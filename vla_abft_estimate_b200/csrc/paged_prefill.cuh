@@ -228,6 +228,19 @@ __device__ __forceinline__ uint64_t ring_desc(uint32_t saddr, uint32_t leading, 
 }
 constexpr uint32_t kIdescBNMajor = 1u << 16;
 
+// Whether the phase is over, without waiting for it.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // mbar_wait that goes on after an abort: for what is still in flight.
 __device__ __forceinline__ void mbar_wait_bounded(uint64_t* bar, uint32_t parity) {
   const uint64_t t0 = global_timer_ns();
@@ -505,7 +518,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       // item they have when both groups' last product is done), if the item is
       // there already.
       const PrefillItem& y = items[(i + 1) & 1];
-      const bool early = __all_sync(0xFFFFFFFFu, mbar_try_wait(&item_full[(i + 1) & 1], ((i + 1) >> 1) & 1));
+      const bool early = __all_sync(0xFFFFFFFFu, mbar_test_wait(&item_full[(i + 1) & 1], ((i + 1) >> 1) & 1));
       bool next = early && y.valid != 0;
       const bool soon = next && has_q(y);
       if (soon && !kShared) load_q(y);
@@ -879,8 +892,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       }
     }
   }
-  if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   tc_fence_after();
   if (warp == 9) tmem_dealloc(tmem, Cfg::kTmemCols);
 }

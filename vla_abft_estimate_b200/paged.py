@@ -127,6 +127,8 @@ class PagedKVCache:
             status = torch.zeros(1, dtype=torch.int32, device=dev)
         else:
             _i32("status", status, 1, dev)
+            if status.shape[0] < 1:
+                raise ValueError("status needs one entry")
         self.k_pages, self.v_pages, self.page_table, self.seq_lens, self.status = k_pages, v_pages, page_table, seq_lens, status
         self.batch, self.max_pages, self.num_pages = batch, max_pages, num_pages
         self.kv_heads, self.page_size, self.head_dim = kv_heads, page_size, head_dim
