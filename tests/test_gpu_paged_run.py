@@ -178,6 +178,77 @@ def test_non_finite_scores_stay_in_the_rows_that_see_them(cuda_device, value):
     assert torch.isfinite(got[:48]).all() and torch.isfinite(got[:, :3]).all() and torch.isfinite(got[199]).all()
 
 
+def test_captured_prefill_follows_boundaries_and_lengths(cuda_device):
+    """One capture over 60 packed rows, replayed as other batches come: other
+    chunk lengths, empty chunks, rows behind the last one."""
+    dev = cuda_device
+    pool = Pool([900, 120, 400], 2, 16, 64, BF16)
+    cache = pool.device_cache(dev, PagedKVCache)
+    q = torch.randn(60, 14, 64, generator=torch.Generator().manual_seed(8)).to(BF16)
+    dq, out = q.to(dev), torch.empty(60, 14, 64, dtype=BF16, device=dev)
+    cu = torch.tensor([0, 20, 40, 60], dtype=torch.int32, device=dev)
+    cache.prefill(dq, cu, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.prefill(dq, cu, out=out)
+    for new, total in (((20, 20, 20), (900, 120, 400)), ((60, 0, 0), (61, 5, 0)), ((1, 1, 1), (900, 1, 33)),
+                       ((0, 50, 7), (0, 50, 399))):
+        cu.copy_(torch.tensor([0, *torch.tensor(new).cumsum(0)], dtype=torch.int32))
+        cache.seq_lens.copy_(torch.tensor(total, dtype=torch.int32))
+        out.fill_(7.0)
+        g.replay()
+        want, tol = attention(pool, q[:sum(new)], owners_of(new, total))
+        close(out[:sum(new)], want, tol)
+        assert (out[sum(new):] == 7.0).all()
+    cache.check_status()
+
+
+def test_many_sequences(cuda_device):
+    """A batch of 1,000 sequences: every scan over the batch takes many rounds."""
+    dev = cuda_device
+    total = [(i * 29) % 61 for i in range(1000)]
+    pool = Pool(total, 1, 16, 64, F16)
+    cache = pool.device_cache(dev, PagedKVCache)
+    q = torch.randn(1000, 3, 64, generator=torch.Generator().manual_seed(9)).to(F16)
+    want, tol = attention(pool, q, list(enumerate(total)))
+    close(cache.decode(q.to(dev)), want, tol)
+    new = [min(1, t) for t in total]
+    rows = [b for b, n in enumerate(new) if n]
+    cu = torch.tensor([0, *torch.tensor(new).cumsum(0)], dtype=torch.int32, device=dev)
+    close(cache.prefill(q[rows].to(dev), cu), want[rows], tol[rows])
+    k = torch.randn(1000, 1, 64, generator=torch.Generator().manual_seed(10)).to(F16).to(dev)
+    cache.append(None, k, k)
+    last = torch.tensor([t - 1 for t in total if t])
+    page_of = pool.table[torch.tensor(rows), last // 16].long()
+    assert torch.equal(cache.v_pages.cpu()[page_of, 0, last % 16], k.cpu()[rows, 0])
+    cache.check_status()
+
+
+def test_result_over_q_and_a_slice_of_a_wider_table(cuda_device):
+    dev = cuda_device
+    pool = Pool([2000, 77, 300], 4, 16, 128, BF16)
+    wide = torch.full((5, 400), -1, dtype=torch.int32, device=dev)
+    wide[1:4, 7:7 + pool.table.shape[1]] = pool.table.to(dev)
+    cache = PagedKVCache(pool.k.to(dev), pool.v.to(dev), wide[1:4, 7:7 + pool.table.shape[1]],
+                         torch.tensor([0, 2000, 77, 300], dtype=torch.int32, device=dev)[1:])
+    q = torch.randn(43, 28, 128, generator=torch.Generator().manual_seed(8)).to(BF16)
+    new = (40, 1, 2)
+    cu = torch.tensor([0, 40, 41, 43], dtype=torch.int32, device=dev)
+    want, tol = attention(pool, q, owners_of(new, (2000, 77, 300)))
+    for splits in (1, 4):
+        x = q.to(dev)
+        assert cache.prefill(x, cu, out=x, num_splits=splits) is x
+        close(x, want, tol)
+    newest = [39, 40, 42]
+    for sms in (0, 5):
+        x = q[newest].to(dev)
+        assert cache.decode(x, out=x, num_sms=sms) is x
+        close(x, want[newest], tol[newest])
+    with pytest.raises(AttributeError):
+        cache.seq_lens = torch.zeros(3, dtype=torch.int32, device=dev)
+
+
 def test_misaligned_rows_are_copied(cuda_device):
     cache, q, k, v, rope = decode_state(cuda_device)
     want_q = cache.append(q, k, v, rope)

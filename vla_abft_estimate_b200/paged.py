@@ -129,7 +129,7 @@ class PagedKVCache:
             _i32("status", status, 1, dev)
             if status.shape[0] < 1:
                 raise ValueError("status needs one entry")
-        self.k_pages, self.v_pages, self.page_table, self.seq_lens, self.status = k_pages, v_pages, page_table, seq_lens, status
+        self._tensors = k_pages, v_pages, page_table, seq_lens, status
         self.batch, self.max_pages, self.num_pages = batch, max_pages, num_pages
         self.kv_heads, self.page_size, self.head_dim = kv_heads, page_size, head_dim
         self.dtype, self.device = k_pages.dtype, dev
@@ -147,6 +147,14 @@ class PagedKVCache:
                  for name in ("abft_kv_append", "abft_paged_decode", "abft_paged_decode_workspace_bytes",
                               "abft_paged_prefill", "abft_paged_prefill_workspace_bytes")]
         self._fast = _host().Calls(bytes(kv), dev.index, *entry)
+
+    # The kernels hold the addresses: the tensors are written in place, not
+    # replaced.
+    k_pages = property(lambda self: self._tensors[0])
+    v_pages = property(lambda self: self._tensors[1])
+    page_table = property(lambda self: self._tensors[2])
+    seq_lens = property(lambda self: self._tensors[3])
+    status = property(lambda self: self._tensors[4])
 
     # ---- argument checks ------------------------------------------------------
     # A call whose arguments are all in order goes to the library through
@@ -258,8 +266,8 @@ class PagedKVCache:
                num_sms: int = 0) -> torch.Tensor:
         """Attention of each sequence's newest token over its cache: ``q``
         [batch, heads, head_dim], returns the same shape. ``scale`` defaults
-        to head_dim^-0.5. A sequence of length 0 gives zeros. ``num_sms``:
-        SMs the caches are shared out to (0: all)."""
+        to head_dim^-0.5. A sequence of length 0 gives zeros. ``out`` may be
+        ``q``. ``num_sms``: SMs the caches are shared out to (0: all)."""
         return self._attention(False, q, None, scale, out, 0, num_sms)
 
     def prefill(self, q: torch.Tensor, cu_seqlens: torch.Tensor, *, scale: Optional[float] = None,
@@ -269,7 +277,8 @@ class PagedKVCache:
         the last tokens of sequence b (``append`` has stored their keys), and
         row i of n sees the slots up to seq_lens[b] - n + i. Chunks of any
         length, 0 and 1 included; rows behind cu[batch] are left as they were
-        in ``out`` (undefined without one). ``num_splits``: pieces the keys of
+        in ``out`` (undefined without one), which may be ``q``.
+        ``num_splits``: pieces the keys of
         a block of query rows are cut into (0: chosen from the rows, the heads
         and the table's width)."""
         return self._attention(True, q, cu_seqlens, scale, out, num_splits, 0)
