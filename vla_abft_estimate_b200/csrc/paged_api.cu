@@ -171,7 +171,7 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
   if (decode && a->tokens != a->kv.batch) return ABFT_ERR_INVALID_ARG;
   if (a->tokens == 0 || a->kv.batch == 0) return ABFT_OK;
   // The list of tiles is counted in 32 bits.
-  if (decode && decode_segments(a) * decode_segment_tiles(a) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
+  if (decode && decode_segments(a) * (decode_segment_tiles(a) + kDecCost) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
   // Grids (blocks x kv heads, rows x heads for the join) stay below 2^31.
   if (a->tokens >= (int64_t{1} << 30) / a->heads) return ABFT_ERR_UNSUPPORTED;
   if (a->q == nullptr || a->out == nullptr || (!decode && a->cu_seqlens == nullptr)) return ABFT_ERR_INVALID_ARG;

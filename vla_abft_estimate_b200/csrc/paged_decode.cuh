@@ -25,15 +25,15 @@
 //
 // Work is one list of 32-key tiles over all (sequence, kv head) segments, cut
 // into equal shares for the warps of one CTA per SM: lengths of any mix keep
-// every SM reading to the end. A warp's ring of loads runs on across segment
-// boundaries. A segment inside one warp's share is finished by that warp;
+// every SM reading to the end. (Where lengths differ much a segment takes
+// kDecCost places in the list more than it has tiles, for its start and end.) A
+// warp's ring of loads runs on across segment boundaries. A segment inside one warp's share is finished by that warp;
 // pieces of a segment that crosses warps are joined in shared memory, those of
 // one that crosses CTAs by a second, small kernel, in a fixed order. A cache
 // too small to be worth sharing out gets a CTA per segment instead: nothing
-// crosses CTAs, and one launch does. (Joined
-// instead by the last CTA to arrive, an atomic counter's choice, 37 pieces of
-// 8 heads took one SM 12 us; spread over one block per head, launch included,
-// 3 us.)
+// crosses CTAs, and one launch does. (Joined instead by the last CTA to arrive,
+// an atomic counter's choice, 37 pieces of 8 heads took one SM 12 us; spread
+// over one block per head, launch included, 3 us.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -115,6 +115,12 @@ struct DecodeParams {
 // 49.5: one SM takes in some 62 GB/s however many warps ask.)
 constexpr int kDecWarps = 4;
 constexpr int kDecTile = 32;
+// Places in the list that a segment takes for its start and end when the
+// longest sequence has over twice the tiles of the shortest: short segments
+// would make some shares late (37 sequences of 1 to 4,097 slots: 17.8 us with
+// 1, 18.3 with 2, 21.6 with 0). Equal ones divide best without (256 of 2,048
+// slots: 44.2 us against 47.9 with 1).
+constexpr int kDecCost = 1;
 
 template <int D, int NT>
 struct DecodeCfg {
@@ -139,11 +145,12 @@ struct DecodeCfg {
 
 // A position in the list of tiles.
 struct TileIter {
-  int left;        // tiles of the share still to come, this one included
+  int u;           // its place in the list
   int b, y;        // sequence; kv head and chunk
   int tile, tiles; // tile within the segment, and the segment's tiles
   int len;
 };
+constexpr int kNoMore = 0x7FFFFFFF;  // the place behind the last tile
 
 template <int kTile>
 __device__ __forceinline__ int tiles_of(const PagedView& kv, int b, int* len, bool* bad) {
@@ -151,23 +158,30 @@ __device__ __forceinline__ int tiles_of(const PagedView& kv, int b, int* len, bo
   return (*len + kTile - 1) / kTile;
 }
 
-// The next tile; only called while left > 1.
+// The next tile; `cost` places lie before a segment's first.
 template <int kTile>
-__device__ __forceinline__ void advance(TileIter& it, const PagedView& kv, int rows) {
-  --it.left;
-  if (++it.tile < it.tiles) return;
-  if (it.y + 1 < rows) {
-    it.tile = 0;
-    ++it.y;
+__device__ __forceinline__ void advance(TileIter& it, const PagedView& kv, int rows, int cost) {
+  if (it.tile + 1 < it.tiles) {
+    ++it.tile;
+    ++it.u;
     return;
   }
-  if (it.b + 1 >= kv.batch) return;
-  it.tile = it.y = 0;
-  bool bad;
-  do {
-    ++it.b;
-    it.tiles = tiles_of<kTile>(kv, it.b, &it.len, &bad);
-  } while (it.tiles == 0 && it.b + 1 < kv.batch);
+  if (it.y + 1 < rows) {
+    ++it.y;
+  } else {
+    bool bad;
+    do {
+      if (it.b + 1 >= kv.batch) {
+        it.u = kNoMore;
+        return;
+      }
+      ++it.b;
+      it.tiles = tiles_of<kTile>(kv, it.b, &it.len, &bad);
+    } while (it.tiles == 0);
+    it.y = 0;
+  }
+  it.tile = 0;
+  it.u += 1 + cost;
 }
 
 template <int D, int NT, bool F16>
@@ -194,7 +208,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
 
   // ---- this warp's share ------------------------------------------------------
   TileIter head;
-  int total, shares, u0, u1;
+  int total, shares, u0, u1, cost = 0;
   if (p.by_segment) {  // the list is one segment, its shares this CTA's warps'
     head.b = blockIdx.x / rows;
     head.y = blockIdx.x - head.b * rows;
@@ -202,36 +216,47 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
     total = head.tiles = tiles_of<kTile>(kv, head.b, &head.len, &bad);
     if (bad && head.y == 0 && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
     shares = kWarps;
-    u0 = head.tile = share_start(total, shares, warp);
+    u0 = head.u = head.tile = share_start(total, shares, warp);
     u1 = share_start(total, shares, warp + 1);
-    head.left = u1 - u0;
   } else {
     int len0 = 0, tiles0 = 0;  // this lane's sequence of the first 32
-    int sum = 0;
+    int sum = 0, held_any = 0, least = kNoMore, most = 0;
     for (int b = lane; b < kv.batch; b += 32) {
       int len;
       bool bad;
       const int tiles = tiles_of<kTile>(kv, b, &len, &bad);
       if (b == lane) len0 = len, tiles0 = tiles;
-      sum += tiles;
+      if (tiles > 0) {
+        sum += tiles;
+        ++held_any;
+        least = min(least, tiles);
+        most = max(most, tiles);
+      }
       if (bad && blockIdx.x == 0 && warp == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
     }
     sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+    least = __reduce_min_sync(0xFFFFFFFFu, least);
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (least < most / 2) {
+      cost = kDecCost;
+      sum += __reduce_add_sync(0xFFFFFFFFu, held_any) * kDecCost;
+    }
     total = sum * rows;  // the host keeps it below 2^31
     shares = gridDim.x * kWarps;
     const int share = blockIdx.x * kWarps + warp;
     u0 = share_start(total, shares, share);
     u1 = share_start(total, shares, share + 1);
 
-    head.left = u1 - u0;
+    head.u = kNoMore;
     head.b = head.y = head.tile = head.tiles = head.len = 0;
-    if (head.left > 0) {  // the sequence that holds tile u0
+    if (u0 < u1) {  // the sequence that holds place u0
       int before = 0;
       for (int i = 0; i < kv.batch; i += 32) {
         int mine = tiles0, len = len0;
         bool bad;
         if (i > 0) mine = i + lane < kv.batch ? tiles_of<kTile>(kv, i + lane, &len, &bad) : 0;
-        int upto = mine;
+        const int places = mine > 0 ? mine + cost : 0;
+        int upto = places;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
@@ -243,9 +268,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
           head.b = i + src;
           head.tiles = __shfl_sync(0xFFFFFFFFu, mine, src);
           head.len = __shfl_sync(0xFFFFFFFFu, len, src);
-          const int in = u0 - (before + __shfl_sync(0xFFFFFFFFu, upto - mine, src)) * rows;
-          head.y = in / head.tiles;
-          head.tile = in - head.y * head.tiles;
+          const int in = u0 - (before + __shfl_sync(0xFFFFFFFFu, upto - places, src)) * rows;
+          head.y = in / (head.tiles + cost);
+          const int off = in - head.y * (head.tiles + cost);
+          head.tile = max(0, off - cost);
+          head.u = u0 - off + cost + head.tile;  // the first tile at or behind u0
           break;
         }
         before += __shfl_sync(0xFFFFFFFFu, upto, 31);
@@ -354,18 +381,17 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
 
   TileIter cur = head;  // consumer; `head` runs kStages - 1 tiles ahead
   if (lane == 0) s_first[warp] = s_last[warp] = 0;
-  if (cur.left > 0) {
+  if (cur.u < u1) {
     entries(head);
     load_q(cur, qf);
     begin_segment();
     bool from_before = cur.tile > 0;  // the segment began in an earlier share
-    int ahead = head.left;            // tiles not yet issued
     int stage = 0;
     auto fill = [&](int sn) {
-      if (ahead > 0) {
+      if (head.u < u1) {
         issue(head, sn);
-        if (--ahead > 0) {
-          advance<kTile>(head, kv, rows);
+        advance<kTile>(head, kv, rows, cost);
+        if (head.u < u1) {
           if (head.tile == 0) {
             entries(head);
           } else if (head.tile - held == kHeld) {
@@ -385,13 +411,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
       // Refill the stage that the previous step emptied.
       fill(stage == 0 ? Cfg::kStages - 1 : stage - 1);
       // The next segment's query rows are asked for under this one's last step.
-      const bool ends = cur.tile + 1 == cur.tiles, stops = cur.left == 1;
+      const bool ends = cur.tile + 1 == cur.tiles;
       uint32_t qn[NT][D / 16][2];
       TileIter next = cur;
-      if (!stops) {
-        advance<kTile>(next, kv, rows);
-        if (ends) load_q(next, qn);
-      }
+      advance<kTile>(next, kv, rows, cost);
+      const bool stops = next.u >= u1;
+      if (ends && !stops) load_q(next, qn);
       const uint32_t ks_base = ring + stage * Cfg::kStageBytes;
       const uint32_t vs_base = ks_base + Cfg::kHalfBytes;
 
@@ -508,7 +533,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
             s_last[warp] = 2;
             s_seg[warp][1][0] = cur.b;
             s_seg[warp][1][1] = cur.y;
-            s_end[warp] = u1 - cur.left + (cur.tiles - 1 - cur.tile);
+            s_end[warp] = cur.u + (cur.tiles - 1 - cur.tile);
           }
         } else {  // the whole segment: its rows are done
           const int hk = cur.y / p.head_chunks, hc = cur.y - hk * p.head_chunks;
