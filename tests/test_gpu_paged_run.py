@@ -225,6 +225,38 @@ def test_many_sequences(cuda_device):
     cache.check_status()
 
 
+@pytest.mark.parametrize("batch", [33, 129, 2100])
+def test_batches_that_a_warp_scans_in_parts(cuda_device, batch):
+    """More sequences than lanes, than boundaries counted at once, and than 32
+    for each lane: empty ones, and none, one or several new tokens each."""
+    dev = cuda_device
+    total = [(i * 29) % 47 for i in range(batch)]
+    new = [min(t, (0, 1, 3)[i % 3]) for i, t in enumerate(total)]
+    pool = Pool(total, 1, 16, 64, BF16)
+    cache = pool.device_cache(dev, PagedKVCache)
+    g = torch.Generator().manual_seed(12)
+    q = torch.randn(batch, 2, 64, generator=g).to(BF16)
+    want, tol = attention(pool, q, list(enumerate(total)))
+    close(cache.decode(q.to(dev)), want, tol)
+    close(cache.decode(q.to(dev), num_sms=3), want, tol)
+    rows = sum(new)
+    cu = torch.tensor([0, *torch.tensor(new).cumsum(0)], dtype=torch.int32, device=dev)
+    q = torch.randn(rows + 5, 2, 64, generator=g).to(BF16)
+    want, tol = attention(pool, q[:rows], owners_of(new, total))
+    for splits in (0, 2):
+        out = torch.full_like(q, 7.0).to(dev)
+        cache.prefill(q.to(dev), cu, out=out, num_splits=splits)
+        close(out[:rows], want, tol)
+        assert (out[rows:] == 7.0).all()
+    v = torch.randn(rows + 5, 1, 64, generator=g).to(BF16)
+    cache.append(None, v.to(dev), v.to(dev), cu_seqlens=cu)
+    place = [(b, t - n + i) for b, (n, t) in enumerate(zip(new, total)) for i in range(n)]
+    b, pos = torch.tensor(place).unbind(1)
+    stored = cache.v_pages.cpu()[pool.table[b, pos // 16].long(), 0, pos % 16]
+    assert torch.equal(stored, v[:rows, 0])
+    cache.check_status()
+
+
 def test_result_over_q_and_a_slice_of_a_wider_table(cuda_device):
     dev = cuda_device
     pool = Pool([2000, 77, 300], 4, 16, 128, BF16)

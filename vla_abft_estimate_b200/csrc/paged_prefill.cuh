@@ -117,44 +117,74 @@ __host__ __device__ __forceinline__ int visible_keys(int len, int n, int i) {
   return v > 0 ? v : 0;
 }
 
-// Block `index` of the packed sequences, each cut into blocks of `per`
-// tokens; called by one warp. Heavier blocks (later tokens) of a sequence
-// come first. Boundaries and lengths are asked for together; *begin, *count
-// and *len are the sequence's packed rows and raw length. Returns false behind
-// the last block.
-__device__ __forceinline__ bool find_block(const PagedView& kv, const int32_t* cu, int tokens, int per, int index, int lane,
-                                           int* seq, int* block, int* begin, int* count, int* len) {
-  int before = 0;
-  for (int i = 0; i < kv.batch; i += 32) {
-    int mine = 0, lo = 0, hi = 0, length = 0;
-    if (i + lane < kv.batch) {
-      length = kv.seq_lens[i + lane];
-      packed_range(cu, i + lane, tokens, &lo, &hi);
-      mine = (hi - lo + per - 1) / per;
+// The packed sequences, each cut into blocks of `per` tokens, as a warp holds
+// them: lane i has the sequences [i * share, (i + 1) * share). Read once per
+// CTA: a scan of the whole batch for every item made 4 tokens for each of
+// 1,024 sequences of 500 slots 381 us instead of 240.
+struct BlockScan {
+  int share;
+  int blocks, upto;       // of this lane's sequences; with those of all lanes before
+  int begin, count, len;  // share 1: the lane's sequence
+};
+
+// A sequence's packed rows and raw length (boundaries and length are asked for
+// together); returns its blocks.
+__device__ __forceinline__ int blocks_of(const PagedView& kv, const int32_t* cu, int tokens, int per, int b, int* begin,
+                                         int* count, int* len) {
+  int end;
+  *len = kv.seq_lens[b];
+  packed_range(cu, b, tokens, begin, &end);
+  *count = end - *begin;
+  return (*count + per - 1) / per;
+}
+
+__device__ __forceinline__ BlockScan scan_blocks(const PagedView& kv, const int32_t* cu, int tokens, int per, int lane) {
+  BlockScan s;
+  s.share = (kv.batch + 31) >> 5;
+  s.blocks = s.begin = s.count = s.len = 0;
+  const int b0 = lane * s.share, b1 = min(kv.batch, b0 + s.share);
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) s.blocks += blocks_of(kv, cu, tokens, per, b, &s.begin, &s.count, &s.len);
+  s.upto = warp_scan(s.blocks, lane);
+  return s;
+}
+
+// Block `index` of the list; called by one warp. Heavier blocks (later tokens)
+// of a sequence come first. Up to 32 sequences are held in registers; of more,
+// the share that has the block is read again. Returns false behind the last
+// block.
+__device__ __forceinline__ bool find_block(const PagedView& kv, const int32_t* cu, int tokens, int per, const BlockScan& s,
+                                           int index, int lane, int* seq, int* block, int* begin, int* count, int* len) {
+  const uint32_t past = __ballot_sync(0xFFFFFFFFu, s.upto > index);
+  if (past == 0) return false;
+  const int owner = __ffs(past) - 1;
+  int before = __shfl_sync(0xFFFFFFFFu, s.upto - s.blocks, owner);
+  int mine = s.blocks, lo = s.begin, n = s.count, length = s.len, src = owner, from = 0;
+  if (s.share > 1) {
+    const int end = min(kv.batch, (owner + 1) * s.share);
+    for (from = owner * s.share;; from += 32) {
+      if (from >= end) return false;  // boundaries that do not rise
+      mine = 0;
+      if (from + lane < end) mine = blocks_of(kv, cu, tokens, per, from + lane, &lo, &n, &length);
+      const int upto = warp_scan(mine, lane);
+      const uint32_t in = __ballot_sync(0xFFFFFFFFu, before + upto > index);
+      if (in != 0) {
+        src = __ffs(in) - 1;
+        before += __shfl_sync(0xFFFFFFFFu, upto - mine, src);
+        break;
+      }
+      before += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > index);
-    if (past != 0) {
-      const int src = __ffs(past) - 1;
-      const int first = before + __shfl_sync(0xFFFFFFFFu, upto - mine, src);
-      const int blocks = __shfl_sync(0xFFFFFFFFu, mine, src);
-      const int at = blocks - 1 - (index - first);
-      if (at < 0 || at >= blocks) return false;  // boundaries that do not rise
-      *seq = i + src;
-      *block = at;
-      *begin = __shfl_sync(0xFFFFFFFFu, lo, src);
-      *count = __shfl_sync(0xFFFFFFFFu, hi - lo, src);
-      *len = __shfl_sync(0xFFFFFFFFu, length, src);
-      return true;
-    }
-    before += __shfl_sync(0xFFFFFFFFu, upto, 31);
   }
-  return false;
+  const int blocks = __shfl_sync(0xFFFFFFFFu, mine, src);
+  const int at = blocks - 1 - (index - before);
+  if (at < 0 || at >= blocks) return false;  // boundaries that do not rise
+  *seq = from + src;
+  *block = at;
+  *begin = __shfl_sync(0xFFFFFFFFu, lo, src);
+  *count = __shfl_sync(0xFFFFFFFFu, n, src);
+  *len = __shfl_sync(0xFFFFFFFFu, length, src);
+  return true;
 }
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* map, uint64_t* bar, int32_t x, int32_t y, int32_t z,
@@ -826,6 +856,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       // ---------------------------------------------------------- work
       int index = blockIdx.x, published = 0, asked = 0;
       bool ok = true;
+      const BlockScan scan = scan_blocks(kv, p.cu, p.tokens, p.block_tokens, lane);
       while (ok) {
         PrefillItem x;
         x.valid = 0;
@@ -836,7 +867,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           const int rest = index - x.split * p.items;
           x.hk = rest % kv.kv_heads;
           int seq = 0, block = 0, raw_len = 0;
-          if (find_block(kv, p.cu, p.tokens, p.block_tokens, rest / kv.kv_heads, lane, &seq, &block, &x.row0, &x.n,
+          if (find_block(kv, p.cu, p.tokens, p.block_tokens, scan, rest / kv.kv_heads, lane, &seq, &block, &x.row0, &x.n,
                          &raw_len)) {
             bool bad_len;
             x.seq = seq;
