@@ -64,18 +64,19 @@ struct PrefillCfg {
   static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kOffRing = 2 * kTileBytes;            // after the two Q tiles
   static constexpr int kOffBar = kOffRing + kSlots * kTileBytes;
-  // full, empty, qfull, sfull, pfull, ofull, item full and empty, work, loaded,
-  // both, drain, one unused (an even number)
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 4 + 1 + 1 + 1 + 1;
+  // full, empty, qfull, sfull, pfull, ofull, sread, item full and empty, work,
+  // loaded, both, drain (an even number)
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 2 + 2 + 4 + 1 + 1 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kOffItems = kOffMisc + 16;  // two items and the launch-control answer
   static constexpr int kSmemBytes = kOffItems + 2 * 48 + 16 + 1024;
   static_assert(kBars % 2 == 0, "the answer is 16-byte aligned");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
   static_assert(kSmemBytes > 232448 / 2, "one CTA per SM: each takes all of TMEM");
-  // TMEM columns: S of both tiles (P over its first half), then O of both.
+  // TMEM columns: S of both tiles (P over its first half), then O of both; with
+  // heads of 64 there is room for a P of their own behind them.
   static constexpr int kTmemCols = 512;
-  static constexpr int kColO = 256;
+  static constexpr int kColO = 256, kColP = kColO + 2 * D;
 };
 
 struct PrefillParams {
@@ -324,6 +325,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                          const PrefillParams p) {
   using Cfg = PrefillCfg<D>;
+  // The next scores are computed while the rows work on the last ones: P does
+  // not take the place of S, and products of O run behind those of S.
+  constexpr bool kAhead = D == 64 && !kShared;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
@@ -332,7 +336,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   uint64_t* sfull = qfull + 2;
   uint64_t* pfull = sfull + 2;
   uint64_t* ofull = pfull + 2;
-  uint64_t* item_full = ofull + 2;
+  uint64_t* sread = ofull + 2;
+  uint64_t* item_full = sread + 2;
   uint64_t* item_empty = item_full + 2;
   uint64_t* work = item_empty + 2;
   uint64_t* loaded_all = work + 1;
@@ -355,6 +360,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       mbar_init(&sfull[t], 1);
       mbar_init(&pfull[t], kPreRows);
       mbar_init(&ofull[t], 1);
+      mbar_init(&sread[t], kPreRows);
       mbar_init(&item_full[t], 1);
       mbar_init(&item_empty[t], 10);  // a lane of each row warp, the loader's and the issuer's
     }
@@ -404,6 +410,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     };
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t ts = lanes + t * 128, to = lanes + Cfg::kColO + t * D;
+    const uint32_t tp = kAhead ? lanes + Cfg::kColP + t * (kPreKeys / 2) : ts;
     const int tile = kShared ? 0 : t;                            // whose rows these are
     const int lag = kShared ? t : 0, stride = kShared ? 2 : 1;  // this group's steps: j0 + lag, by stride
     int met = 0;  // times the groups have waited for each other
@@ -465,15 +472,16 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       float m = -INFINITY, l = 0.f;                         // m: maximum that P refers to (raw scores)
       const int begin = j0 + lag;
       for (int j = begin; j < end; j += stride, ++count) {
-        if (!mbar_wait(&sfull[t], count & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
+        ok = mbar_wait(&sfull[t], count & 1, abort_flag);
         tc_fence_after();
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + c * 32, s[c]);
         tmem_ld_wait();
+        if (kAhead) {
+          tc_fence_before();
+          mbar_arrive(&sread[t]);
+        }
         if (p.negate) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -499,7 +507,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);  // NaN if a score is
         // Also true from m = -inf and for NaN, but not while all is -inf.
         const bool raise = !((mn - m) * p.scale_log2 <= 8.f) && mn != -INFINITY;
-        if (j == begin || __any_sync(0xFFFFFFFFu, raise)) {
+        if (kAhead && j > begin) {  // the last product has read P and written O
+          ok = mbar_wait(&ofull[t], (count - 1) & 1, abort_flag) && ok;
+          tc_fence_after();
+        }
+        if (j == begin || __any_sync(0xFFFFFFFFu, raise || !ok)) {
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
           if (mn == INFINITY) mn = __int_as_float(0x7FC00000);  // inf - inf: the row is NaN
           const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * p.scale_log2);
           m = mn;
@@ -534,7 +548,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
               sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], y);
               pk[c * 16 + (k >> 1)] = pack2<F16>(y.x, y.y);
             }
-          tmem_st_32x32b_x32(ts + h * 32, pk);
+          tmem_st_32x32b_x32(tp + h * 32, pk);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_st_wait();
@@ -554,7 +568,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (soon && !kShared) load_q(y);
       const bool any = end > begin;
       if (any) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[t], used & 1, abort_flag));
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[t], (kAhead ? count - 1 : used) & 1, abort_flag));
         tc_fence_after();
         ++used;
       }
@@ -679,7 +693,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         };
         // Keys come `lead` steps before the values: K of the first steps, then
         // V and the next K in turn, as the issuer uses them.
-        const int lead = kShared ? 2 : 1;
+        const int lead = kShared || kAhead ? 2 : 1;
         int ids[3];  // table entries of steps j, j + 1, j + 2
 #pragma unroll
         for (int k = 0; k < 3; ++k) ids[k] = x.j0 + k < x.j1 ? entry(x.j0 + k) : 0;
@@ -739,7 +753,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         tc_fence_after();
         return ok;
       };
-      const int lead = kShared ? 2 : 1;  // steps between a group's own
+      constexpr int kStride = kShared ? 2 : 1;        // steps between a group's own
+      constexpr int kLead = kShared || kAhead ? 2 : 1;  // steps that scores come before the product of O
       auto scores = [&](int t, int at) {
         if (elect_one()) {
           const uint64_t dq = desc_q + (kShared ? 0 : t) * (Cfg::kTileBytes >> 4), dk = desc_k + at * (Cfg::kTileBytes >> 4);
@@ -751,6 +766,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           umma_commit(&sfull[t]);
         }
         __syncwarp();
+      };
+      auto seen = [&](int t) {  // the rows have the scores of step pcount[t] in registers
+        ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&sread[t], pcount[t] & 1, abort_flag));
+        tc_fence_after();
+        return ok;
       };
       auto release = [&](int at) {  // once the MMAs so far have read the slot
         if (elect_one()) umma_commit(&empty[at]);
@@ -782,9 +802,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (!ok) break;
         release(slot);
         step_ring();
-        if (kShared && first_j + 1 < last_j) {
+        if (kLead == 2 && first_j + 1 < last_j) {
           if (!ready(slot, phase)) break;
-          scores(1, slot);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (kShared && t == 0) continue;
+            if (kAhead && (first_j + 1 >= stop[t] || !seen(t))) continue;
+            scores(t, slot);
+          }
+          if (!ok) break;
           release(slot);
           step_ring();
         }
@@ -819,8 +845,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 tc_fence_after();
                 if (elect_one()) {
                   const uint64_t dv = desc_v + vs * (Cfg::kTileBytes >> 4);
-                  const uint32_t d = tm + Cfg::kColO + t * D, a = tm + t * 128;
-                  umma_f16_ts(d, a, dv, idesc_o, j >= first_j + lead);
+                  const uint32_t d = tm + Cfg::kColO + t * D;
+                  const uint32_t a = kAhead ? tm + Cfg::kColP + t * (kPreKeys / 2) : tm + t * 128;
+                  umma_f16_ts(d, a, dv, idesc_o, j >= first_j + kStride);
                   if (groups == kPreKeys / 16) {
 #pragma unroll
                     for (int k = 1; k < kPreKeys / 16; ++k)
@@ -829,14 +856,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                     for (int k = 1; k < groups; ++k)
                       umma_f16_ts(d, a + k * 8, dv + k * (2 * Cfg::kGroupBytes >> 4), idesc_o, 1);
                   }
-                  if (j + lead >= stop[t]) umma_commit(&ofull[t]);
+                  if (kAhead || j + kStride >= stop[t]) umma_commit(&ofull[t]);
                 }
                 __syncwarp();
               }
             }
-            if (j + lead < stop[t] && ok) {
+            if (j + kLead < stop[t] && ok) {
               if (!loaded) ready(slot, phase);
               loaded = true;
+              if (kAhead && ok) seen(t);
               if (ok) scores(t, slot);
             }
           }
