@@ -14,7 +14,9 @@
 // a short chunk fills its rows. Per 128 keys:
 //   S = Q K^T   tcgen05.mma, both operands in shared memory, S in TMEM
 //   P = 2^(x - m) by one thread per row (no exchange between lanes): S is read
-//       from TMEM, P goes back over it as 16-bit operand
+//       from TMEM, P goes back over it as 16-bit operand (heads of 64: beside
+//       it, and the next S is computed meanwhile; 8,192 tokens of 32 heads: 366
+//       us, 395 without)
 //   O += P V    tcgen05.mma with P from TMEM, V as N-major operand
 // The two tiles alternate: while the tensor core works on one, the other's
 // rows are exponentiated. O stays in TMEM; it is rescaled only when a row's
