@@ -318,7 +318,8 @@ class PagedKVCache:
     def check_status(self) -> None:
         """Raises ValueError when a call since the last check met a bad page
         entry, length or position on the device (which it skipped), and
-        clears the record. Synchronises."""
+        clears the record. Synchronises with the current stream: work queued on
+        others is waited for by the caller."""
         bits = int(self.status.cpu()[0])
         if not bits:
             return
