@@ -257,6 +257,32 @@ def test_batches_that_a_warp_scans_in_parts(cuda_device, batch):
     cache.check_status()
 
 
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("kv_heads,group", [(1, 3), (2, 12), (4, 7), (1, 24)])
+@pytest.mark.parametrize("lens", [(510,), (0,), (1, 33, 0), (500, 130, 31, 257, 64, 448, 5), [37 * i % 513 for i in range(16)]])
+def test_decode_by_clusters(cuda_device, lens, kv_heads, group, d, dtype):
+    """Tables of 512 slots: clusters of 8, 4 or 2 CTAs a segment by the number of
+    segments (1 to 64); lengths that leave CTAs, or all, without a tile."""
+    dev = cuda_device
+    pool = Pool(lens, kv_heads, 16, d, dtype, extra_columns=32 - max(1, (max(lens) + 15) // 16))
+    cache = pool.device_cache(dev, PagedKVCache)
+    assert cache.max_pages == 32
+    q = torch.randn(len(lens), kv_heads * group, d, generator=torch.Generator().manual_seed(13)).to(dtype)
+    want, tol = attention(pool, q, list(enumerate(lens)))
+    x = q.to(dev)
+    for sms in (0, 1, 9):  # 1: the list on one SM
+        close(cache.decode(x, num_sms=sms), want, tol)
+    first = cache.decode(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.decode(x)
+    for _ in range(3):
+        out.fill_(7.0)
+        graph.replay()
+        assert torch.equal(out, first)
+    cache.check_status()
+
+
 def test_result_over_q_and_a_slice_of_a_wider_table(cuda_device):
     dev = cuda_device
     pool = Pool([2000, 77, 300], 4, 16, 128, BF16)

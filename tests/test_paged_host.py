@@ -229,9 +229,11 @@ def test_workspace_sizes():
     a.num_sms = 3
     assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 3 * cta
     a.num_sms = 148
-    a.kv.max_pages = a.kv.table_stride = 64  # 32 tiles each: shared out over 144 SMs, 18 for each segment
-    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 64 * cta  # 256 tiles for 64 CTAs' warps
-    a.kv.max_pages = a.kv.table_stride = 640
+    a.kv.max_pages = a.kv.table_stride = 64  # 1,024 slots: a cluster of 8 CTAs each and no scratch
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 0
+    a.kv.max_pages = a.kv.table_stride = 130  # 65 tiles each, shared out: 520 tiles for 130 CTAs' warps
+    assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 130 * cta
+    a.kv.max_pages = a.kv.table_stride = 640  # 144 SMs, 18 for each segment
     assert N.lib().abft_paged_decode_workspace_bytes(ctypes.byref(a)) == 144 * cta
     a.kv.max_pages = a.kv.table_stride = 3
     a.num_splits = 1

@@ -73,22 +73,30 @@ inline bool off8el(int64_t s) { return (s & 7) != 0; }
 // Launch with programmatic serialization: the kernel waits
 // (griddepcontrol.wait) before any global access.
 template <typename K, typename... P>
-int launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const P&... p) {
+int launch_clusters(int cluster, K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const P&... p) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kernel, p...) != cudaSuccess) {
     cudaGetLastError();
     return ABFT_ERR_CUDA;
   }
   return launch_result();
+}
+
+template <typename K, typename... P>
+int launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, const P&... p) {
+  return launch_clusters(1, kernel, grid, block, smem, s, p...);
 }
 
 int check_kv(const abft_paged_kv& c) {
@@ -181,18 +189,27 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
   return ABFT_OK;
 }
 
-// A CTA per segment, instead of equal shares of the list, when the SMs hold
-// them all and they are short: sharing out costs a second launch and the
-// joins. Measured (equal lengths, group 7 or 4 of 128): 4 segments of 128 / 256
-// / 512 slots: 4.8 / 5.9 / 8.4 us against 6.4 / 7.5 / 7.5; 128 segments of 512 /
-// 1,280 slots: 9.2 / 17.3 against 11.7 / 21.8. Longer ones are shared out all
-// the same, since lengths may differ by more than that.
-bool decode_by_segment(const abft_paged_attn_args* a, int sms) {
+// CTAs per segment (a cluster of them), or 0: equal shares of the list. When
+// the SMs hold all segments and they are short, sharing out costs more (a
+// second launch and pieces through memory) than it saves. Measured (equal
+// lengths, group 7 of 128; one CTA / a cluster / the list): 4 segments, clusters
+// of 8: 190 slots 5.9 / 6.3 / -, 310 slots 7.1 / 6.4 / -, 500 slots - / 6.5 /
+// 7.5, 2,000 slots - / 7.8 / 8.0; 32 segments, clusters of 4: 500 slots - / 6.9 /
+// 8.3, 1,000 slots - / 8.0 / 9.6; 64 segments, clusters of 2: 370 slots 7.7 / 8.0 /
+// -, 500 slots - / 8.2 / 9.7; 128 segments of 512 / 1,280 slots: 9.2 / 17.3 us
+// against the list's 11.7 / 21.8. Longer ones are shared out all the same, since
+// lengths may differ by more than that. Clusters have to fit the device's groups
+// of SMs: 15 of 8 and 33 of 4 run at once, a second wave costs 4 us.
+int decode_by_segment(const abft_paged_attn_args* a, int sms) {
   const int64_t segments = decode_segments(a), slots = static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size;
-  return segments <= sms && slots <= (2 * segments >= sms ? 1280 : 384);
+  if (segments > sms) return 0;
+  if (2 * segments > sms) return slots <= 1280 ? 1 : 0;
+  const int c = 8 * segments <= sms * 3 / 4 ? 8 : 4 * segments <= sms * 7 / 8 ? 4 : 2;
+  if (slots <= (c == 2 ? 384 : 256)) return 1;
+  return slots <= 256 * c ? c : 0;
 }
 
-// CTAs of a decode launch: one per segment, or one per SM, fewer when the
+// CTAs of a decode launch: those of the segments' clusters, or one per SM, fewer when the
 // cache cannot hold a tile for each of their warps. Of the last fifth of the
 // SMs some are left out if the segments then divide evenly among the rest:
 // those of equal length do not cross CTAs (256 segments of 8,192 slots: 128
@@ -200,7 +217,7 @@ bool decode_by_segment(const abft_paged_attn_args* a, int sms) {
 // fifths of the SMs already read at full speed (120 CTAs: 168 and 49).
 int decode_grid(const abft_paged_attn_args* a, int sms) {
   const int64_t segments = decode_segments(a);
-  if (decode_by_segment(a, sms)) return static_cast<int>(segments);
+  if (const int c = decode_by_segment(a, sms)) return static_cast<int>(segments) * c;
   const int64_t ctas = (segments * decode_segment_tiles(a) + kDecWarps - 1) / kDecWarps;
   if (ctas <= sms) return static_cast<int>(ctas);
   for (int g = sms; 5 * g >= 4 * sms; --g)
@@ -221,7 +238,7 @@ int launch_decode(int dev, int slot, const DecodeParams& p, int grid, cudaStream
   using Cfg = DecodeCfg<D, NT>;
   int rc = raise_smem(dev, slot, paged_decode_kernel<D, NT, F16>, Cfg::kSmemBytes);
   if (rc != ABFT_OK) return rc;
-  rc = launch(paged_decode_kernel<D, NT, F16>, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmemBytes, s, p);
+  rc = launch_clusters(p.by_segment, paged_decode_kernel<D, NT, F16>, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmemBytes, s, p);
   if (rc != ABFT_OK || p.by_segment) return rc;
   JoinParams j;
   j.out = p.out;
@@ -416,6 +433,7 @@ int abft_paged_decode(const abft_paged_attn_args* a, void* stream) {
   p.scale_log2 = a->scale * 1.44269504088896340736f;
   const int grid = decode_grid(a, sms);
   p.by_segment = decode_by_segment(a, sms);
+  for (p.cluster_shift = 0; 1 << (p.cluster_shift + 1) <= p.by_segment;) ++p.cluster_shift;
   const size_t need = decode_bytes(a, sms);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
   if (off16(a->workspace)) return ABFT_ERR_ALIGNMENT;

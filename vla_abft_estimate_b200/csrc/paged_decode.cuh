@@ -27,13 +27,16 @@
 // into equal shares for the warps of one CTA per SM: lengths of any mix keep
 // every SM reading to the end. (Where lengths differ much a segment takes
 // kDecCost places in the list more than it has tiles, for its start and end.) A
-// warp's ring of loads runs on across segment boundaries. A segment inside one warp's share is finished by that warp;
-// pieces of a segment that crosses warps are joined in shared memory, those of
-// one that crosses CTAs by a second, small kernel, in a fixed order. A cache
-// too small to be worth sharing out gets a CTA per segment instead: nothing
-// crosses CTAs, and one launch does. (Joined instead by the last CTA to arrive,
-// an atomic counter's choice, 37 pieces of 8 heads took one SM 12 us; spread
-// over one block per head, launch included, 3 us.)
+// warp's ring of loads runs on across segment boundaries. A segment inside one
+// warp's share is finished by that warp; pieces of a segment that crosses warps
+// are joined in shared memory, those of one that crosses CTAs by a second, small
+// kernel, in a fixed order. (Joined instead by the last CTA to arrive, an atomic
+// counter's choice, 37 pieces of 8 heads took one SM 12 us; spread over one block
+// per head, launch included, 3 us.)
+//
+// A cache too small to be worth sharing out so gets a CTA or a cluster of CTAs
+// per segment: one launch, and the cluster's pieces are read from each other's
+// shared memory (1 sequence of 500 slots and 4 kv heads: 6.5 us, 7.5 by the list).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -95,6 +98,21 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The address of the same place in the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t to;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
+  return to;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 struct DecodeParams {
   PagedView kv;
   const void* q;
@@ -102,7 +120,8 @@ struct DecodeParams {
   int64_t qt, qh, ot, oh;  // token and head strides, elements
   int32_t group;           // query heads per kv head
   int32_t head_chunks;     // segments that share a kv head's query heads
-  int32_t by_segment;      // a CTA per segment; no pieces in memory, no second kernel
+  int32_t by_segment;      // CTAs (a cluster) per segment, no pieces in memory, no second kernel; 0: the list
+  int32_t cluster_shift;   // log2 of by_segment
   float scale_log2;        // scale * log2(e)
   float* part_o;           // [grid][2][heads of a segment][head_dim]: pieces of segments that cross CTAs
   float2* part_ml;         // [grid][2][heads of a segment] (m, l)
@@ -114,6 +133,7 @@ struct DecodeParams {
 // 128 segments of 2,048 slots 26.1 against 24.6 us, the long list 50.6 against
 // 49.5: one SM takes in some 62 GB/s however many warps ask.)
 constexpr int kDecWarps = 4;
+constexpr int kDecCluster = 8;  // CTAs of a segment at most
 constexpr int kDecTile = 32;
 // Places in the list that a segment takes for its start and end when the
 // longest sequence has over twice the tiles of the shortest: short segments
@@ -137,7 +157,7 @@ struct DecodeCfg {
   // bank conflicts) and (m, l) of each.
   static constexpr int kPitch = D + 4;
   static constexpr int kPieceBytes = kHeads * (kPitch + 2) * 4;
-  static_assert(kPieceBytes <= kWarpBytes, "a warp's last piece takes the place of its ring");
+  static_assert(2 * kPieceBytes <= kWarpBytes, "a warp's last piece takes the place of its ring, and the CTA's follows");
   static constexpr int kOffFirst = kWarps * kWarpBytes;  // the warps' first pieces
   static constexpr int kSmemBytes = kOffFirst + kWarps * kPieceBytes;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
@@ -219,15 +239,17 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
   // ---- this warp's share ------------------------------------------------------
   TileIter head;
   int total, shares, u0, u1, cost = 0;
-  if (p.by_segment) {  // the list is one segment, its shares this CTA's warps'
-    head.b = blockIdx.x / rows;
-    head.y = blockIdx.x - head.b * rows;
+  const int rank = static_cast<int>(blockIdx.x) & (p.by_segment - 1);  // of the cluster's CTAs
+  if (p.by_segment) {  // the list is one segment, its shares the cluster's warps'
+    const int segment = static_cast<int>(blockIdx.x) >> p.cluster_shift;
+    head.b = segment / rows;
+    head.y = segment - head.b * rows;
     bool bad;
     total = head.tiles = tiles_of<kTile>(kv, head.b, &head.len, &bad);
-    if (bad && head.y == 0 && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
-    shares = kWarps;
-    u0 = head.u = head.tile = share_start(total, shares, warp);
-    u1 = share_start(total, shares, warp + 1);
+    if (bad && head.y == 0 && rank == 0 && threadIdx.x == 0 && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_LEN);
+    shares = p.by_segment * kWarps;
+    u0 = head.u = head.tile = share_start(total, shares, rank * kWarps + warp);
+    u1 = share_start(total, shares, rank * kWarps + warp + 1);
   } else {
     // Lane i counts the sequences [i * part, (i + 1) * part): the lane that
     // holds a place is found by one scan, its sequence by another (1,024
@@ -601,6 +623,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
   // as the segment goes; the chain before warp 0 lacks its start (in an earlier
   // CTA). 16 threads take a head, each D / 16 of its elements, and read all
   // pieces at once.
+  // The CTA's piece for the others of its cluster.
+  float* piece = reinterpret_cast<float*>(smem + Cfg::kPieceBytes);
+  float2* piece_ml = reinterpret_cast<float2*>(piece + Cfg::kHeads * Cfg::kPitch);
+  if (p.by_segment > 1 && s_first[0] == 0 && s_last[0] == 0 && threadIdx.x < Cfg::kHeads)
+    piece_ml[threadIdx.x] = make_float2(-INFINITY, 0.f);  // no share, or the whole segment
   int over = -1;  // warp whose last piece goes on in the next CTA
 #pragma unroll 1
   for (int w = -1; w < kWarps; ++w) {
@@ -657,14 +684,54 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
           *reinterpret_cast<uint2*>(dst + i) =
               make_uint2(pack2<F16>(x[i] * inv, x[i + 1] * inv), pack2<F16>(x[i + 2] * inv, x[i + 3] * inv));
       } else {
-        float* dst = p.part_o + (slot + h) * D + d;
+        float* dst = p.by_segment ? piece + h * Cfg::kPitch + d : p.part_o + (slot + h) * D + d;
 #pragma unroll
         for (int i = 0; i < kPer; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-        if (d == 0) p.part_ml[slot + h] = make_float2(top, l_sum);
+        if (d == 0) (p.by_segment ? piece_ml + h : p.part_ml + slot + h)[0] = make_float2(top, l_sum);
       }
     }
   }
-  if (p.by_segment) return;
+  if (p.by_segment) {
+    if (p.by_segment == 1) return;
+    // The cluster's pieces, in the order of its CTAs; each CTA joins every
+    // by_segment-th head, D / 2 threads a head.
+    cluster_barrier();
+    const bool in_first = share_start(total, shares, kWarps) >= total;  // joined already
+    const int b = blockIdx.x / (rows << p.cluster_shift), y = (blockIdx.x >> p.cluster_shift) - b * rows;
+    const int hk = y / p.head_chunks, hc = y - hk * p.head_chunks;
+    const int nheads = in_first ? 0 : min(Cfg::kHeads, p.group - hc * Cfg::kHeads);
+    const int d = (threadIdx.x % (D / 2)) * 2;
+    for (int h = rank + (threadIdx.x / (D / 2) << p.cluster_shift); h < nheads;
+         h += (Cfg::kThreads / (D / 2)) << p.cluster_shift) {
+      const uint32_t at = smem_u32(piece + h * Cfg::kPitch + d), at_ml = smem_u32(piece_ml + h);
+      float2 ml[kDecCluster], v[kDecCluster];
+      float top = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < kDecCluster; ++r) {
+        ml[r] = make_float2(-INFINITY, 0.f);
+        if (r < p.by_segment) {
+          ml[r] = ld_cluster_f2(map_rank(at_ml, r));
+          v[r] = ld_cluster_f2(map_rank(at, r));
+        }
+        top = fmaxf(top, ml[r].x);
+      }
+      const float ms = top == -INFINITY ? 0.f : top;
+      float l_sum = 0.f, x = 0.f, z = 0.f;
+#pragma unroll
+      for (int r = 0; r < kDecCluster; ++r) {
+        if (ml[r].y == 0.f) continue;  // no piece: v was not written
+        const float f = exp2_approx(ml[r].x - ms);
+        l_sum += ml[r].y * f;
+        x += v[r].x * f;
+        z += v[r].y * f;
+      }
+      const float inv = l_sum > 0.f ? 1.f / l_sum : (l_sum == 0.f ? 0.f : l_sum);
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + b * p.ot + (hk * p.group + hc * Cfg::kHeads + h) * p.oh +
+                                   d) = pack2<F16>(x * inv, z * inv);
+    }
+    cluster_barrier();  // shared memory stays until it has been read
+    return;
+  }
   if (threadIdx.x == 0) {
     int4 spill = make_int4(0, 0, 0, 0);
     if (over >= 0)
