@@ -483,7 +483,6 @@ int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
   p.block_tokens = plan.block_tokens;
   p.splits = plan.splits;
   p.piece = plan.piece;
-  p.items = static_cast<int32_t>(plan.items / plan.splits);
   const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
   p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
   p.negate = a->scale < 0.f;

@@ -91,9 +91,8 @@ struct PrefillParams {
   int32_t group;           // query heads per kv head
   int32_t tile_tokens;     // tokens of one tile: 128 / group
   int32_t block_tokens;    // tokens of an item: one tile's or two's
-  int32_t splits;          // pieces of an item's keys at most: blocks of the grid for it
+  int32_t splits;          // pieces of an item's keys at most
   int32_t piece;           // steps of a piece
-  int32_t items;           // blocks of the grid for one piece of every item
   float scale_log2;        // |scale| * log2(e), never 0
   int32_t negate;          // scale < 0
   uint32_t group_inv;      // ceil(2^16 / group): row_token()
@@ -114,61 +113,69 @@ __host__ __device__ __forceinline__ int row_token(int row, uint32_t group_inv) {
   return static_cast<int>((static_cast<uint32_t>(row) * group_inv) >> 16);
 }
 
+// Pieces of `piece` steps that `steps` steps are cut into, one at least.
+__host__ __device__ __forceinline__ int pieces_of(int steps, int piece) {
+  return steps <= piece ? 1 : (steps + piece - 1) / piece;
+}
+
 // Keys that local token i of n sees in a sequence of length len.
 __host__ __device__ __forceinline__ int visible_keys(int len, int n, int i) {
   const int v = len - n + i + 1;
   return v > 0 ? v : 0;
 }
 
-// The packed sequences, each cut into blocks of `per` tokens, as a warp holds
-// them: lane i has the sequences [i * share, (i + 1) * share). Read once per
-// CTA: a scan of the whole batch for every item made 4 tokens for each of
-// 1,024 sequences of 500 slots 381 us instead of 240.
-struct BlockScan {
+// The list of work: the packed sequences, each cut into blocks of tokens, their
+// keys into pieces (as many for each block as the sequence's length gives, so
+// that places without work are few and at the end), as a warp holds it: lane i
+// has the sequences [i * share, (i + 1) * share). Read once per CTA: a scan of
+// the whole batch for every item made 4 tokens for each of 1,024 sequences of
+// 500 slots 381 us instead of 240.
+struct WorkScan {
   int share;
-  int blocks, upto;       // of this lane's sequences; with those of all lanes before
+  int places, upto;       // of this lane's sequences; with those of all lanes before
   int begin, count, len;  // share 1: the lane's sequence
 };
 
 // A sequence's packed rows and raw length (boundaries and length are asked for
-// together); returns its blocks.
-__device__ __forceinline__ int blocks_of(const PagedView& kv, const int32_t* cu, int tokens, int per, int b, int* begin,
-                                         int* count, int* len) {
+// together); returns its places in the list.
+__device__ __forceinline__ int places_of(const PrefillParams& p, int b, int* begin, int* count, int* len) {
   int end;
-  *len = kv.seq_lens[b];
-  packed_range(cu, b, tokens, begin, &end);
+  bool bad;
+  *len = p.kv.seq_lens[b];
+  packed_range(p.cu, b, p.tokens, begin, &end);
   *count = end - *begin;
-  return (*count + per - 1) / per;
+  const int keys = paged_clamp_len(*len, p.kv.max_pages, p.kv.page_shift, &bad);
+  return (*count + p.block_tokens - 1) / p.block_tokens * pieces_of((keys + kPreKeys - 1) / kPreKeys, p.piece);
 }
 
-__device__ __forceinline__ BlockScan scan_blocks(const PagedView& kv, const int32_t* cu, int tokens, int per, int lane) {
-  BlockScan s;
-  s.share = (kv.batch + 31) >> 5;
-  s.blocks = s.begin = s.count = s.len = 0;
-  const int b0 = lane * s.share, b1 = min(kv.batch, b0 + s.share);
+__device__ __forceinline__ WorkScan scan_work(const PrefillParams& p, int lane) {
+  WorkScan s;
+  s.share = (p.kv.batch + 31) >> 5;
+  s.places = s.begin = s.count = s.len = 0;
+  const int b0 = lane * s.share, b1 = min(p.kv.batch, b0 + s.share);
 #pragma unroll 4
-  for (int b = b0; b < b1; ++b) s.blocks += blocks_of(kv, cu, tokens, per, b, &s.begin, &s.count, &s.len);
-  s.upto = warp_scan(s.blocks, lane);
+  for (int b = b0; b < b1; ++b) s.places += places_of(p, b, &s.begin, &s.count, &s.len);
+  s.upto = warp_scan(s.places, lane);
   return s;
 }
 
-// Block `index` of the list; called by one warp. Heavier blocks (later tokens)
-// of a sequence come first. Up to 32 sequences are held in registers; of more,
-// the share that has the block is read again. Returns false behind the last
-// block.
-__device__ __forceinline__ bool find_block(const PagedView& kv, const int32_t* cu, int tokens, int per, const BlockScan& s,
-                                           int index, int lane, int* seq, int* block, int* begin, int* count, int* len) {
+// Place `index` of the list; called by one warp. First pieces of a sequence
+// come first, of them the heavier blocks (later tokens). Up to 32 sequences are
+// held in registers; of more, the share that has the place is read again.
+// Returns false behind the last place.
+__device__ __forceinline__ bool find_work(const PrefillParams& p, const WorkScan& s, int index, int lane, int* seq, int* block,
+                                          int* split, int* begin, int* count, int* len) {
   const uint32_t past = __ballot_sync(0xFFFFFFFFu, s.upto > index);
   if (past == 0) return false;
   const int owner = __ffs(past) - 1;
-  int before = __shfl_sync(0xFFFFFFFFu, s.upto - s.blocks, owner);
-  int mine = s.blocks, lo = s.begin, n = s.count, length = s.len, src = owner, from = 0;
+  int before = __shfl_sync(0xFFFFFFFFu, s.upto - s.places, owner);
+  int mine = s.places, lo = s.begin, n = s.count, length = s.len, src = owner, from = 0;
   if (s.share > 1) {
-    const int end = min(kv.batch, (owner + 1) * s.share);
+    const int end = min(p.kv.batch, (owner + 1) * s.share);
     for (from = owner * s.share;; from += 32) {
       if (from >= end) return false;  // boundaries that do not rise
       mine = 0;
-      if (from + lane < end) mine = blocks_of(kv, cu, tokens, per, from + lane, &lo, &n, &length);
+      if (from + lane < end) mine = places_of(p, from + lane, &lo, &n, &length);
       const int upto = warp_scan(mine, lane);
       const uint32_t in = __ballot_sync(0xFFFFFFFFu, before + upto > index);
       if (in != 0) {
@@ -179,14 +186,15 @@ __device__ __forceinline__ bool find_block(const PagedView& kv, const int32_t* c
       before += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
   }
-  const int blocks = __shfl_sync(0xFFFFFFFFu, mine, src);
-  const int at = blocks - 1 - (index - before);
-  if (at < 0 || at >= blocks) return false;  // boundaries that do not rise
+  const int at = index - before;
+  if (at < 0 || at >= __shfl_sync(0xFFFFFFFFu, mine, src)) return false;  // boundaries that do not rise
   *seq = from + src;
-  *block = at;
   *begin = __shfl_sync(0xFFFFFFFFu, lo, src);
   *count = __shfl_sync(0xFFFFFFFFu, n, src);
   *len = __shfl_sync(0xFFFFFFFFu, length, src);
+  const int blocks = (*count + p.block_tokens - 1) / p.block_tokens;
+  *split = at / blocks;
+  *block = blocks - 1 - (at - *split * blocks);
   return true;
 }
 
@@ -886,19 +894,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       // ---------------------------------------------------------- work
       int index = blockIdx.x, published = 0, asked = 0;
       bool ok = true;
-      const BlockScan scan = scan_blocks(kv, p.cu, p.tokens, p.block_tokens, lane);
+      const WorkScan scan = scan_work(p, lane);
       while (ok) {
         PrefillItem x;
         x.valid = 0;
         bool publish = index < 0;
         if (index >= 0) {
-          // First pieces first: every item has one, few have the last.
-          x.split = index / p.items;
-          const int rest = index - x.split * p.items;
-          x.hk = rest % kv.kv_heads;
+          x.hk = index % kv.kv_heads;
           int seq = 0, block = 0, raw_len = 0;
-          if (find_block(kv, p.cu, p.tokens, p.block_tokens, scan, rest / kv.kv_heads, lane, &seq, &block, &x.row0, &x.n,
-                         &raw_len)) {
+          if (find_work(p, scan, index / kv.kv_heads, lane, &seq, &block, &x.split, &x.row0, &x.n, &raw_len)) {
             bool bad_len;
             x.seq = seq;
             x.len = paged_clamp_len(raw_len, kv.max_pages, kv.page_shift, &bad_len);
