@@ -283,6 +283,42 @@ def test_decode_by_clusters(cuda_device, lens, kv_heads, group, d, dtype):
     cache.check_status()
 
 
+@pytest.mark.parametrize("kv_heads,group,d,lens,new", [
+    (1, 7, 128, (5000, 3, 700), (9, 3, 5)),             # one sequence cut, the others whole
+    (4, 2, 64, (4097,), (70,)),                          # blocks of unlike length
+    (2, 16, 128, (2300, 2299, 0, 1), (1, 20, 0, 1)),
+    (1, 4, 64, [3000] + [40 + i for i in range(39)], [33] + [1 + i % 3 for i in range(39)]),  # two sequences a lane
+])
+def test_pieces_chosen_for_the_lengths(cuda_device, kv_heads, group, d, lens, new):
+    """Tables far wider than the sequences; lengths that change between the
+    replays of a graph, whose pieces are chosen each time."""
+    dev = cuda_device
+    pool = Pool(lens, kv_heads, 16, d, BF16, extra_columns=1500)
+    cache = pool.device_cache(dev, PagedKVCache)
+    rows = sum(new)
+    cu = torch.tensor([0, *torch.tensor(new).cumsum(0)], dtype=torch.int32, device=dev)
+    q = torch.randn(rows + 3, kv_heads * group, d, generator=torch.Generator().manual_seed(14)).to(BF16)
+    x, out = q.to(dev), torch.empty_like(q, device=dev)
+    cache.prefill(x, cu, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.prefill(x, cu, out=out)
+    for short in (0, 1, 0):
+        now = [max(n, t - short * 900) for t, n in zip(lens, new)]
+        cache.seq_lens.copy_(torch.tensor(now, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        want, tol = attention(pool, q[:rows], owners_of(new, now))
+        close(out[:rows], want, tol)
+        assert (out[rows:] == 7.0).all()
+    cache.check_status()
+    cache.seq_lens.zero_()  # rows without keys
+    graph.replay()
+    assert (out[:rows] == 0).all()
+    with pytest.raises(ValueError, match="length"):
+        cache.check_status()
+
+
 def test_result_over_q_and_a_slice_of_a_wider_table(cuda_device):
     dev = cuda_device
     pool = Pool([2000, 77, 300], 4, 16, 128, BF16)

@@ -299,6 +299,7 @@ int page_map(CUtensorMap* m, const abft_paged_kv& c, const void* pages, int64_t 
 // kv head, their keys in pieces of `piece` steps.
 struct PrefillPlan {
   int tile_tokens, block_tokens, splits, piece;
+  bool choose;    // the kernel chooses the piece, for `splits` pieces at most
   int64_t items;  // blocks of the grid
 };
 
@@ -312,33 +313,36 @@ PrefillPlan prefill_plan(const abft_paged_attn_args* a, int sms) {
   if (blocks(r.tile_tokens) <= sms) r.block_tokens = r.tile_tokens;
   const int64_t base = blocks(r.block_tokens);
   const int64_t steps = (static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size + kPreKeys - 1) / kPreKeys;
-  // Pieces, of four steps at least: as many as give each SM one item, counted
-  // without the blocks that only ragged chunks have, and twice as many for
-  // several sequences, whose lengths may differ, if one each is not enough.
-  // (One sequence, 64 tokens on 16,384 slots: 1 piece 159 us, 8 pieces 34, 16
-  // 44; 512 tokens on 8,192, 116 items: 1 piece 86, 2 pieces 100, for the sums
-  // that go through memory. Nine sequences of 5 tokens on up to 7,777: 4 pieces
-  // 29, 8 pieces 21; four of 16 on 32,768 each: 4 pieces 101, 8 pieces 103.)
+  // Without a number of pieces given, the kernel chooses their length for the
+  // sequences it finds (scan_work); here their number is bounded: room for each
+  // SM to have one, for several sequences, whose lengths may differ, four. One
+  // where the blocks alone fill the SMs. (One sequence, 64 tokens on 16,384
+  // slots: 1 piece 159 us, 8 pieces 34, 16 40; 512 tokens on 8,192, 116 items: 1
+  // piece 81, 2 pieces 96, for the sums that go through memory. Nine sequences of
+  // 5 tokens, 36 items, on up to 7,777 slots: 4 pieces 29, 8 21, 16 18; on 7,777
+  // each: 4 pieces 36, 8 37, 16 46. Chosen in the kernel: 36, 79, 19, 38; in tables
+  // of 32,768 slots 64 tokens on 4,000 22 us, 46 in pieces of the table's width.)
   int64_t n = a->num_splits;
   if (n == 0) {
     int64_t least = (a->tokens + r.block_tokens - 1) / r.block_tokens;
     if (least < a->kv.batch) least = a->kv.batch;
     n = sms / (least * a->kv.kv_heads);
-    if (n > 1 && a->kv.batch > 1) n *= 2;
-    if (n > steps / 4) n = steps / 4;
+    if (a->kv.batch > 1) n *= 4;
+    if (n > (steps + kPreLeast - 1) / kPreLeast) n = (steps + kPreLeast - 1) / kPreLeast;
   }
   if (n > steps) n = steps;
   if (n < 1) n = 1;
+  r.choose = a->num_splits == 0 && n > 1;
   r.piece = static_cast<int>((steps + n - 1) / n);
   r.splits = static_cast<int>((steps + r.piece - 1) / r.piece);
-  r.items = base * r.splits;
+  r.items = r.choose ? (base > sms ? base : sms) : base * r.splits;
   return r;
 }
 
-size_t prefill_bytes(const abft_paged_attn_args* a, int splits) {
-  if (splits <= 1) return 0;
-  const size_t rows = static_cast<size_t>(a->tokens) * a->heads * splits;
-  return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2));
+size_t prefill_bytes(const abft_paged_attn_args* a, const PrefillPlan& plan) {
+  if (plan.splits <= 1) return 0;
+  const size_t rows = static_cast<size_t>(a->tokens) * a->heads * plan.splits;
+  return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2)) + (plan.choose ? 16 : 0);
 }
 
 template <int D, bool F16, bool kShared>
@@ -360,6 +364,7 @@ int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUten
   j.heads = a->heads;
   j.splits = p.splits;
   j.piece = p.piece;
+  j.chosen = p.chosen;
   j.block_tokens = p.block_tokens;
   j.part_o = p.part_o;
   j.part_ml = p.part_ml;
@@ -460,7 +465,7 @@ size_t abft_paged_prefill_workspace_bytes(const abft_paged_attn_args* a) {
   if (attn_check(a, false) != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return 0;
   int dev = 0, sms = a->num_sms;
   if (sms == 0 && paged_device(&dev, &sms) != ABFT_OK) sms = 148;
-  return prefill_bytes(a, prefill_plan(a, sms).splits);
+  return prefill_bytes(a, prefill_plan(a, sms));
 }
 
 int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
@@ -482,17 +487,20 @@ int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
   p.tile_tokens = plan.tile_tokens;
   p.block_tokens = plan.block_tokens;
   p.splits = plan.splits;
-  p.piece = plan.piece;
+  p.piece = plan.choose ? 0 : plan.piece;
+  p.sms = sms;
   const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
   p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
   p.negate = a->scale < 0.f;
   p.group_inv = (65536u + p.group - 1) / p.group;
-  const size_t need = prefill_bytes(a, p.splits);
+  const size_t need = prefill_bytes(a, plan);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
   if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float2*>(
       p.part_o + static_cast<size_t>(a->tokens) * a->heads * p.splits * a->kv.head_dim);
+  p.chosen = plan.choose ? reinterpret_cast<int32_t*>(p.part_ml + static_cast<size_t>(a->tokens) * a->heads * p.splits)
+                         : nullptr;
   CUtensorMap tm_k, tm_v;
   if ((rc = page_map(&tm_k, a->kv, a->kv.k_pages, a->kv.k_page_stride)) != ABFT_OK) return rc;
   if ((rc = page_map(&tm_v, a->kv, a->kv.v_pages, a->kv.v_page_stride)) != ABFT_OK) return rc;

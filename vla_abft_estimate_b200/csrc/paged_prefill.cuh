@@ -92,7 +92,9 @@ struct PrefillParams {
   int32_t tile_tokens;     // tokens of one tile: 128 / group
   int32_t block_tokens;    // tokens of an item: one tile's or two's
   int32_t splits;          // pieces of an item's keys at most
-  int32_t piece;           // steps of a piece
+  int32_t piece;           // steps of a piece; 0: chosen by the kernel, for the lengths it finds
+  int32_t sms;             // items that run at once
+  int32_t* chosen;         // [1] the piece chosen, for the join
   float scale_log2;        // |scale| * log2(e), never 0
   int32_t negate;          // scale < 0
   uint32_t group_inv;      // ceil(2^16 / group): row_token()
@@ -131,30 +133,74 @@ __host__ __device__ __forceinline__ int visible_keys(int len, int n, int i) {
 // the whole batch for every item made 4 tokens for each of 1,024 sequences of
 // 500 slots 381 us instead of 240.
 struct WorkScan {
-  int share;
+  int share, piece;
   int places, upto;       // of this lane's sequences; with those of all lanes before
   int begin, count, len;  // share 1: the lane's sequence
 };
 
 // A sequence's packed rows and raw length (boundaries and length are asked for
-// together); returns its places in the list.
-__device__ __forceinline__ int places_of(const PrefillParams& p, int b, int* begin, int* count, int* len) {
+// together); returns its blocks and the steps of its whole length.
+__device__ __forceinline__ int blocks_of(const PrefillParams& p, int b, int* begin, int* count, int* len, int* steps) {
   int end;
   bool bad;
   *len = p.kv.seq_lens[b];
   packed_range(p.cu, b, p.tokens, begin, &end);
   *count = end - *begin;
   const int keys = paged_clamp_len(*len, p.kv.max_pages, p.kv.page_shift, &bad);
-  return (*count + p.block_tokens - 1) / p.block_tokens * pieces_of((keys + kPreKeys - 1) / kPreKeys, p.piece);
+  *steps = (keys + kPreKeys - 1) / kPreKeys;
+  return (*count + p.block_tokens - 1) / p.block_tokens;
 }
+
+// A piece chosen here leaves no more items than run at once, so that the longest
+// sequences, whatever their share of the table, are cut and the others are not;
+// kPreLeast steps at least. When the blocks alone are as many, nothing is cut.
+// Every CTA finds the same.
+constexpr int kPreLeast = 4;
 
 __device__ __forceinline__ WorkScan scan_work(const PrefillParams& p, int lane) {
   WorkScan s;
   s.share = (p.kv.batch + 31) >> 5;
-  s.places = s.begin = s.count = s.len = 0;
+  s.piece = p.piece;
+  s.begin = s.count = s.len = 0;
   const int b0 = lane * s.share, b1 = min(p.kv.batch, b0 + s.share);
+  int blocks = 0, steps = 0, most = 0, weight = 0, weight8 = 0;
 #pragma unroll 4
-  for (int b = b0; b < b1; ++b) s.places += places_of(p, b, &s.begin, &s.count, &s.len);
+  for (int b = b0; b < b1; ++b) {
+    const int mine = blocks_of(p, b, &s.begin, &s.count, &s.len, &steps);
+    blocks += mine;
+    weight += mine * steps;
+    weight8 += mine * ((steps + 255) >> 8);
+    if (mine > 0) most = max(most, steps);
+  }
+  auto places = [&](int piece) {  // of this lane's sequences
+    if (s.share == 1) return blocks * pieces_of(steps, piece);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      int begin, count, len, of;
+      const int mine = blocks_of(p, b, &begin, &count, &len, &of);
+      sum += mine * pieces_of(of, piece);
+    }
+    return sum;
+  };
+  if (s.piece == 0) {
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    const int all = __reduce_add_sync(0xFFFFFFFFu, blocks);
+    const int room = p.sms / p.kv.kv_heads;
+    s.piece = max(most, 1);
+    if (all < room) {
+      // blocks of w steps in all are ceil(steps / piece) <= (w - all) / piece +
+      // all items; 2^16 steps and more are counted in units of 2^8.
+      const int shift = most >= 65536 ? 8 : 0;
+      const int w = __reduce_add_sync(0xFFFFFFFFu, shift ? weight8 : weight);
+      const int enough = (max(w - (shift ? 0 : all), 0) / (room - all) + 1) << shift;
+      s.piece = max(max(enough, kPreLeast), (most + p.splits - 1) / p.splits);
+      // The longest sequence in as many pieces, of equal length, if the others
+      // allow it.
+      const int even = max(kPreLeast, pieces_of(most, pieces_of(most, s.piece)));
+      if (even < s.piece && static_cast<int>(__reduce_add_sync(0xFFFFFFFFu, places(even))) <= room) s.piece = even;
+    }
+  }
+  s.places = places(s.piece);
   s.upto = warp_scan(s.places, lane);
   return s;
 }
@@ -175,7 +221,11 @@ __device__ __forceinline__ bool find_work(const PrefillParams& p, const WorkScan
     for (from = owner * s.share;; from += 32) {
       if (from >= end) return false;  // boundaries that do not rise
       mine = 0;
-      if (from + lane < end) mine = places_of(p, from + lane, &lo, &n, &length);
+      if (from + lane < end) {
+        int steps;
+        mine = blocks_of(p, from + lane, &lo, &n, &length, &steps);
+        mine *= pieces_of(steps, s.piece);
+      }
       const int upto = warp_scan(mine, lane);
       const uint32_t in = __ballot_sync(0xFFFFFFFFu, before + upto > index);
       if (in != 0) {
@@ -186,15 +236,19 @@ __device__ __forceinline__ bool find_work(const PrefillParams& p, const WorkScan
       before += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
   }
-  const int at = index - before;
-  if (at < 0 || at >= __shfl_sync(0xFFFFFFFFu, mine, src)) return false;  // boundaries that do not rise
+  const int at = index - before, places = __shfl_sync(0xFFFFFFFFu, mine, src);
+  if (at < 0 || at >= places) return false;  // boundaries that do not rise
   *seq = from + src;
   *begin = __shfl_sync(0xFFFFFFFFu, lo, src);
   *count = __shfl_sync(0xFFFFFFFFu, n, src);
   *len = __shfl_sync(0xFFFFFFFFu, length, src);
   const int blocks = (*count + p.block_tokens - 1) / p.block_tokens;
-  *split = at / blocks;
-  *block = blocks - 1 - (at - *split * blocks);
+  *split = -1;
+  *block = blocks - 1 - at;
+  if (places != blocks) {
+    *split = at / blocks;
+    *block += *split * blocks;
+  }
   return true;
 }
 
@@ -293,7 +347,7 @@ __device__ __forceinline__ void mbar_wait_bounded(uint64_t* bar, uint32_t parity
 struct __align__(16) PrefillItem {
   int32_t valid;    // 0: no more work
   int32_t hk;       // kv head
-  int32_t split;    // piece
+  int32_t split;    // piece; -1: the only one, its rows are results
   int32_t seq, len; // sequence, its keys
   int32_t row0, n;  // its first packed row and its rows
   int32_t tok0;     // first token of the item within them
@@ -593,7 +647,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.ot + head * p.oh;
       if (kShared ? end == j0 : !any) {  // no keys
         if (live && (t == 0 || !kShared)) {
-          if (p.splits == 1)
+          if (x.split < 0)
             for (int k = 0; k < D; k += 8) *reinterpret_cast<uint4*>(dst + k) = make_uint4(0u, 0u, 0u, 0u);
           else
             p.part_ml[at] = make_float2(-INFINITY, 0.f);
@@ -625,7 +679,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           c0 = t * (D / 2);
           c1 = c0 + D / 2;
         }
-        if (p.splits > 1) {
+        if (x.split >= 0) {
           if (live && c0 == 0) p.part_ml[at] = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
         } else {
           const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
@@ -649,7 +703,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(z[k]), f1, __uint_as_float(o[k])));
           }
           if (!live) continue;
-          if (p.splits > 1) {
+          if (x.split >= 0) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
               *reinterpret_cast<uint4*>(p.part_o + at * D + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
@@ -900,6 +954,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         x.valid = 0;
         bool publish = index < 0;
         if (index >= 0) {
+          if (index == 0 && p.chosen != nullptr && lane == 0) *p.chosen = scan.piece;
           x.hk = index % kv.kv_heads;
           int seq = 0, block = 0, raw_len = 0;
           if (find_work(p, scan, index / kv.kv_heads, lane, &seq, &block, &x.split, &x.row0, &x.n, &raw_len)) {
@@ -918,12 +973,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
               steps[t] = last >= first ? (visible_keys(x.len, x.n, last) + kPreKeys - 1) / kPreKeys : 0;
             }
             const int most = max(steps[0], steps[1]);
-            x.j0 = min(x.split * p.piece, most);
-            x.j1 = min(x.j0 + p.piece, most);
+            x.j0 = min(max(x.split, 0) * scan.piece, most);
+            x.j1 = min(x.j0 + scan.piece, most);
             x.end0 = max(x.j0, min(x.j1, steps[0]));
             x.end1 = kShared ? x.end0 : max(x.j0, min(x.j1, steps[1]));
             // Without keys the rows still get their zeros when no join follows.
-            publish = x.j0 < x.j1 || p.splits == 1;
+            publish = x.j0 < x.j1 || x.split < 0;
             x.valid = 1;
           }
         }
@@ -971,6 +1026,7 @@ struct PrefillJoinParams {
   void* out;
   int64_t ot, oh;
   int32_t tokens, heads, splits, piece, block_tokens;
+  const int32_t* chosen;  // the piece, or NULL: `piece`
   const float* part_o;
   const float2* part_ml;
 };
@@ -984,6 +1040,7 @@ __global__ void __launch_bounds__(32 * kPreJoinWarps) paged_prefill_join_kernel(
   const int index = blockIdx.x * kPreJoinWarps + (threadIdx.x >> 5);
   const int row = index / p.heads, h = index - row * p.heads;
   if (row >= p.tokens) return;
+  const int piece = p.chosen != nullptr ? *p.chosen : p.piece;
   const int b = owner_of(p.cu, p.kv.batch, row, lane);
   if (b >= p.kv.batch) return;  // behind the last sequence
   int row0, row_end;
@@ -992,9 +1049,10 @@ __global__ void __launch_bounds__(32 * kPreJoinWarps) paged_prefill_join_kernel(
   const int n = row_end - row0;
   bool bad;
   const int len = paged_clamp_len(p.kv.seq_lens[b], p.kv.max_pages, p.kv.page_shift, &bad);
+  if (pieces_of((len + kPreKeys - 1) / kPreKeys, piece) == 1) return;  // the row is done
   // Pieces of the row's item.
   const int last = min(((row - row0) / p.block_tokens + 1) * p.block_tokens, n) - 1;
-  const int count = ((visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys + p.piece - 1) / p.piece;
+  const int count = ((visible_keys(len, n, last) + kPreKeys - 1) / kPreKeys + piece - 1) / piece;
   const int64_t at = (static_cast<int64_t>(row) * p.heads + h) * p.splits;
   // The maximum of all pieces first, then sums that do not wait for each other.
   float top = -INFINITY;

@@ -279,8 +279,8 @@ class PagedKVCache:
         length, 0 and 1 included; rows behind cu[batch] are left as they were
         in ``out`` (undefined without one), which may be ``q``.
         ``num_splits``: pieces the keys of
-        a block of query rows are cut into (0: chosen from the rows, the heads
-        and the table's width)."""
+        a block of query rows are cut into (0: chosen on the device for the
+        sequences' lengths)."""
         return self._attention(True, q, cu_seqlens, scale, out, num_splits, 0)
 
     def _attention(self, prefill, q, cu, scale, out, num_splits, num_sms):
