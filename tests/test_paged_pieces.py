@@ -1,0 +1,70 @@
+"""Paged prefill's list of work on the host: the pieces chosen for a batch fit
+the grid and the scratch, whatever its lengths."""
+import subprocess
+
+import pytest
+
+from vla_abft_estimate_b200 import _build
+
+from .test_paged_host import _have_nvcc
+
+PROGRAM = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "paged_prefill.cuh"
+using namespace abft;
+static uint64_t state = 88172645463325252ull;
+static int below(int n) {
+  state ^= state << 13, state ^= state >> 7, state ^= state << 17;
+  return static_cast<int>((state >> 11) % n);
+}
+int main() {
+  static int blocks[256], steps[256];
+  for (int piece : {1, 4, 100})
+    for (int s = 0; s < 1000; ++s) {
+      const int n = pieces_of(s, piece);
+      if (n < 1 || (s > 0 && ((n - 1) * piece >= s || n * piece < s))) return std::printf("pieces_of %d %d\n", s, piece), 1;
+    }
+  long cut = 0, tight = 0;
+  for (int round = 0; round < 300000; ++round) {
+    const int batch = 1 + below(1 << below(8)), room = 1 + below(200), splits = 1 + below(200);
+    const int top = 1 + below(1 << (1 + below(round % 50 == 0 ? 22 : 12))), idle = below(4);
+    WorkSums all = {0, 0, 0, 0};
+    for (int b = 0; b < batch; ++b) {
+      blocks[b] = below(4) == 0 ? 0 : 1 + below(3);
+      steps[b] = below(4) < idle ? 0 : 1 + below(top);
+      all.add(blocks[b], steps[b]);
+    }
+    const int piece = fitting_piece(all, room, splits);
+    auto places = [&](int of) {
+      long sum = 0;
+      for (int b = 0; b < batch; ++b) sum += static_cast<long>(blocks[b]) * pieces_of(steps[b], of);
+      return sum;
+    };
+    const long limit = all.blocks < room ? room : all.blocks;
+    if (places(piece) > limit) return std::printf("%ld places for %ld\n", places(piece), limit), 1;
+    for (int b = 0; b < batch; ++b)
+      if (blocks[b] > 0 && pieces_of(steps[b], piece) > splits) return std::printf("more pieces than scratch\n"), 1;
+    cut += places(piece) > all.blocks;
+    tight += places(piece) > all.blocks && places(piece) == room - 1;  // (weight - blocks) / piece < room - blocks
+  }
+  std::printf("%ld %ld\n", cut, tight);
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(not _have_nvcc(), reason="needs nvcc")
+def test_chosen_pieces_fit_the_grid(tmp_path):
+    """Random batches, sequences without keys and without new rows among them:
+    no more places than items that run at once (or than blocks, when those alone
+    are more), no sequence in more pieces than the scratch holds."""
+    src = tmp_path / "pieces.cu"
+    src.write_text(PROGRAM)
+    exe = tmp_path / "pieces"
+    subprocess.check_call([_build._nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O2",
+                           f"-I{_build.CSRC_DIR}", f"-I{_build.INCLUDE_DIR}", str(src), "-o", str(exe)])
+    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+    cut, tight = (int(x) for x in out.stdout.split())
+    assert cut > 10_000 and tight > 100  # batches that are cut, and lists that reach the bound

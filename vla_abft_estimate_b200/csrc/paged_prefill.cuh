@@ -151,11 +151,36 @@ __device__ __forceinline__ int blocks_of(const PrefillParams& p, int b, int* beg
   return (*count + p.block_tokens - 1) / p.block_tokens;
 }
 
-// A piece chosen here leaves no more items than run at once, so that the longest
-// sequences, whatever their share of the table, are cut and the others are not;
-// kPreLeast steps at least. When the blocks alone are as many, nothing is cut.
-// Every CTA finds the same.
+// Blocks of sequences, and what the choice of the piece needs of their steps. A
+// block without keys still takes a place in the list, so it weighs a step.
+struct WorkSums {
+  int blocks, most;        // blocks; the most steps of one
+  int weight, weight256;   // steps of all blocks, and in units of 256 (rounded up)
+  __host__ __device__ void add(int count, int steps) {
+    blocks += count;
+    weight += count * (steps > 1 ? steps : 1);
+    weight256 += count * (steps > 256 ? (steps + 255) >> 8 : 1);
+    if (count > 0 && steps > most) most = steps;
+  }
+  __host__ __device__ bool units() const { return most >= 65536; }
+};
+
+// A piece that leaves no more than `room` items, those that run at once, so that
+// the longest sequences, whatever their share of the table, are cut and the
+// others are not; kPreLeast steps at least, and `splits` pieces of a sequence at
+// most. When the blocks alone are as many, nothing is cut. A block of s >= 1
+// steps is ceil(s / piece) <= (s - 1) / piece + 1 items, so all are at most
+// (weight - blocks) / piece + blocks; 2^16 steps and more are counted in units.
 constexpr int kPreLeast = 4;
+
+__host__ __device__ __forceinline__ int fitting_piece(const WorkSums& all, int room, int splits) {
+  if (all.blocks >= room) return all.most > 1 ? all.most : 1;
+  int piece = ((all.units() ? all.weight256 : all.weight) - all.blocks) / (room - all.blocks) + 1;
+  if (all.units()) piece <<= 8;
+  if (piece < kPreLeast) piece = kPreLeast;
+  const int least = (all.most + splits - 1) / splits;
+  return piece > least ? piece : least;
+}
 
 __device__ __forceinline__ WorkScan scan_work(const PrefillParams& p, int lane) {
   WorkScan s;
@@ -163,17 +188,15 @@ __device__ __forceinline__ WorkScan scan_work(const PrefillParams& p, int lane) 
   s.piece = p.piece;
   s.begin = s.count = s.len = 0;
   const int b0 = lane * s.share, b1 = min(p.kv.batch, b0 + s.share);
-  int blocks = 0, steps = 0, most = 0, weight = 0, weight8 = 0;
+  WorkSums sums = {0, 0, 0, 0};
+  int steps = 0;
 #pragma unroll 4
   for (int b = b0; b < b1; ++b) {
     const int mine = blocks_of(p, b, &s.begin, &s.count, &s.len, &steps);
-    blocks += mine;
-    weight += mine * steps;
-    weight8 += mine * ((steps + 255) >> 8);
-    if (mine > 0) most = max(most, steps);
+    sums.add(mine, steps);
   }
   auto places = [&](int piece) {  // of this lane's sequences
-    if (s.share == 1) return blocks * pieces_of(steps, piece);
+    if (s.share == 1) return sums.blocks * pieces_of(steps, piece);
     int sum = 0;
     for (int b = b0; b < b1; ++b) {
       int begin, count, len, of;
@@ -182,21 +205,17 @@ __device__ __forceinline__ WorkScan scan_work(const PrefillParams& p, int lane) 
     }
     return sum;
   };
-  if (s.piece == 0) {
-    most = __reduce_max_sync(0xFFFFFFFFu, most);
-    const int all = __reduce_add_sync(0xFFFFFFFFu, blocks);
+  if (s.piece == 0) {  // chosen here; every CTA finds the same
+    WorkSums all;
+    all.most = __reduce_max_sync(0xFFFFFFFFu, sums.most);
+    all.blocks = __reduce_add_sync(0xFFFFFFFFu, sums.blocks);
+    all.weight = all.weight256 = __reduce_add_sync(0xFFFFFFFFu, all.units() ? sums.weight256 : sums.weight);
     const int room = p.sms / p.kv.kv_heads;
-    s.piece = max(most, 1);
-    if (all < room) {
-      // blocks of w steps in all are ceil(steps / piece) <= (w - all) / piece +
-      // all items; 2^16 steps and more are counted in units of 2^8.
-      const int shift = most >= 65536 ? 8 : 0;
-      const int w = __reduce_add_sync(0xFFFFFFFFu, shift ? weight8 : weight);
-      const int enough = (max(w - (shift ? 0 : all), 0) / (room - all) + 1) << shift;
-      s.piece = max(max(enough, kPreLeast), (most + p.splits - 1) / p.splits);
+    s.piece = fitting_piece(all, room, p.splits);
+    if (all.blocks < room) {
       // The longest sequence in as many pieces, of equal length, if the others
       // allow it.
-      const int even = max(kPreLeast, pieces_of(most, pieces_of(most, s.piece)));
+      const int even = max(kPreLeast, pieces_of(all.most, pieces_of(all.most, s.piece)));
       if (even < s.piece && static_cast<int>(__reduce_add_sync(0xFFFFFFFFu, places(even))) <= room) s.piece = even;
     }
   }
