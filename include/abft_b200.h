@@ -421,6 +421,13 @@ int abft_check_only_noalloc(const abft_check_args* args, void* stream);
  *                         position; attention gives them 0);
  *   ABFT_PAGED_BAD_ANGLE  a position at or beyond max_positions of the
  *                         rotation table: append skips the token;
+ *   ABFT_PAGED_BAD_ROWS   cu_seqlens that does not start at 0, falls, or passes
+ *                         `tokens`: rows before the first sequence, and those
+ *                         of a sequence whose boundaries fall or lie outside
+ *                         [0, tokens], are left as they were and nothing is
+ *                         appended for them; where boundaries fall, rows that
+ *                         more than one sequence could claim are not appended
+ *                         either, and attention leaves them undefined;
  *   ABFT_PAGED_TIMEOUT    a bounded wait of the prefill kernel gave up: its
  *                         output is incomplete.
  * Slots at or beyond a sequence's length are never used: they may hold
@@ -429,6 +436,7 @@ int abft_check_only_noalloc(const abft_check_args* args, void* stream);
 #define ABFT_PAGED_BAD_LEN   2u
 #define ABFT_PAGED_BAD_ANGLE 4u
 #define ABFT_PAGED_TIMEOUT   8u
+#define ABFT_PAGED_BAD_ROWS  16u
 
 /* A page pool and the sequences in it. */
 typedef struct abft_paged_kv {

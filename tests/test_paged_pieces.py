@@ -1,4 +1,5 @@
-"""Paged prefill's list of work on the host: the pieces chosen for a batch fit
+"""Paged prefill's list of work on the host: the rows of a sequence lie within
+the call's whatever the boundaries say, and the pieces chosen for a batch fit
 the grid and the scratch, whatever its lengths."""
 import subprocess
 
@@ -24,6 +25,15 @@ int main() {
     for (int s = 0; s < 1000; ++s) {
       const int n = pieces_of(s, piece);
       if (n < 1 || (s > 0 && ((n - 1) * piece >= s || n * piece < s))) return std::printf("pieces_of %d %d\n", s, piece), 1;
+    }
+  const int edge[] = {-2147483647 - 1, -5, -1, 0, 1, 3, 7, 59, 60, 61, 900, 2147483647};
+  for (int lo : edge)
+    for (int hi : edge) {
+      const int cu[2] = {lo, hi};
+      int begin, end;
+      packed_range(cu, 0, 60, &begin, &end);
+      const bool ok = 0 <= lo && lo <= hi && hi <= 60;
+      if (ok ? begin != lo || end != hi : begin != 0 || end != 0) return std::printf("packed_range %d %d\n", lo, hi), 1;
     }
   long cut = 0, tight = 0;
   for (int round = 0; round < 300000; ++round) {
@@ -58,7 +68,8 @@ int main() {
 def test_chosen_pieces_fit_the_grid(tmp_path):
     """Random batches, sequences without keys and without new rows among them:
     no more places than items that run at once (or than blocks, when those alone
-    are more), no sequence in more pieces than the scratch holds."""
+    are more), no sequence in more pieces than the scratch holds. Boundaries that fall or lie
+    outside the rows give a sequence none."""
     src = tmp_path / "pieces.cu"
     src.write_text(PROGRAM)
     exe = tmp_path / "pieces"

@@ -82,6 +82,7 @@ PAGED_BAD_PAGE = 1
 PAGED_BAD_LEN = 2
 PAGED_BAD_ANGLE = 4
 PAGED_TIMEOUT = 8
+PAGED_BAD_ROWS = 16
 
 
 class AbftError(RuntimeError):

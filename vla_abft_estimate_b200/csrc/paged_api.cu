@@ -147,7 +147,7 @@ int launch_append(AppendParams p, int sms, cudaStream_t s) {
   // Halve the warps of a token while a full set of the SMs' blocks is left.
   p.warps_shift = 3;
   while (p.warps_shift > 0 && (p.tokens << (p.warps_shift - 1)) >= int64_t{16} * sms) --p.warps_shift;
-  const int64_t blocks = ((p.tokens << p.warps_shift) + kAppendWarps - 1) / kAppendWarps;
+  const int64_t blocks = ((p.tokens << p.warps_shift) + kAppendWarps - 1) / kAppendWarps + (p.cu != nullptr);
   return launch(kv_append_kernel<D, F16>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, s, p);
 }
 

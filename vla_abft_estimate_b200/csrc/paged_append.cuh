@@ -70,6 +70,17 @@ __device__ __forceinline__ int owner_of(const int32_t* cu, int batch, int64_t t,
   return n;
 }
 
+// One warp of a launch looks at all boundaries; they start at 0, do not fall
+// and end within the rows.
+__device__ __forceinline__ void check_boundaries(const int32_t* cu, int batch, int64_t tokens, int lane, uint32_t* status) {
+  bool bad = false;
+  for (int b = lane; b < batch; b += 32) {
+    const int lo = cu[b], hi = cu[b + 1];
+    bad = bad || hi < lo || hi > tokens || (b == 0 && lo != 0);
+  }
+  if (bad && status != nullptr) atomicOr(status, ABFT_PAGED_BAD_ROWS);
+}
+
 // One thread owns chunk c of a row's pairs: elements [8c, 8c + 8) and their
 // partners [D/2 + 8c, D/2 + 8c + 8). D / 16 threads cover a row, a warp 512 / D
 // rows of one token. `warps` warps share a token's rows (q's heads, then k's,
@@ -88,14 +99,21 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
   const int64_t w = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
   const int64_t t = w >> p.warps_shift;
   const int sub = static_cast<int>(w) & ((1 << p.warps_shift) - 1);
-  if (t >= p.tokens) return;
   const PagedView& kv = p.kv;
+  if (t >= p.tokens) {
+    // With boundaries the last block has no row: its first warp checks them.
+    if (p.cu != nullptr && blockIdx.x == gridDim.x - 1 && threadIdx.x < 32)
+      check_boundaries(p.cu, kv.batch, p.tokens, lane, kv.status);
+    return;
+  }
   int b, pos, place = 0, n = 1;
   if (p.cu != nullptr) {
     b = owner_of(p.cu, kv.batch, t, lane);
     if (b >= kv.batch) return;  // behind the last sequence
-    const int begin = p.cu[b];
-    n = p.cu[b + 1] - begin;
+    int begin, end;
+    packed_range(p.cu, b, static_cast<int>(p.tokens), &begin, &end);
+    if (t < begin || t >= end) return;  // bad boundaries: the row is no sequence's, or two claim it
+    n = end - begin;
     place = static_cast<int>(t) - begin;
   } else {
     b = static_cast<int>(t);

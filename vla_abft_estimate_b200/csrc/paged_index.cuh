@@ -38,6 +38,15 @@ __host__ __device__ __forceinline__ int64_t paged_offset(int page, int64_t page_
          ((((static_cast<int64_t>(head)) << page_shift) + slot) << hd_shift);
 }
 
+// A sequence's packed rows [begin, end), within [0, tokens] whatever cu holds:
+// none when its boundaries fall or lie outside.
+__host__ __device__ __forceinline__ void packed_range(const int32_t* cu, int b, int tokens, int* begin, int* end) {
+  const int lo = cu[b], hi = cu[b + 1];
+  const bool ok = lo >= 0 && lo <= hi && hi <= tokens;
+  *begin = ok ? lo : 0;
+  *end = ok ? hi : 0;
+}
+
 // Tiles [begin, end) of piece `split` when `tiles` tiles are cut into at
 // most `splits` pieces of equal size (the last one shorter, later ones empty).
 __host__ __device__ __forceinline__ void split_tiles(int tiles, int splits, int split, int* begin, int* end) {

@@ -102,13 +102,6 @@ struct PrefillParams {
   float2* part_ml;         // [tokens * heads][splits]
 };
 
-// A sequence's share of the packed rows, safe for any cu: begin <= end <= tokens.
-__host__ __device__ __forceinline__ void packed_range(const int32_t* cu, int b, int tokens, int* begin, int* end) {
-  const int lo = cu[b], hi = cu[b + 1];
-  *begin = lo < 0 ? 0 : (lo > tokens ? tokens : lo);
-  *end = hi < *begin ? *begin : (hi > tokens ? tokens : hi);
-}
-
 // row / group for a row of a tile: exact for rows below 128 and groups up to 64
 // (the product overshoots the quotient by less than 128 / 2^16 < 1 / 64).
 __host__ __device__ __forceinline__ int row_token(int row, uint32_t group_inv) {
@@ -1029,6 +1022,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         fence_proxy_async_smem();  // read before the next answer is written there
         __syncwarp();
       }
+      if (blockIdx.x == 0) check_boundaries(p.cu, kv.batch, p.tokens, lane, kv.status);
     }
   }
   __syncthreads();

@@ -317,8 +317,8 @@ class PagedKVCache:
 
     def check_status(self) -> None:
         """Raises ValueError when a call since the last check met a bad page
-        entry, length or position on the device (which it skipped), and
-        clears the record. Synchronises with the current stream: work queued on
+        entry, length, position or boundary on the device (which it skipped),
+        and clears the record. Synchronises with the current stream: work queued on
         others is waited for by the caller."""
         bits = int(self.status.cpu()[0])
         if not bits:
@@ -327,5 +327,6 @@ class PagedKVCache:
         said = [text for bit, text in ((N.PAGED_BAD_PAGE, "a page_table entry outside the pool"),
                                        (N.PAGED_BAD_LEN, "a length below 0, beyond the table or below the new tokens"),
                                        (N.PAGED_BAD_ANGLE, "a position beyond the rotation table"),
+                                       (N.PAGED_BAD_ROWS, "cu_seqlens that does not start at 0, falls or passes the rows"),
                                        (N.PAGED_TIMEOUT, "a bounded device wait gave up")) if bits & bit]
         raise ValueError("paged cache: " + "; ".join(said))
