@@ -21,7 +21,10 @@
 //
 // P is rounded to 16 bits for the product, as hi + lo (two products), so
 // that the output's own rounding stays the only one that counts: the second
-// product hides behind the loads.
+// product hides behind the loads. fp16 ends at 2^-24, and the many keys of a
+// long cache may weigh less than that each and still count together: there the
+// weights are lifted by 2^15 (the greatest becomes 2^15, within the format), and
+// the quotient takes it out again.
 //
 // Work is one list of 32-key tiles over all (sequence, kv head) segments, cut
 // into equal shares for the warps of one CTA per SM: lengths of any mix keep
@@ -141,6 +144,9 @@ constexpr int kDecTile = 32;
 // 1, 18.3 with 2, 21.6 with 0). Equal ones divide best without (256 of 2,048
 // slots: 44.2 us against 47.9 with 1).
 constexpr int kDecCost = 1;
+// What the weights are lifted by (a power of 2): fp16's greatest is below 2^16.
+template <bool F16>
+constexpr float kDecLift = F16 ? 15.f : 0.f;
 
 template <int D, int NT>
 struct DecodeCfg {
@@ -499,6 +505,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
           const float mn = fmaxf(m[nt][e], top);
           const float ms = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: weights 0, not NaN
+          const float base = ms - kDecLift<F16>;
           scale[nt][e] = exp2_approx(m[nt][e] - ms);
           m[nt][e] = mn;
           float sum_p = 0.f;
@@ -507,7 +514,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) paged_decode_kernel(const D
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               float& x = s[mt][nt][half * 2 + e];
-              x = exp2_approx(x - ms);
+              x = exp2_approx(x - base);
               sum_p += x;
             }
           l[nt][e] = l[nt][e] * scale[nt][e] + sum_p;

@@ -20,9 +20,12 @@
 //   O += P V    tcgen05.mma with P from TMEM, V as N-major operand
 // The two tiles alternate: while the tensor core works on one, the other's
 // rows are exponentiated. O stays in TMEM; it is rescaled only when a row's
-// maximum has risen by more than 2^8 since the last rescaling (P and the sum
-// l then still fit their formats, and the quotient is unchanged), which after
-// the first tiles of a row hardly happens.
+// maximum has risen by more than 2^8 (fp16: 2^5) since the last rescaling, which
+// after the first tiles of a row hardly happens: P and the sum l then still fit
+// their formats. fp16 ends at 2^-24, and the many keys of a long cache may weigh
+// less than that each and still count together: there P is lifted by 2^10 (2^15
+// at most, within the format), so that weights down to 2^-24 of the greatest keep
+// all their bits, smaller ones steps of 2^-34; the quotient takes it out again.
 //
 // A call with few rows takes one tile an item, and both groups of row warps
 // work on it, on every other step each ("shared" below), with an O of their
@@ -57,6 +60,14 @@ constexpr int kPreThreads = 384;
 // 256 * 200 + 128 * 104 = 64,512. (The issuer's loop in local memory for want
 // of registers doubles the kernel's time.)
 constexpr int kPreRegsRows = 200, kPreRegsOther = 104;
+// How far (powers of 2) a row's maximum may have risen above the one that P
+// refers to, and what P is lifted by: lag + lift stay below fp16's 2^16. (fp16,
+// 8,192 tokens, 28 heads of 128 / 32 of 64, chunks on a prefix: lag 8 417 / 392 /
+// 88.4 us, 5 414 / 403 / 88.4, 3 430 / 408 / 90.9, 2 456 / 418 / 92.4.)
+template <bool F16>
+constexpr float kPreLag = F16 ? 5.f : 8.f;
+template <bool F16>
+constexpr float kPreLift = F16 ? 10.f : 0.f;
 
 template <int D>
 struct PrefillCfg {
@@ -582,7 +593,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);  // NaN if a score is
         // Also true from m = -inf and for NaN, but not while all is -inf.
-        const bool raise = !((mn - m) * p.scale_log2 <= 8.f) && mn != -INFINITY;
+        const bool raise = !((mn - m) * p.scale_log2 <= kPreLag<F16>) && mn != -INFINITY;
         if (kAhead && j > begin) {  // the last product has read P and written O
           ok = mbar_wait(&ofull[t], (count - 1) & 1, abort_flag) && ok;
           tc_fence_after();
@@ -607,7 +618,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             tmem_st_wait();
           }
         }
-        const float shift = m == -INFINITY ? 0.f : -m * p.scale_log2;
+        const float shift = m == -INFINITY ? 0.f : fmaf(-m, p.scale_log2, kPreLift<F16>);
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
