@@ -54,3 +54,28 @@ def test_small_weights_are_kept(cuda_device, n, at, gap, d, dtype):
     want, tol = attention(pool, q[rows], [(0, n - 298), (0, n - 198), (0, n), (1, 70)], 1.0)
     close(got[rows], want, tol)
     cache.check_status()
+
+
+@pytest.mark.parametrize("dtype,lag", [(BF16, 8), (F16, 5)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_greatest_weight_above_a_lagging_maximum(cuda_device, d, dtype, lag):
+    """One key has nearly all the weight, 128 slots behind the one the row's
+    maximum still refers to, by less than the maximum may lag: its weight is then
+    rounded like any other, where an exact maximum makes it 1. Two half steps in
+    all: the weight's and the output's."""
+    dev = cuda_device
+    rows = 64
+    pool = Pool([400], 1, 64, d, dtype)
+    held = pool.table[0].long()
+    key = torch.full((7 * 64, d), -16.0)  # the others: far below
+    key[10], key[200] = 0.0, 1.0 / 16
+    key[400:] = float("nan")
+    pool.k[held] = key.view(7, 1, 64, d).to(dtype)
+    cache = pool.device_cache(dev, PagedKVCache)
+    # rows' scores of key 200 rise from 0 to `lag` powers of 2 above key 10's
+    rise = torch.linspace(0.05, 0.95 * lag, rows) * 0.6931
+    q = (rise * 16 / d)[:, None, None].expand(rows, 3, d).to(dtype).contiguous()
+    want, tol = attention(pool, q, [(0, 337 + i) for i in range(rows)], 1.0)
+    cu = torch.tensor([0, rows], dtype=torch.int32, device=dev)
+    for splits in (0, 1):
+        close(cache.prefill(q.to(dev), cu, scale=1.0, num_splits=splits), want, tol)
