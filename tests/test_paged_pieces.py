@@ -1,13 +1,15 @@
 """Paged prefill's list of work on the host: the rows of a sequence lie within
 the call's whatever the boundaries say, and the pieces chosen for a batch fit
 the grid and the scratch, whatever its lengths."""
+import ctypes
 import subprocess
 
 import pytest
 
 from vla_abft_estimate_b200 import _build
+from vla_abft_estimate_b200 import _native as N
 
-from .test_paged_host import _have_nvcc
+from .test_paged_host import _have_nvcc, _kv
 
 PROGRAM = r"""
 #include <cstdio>
@@ -79,3 +81,19 @@ def test_chosen_pieces_fit_the_grid(tmp_path):
     assert out.returncode == 0, out.stdout
     cut, tight = (int(x) for x in out.stdout.split())
     assert cut > 10_000 and tight > 100  # batches that are cut, and lists that reach the bound
+
+
+def test_decode_list_is_counted_in_32_bits():
+    """2^31 places in the list of tiles are refused, the batch below is not (the
+    table, 2^30 - 16 slots, is the widest that any call takes)."""
+    L = N.lib()
+
+    def scratch(batch):
+        a = N.PagedAttnArgs()
+        a.kv, a.q, a.out, a.tokens, a.heads, a.scale, a.num_sms = _kv(), 0x50000, 0x60000, batch, 28, 0.1, 148
+        a.kv.max_pages = a.kv.table_stride = (1 << 26) - 1
+        a.kv.batch = batch
+        return L.abft_paged_decode_workspace_bytes(ctypes.byref(a))  # 0 for a call that is refused
+
+    assert scratch(16) == 0  # 64 segments of 2^25 tiles
+    assert scratch(15) > 0
