@@ -9,6 +9,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
@@ -16,6 +17,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <math.h>
 #include <string.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -35,11 +37,27 @@ struct Calls {
   AppendFn append;
   AttnFn attend[2];    // decode, prefill
   BytesFn scratch[2];
+  PyObject* pages[2];  // the tensors behind kv, or NULL
 };
 
 const at::Tensor* tensor_of(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 at::ScalarType type_of(const Calls* c) { return c->kv.dtype == ABFT_DTYPE_F16 ? at::kHalf : at::kBFloat16; }
+
+bool differentiated(const at::Tensor* t) { return t->requires_grad() && c10::GradMode::is_enabled(); }
+
+// The cache is known and asks for no gradient; nothing is traced, and no level
+// of forward mode is open, in which any tensor may be a dual.
+bool ready(const Calls* c) {
+  return c->append != nullptr && c10::cuda::current_device() == c->device && c->pages[0] != nullptr &&
+         !at::tracer::impl::is_dispatch_enabled() && torch::autograd::ForwardADLevel::try_get_by_idx(0) == nullptr &&
+         !differentiated(&THPVariable_Unpack(c->pages[0])) && !differentiated(&THPVariable_Unpack(c->pages[1]));
+}
+
+// Autograd learns that the tensor has been written.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // [tokens, heads, head_dim] rows the kernels can read or write in place.
 bool rows(const Calls* c, const at::Tensor* t, int64_t tokens, int64_t heads) {
@@ -49,8 +67,7 @@ bool rows(const Calls* c, const at::Tensor* t, int64_t tokens, int64_t heads) {
   const auto stride = t->strides();
   return size[2] == c->kv.head_dim && (tokens < 0 || size[0] == tokens) && (heads < 0 || size[1] == heads) &&
          stride[2] == 1 && stride[0] % 8 == 0 && stride[1] % 8 == 0 &&
-         (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15u) == 0 &&
-         !(t->requires_grad() && c10::GradMode::is_enabled());
+         (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15u) == 0 && !differentiated(t);
 }
 
 bool repeats(const at::Tensor* t) {
@@ -76,7 +93,7 @@ at::Tensor fresh(const Calls* c, at::IntArrayRef size, at::ScalarType type) {
 // rotated q; None when the call needs the long way; a status code.
 PyObject* calls_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   const Calls* c = reinterpret_cast<const Calls*>(self);
-  if (n != 6 || c->append == nullptr || c10::cuda::current_device() != c->device) Py_RETURN_NONE;
+  if (n != 6 || !ready(c)) Py_RETURN_NONE;
   const at::Tensor *q = tensor_of(a[0]), *k = tensor_of(a[1]), *v = tensor_of(a[2]);
   const at::Tensor *rope = tensor_of(a[3]), *cu = tensor_of(a[4]), *out = tensor_of(a[5]);
   if (!rows(c, k, -1, c->kv.kv_heads)) Py_RETURN_NONE;
@@ -87,7 +104,7 @@ PyObject* calls_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   if (a[3] != Py_None) {
     if (rope == nullptr || !rope->is_cuda() || rope->get_device() != c->device || rope->scalar_type() != at::kFloat ||
         rope->dim() != 3 || rope->size(0) == 0 || rope->size(1) * 2 != c->kv.head_dim || rope->size(2) != 2 ||
-        !rope->is_contiguous() || (reinterpret_cast<uintptr_t>(rope->const_data_ptr()) & 15u) != 0)
+        !rope->is_contiguous() || differentiated(rope) || (reinterpret_cast<uintptr_t>(rope->const_data_ptr()) & 15u) != 0)
       Py_RETURN_NONE;
     args.rope = static_cast<const float*>(rope->const_data_ptr());
     args.max_positions = rope->size(0);
@@ -118,7 +135,10 @@ PyObject* calls_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   int rc;
   Py_BEGIN_ALLOW_THREADS rc = c->append(&args, stream);
   Py_END_ALLOW_THREADS if (rc != ABFT_OK) return PyLong_FromLong(rc);
+  written(THPVariable_Unpack(c->pages[0]));
+  written(THPVariable_Unpack(c->pages[1]));
   if (a[5] != Py_None) {
+    written(*out);
     Py_INCREF(a[5]);
     return a[5];
   }
@@ -129,7 +149,7 @@ PyObject* calls_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 // num_splits, num_sms): the output; None; a status code.
 PyObject* calls_attend(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   const Calls* c = reinterpret_cast<const Calls*>(self);
-  if (n != 7 || c->append == nullptr || c10::cuda::current_device() != c->device) Py_RETURN_NONE;
+  if (n != 7 || !ready(c)) Py_RETURN_NONE;
   const int which = a[0] == Py_True ? 1 : 0;
   const at::Tensor *q = tensor_of(a[1]), *cu = tensor_of(a[2]), *out = tensor_of(a[4]);
   if (!rows(c, q, which == 0 ? c->kv.batch : -1, -1) || !group(c, q->size(1))) Py_RETURN_NONE;
@@ -180,6 +200,7 @@ PyObject* calls_attend(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   Py_BEGIN_ALLOW_THREADS rc = c->attend[which](&args, stream);
   Py_END_ALLOW_THREADS if (rc != ABFT_OK) return PyLong_FromLong(rc);
   if (a[4] != Py_None) {
+    written(*out);
     Py_INCREF(a[4]);
     return a[4];
   }
@@ -201,6 +222,27 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
   return nullptr;
+}
+
+// hold(k_pages, v_pages): the tensors whose addresses the cache struct has.
+PyObject* calls_hold(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  Calls* c = reinterpret_cast<Calls*>(self);
+  if (n != 2 || !THPVariable_Check(a[0]) || !THPVariable_Check(a[1])) {
+    PyErr_SetString(PyExc_TypeError, "hold takes the two page tensors");
+    return nullptr;
+  }
+  for (int i = 0; i < 2; ++i) {
+    Py_INCREF(a[i]);
+    Py_XSETREF(c->pages[i], a[i]);
+  }
+  Py_RETURN_NONE;
+}
+
+void calls_dealloc(PyObject* self) {
+  Calls* c = reinterpret_cast<Calls*>(self);
+  Py_CLEAR(c->pages[0]);
+  Py_CLEAR(c->pages[1]);
+  Py_TYPE(self)->tp_free(self);
 }
 
 // Calls(kv bytes, device, addresses of append, decode, its scratch size,
@@ -227,6 +269,7 @@ int calls_init(PyObject* self, PyObject* args, PyObject*) {
 PyMethodDef methods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<calls_append>)), METH_FASTCALL, nullptr},
     {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<calls_attend>)), METH_FASTCALL, nullptr},
+    {"hold", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<calls_hold>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyTypeObject calls_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
@@ -241,6 +284,7 @@ PyMODINIT_FUNC PyInit__paged_host(void) {
   calls_type.tp_flags = Py_TPFLAGS_DEFAULT;
   calls_type.tp_new = PyType_GenericNew;
   calls_type.tp_init = calls_init;
+  calls_type.tp_dealloc = calls_dealloc;
   calls_type.tp_methods = methods;
   if (PyType_Ready(&calls_type) < 0) return nullptr;
   PyObject* m = PyModule_Create(&module_def);

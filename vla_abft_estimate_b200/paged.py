@@ -18,7 +18,9 @@ kernels, so a captured step (``torch.cuda.graph``) replays with the lengths
 and pages of the moment. Bad entries never lead outside the tensors; they set
 bits that ``check_status`` turns into an error. Calls are queued on the
 current stream of the cache's device; results and workspaces are allocated
-there, per call.
+there, per call. No derivatives: tensors that require a gradient (under grad
+mode) or have a tangent are refused, and so are calls under a tracer; what a
+call writes counts as modified in place.
 """
 from __future__ import annotations
 
@@ -147,6 +149,7 @@ class PagedKVCache:
                  for name in ("abft_kv_append", "abft_paged_decode", "abft_paged_decode_workspace_bytes",
                               "abft_paged_prefill", "abft_paged_prefill_workspace_bytes")]
         self._fast = _host().Calls(bytes(kv), dev.index, *entry)
+        self._fast.hold(k_pages, v_pages)
 
     # The kernels hold the addresses: the tensors are written in place, not
     # replaced.
@@ -171,12 +174,31 @@ class PagedKVCache:
             raise ValueError(f"{name} must be a {self.dtype} tensor [{'tokens' if tokens is None else tokens}, "
                              f"{'heads' if heads is None else heads}, {self.head_dim}] on {self.device}, got {t.dtype} "
                              f"{tuple(shape)} on {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires a gradient, which the paged cache operators do not give: call them under "
-                             "torch.no_grad()")
+        self._no_derivative(name, t)
         if not self._in_place(t):
             return t.clone(memory_format=torch.contiguous_format)
         return t
+
+    @staticmethod
+    def _no_derivative(name: str, t: torch.Tensor) -> None:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient, which the paged cache operators do not give: call them under "
+                             "torch.no_grad()")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has a tangent, which the paged cache operators do not carry on")
+
+    def _callable(self) -> None:
+        if torch._C._get_tracing_state() is not None:
+            raise ValueError("the paged cache operators cannot be traced: a trace would hold their results as constants")
+        self._no_derivative("k_pages", self.k_pages)
+        self._no_derivative("v_pages", self.v_pages)
+
+    @staticmethod
+    def _written(*tensors: Optional[torch.Tensor]) -> None:
+        """Autograd learns that the tensors have been written."""
+        for t in tensors:
+            if t is not None and not t.is_inference():
+                torch.autograd.graph.increment_version(t)
 
     @staticmethod
     def _in_place(t: torch.Tensor) -> bool:
@@ -230,6 +252,7 @@ class PagedKVCache:
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
                 return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
+        self._callable()
         args = N.KvAppendArgs()
         args.kv = self._kv
         k = self._rows("k", k, None, self.kv_heads)
@@ -246,6 +269,7 @@ class PagedKVCache:
                     or not rope.is_contiguous() or rope.shape[0] == 0 or rope.data_ptr() % 16):
                 raise ValueError(f"rope must be a contiguous, 16-byte aligned float32 [positions, {self.head_dim // 2}, 2] "
                                  f"tensor on {self.device}")
+            self._no_derivative("rope", rope)
             args.rope, args.max_positions = rope.data_ptr(), rope.shape[0]
         if q is not None:
             self._group(q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0)
@@ -260,6 +284,7 @@ class PagedKVCache:
         args.k_token_stride, args.k_head_stride, _ = k.stride()
         args.v_token_stride, args.v_head_stride, _ = v.stride()
         self._call("abft_kv_append", args)
+        self._written(self.k_pages, self.v_pages, q_out)
         return q_out
 
     def decode(self, q: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
@@ -291,6 +316,7 @@ class PagedKVCache:
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
                 return self._attention(prefill, q, cu, scale, out, num_splits, num_sms)
+        self._callable()
         args = N.PagedAttnArgs()
         args.kv = self._kv
         if prefill:
@@ -313,6 +339,7 @@ class PagedKVCache:
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)  # of this call alone
             args.workspace, args.workspace_bytes = ws.data_ptr(), need
         self._call(name, args)
+        self._written(out)
         return out
 
     def check_status(self) -> None:
