@@ -1,5 +1,10 @@
-"""Build libabft_b200.so in-tree with nvcc for sm_100a, and _paged_host.so,
-the extension that takes Python calls of the paged cache to it.
+"""Build libabft_b200.so in-tree with nvcc for sm_100a, and _paged_host, the
+extension that takes Python calls of the paged cache to it.
+
+The library needs nvcc alone. The extension needs g++ and the headers of the
+installed torch, and serves that torch and Python only (its file is named after
+them); where it cannot be built the library is built all the same, and the
+paged cache takes its longer way through ctypes.
 
 Both land in ``vla_abft_estimate_b200/_lib/`` next to the
 package so that they travel with the source tree; nothing is installed into
@@ -10,15 +15,18 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
+from typing import Optional
 
 PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
 CSRC_DIR = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libabft_b200.so"
-HOST_PATH = LIB_DIR / "_paged_host.so"
 HOST_SOURCE = CSRC_DIR / "paged_host.cpp"
 INCLUDE_DIR = REPO_DIR / "include"
 
@@ -58,8 +66,21 @@ def _newer(out: Path, inputs: list[Path]) -> bool:
     return all(p.stat().st_mtime <= t for p in inputs)
 
 
+def _torch_version() -> Optional[str]:
+    """Of the installed torch, without importing it; None when there is none."""
+    try:
+        return metadata.version("torch")
+    except metadata.PackageNotFoundError:
+        return None
+
+
+def host_path() -> Path:
+    """The extension's file for this torch and Python."""
+    return LIB_DIR / f"_paged_host.torch-{_torch_version()}.{sysconfig.get_config_var('SOABI')}.so"
+
+
 def _host_stale() -> bool:
-    return not _newer(HOST_PATH, [HOST_SOURCE, INCLUDE_DIR / "abft_b200.h"])
+    return _torch_version() is not None and not _newer(host_path(), [HOST_SOURCE, INCLUDE_DIR / "abft_b200.h"])
 
 
 def is_stale() -> bool:
@@ -69,8 +90,6 @@ def is_stale() -> bool:
 def _host_cmd(out: Path) -> list[str]:
     """g++ on the extension, against the headers and libraries of the torch
     that is installed (it reads torch tensors without Python's attributes)."""
-    import sysconfig
-
     import torch
 
     root = Path(torch.__file__).resolve().parent
@@ -92,7 +111,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the library if it is missing or older than its sources (the
-    sources that changed, side by side, then one link)."""
+    sources that changed, side by side, then one link), and the extension of the
+    paged cache; a failure of that one is a warning."""
     if not force and not is_stale():
         return LIB_PATH
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
@@ -106,20 +126,33 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         for _, _, cmd in jobs:
             cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd))
-    if force or _host_stale():
-        tmp = HOST_PATH.with_suffix(".so.tmp")
-        jobs.append((tmp, HOST_PATH, _host_cmd(tmp)))
-    with ThreadPoolExecutor(max(1, len(jobs))) as pool:
+    with ThreadPoolExecutor(len(jobs) + 1) as pool:
+        host = pool.submit(_build_host, verbose) if force or _host_stale() else None
         list(pool.map(lambda j: _run(j[2], verbose), jobs))
-    for tmp, obj, _ in jobs:
-        os.replace(tmp, obj)
+        for tmp, obj, _ in jobs:
+            os.replace(tmp, obj)
+        _link(force, verbose)
+        try:
+            if host is not None:
+                host.result()
+        except Exception as e:  # no torch, no g++, other headers: the library is complete without it
+            warnings.warn(f"the host extension of the paged cache was not built, its calls take the longer way: {e}")
+    return LIB_PATH
+
+
+def _build_host(verbose: bool) -> None:
+    tmp = host_path().with_suffix(".so.tmp")
+    _run(_host_cmd(tmp), verbose)
+    os.replace(tmp, host_path())
+
+
+def _link(force: bool, verbose: bool) -> None:
     if not force and all(_newer(LIB_PATH, _inputs(s)) for s in SOURCES):
-        return LIB_PATH
+        return
     tmp = LIB_PATH.with_suffix(".so.tmp")
     _run([_nvcc(), *NVCC_FLAGS[:2], "-shared", *[str(OBJ_DIR / (Path(s).stem + ".o")) for s in SOURCES],
           "-o", str(tmp)], verbose)
     os.replace(tmp, LIB_PATH)
-    return LIB_PATH
 
 
 if __name__ == "__main__":
