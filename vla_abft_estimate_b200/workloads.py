@@ -64,7 +64,8 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
     over ``model.new_paged_caches(...)``: rotation, cache writes and attention
     by the library's paged operators (head_dim 64 or 128, CUDA). ids are the
     packed new tokens; cu_seqlens bounds each sequence's (prompts and chunks
-    of any length), or is None for one token per sequence.
+    of any length; rows behind the last sequence attend to nothing), or is
+    None for one token per sequence.
     ``caches.lens`` counts the new tokens already: advance it first.
     ``dtype``: bfloat16 (default) or float16, the reference driver's
     ``--dtype`` (qwen_abft_benchmark.py:26)."""
@@ -126,7 +127,8 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
             t = x.shape[0]
             q, k, v = self.qkv(self.ln1(x)).split([nh * hd, nkv * hd, nkv * hd], dim=-1)
             q = cache.append(q.view(t, nh, hd), k.view(t, nkv, hd), v.view(t, nkv, hd), rope, cu_seqlens=cu_seqlens)
-            a = cache.decode(q) if cu_seqlens is None else cache.prefill(q, cu_seqlens)
+            # Rows of no sequence go on through the checked linears: zeros, not what memory held.
+            a = cache.decode(q) if cu_seqlens is None else cache.prefill(q, cu_seqlens, out=torch.zeros_like(q))
             x = x + self.o(a.view(t, nh * hd))
             g, u = self.gate_up(self.ln2(x)).chunk(2, dim=-1)
             return x + self.down(F.silu(g) * u)
