@@ -980,12 +980,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       int index = blockIdx.x, published = 0, asked = 0;
       bool ok = true;
       const WorkScan scan = scan_work(p, lane);
+      // Every CTA writes the same: the join reads it even if the CTA that took an
+      // item gave up.
+      if (p.chosen != nullptr && lane == 0) *p.chosen = scan.piece;
       while (ok) {
         PrefillItem x;
         x.valid = 0;
         bool publish = index < 0;
         if (index >= 0) {
-          if (index == 0 && p.chosen != nullptr && lane == 0) *p.chosen = scan.piece;
           x.hk = index % kv.kv_heads;
           int seq = 0, block = 0, raw_len = 0;
           if (find_work(p, scan, index / kv.kv_heads, lane, &seq, &block, &x.split, &x.row0, &x.n, &raw_len)) {
