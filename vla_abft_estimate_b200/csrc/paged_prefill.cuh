@@ -978,7 +978,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     } else if (warp == 10) {
       // ---------------------------------------------------------- work
       int index = blockIdx.x, published = 0, asked = 0;
-      bool ok = true;
+      bool ok = true, first = false;
       const WorkScan scan = scan_work(p, lane);
       // Every CTA writes the same: the join reads it even if the CTA that took an
       // item gave up.
@@ -988,6 +988,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         x.valid = 0;
         bool publish = index < 0;
         if (index >= 0) {
+          first = first || index == 0;
           x.hk = index % kv.kv_heads;
           int seq = 0, block = 0, raw_len = 0;
           if (find_work(p, scan, index / kv.kv_heads, lane, &seq, &block, &x.split, &x.row0, &x.n, &raw_len)) {
@@ -1043,7 +1044,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         fence_proxy_async_smem();  // read before the next answer is written there
         __syncwarp();
       }
-      if (blockIdx.x == 0) check_boundaries(p.cu, kv.batch, p.tokens, lane, kv.status);
+      // By the CTA that had item 0, its own or taken over.
+      if (first) check_boundaries(p.cu, kv.batch, p.tokens, lane, kv.status);
     }
   }
   __syncthreads();
