@@ -198,7 +198,9 @@ int attn_check(const abft_paged_attn_args* a, bool decode) {
 // 8.3, 1,000 slots - / 8.0 / 9.6; 64 segments, clusters of 2: 370 slots 7.7 / 8.0 /
 // -, 500 slots - / 8.2 / 9.7; 128 segments of 512 / 1,280 slots: 9.2 / 17.3 us
 // against the list's 11.7 / 21.8. Longer ones are shared out all the same, since
-// lengths may differ by more than that. Clusters have to fit the device's groups
+// lengths may differ by more than that. (The lengths are on the device: what is
+// known here, and decides, is the width of the table, which is measured where the
+// caches fill it. 500 slots in a table of 32,768 go by the list.) Clusters have to fit the device's groups
 // of SMs: 15 of 8 and 33 of 4 run at once, a second wave costs 4 us.
 int decode_by_segment(const abft_paged_attn_args* a, int sms) {
   const int64_t segments = decode_segments(a), slots = static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size;

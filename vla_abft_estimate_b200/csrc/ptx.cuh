@@ -57,8 +57,10 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Wall-clock bound on any single wait. A healthy wait in this library lasts
-// at most one output tile's main loop (well under a millisecond).
+// Wall-clock bound on any single wait. A healthy wait lasts at most one output
+// tile's main loop (GEMM: well under a millisecond) or one work item (paged
+// prefill: some 1.2 us for each 128 keys of its piece, so that the bound is
+// met by an uncut piece of some 2 * 10^8 slots).
 constexpr uint64_t kWaitTimeoutNs = 2000000000ull;
 
 // Bounded wait for the phase of `bar` with parity `parity` to complete.
