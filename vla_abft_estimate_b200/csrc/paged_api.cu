@@ -443,7 +443,7 @@ int abft_paged_decode(const abft_paged_attn_args* a, void* stream) {
   for (p.cluster_shift = 0; 1 << (p.cluster_shift + 1) <= p.by_segment;) ++p.cluster_shift;
   const size_t need = decode_bytes(a, sms);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
-  if (off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
+  if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
   const size_t rows = static_cast<size_t>(grid) * 2 * 8 * nt;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * a->kv.head_dim);
