@@ -437,6 +437,8 @@ int abft_check_only_noalloc(const abft_check_args* args, void* stream);
 #define ABFT_PAGED_BAD_ANGLE 4u
 #define ABFT_PAGED_TIMEOUT   8u
 #define ABFT_PAGED_BAD_ROWS  16u
+#define ABFT_PAGED_BAD_DRAFT 32u  /* a tree's parents, or rows to keep: see abft_paged_tree, abft_kv_keep */
+#define ABFT_PAGED_BAD_FORK  64u  /* see abft_kv_fork                                                     */
 
 /* A page pool and the sequences in it. */
 typedef struct abft_paged_kv {
@@ -513,6 +515,109 @@ int abft_paged_decode(const abft_paged_attn_args* args, void* stream);
  * not see it (its weight there is 0, and 0 * inf is not). */
 size_t abft_paged_prefill_workspace_bytes(const abft_paged_attn_args* args);
 int abft_paged_prefill(const abft_paged_attn_args* args, void* stream);
+
+/* ---- Drafted trees and forks over the paged cache --------------------------
+ *
+ * A step that looks at several continuations of each sequence at once: the n
+ * new tokens of a sequence form a tree (or several), given by parents[row], the
+ * parent's place among the sequence's new rows or -1; parents come before
+ * their children. They are appended behind the cache in row order, attended to
+ * as trees, and those that the model confirms are kept. No counterpart in the
+ * reference. */
+
+/* Append by positions of the caller's: slots go by the lengths as in
+ * abft_kv_append, the rotation by positions[axis][token], pair j by the axis
+ * whose section holds it: sections[0] pairs by axis 0, the next sections[1] by
+ * axis 1, and so on. Several axes serve image and video tokens (time, height,
+ * width), one a drafted token's depth. A position outside [0, max_positions)
+ * on any axis sets ABFT_PAGED_BAD_ANGLE and the token is skipped. */
+#define ABFT_MOST_AXES 4
+typedef struct abft_kv_append_at_args {
+  abft_kv_append_args append;  /* rope not NULL                                          */
+  const int32_t* positions;    /* [axes, position_stride], `tokens` of a row used; rows   */
+  int64_t position_stride;     /* may overlap (0: one row for all axes)                   */
+  int32_t axes;                /* 1 to ABFT_MOST_AXES                                    */
+  int32_t sections[ABFT_MOST_AXES];  /* pairs of each axis, head_dim / 2 in all          */
+  int32_t reserved;
+} abft_kv_append_at_args;
+int abft_kv_append_at(const abft_kv_append_at_args* args, void* stream);
+
+/* Tree attention: query row i of the n new tokens of sequence b sees the slots
+ * before the new ones (j < seq_lens[b] - n), its own and its ancestors'.
+ * Everything else is as for abft_paged_prefill. A parent that is below -1 or
+ * does not come before its child sets ABFT_PAGED_BAD_DRAFT; the way up ends
+ * there. */
+typedef struct abft_paged_tree_args {
+  abft_paged_attn_args attn;
+  const int32_t* parents;      /* [tokens]                                               */
+} abft_paged_tree_args;
+size_t abft_paged_tree_workspace_bytes(const abft_paged_tree_args* args);
+int abft_paged_tree(const abft_paged_tree_args* args, void* stream);
+
+/* Accept: of each sequence's tree the path to keep. Row i, with token ids[i], is
+ * confirmed when it has no parent, or its parent is confirmed and answers[parent]
+ * == ids[i] (answers: the token that the model gives behind each row). The path
+ * ends at the deepest confirmed row, the lowest of equals. kept[cu[b] + k]: its
+ * rows from the top, then -1; rows behind cu[batch] -1; counts[b]: their
+ * number; next[b]: the last one's answer, or -1 where there is none. A bad parent
+ * (as above) sets ABFT_PAGED_BAD_DRAFT and confirms nothing. */
+typedef struct abft_draft_accept_args {
+  const int32_t* cu_seqlens;   /* [batch + 1]                                            */
+  const int32_t* parents;      /* [tokens]                                               */
+  const void* ids;             /* [tokens], of id_bytes each                             */
+  const void* answers;         /* [tokens]                                               */
+  int32_t* kept;               /* [tokens]                                               */
+  int32_t* counts;             /* [batch]                                                */
+  void* next;                  /* [batch]                                                */
+  uint32_t* status;            /* ABFT_PAGED_* bits, or NULL                             */
+  int64_t tokens;
+  int32_t batch;               /* at most 65535                                          */
+  int32_t id_bytes;            /* 4 or 8                                                 */
+} abft_draft_accept_args;
+int abft_draft_accept(const abft_draft_accept_args* args, void* stream);
+
+/* Keep: of the n new tokens of sequence b the rows kept[cu[b] + i], i <
+ * counts[b], rising, move to the slots of rows 0, 1, ... in every layer, and
+ * lens_out[b] = seq_lens[b] - n + counts[b] (lens_out may be kv.seq_lens itself).
+ * The layers share kv's geometry, strides, table and lengths; their pools are
+ * pools[2 * layer] (keys) and pools[2 * layer + 1] (values), device memory of
+ * 16-byte aligned addresses, or, with pools NULL and one layer, kv's. A sequence
+ * with bad boundaries, count or rows (ABFT_PAGED_BAD_ROWS, ABFT_PAGED_BAD_DRAFT), a
+ * length below n or beyond the table, or a bad page under one of those slots is
+ * left as it was, its length too. */
+typedef struct abft_kv_keep_args {
+  abft_paged_kv kv;
+  const void* const* pools;
+  const int32_t* cu_seqlens;   /* [batch + 1]                                            */
+  const int32_t* kept;         /* [tokens]                                               */
+  const int32_t* counts;       /* [batch]                                                */
+  int32_t* lens_out;           /* [batch]                                                */
+  int64_t tokens;
+  int32_t layers;              /* 1 to 4096                                              */
+  int32_t reserved;
+} abft_kv_keep_args;
+int abft_kv_keep(const abft_kv_keep_args* args, void* stream);
+
+/* Fork: for each pair i sequence dst[i] gets the cache of sequence src[i]: its
+ * row of kv.page_table the source's full pages, kv.seq_lens[dst[i]] the source's
+ * length (both arrays are written), and where the length ends inside a page,
+ * page pages[i], which no sequence may hold, a copy of the slots in use of the
+ * source's last page in every layer, and its place in the row. pages[i] is not
+ * looked at where the length ends with a page. -1 for src[i] or dst[i]: no pair.
+ * A pair is left undone, with ABFT_PAGED_BAD_FORK, when src or dst is outside the
+ * batch, dst is also a source or named by another pair, or the page it needs is
+ * named by another pair; with ABFT_PAGED_BAD_LEN or ABFT_PAGED_BAD_PAGE when the
+ * source's length or either page is bad or both pages are the same. */
+typedef struct abft_kv_fork_args {
+  abft_paged_kv kv;
+  const void* const* pools;    /* as for abft_kv_keep                                    */
+  const int32_t* src;          /* [pairs]                                                */
+  const int32_t* dst;
+  const int32_t* pages;
+  int32_t pairs;               /* at most 65535                                          */
+  int32_t layers;
+} abft_kv_fork_args;
+int abft_kv_fork(const abft_kv_fork_args* args, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

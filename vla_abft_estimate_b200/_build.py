@@ -37,7 +37,9 @@ OBJ_DIR = LIB_DIR / "obj"
 SOURCES = {
     "abft_api.cu": ["ptx.cuh", "gemm_kernel.cuh", "aux_kernels.cuh"],
     "paged_api.cu": ["ptx.cuh", "paged_index.cuh", "paged_append.cuh", "paged_decode.cuh",
-                     "paged_prefill.cuh"],
+                     "paged_prefill.cuh", "paged_launch.cuh"],
+    "paged_draft_api.cu": ["ptx.cuh", "paged_index.cuh", "paged_append.cuh", "paged_decode.cuh",
+                           "paged_prefill.cuh", "paged_launch.cuh", "paged_draft.cuh"],
 }
 
 NVCC_FLAGS = [

@@ -73,6 +73,12 @@ EXPORTED_SYMBOLS = (
     "abft_paged_decode",
     "abft_paged_prefill_workspace_bytes",
     "abft_paged_prefill",
+    "abft_kv_append_at",
+    "abft_paged_tree_workspace_bytes",
+    "abft_paged_tree",
+    "abft_draft_accept",
+    "abft_kv_keep",
+    "abft_kv_fork",
 )
 
 NO_ALLOC_SCRATCH_BYTES = 4 << 20
@@ -83,6 +89,10 @@ PAGED_BAD_LEN = 2
 PAGED_BAD_ANGLE = 4
 PAGED_TIMEOUT = 8
 PAGED_BAD_ROWS = 16
+PAGED_BAD_DRAFT = 32
+PAGED_BAD_FORK = 64
+
+MOST_AXES = 4  # of the positions of abft_kv_append_at
 
 
 class AbftError(RuntimeError):
@@ -255,6 +265,76 @@ class PagedAttnArgs(ctypes.Structure):
     ]
 
 
+class KvAppendAtArgs(ctypes.Structure):
+    """Mirror of ``abft_kv_append_at_args``."""
+
+    _fields_ = [
+        ("append", KvAppendArgs),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_int64),
+        ("axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * MOST_AXES),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class PagedTreeArgs(ctypes.Structure):
+    """Mirror of ``abft_paged_tree_args``."""
+
+    _fields_ = [
+        ("attn", PagedAttnArgs),
+        ("parents", ctypes.c_void_p),
+    ]
+
+
+class DraftAcceptArgs(ctypes.Structure):
+    """Mirror of ``abft_draft_accept_args``."""
+
+    _fields_ = [
+        ("cu_seqlens", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("ids", ctypes.c_void_p),
+        ("answers", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("next", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("id_bytes", ctypes.c_int32),
+    ]
+
+
+class KvKeepArgs(ctypes.Structure):
+    """Mirror of ``abft_kv_keep_args``."""
+
+    _fields_ = [
+        ("kv", PagedKv),
+        ("pools", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("lens_out", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("layers", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class KvForkArgs(ctypes.Structure):
+    """Mirror of ``abft_kv_fork_args``."""
+
+    _fields_ = [
+        ("kv", PagedKv),
+        ("pools", ctypes.c_void_p),
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("pages", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+    ]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -325,6 +405,18 @@ def lib() -> ctypes.CDLL:
     L.abft_paged_prefill_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs)]
     L.abft_paged_prefill.restype = ctypes.c_int
     L.abft_paged_prefill.argtypes = [ctypes.POINTER(PagedAttnArgs), vp]
+    L.abft_kv_append_at.restype = ctypes.c_int
+    L.abft_kv_append_at.argtypes = [ctypes.POINTER(KvAppendAtArgs), vp]
+    L.abft_paged_tree_workspace_bytes.restype = sz
+    L.abft_paged_tree_workspace_bytes.argtypes = [ctypes.POINTER(PagedTreeArgs)]
+    L.abft_paged_tree.restype = ctypes.c_int
+    L.abft_paged_tree.argtypes = [ctypes.POINTER(PagedTreeArgs), vp]
+    L.abft_draft_accept.restype = ctypes.c_int
+    L.abft_draft_accept.argtypes = [ctypes.POINTER(DraftAcceptArgs), vp]
+    L.abft_kv_keep.restype = ctypes.c_int
+    L.abft_kv_keep.argtypes = [ctypes.POINTER(KvKeepArgs), vp]
+    L.abft_kv_fork.restype = ctypes.c_int
+    L.abft_kv_fork.argtypes = [ctypes.POINTER(KvForkArgs), vp]
     _LIB = L
     return L
 

@@ -33,6 +33,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+constexpr int kMostAxes = 4;
+
 struct AppendParams {
   PagedView kv;
   const void *q, *k, *v;
@@ -44,6 +46,10 @@ struct AppendParams {
   int64_t tokens;
   int32_t heads;
   int32_t warps_shift;  // log2 of the warps that share a token
+  const int32_t* positions;  // [axes][position_stride]: what a token is rotated by, where that is not its slot's place
+  int64_t position_stride;
+  int32_t axes;
+  int32_t axis_end[kMostAxes];  // pairs [axis_end[a - 1], axis_end[a]) turn by axis a
 };
 
 // Sequence that owns packed token t: the number of boundaries cu[1..batch]
@@ -90,7 +96,12 @@ __device__ __forceinline__ void check_boundaries(const int32_t* cu, int batch, i
 constexpr int kAppendWarps = 8;
 constexpr int kAppendThreads = 32 * kAppendWarps;
 
-template <int D, bool F16>
+//
+// kAxes: the rotation goes by positions of the caller's, of several axes (images
+// and video: time, height, width) or one (a drafted token's depth), each for its
+// share of the pairs:  (c_j, s_j) = rope[positions[axis of j][t]][j]. They are
+// asked for before the chain (sequence, length, page) begins.
+template <int D, bool F16, bool kAxes = false>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
   constexpr int kChunks = D / 16;  // threads per row
   griddep_wait();
@@ -105,6 +116,11 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
     if (p.cu != nullptr && blockIdx.x == gridDim.x - 1 && threadIdx.x < 32)
       check_boundaries(p.cu, kv.batch, p.tokens, lane, kv.status);
     return;
+  }
+  int turn_by[kMostAxes];
+  if constexpr (kAxes) {
+#pragma unroll
+    for (int a = 0; a < kMostAxes; ++a) turn_by[a] = p.positions[(a < p.axes ? a : 0) * p.position_stride + t];
   }
   int b, pos, place = 0, n = 1;
   if (p.cu != nullptr) {
@@ -124,7 +140,13 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
   uint32_t bad = 0;
   if (pos64 < 0 || pos64 >= (static_cast<int64_t>(kv.max_pages) << kv.page_shift)) bad = ABFT_PAGED_BAD_LEN;
   pos = static_cast<int>(pos64);
-  if (bad == 0 && p.rope != nullptr && pos >= p.max_positions) bad = ABFT_PAGED_BAD_ANGLE;
+  if constexpr (kAxes) {
+#pragma unroll
+    for (int a = 0; a < kMostAxes; ++a)
+      if (bad == 0 && (turn_by[a] < 0 || turn_by[a] >= p.max_positions)) bad = ABFT_PAGED_BAD_ANGLE;
+  } else {
+    if (bad == 0 && p.rope != nullptr && pos >= p.max_positions) bad = ABFT_PAGED_BAD_ANGLE;
+  }
   int page = 0;
   if (bad == 0) {
     page = kv.page_table[b * kv.table_stride + (pos >> kv.page_shift)];
@@ -138,7 +160,17 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
   const int slot = pos & ((1 << kv.page_shift) - 1);
   constexpr int kShift = D == 128 ? 7 : 6;
   float cs[16];  // this chunk's (cos, sin) pairs
-  if (p.rope != nullptr) {
+  if constexpr (kAxes) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int pair = 8 * c + i;
+      int by = turn_by[0];
+#pragma unroll
+      for (int a = 1; a < kMostAxes; ++a) by = pair >= p.axis_end[a - 1] ? turn_by[a] : by;
+      const float2 x = __ldg(reinterpret_cast<const float2*>(p.rope + static_cast<int64_t>(by) * D) + pair);
+      cs[2 * i] = x.x, cs[2 * i + 1] = x.y;
+    }
+  } else if (p.rope != nullptr) {
     const float4* r = reinterpret_cast<const float4*>(p.rope + static_cast<int64_t>(pos) * D) + c * 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -182,7 +214,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
       else
         dst = static_cast<uint16_t*>(kv.v_pages) +
               paged_offset(page, kv.v_page_stride, r - p.heads - kv.kv_heads, slot, kv.page_shift, kShift);
-      if (p.rope != nullptr && r < p.heads + kv.kv_heads) {
+      if ((kAxes || p.rope != nullptr) && r < p.heads + kv.kv_heads) {
         uint32_t* a = reinterpret_cast<uint32_t*>(&lo[k]);
         uint32_t* z = reinterpret_cast<uint32_t*>(&hi[k]);
 #pragma unroll

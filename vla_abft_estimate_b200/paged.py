@@ -13,6 +13,18 @@ libabft_b200.so; tensors are CUDA bf16 or fp16 on an sm_100 device.
     q = cache.append(q, k, v, rope)                  # one token per sequence
     o = cache.decode(q)
 
+Drafted tokens, several continuations of a sequence at once, form trees: row i
+of a sequence's new tokens has the row ``parents[i]`` above it (-1: none).
+
+    layers = PagedLayers(caches)                     # every decoder layer's
+    # in each layer: rotated by depth, not by slot; each row sees its ancestors
+    q = cache.append(q, k, v, rope, cu_seqlens=cu, positions=positions)
+    o = cache.tree(q, cu, parents)
+    # once per step, for all layers: the path the model confirms, moved up
+    kept, counts, token = layers.accept(cu, parents, ids, answers)
+    layers.keep(cu, kept, counts)
+    layers.fork(src, dst, pages)                     # samples or beams of one prompt
+
 ``page_table`` and ``seq_lens`` stay on the device and are read by the
 kernels, so a captured step (``torch.cuda.graph``) replays with the lengths
 and pages of the moment. Bad entries never lead outside the tensors; they set
@@ -28,7 +40,7 @@ import ctypes
 import importlib.util
 import math
 import warnings
-from typing import Optional
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -78,6 +90,25 @@ class _LongWay:
         def attend(self, *args):
             return None
 
+        def drafts(self, *entries):
+            pass
+
+        def tree(self, *args):
+            return None
+
+    class Layers:
+        def __init__(self, *caches_and_entries):
+            pass
+
+        def accept(self, *args):
+            return None
+
+        def keep(self, *args):
+            return None
+
+        def fork(self, *args):
+            return None
+
 
 def _host():
     """The extension of csrc/paged_host.cpp, built next to the library for the
@@ -95,6 +126,43 @@ def _host():
                           "`python -m vla_abft_estimate_b200._build`")
             _HOST = _LongWay
     return _HOST
+
+
+def _addresses(*names: str) -> list:
+    return [ctypes.cast(getattr(N.lib(), name), ctypes.c_void_p).value for name in names]
+
+
+def _derivative_free(name: str, t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which the paged cache operators do not give: call them under "
+                         "torch.no_grad()")
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a tangent, which the paged cache operators do not carry on")
+
+
+def _not_traced() -> None:
+    if torch._C._get_tracing_state() is not None:
+        raise ValueError("the paged cache operators cannot be traced: a trace would hold their results as constants")
+
+
+def _mark_written(*tensors: Optional[torch.Tensor]) -> None:
+    """Autograd learns that the tensors have been written."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
+def _raise_status(bits: int) -> None:
+    said = [text for bit, text in ((N.PAGED_BAD_PAGE, "a page_table entry outside the pool, or a page to fork into that is"),
+                                   (N.PAGED_BAD_LEN, "a length below 0, beyond the table or below the new tokens"),
+                                   (N.PAGED_BAD_ANGLE, "a position beyond the rotation table"),
+                                   (N.PAGED_BAD_ROWS, "cu_seqlens that does not start at 0, falls or passes the rows"),
+                                   (N.PAGED_TIMEOUT, "a bounded device wait gave up"),
+                                   (N.PAGED_BAD_DRAFT, "a tree's parent that does not come before its child, or rows to keep "
+                                                       "that do not rise within the new ones"),
+                                   (N.PAGED_BAD_FORK, "a fork from or to a sequence outside the batch, to one that another "
+                                                      "fork names, or into a page that another needs")) if bits & bit]
+    raise ValueError("paged cache: " + "; ".join(said))
 
 
 class PagedKVCache:
@@ -167,12 +235,11 @@ class PagedKVCache:
         kv.batch, kv.max_pages, kv.dtype = batch, max_pages, _DTYPES[k_pages.dtype]
         self._kv = kv
         self._index = dev.index
-        L = N.lib()
-        entry = [ctypes.cast(getattr(L, name), ctypes.c_void_p).value
-                 for name in ("abft_kv_append", "abft_paged_decode", "abft_paged_decode_workspace_bytes",
-                              "abft_paged_prefill", "abft_paged_prefill_workspace_bytes")]
+        entry = _addresses("abft_kv_append", "abft_paged_decode", "abft_paged_decode_workspace_bytes",
+                           "abft_paged_prefill", "abft_paged_prefill_workspace_bytes")
         self._fast = _host().Calls(bytes(kv), dev.index, *entry)
         self._fast.hold(k_pages, v_pages)
+        self._fast.drafts(*_addresses("abft_kv_append_at", "abft_paged_tree", "abft_paged_tree_workspace_bytes"))
 
     # The kernels hold the addresses: the tensors are written in place, not
     # replaced.
@@ -202,26 +269,13 @@ class PagedKVCache:
             return t.clone(memory_format=torch.contiguous_format)
         return t
 
-    @staticmethod
-    def _no_derivative(name: str, t: torch.Tensor) -> None:
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires a gradient, which the paged cache operators do not give: call them under "
-                             "torch.no_grad()")
-        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
-            raise ValueError(f"{name} has a tangent, which the paged cache operators do not carry on")
+    _no_derivative = staticmethod(_derivative_free)
+    _written = staticmethod(_mark_written)
 
     def _callable(self) -> None:
-        if torch._C._get_tracing_state() is not None:
-            raise ValueError("the paged cache operators cannot be traced: a trace would hold their results as constants")
+        _not_traced()
         self._no_derivative("k_pages", self.k_pages)
         self._no_derivative("v_pages", self.v_pages)
-
-    @staticmethod
-    def _written(*tensors: Optional[torch.Tensor]) -> None:
-        """Autograd learns that the tensors have been written."""
-        for t in tensors:
-            if t is not None and not t.is_inference():
-                torch.autograd.graph.increment_version(t)
 
     @staticmethod
     def _in_place(t: torch.Tensor) -> bool:
@@ -254,7 +308,9 @@ class PagedKVCache:
 
     # ---- operators --------------------------------------------------------------
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rope: Optional[torch.Tensor] = None, *,
-               cu_seqlens: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+               cu_seqlens: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+               positions: Optional[torch.Tensor] = None,
+               sections: Optional[Sequence[int]] = None) -> Optional[torch.Tensor]:
         """Stores the new tokens' keys and values and returns the rotated q.
 
         ``q`` [tokens, heads, head_dim], ``k`` and ``v`` [tokens, kv_heads,
@@ -268,15 +324,30 @@ class PagedKVCache:
         (may be ``q``, but not overlap it otherwise) receives q; rows of no
         sequence are left as they were (undefined without ``q_out``). q None
         stores k and v only.
+
+        ``positions``: int32 [tokens] or [axes, tokens] (up to 4 axes), what the
+        rotation goes by in place of the slots' places, which stay those of the
+        lengths: a drafted token's depth behind the cache, an image patch's
+        time, height and width. With several axes ``sections`` says how many
+        pairs turn by each, in their order, head_dim / 2 in all.
         """
-        done = self._fast.append(q, k, v, rope, cu_seqlens, q_out)
+        name = "abft_kv_append"
+        if positions is None:
+            if sections is not None:
+                raise ValueError("sections without positions")
+            done = self._fast.append(q, k, v, rope, cu_seqlens, q_out)
+        else:
+            name = "abft_kv_append_at"
+            positions, sections = self._axes(positions, sections)
+            done = self._fast.append(q, k, v, rope, cu_seqlens, q_out, positions, sections)
         if done is not None:
-            return done if type(done) is not int else N.check("abft_kv_append", done)
+            return done if type(done) is not int else N.check(name, done)
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
-                return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out)
+                return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out, positions=positions, sections=sections)
         self._callable()
-        args = N.KvAppendArgs()
+        by = N.KvAppendAtArgs()
+        args = by.append
         args.kv = self._kv
         k = self._rows("k", k, None, self.kv_heads)
         tokens = k.shape[0]
@@ -306,9 +377,32 @@ class PagedKVCache:
         args.k, args.v, args.tokens = k.data_ptr(), v.data_ptr(), tokens
         args.k_token_stride, args.k_head_stride, _ = k.stride()
         args.v_token_stride, args.v_head_stride, _ = v.stride()
-        self._call("abft_kv_append", args)
+        if positions is not None:
+            if rope is None:
+                raise ValueError("positions without rope")
+            _i32("positions", positions, 2, self.device)
+            if positions.shape[1] != tokens or len(sections) != positions.shape[0]:
+                raise ValueError(f"positions must be [tokens] or [axes, tokens] with a section for each axis, got "
+                                 f"{tuple(positions.shape)} for {tokens} tokens and sections {sections}")
+            if (not 1 <= len(sections) <= N.MOST_AXES or any(type(x) is not int or x < 0 for x in sections)
+                    or sum(sections) * 2 != self.head_dim):
+                raise ValueError(f"sections must be 1 to {N.MOST_AXES} whole numbers, {self.head_dim // 2} in all, got {sections}")
+            by.positions, by.position_stride, by.axes = positions.data_ptr(), positions.stride(0), len(sections)
+            for i, x in enumerate(sections):
+                by.sections[i] = x
+        self._call(name, args if positions is None else by)
         self._written(self.k_pages, self.v_pages, q_out)
         return q_out
+
+    def _axes(self, positions, sections):
+        """positions as [axes, tokens], sections as a tuple."""
+        if not isinstance(positions, torch.Tensor):
+            raise TypeError(f"positions must be a torch.Tensor, got {type(positions).__name__}")
+        if sections is None:
+            sections = (self.head_dim // 2,)
+        elif type(sections) is not tuple:
+            sections = tuple(sections)
+        return (positions[None] if positions.dim() == 1 else positions), sections
 
     def decode(self, q: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                num_sms: int = 0) -> torch.Tensor:
@@ -331,16 +425,30 @@ class PagedKVCache:
         sequences' lengths)."""
         return self._attention(True, q, cu_seqlens, scale, out, num_splits, 0)
 
-    def _attention(self, prefill, q, cu, scale, out, num_splits, num_sms):
-        done = self._fast.attend(prefill, q, cu, scale, out, num_splits, num_sms)
-        name = "abft_paged_prefill" if prefill else "abft_paged_decode"
+    def tree(self, q: torch.Tensor, cu_seqlens: torch.Tensor, parents: torch.Tensor, *, scale: Optional[float] = None,
+             out: Optional[torch.Tensor] = None, num_splits: int = 0) -> torch.Tensor:
+        """Attention of a tree of drafted tokens for each sequence: rows as in
+        ``prefill``, but row i of n sees the slots before the n new ones, its
+        own and its ancestors'. ``parents`` int32 [tokens]: the place of row
+        i's parent among its sequence's new rows, below i, or -1 for none (a row
+        that follows the cached tokens directly; there may be several). Trees of
+        any size, one row included. Everything else is as in ``prefill``."""
+        return self._attention(True, q, cu_seqlens, scale, out, num_splits, 0, parents, True)
+
+    def _attention(self, prefill, q, cu, scale, out, num_splits, num_sms, parents=None, tree=False):
+        if tree:
+            done = self._fast.tree(q, cu, parents, scale, out, num_splits, num_sms)
+        else:
+            done = self._fast.attend(prefill, q, cu, scale, out, num_splits, num_sms)
+        name = "abft_paged_tree" if tree else "abft_paged_prefill" if prefill else "abft_paged_decode"
         if done is not None:
             return done if type(done) is not int else N.check(name, done)
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
-                return self._attention(prefill, q, cu, scale, out, num_splits, num_sms)
+                return self._attention(prefill, q, cu, scale, out, num_splits, num_sms, parents, tree)
         self._callable()
-        args = N.PagedAttnArgs()
+        call = N.PagedTreeArgs()
+        args = call.attn
         args.kv = self._kv
         if prefill:
             self._boundaries(cu)
@@ -349,6 +457,11 @@ class PagedKVCache:
             raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
         self._group(q.shape[1] if q.dim() == 3 else 0)
         q = self._rows("q", q, None if prefill else self.batch, None)
+        if tree:
+            _i32("parents", parents, 1, self.device)
+            if parents.shape[0] != q.shape[0]:
+                raise ValueError(f"parents must have an entry for each of the {q.shape[0]} rows, got {parents.shape[0]}")
+            call.parents = parents.data_ptr()
         out = self._result("out", out, q)
         args.q, args.out, args.tokens, args.heads = q.data_ptr(), out.data_ptr(), q.shape[0], q.shape[1]
         args.q_token_stride, args.q_head_stride, _ = q.stride()
@@ -357,11 +470,12 @@ class PagedKVCache:
         if int(num_splits) < 0 or int(num_sms) < 0 or not math.isfinite(args.scale):
             raise ValueError(f"scale must be finite, num_splits and num_sms at least 0, got {scale}, {num_splits}, {num_sms}")
         args.num_splits, args.num_sms = int(num_splits), int(num_sms)
-        need = int(getattr(N.lib(), name + "_workspace_bytes")(ctypes.byref(args)))
+        given = call if tree else args
+        need = int(getattr(N.lib(), name + "_workspace_bytes")(ctypes.byref(given)))
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)  # of this call alone
             args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        self._call(name, args)
+        self._call(name, given)
         self._written(out)
         return out
 
@@ -374,9 +488,162 @@ class PagedKVCache:
         if not bits:
             return
         self.status.zero_()
-        said = [text for bit, text in ((N.PAGED_BAD_PAGE, "a page_table entry outside the pool"),
-                                       (N.PAGED_BAD_LEN, "a length below 0, beyond the table or below the new tokens"),
-                                       (N.PAGED_BAD_ANGLE, "a position beyond the rotation table"),
-                                       (N.PAGED_BAD_ROWS, "cu_seqlens that does not start at 0, falls or passes the rows"),
-                                       (N.PAGED_TIMEOUT, "a bounded device wait gave up")) if bits & bit]
-        raise ValueError("paged cache: " + "; ".join(said))
+        _raise_status(bits)
+
+
+class PagedLayers:
+    """The caches of a model's layers, for what is done in all of them at once.
+
+    ``layers``: a ``PagedKVCache`` for each, with one page table, one array of
+    lengths, one type and one geometry, and pools of their own. Make it outside
+    of a graph capture; the calls may be captured. What the status tells of these
+    calls is in the first layer's.
+    """
+
+    def __init__(self, layers: Sequence[PagedKVCache]):
+        layers = tuple(layers)
+        if not layers or not all(isinstance(c, PagedKVCache) for c in layers):
+            raise TypeError("layers must be PagedKVCache objects, one at least")
+        first = layers[0]
+
+        def shared(c):
+            kv = c._kv
+            return (kv.page_table, kv.table_stride, kv.seq_lens, kv.k_page_stride, kv.v_page_stride, c.device, c.dtype,
+                    c.batch, c.max_pages, c.num_pages, c.kv_heads, c.page_size, c.head_dim)
+
+        if any(shared(c) != shared(first) for c in layers):
+            raise ValueError("layers must share page table, lengths, type, shape and page strides")
+        pools = [x for c in layers for x in (c._kv.k_pages or 0, c._kv.v_pages or 0)]
+        if first.num_pages and len(set(pools)) != len(pools):
+            raise ValueError("layers must have pools of their own, for keys and for values")
+        self.layers, self.batch, self.device = layers, first.batch, first.device
+        self._kv, self._index = first._kv, first._index
+        self._pools = torch.tensor(pools, dtype=torch.int64, device=self.device)
+        self._pages = tuple(x for c in layers for x in (c.k_pages, c.v_pages))
+        self._fast = _host().Layers(bytes(self._kv), self._index, len(layers), self._pools.data_ptr(),
+                                    *_addresses("abft_draft_accept", "abft_kv_keep", "abft_kv_fork"),
+                                    self._pages, first.page_table, first.seq_lens)
+
+    page_table = property(lambda self: self.layers[0].page_table)
+    seq_lens = property(lambda self: self.layers[0].seq_lens)
+
+    def _list(self, name: str, t: torch.Tensor, size: int) -> None:
+        _i32(name, t, 1, self.device)
+        if t.shape[0] != size:
+            raise ValueError(f"{name} must have {size} entries, got {t.shape[0]}")
+
+    def _callable(self) -> None:
+        _not_traced()
+        for c in self.layers:
+            c._callable()
+
+    def _call(self, name: str, args) -> None:
+        stream = torch._C._cuda_getCurrentRawStream(self._index)
+        N.check(name, getattr(N.lib(), name)(ctypes.byref(args), stream))
+
+    def accept(self, cu_seqlens: torch.Tensor, parents: torch.Tensor, ids: torch.Tensor,
+               answers: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Which rows of each sequence's tree the model confirms: (kept,
+        counts, token). ``ids`` int32 or int64 [tokens], the drafted tokens;
+        ``answers`` of the same type, the token that the model gives behind each
+        row. A row is confirmed when it has no parent (it was sampled already),
+        or its parent is confirmed and ``answers[parent] == ids[row]``. ``kept``
+        int32 [tokens]: for each sequence the path to its deepest confirmed row
+        (the lowest of equals), as places among its new rows, then -1;
+        ``counts`` int32 [batch] its length; ``token`` [batch] the last row's
+        answer, -1 for a sequence without rows."""
+        done = self._fast.accept(cu_seqlens, parents, ids, answers)
+        if done is not None:
+            return done if type(done) is not int else N.check("abft_draft_accept", done)
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                return self.accept(cu_seqlens, parents, ids, answers)
+        _not_traced()
+        self._list("cu_seqlens", cu_seqlens, self.batch + 1)
+        for name, t in (("ids", ids), ("answers", answers)):
+            if (not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.dim() != 1
+                    or t.device != self.device or t.dtype != ids.dtype or t.shape != ids.shape):
+                raise ValueError(f"{name} must be a 1-D int32 or int64 tensor on {self.device}, ids and answers alike")
+        self._list("parents", parents, ids.shape[0])
+        ids, answers = ids.contiguous(), answers.contiguous()
+        kept = torch.empty(ids.shape, dtype=torch.int32, device=self.device)
+        counts = torch.empty(self.batch, dtype=torch.int32, device=self.device)
+        token = torch.empty(self.batch, dtype=ids.dtype, device=self.device)
+        args = N.DraftAcceptArgs()
+        args.cu_seqlens, args.parents = cu_seqlens.data_ptr(), parents.data_ptr()
+        args.ids, args.answers = ids.data_ptr(), answers.data_ptr()
+        args.kept, args.counts, args.next = kept.data_ptr(), counts.data_ptr(), token.data_ptr()
+        args.status, args.tokens, args.batch = self._kv.status, ids.shape[0], self.batch
+        args.id_bytes = ids.element_size()
+        self._call("abft_draft_accept", args)
+        return kept, counts, token
+
+    def keep(self, cu_seqlens: torch.Tensor, kept: torch.Tensor, counts: torch.Tensor, *,
+             lens_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Of each sequence's n new tokens (rows cu[b] to cu[b + 1] of the step)
+        keeps the rows ``kept[cu[b]]`` to ``kept[cu[b] + counts[b] - 1]``, rising
+        places among them: their keys and values move up to the slots behind
+        the cache, in all layers, and ``seq_lens[b]`` falls by ``n - counts[b]``.
+        ``lens_out``: int32 [batch] that gets the lengths instead, ``seq_lens``
+        stays. Pages behind the new lengths stay in the table, for the caller to
+        use again. A sequence with bad rows, boundaries, length or pages is left
+        as it was, and the status tells. Returns the array of lengths written."""
+        out = self.seq_lens if lens_out is None else lens_out
+        done = self._fast.keep(cu_seqlens, kept, counts, out)
+        if done is not None:
+            N.check("abft_kv_keep", done)
+            return out
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                return self.keep(cu_seqlens, kept, counts, lens_out=lens_out)
+        self._callable()
+        self._list("cu_seqlens", cu_seqlens, self.batch + 1)
+        _i32("kept", kept, 1, self.device)
+        self._list("counts", counts, self.batch)
+        self._list("lens_out", out, self.batch)
+        args = N.KvKeepArgs()
+        args.kv, args.pools, args.layers = self._kv, self._pools.data_ptr(), len(self.layers)
+        args.cu_seqlens, args.kept, args.counts = cu_seqlens.data_ptr(), kept.data_ptr(), counts.data_ptr()
+        args.lens_out, args.tokens = out.data_ptr(), kept.shape[0]
+        self._call("abft_kv_keep", args)
+        _mark_written(*self._pages, out)
+        return out
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor, pages: torch.Tensor) -> None:
+        """Lets sequences go on from others' caches: for each pair i (int32
+        [pairs] each) sequence ``dst[i]`` gets the length and the full pages of
+        ``src[i]``, which they share from now on, and, where the length ends
+        inside a page, a copy of that page's slots in use, in all layers, in
+        page ``pages[i]``, which no sequence may hold and which its row of the
+        table names then (not looked at where the length ends with a page). -1
+        in ``src`` or ``dst``: no pair. Sources may be named by several pairs;
+        a destination that is also a source or named twice, or a page that
+        another pair names too, is refused: the pair is left undone, and the
+        status tells."""
+        done = self._fast.fork(src, dst, pages)
+        if done is not None:
+            return N.check("abft_kv_fork", done)
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                return self.fork(src, dst, pages)
+        self._callable()
+        _i32("src", src, 1, self.device)
+        self._list("dst", dst, src.shape[0])
+        self._list("pages", pages, src.shape[0])
+        args = N.KvForkArgs()
+        args.kv, args.pools, args.layers = self._kv, self._pools.data_ptr(), len(self.layers)
+        args.src, args.dst, args.pages, args.pairs = src.data_ptr(), dst.data_ptr(), pages.data_ptr(), src.shape[0]
+        self._call("abft_kv_fork", args)
+        _mark_written(*self._pages, self.page_table, self.seq_lens)
+
+    def check_status(self) -> None:
+        """``PagedKVCache.check_status`` for all layers at once."""
+        words = {c.status.data_ptr(): c.status for c in self.layers}.values()
+        bits = 0
+        for x in torch.cat([w[:1] for w in words]).tolist():
+            bits |= x
+        if not bits:
+            return
+        for w in words:
+            w.zero_()
+        _raise_status(bits)
