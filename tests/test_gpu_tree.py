@@ -13,7 +13,7 @@ from .test_gpu_paged import BF16, F16, bits, close
 pytestmark = pytest.mark.gpu
 
 
-def run_tree(dev, trees, total, heads, kv_heads, d, page, dtype, *, seed=0, pad=0, scale=None, splits=0, joint=False,
+def run_tree(dev, trees, total, heads, kv_heads, d, page, dtype, *, seed=0, pad=0, scale=None, sms=0, joint=False,
              strided=False, in_place=False, extra_columns=0):
     pool = Pool(total, kv_heads, page, d, dtype, seed=seed, joint=joint, extra_columns=extra_columns)
     cache = pool.device_cache(dev, PagedKVCache)
@@ -28,7 +28,7 @@ def run_tree(dev, trees, total, heads, kv_heads, d, page, dtype, *, seed=0, pad=
         dq = wide[:, 1:heads + 1]
     out = dq if in_place else torch.full((tokens, heads, d), 7.0, dtype=dtype, device=dev)
     before = bits(cache.k_pages), bits(cache.v_pages)
-    got = cache.tree(dq, i32(cu, dev), i32(parents + [-1] * pad, dev), scale=scale, out=out, num_splits=splits)
+    got = cache.tree(dq, i32(cu, dev), i32(parents + [-1] * pad, dev), scale=scale, out=out, num_sms=sms)
     assert got is out
     cache.check_status()
     rows = [(b, visible_slots(tree, i, total[b])) for b, tree in enumerate(trees) for i in range(len(tree))]
@@ -53,11 +53,11 @@ def test_lengths(cuda_device, n, total, page):
     run_tree(cuda_device, [random_tree(n, n + total)], [total], 7, 1, 128, page, BF16)
 
 
-@pytest.mark.parametrize("splits", [0, 1, 2, 5])
+@pytest.mark.parametrize("sms", [0, 1, 2, 5, 37])
 @pytest.mark.parametrize("d", [64, 128])
-def test_long_caches_in_pieces(cuda_device, d, splits):
+def test_long_caches_in_pieces(cuda_device, d, sms):
     trees = [random_tree(26, 5), random_tree(3, 6), [], random_tree(61, 7)]
-    run_tree(cuda_device, trees, [3000, 700, 0, 1111], 14, 2, d, 32, BF16, splits=splits)
+    run_tree(cuda_device, trees, [3000, 700, 0, 1111], 14, 2, d, 32, BF16, sms=sms)
 
 
 @pytest.mark.parametrize("shape", ["chain", "star", "many roots", "two deep", "roots only"])
@@ -123,8 +123,8 @@ def test_hidden_rows_do_not_count_however_large(cuda_device):
     close(got[odd], want[odd], tol[odd])
 
 
-@pytest.mark.parametrize("splits", [0, 1, 3])
-def test_bad_parents_end_the_way_up(cuda_device, splits):
+@pytest.mark.parametrize("sms", [0, 1, 3])
+def test_bad_parents_end_the_way_up(cuda_device, sms):
     dev = cuda_device
     tree = random_tree(40, 3)
     tree[7], tree[11], tree[20], tree[39] = 7, 30, -9, 2 ** 31 - 1
@@ -133,7 +133,7 @@ def test_bad_parents_end_the_way_up(cuda_device, splits):
     pool = Pool([700], 2, 16, 64, BF16)
     cache = pool.device_cache(dev, PagedKVCache)
     q = torch.randn(40, 4, 64, generator=torch.Generator().manual_seed(4)).to(BF16)
-    got = cache.tree(q.to(dev), i32([0, 40], dev), i32(tree, dev), num_splits=splits)
+    got = cache.tree(q.to(dev), i32([0, 40], dev), i32(tree, dev), num_sms=sms)
     close(got, *attention_over(pool, q, [(0, visible_slots(tree, i, 700)) for i in range(40)]))
     with pytest.raises(ValueError, match="parent"):
         cache.check_status()
@@ -243,7 +243,7 @@ def test_refusals(cuda_device):
     with pytest.raises(ValueError):
         cache.tree(q, cu, up, scale=math.inf)
     with pytest.raises(ValueError):
-        cache.tree(q, cu, up, num_splits=-1)
+        cache.tree(q, cu, up, num_sms=-1)
     with pytest.raises(ValueError, match="q must be"):
         cache.tree(q.half(), cu, up)
     with pytest.raises(ValueError, match="heads"):
@@ -253,3 +253,83 @@ def test_refusals(cuda_device):
     with pytest.raises(ValueError, match="gradient"):
         cache.tree(q.clone().requires_grad_(), cu, up)
     assert cache.tree(q[:0], i32([0, 0], dev), up[:0]).shape == (0, 4, 64)
+
+
+# The table's width decides whether a segment has a cluster of CTAs or a part of the
+# list, the number of rows how many segments there are.
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("columns", [0, 2000])
+@pytest.mark.parametrize("heads,kv_heads,n", [(4, 4, 5), (8, 2, 4), (14, 2, 4), (16, 2, 8), (7, 1, 16), (64, 1, 3)])
+def test_small_trees(cuda_device, heads, kv_heads, n, columns, d, dtype):
+    for sizes, total in (([n], [600]), ([n], [n]), ([n], [64 + n]), ([n, n, 1, 0, n], [129, 64, 1, 0, 2000]),
+                         ([n] * 9, [n + 61 * b for b in range(9)])):
+        run_tree(cuda_device, [random_tree(x, 3 + i) for i, x in enumerate(sizes)], total, heads, kv_heads, d, 16, dtype,
+                 extra_columns=columns)
+
+
+@pytest.mark.parametrize("columns", [0, 1000])
+def test_uneven_small_trees(cuda_device, columns):
+    """Trees of several times the average's rows: more segments than one, and idle sequences."""
+    for seed in range(4):
+        sizes = [1, 60, 0, 2, 0, 33, 1, 1, 0, 5, 1, 2]
+        total = [1, 900, 0, 40, 0, 33, 700, 64, 0, 300, 2, 129]
+        run_tree(cuda_device, [random_tree(n, seed + n) for n in sizes], total, 12, 2, 128, 16, BF16, seed=seed, pad=5,
+                 extra_columns=columns)
+
+
+def test_long_caches_of_small_trees(cuda_device):
+    """Segments that cross many CTAs, whole ones inside one, and many sequences."""
+    run_tree(cuda_device, [random_tree(6, 1)], [20000], 8, 1, 128, 64, BF16)
+    run_tree(cuda_device, [random_tree(6, 1), random_tree(3, 2)], [9000, 30], 20, 2, 64, 32, F16)
+    run_tree(cuda_device, [random_tree(4, b) for b in range(40)], [30 + 97 * (b * b % 41) for b in range(40)], 8, 4, 64, 16, BF16)
+    run_tree(cuda_device, [random_tree(1 + b % 3, b) for b in range(1100)], [3 + b % 70 for b in range(1100)], 2, 1, 64, 16, BF16)
+
+
+def test_small_trees_say_what_is_wrong(cuda_device):
+    """Bad lengths, pages, parents and boundaries, by cluster and by list."""
+    dev = cuda_device
+    for columns in (0, 1000):
+        trees, total = [random_tree(6, 1), random_tree(5, 2), random_tree(4, 3)], [40, 100, 3]
+        cu, parents = packed(trees)
+        q = torch.randn(cu[-1], 4, 64, generator=torch.Generator().manual_seed(4)).to(BF16)
+
+        def answer(change, match, want=None, total=total, cu=cu, parents=parents):
+            pool = Pool([40, 100, 10], 2, 16, 64, BF16, extra_columns=columns)
+            cache = pool.device_cache(dev, PagedKVCache)
+            cache.seq_lens.copy_(i32(total))
+            change(cache)
+            out = torch.full((len(q), 4, 64), 7.0, dtype=BF16, device=dev)
+            cache.tree(q.to(dev), i32(cu, dev), i32(parents, dev), out=out)
+            with pytest.raises(ValueError, match=match):
+                cache.check_status()
+            cache.check_status()
+            return pool, out
+
+        pool, out = answer(lambda c: None, "length")  # sequence 2 has more rows than tokens
+        close(out, *attention_over(pool, q, [(b, visible_slots(t, i, total[b])) for b, t in enumerate(trees)
+                                             for i in range(len(t))]))
+        for lens in ([40, 100, 0], [40, 100, -5]):
+            pool, out = answer(lambda c: None, "length", total=lens)
+            assert (out[cu[2]:] == 0).all()
+            close(out[:cu[2]], *attention_over(pool, q[:cu[2]], [(b, visible_slots(trees[b], i, total[b])) for b in (0, 1)
+                                                                 for i in range(len(trees[b]))]))
+
+        def spoil(c):
+            c.page_table[1, 2] = -7
+
+        pool, out = answer(spoil, "page_table")
+        for x in (pool.k, pool.v):
+            x[pool.table[1, 2].long()] = 0
+        rows = [(b, visible_slots(t, i, total[b])) for b, t in enumerate(trees) for i in range(len(t))]
+        close(out, *attention_over(pool, q, rows))
+        wrong = list(parents)
+        wrong[8], wrong[14] = 4, -3
+        pool, out = answer(lambda c: None, "parent", parents=wrong, total=[40, 100, 10])
+        bad = [wrong[a:b] for a, b in zip(cu, cu[1:])]
+        close(out, *attention_over(pool, q, [(b, visible_slots(t, i, (40, 100, 10)[b])) for b, t in enumerate(bad)
+                                             for i in range(len(t))]))
+        pool, out = answer(lambda c: None, "cu_seqlens", cu=[0, 6, 40, 50], total=[40, 100, 10])
+        close(out[:6], *attention_over(pool, q[:6], rows[:6]))
+        assert (out[6:] == 7.0).all()
+        answer(lambda c: None, "cu_seqlens", cu=[-1, -1, -1, -1], total=[40, 100, 10])

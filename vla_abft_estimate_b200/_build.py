@@ -39,7 +39,7 @@ SOURCES = {
     "paged_api.cu": ["ptx.cuh", "paged_index.cuh", "paged_append.cuh", "paged_decode.cuh",
                      "paged_prefill.cuh", "paged_launch.cuh"],
     "paged_draft_api.cu": ["ptx.cuh", "paged_index.cuh", "paged_append.cuh", "paged_decode.cuh",
-                           "paged_prefill.cuh", "paged_launch.cuh", "paged_draft.cuh"],
+                           "paged_prefill.cuh", "paged_tree.cuh", "paged_launch.cuh", "paged_draft.cuh"],
 }
 
 NVCC_FLAGS = [

@@ -93,6 +93,57 @@ size_t abft_paged_prefill_workspace_bytes(const abft_paged_attn_args* a) {
   return prefill_bytes(a, prefill_plan(a, sms));
 }
 
-int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) { return prefill_call<false>(a, nullptr, stream); }
+int abft_paged_prefill(const abft_paged_attn_args* a, void* stream) {
+  int rc = attn_check(a, false);
+  if (rc != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return rc;
+  int dev = 0, sms = 0;
+  if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
+  if (a->num_sms > 0) sms = a->num_sms;
+  PrefillParams p;
+  p.kv = view_of(a->kv);
+  p.q = a->q, p.out = a->out;
+  p.qt = a->q_token_stride, p.qh = a->q_head_stride;
+  p.ot = a->o_token_stride, p.oh = a->o_head_stride;
+  p.cu = a->cu_seqlens;
+  p.tokens = static_cast<int32_t>(a->tokens);
+  p.group = a->heads / a->kv.kv_heads;
+  const PrefillPlan plan = prefill_plan(a, sms);
+  if (plan.items >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
+  p.tile_tokens = plan.tile_tokens;
+  p.block_tokens = plan.block_tokens;
+  p.splits = plan.splits;
+  p.piece = plan.choose ? 0 : plan.piece;
+  p.sms = sms;
+  const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
+  p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
+  p.negate = a->scale < 0.f;
+  p.group_inv = (65536u + p.group - 1) / p.group;
+  const size_t need = prefill_bytes(a, plan);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
+  if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(
+      p.part_o + static_cast<size_t>(a->tokens) * a->heads * p.splits * a->kv.head_dim);
+  p.chosen = plan.choose ? reinterpret_cast<int32_t*>(p.part_ml + static_cast<size_t>(a->tokens) * a->heads * p.splits)
+                         : nullptr;
+  CUtensorMap tm_k, tm_v;
+  if ((rc = page_map(&tm_k, a->kv, a->kv.k_pages, a->kv.k_page_stride)) != ABFT_OK) return rc;
+  if ((rc = page_map(&tm_v, a->kv, a->kv.v_pages, a->kv.v_page_stride)) != ABFT_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
+  const bool shared = plan.block_tokens == plan.tile_tokens;
+  const int slot = 8 + (a->kv.head_dim == 128 ? 4 : 0) + (f16 ? 2 : 0) + (shared ? 1 : 0);
+  const int64_t items = plan.items;
+  switch (slot - 8) {
+    case 0: return launch_prefill<64, false, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 1: return launch_prefill<64, false, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 2: return launch_prefill<64, true, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 3: return launch_prefill<64, true, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 4: return launch_prefill<128, false, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 5: return launch_prefill<128, false, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+    case 6: return launch_prefill<128, true, false>(dev, slot, a, tm_k, tm_v, p, items, s);
+    default: return launch_prefill<128, true, true>(dev, slot, a, tm_k, tm_v, p, items, s);
+  }
+}
 
 }  // extern "C"

@@ -153,15 +153,18 @@ struct KeepParams {
   int32_t tokens;
   int32_t cluster;  // CTAs of a sequence
 };
-constexpr int kKeepThreads = 512;
+constexpr int kKeepThreads = 512;  // at most
 constexpr int kKeepHeld = 256;  // rows whose places are in shared memory at a time
 constexpr int kKeepCluster = 8;
 
 template <int D>
-__global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const KeepParams p) {
-  __shared__ int4 s_move[kKeepHeld];  // page and slot of the source, of the destination
+__global__ void __launch_bounds__(kKeepThreads, 3) kv_keep_kernel(const KeepParams p) {
+  // Where a row comes from (-1: it stays) and goes, in elements of head 0: in the
+  // key pools, in the value pools.
+  __shared__ longlong2 s_move[2][kKeepHeld];
   constexpr int kShift = D == 128 ? 7 : 6, kChunks = D / 8;
   griddep_wait();
+  const int threads = blockDim.x;
   const PagedView& kv = p.kv;
   const int b = blockIdx.x / p.cluster, rank = blockIdx.x - b * p.cluster;
   int begin, end;
@@ -185,13 +188,20 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const KeepParams 
   auto stage = [&](int i) {  // row i's move; what is wrong with it
     const int from = p.kept[begin + i], last = i > 0 ? p.kept[begin + i - 1] : -1;
     if (from <= last || from >= n || from < 0) return ABFT_PAGED_BAD_DRAFT;
-    int4 move;
-    const bool ok = place(from, &move.x, &move.y) & place(i, &move.z, &move.w);
-    s_move[i % kKeepHeld] = move;
+    int page0, slot0, page1, slot1;
+    const bool ok = place(from, &page0, &slot0) & place(i, &page1, &slot1);
+#pragma unroll
+    for (int values = 0; values < 2; ++values) {
+      const int64_t stride = values ? kv.v_page_stride : kv.k_page_stride;
+      longlong2 move;
+      move.x = from == i ? -1 : paged_offset(page0, stride, 0, slot0, kv.page_shift, kShift);
+      move.y = paged_offset(page1, stride, 0, slot1, kv.page_shift, kShift);
+      s_move[values][i % kKeepHeld] = move;
+    }
     return ok ? 0u : ABFT_PAGED_BAD_PAGE;
   };
   if (bad == 0)  // looks at all rows; those of a path that fits are staged for good
-    for (int i = threadIdx.x; i < m; i += kKeepThreads) bad |= stage(i);
+    for (int i = threadIdx.x; i < m; i += threads) bad |= stage(i);
   const bool wrong = __syncthreads_or(bad != 0);
   if (bad != 0 && rank == 0 && kv.status != nullptr) atomicOr(kv.status, bad);
   if (p.cluster > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -201,28 +211,23 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const KeepParams 
       const int here = min(kKeepHeld, m - i0);
       if (m > kKeepHeld) {
         __syncthreads();
-        for (int i = threadIdx.x; i < here; i += kKeepThreads) stage(i0 + i);
+        for (int i = threadIdx.x; i < here; i += threads) stage(i0 + i);
         __syncthreads();
       }
-      for (int column = rank * kKeepThreads + threadIdx.x; column < columns; column += p.cluster * kKeepThreads) {
+      for (int column = rank * threads + threadIdx.x; column < columns; column += p.cluster * threads) {
         const int c = column % kChunks, row = column / kChunks;
         const int head = row % kv.kv_heads, pool = row / kv.kv_heads, values = pool & 1;
-        uint16_t* at = pool_of(kv, p.layers, pool >> 1, values) + c * 8;
-        const int64_t stride = values ? kv.v_page_stride : kv.k_page_stride;
+        uint16_t* at = pool_of(kv, p.layers, pool >> 1, values) + (static_cast<int64_t>(head) << kv.page_shift << kShift) + c * 8;
+        const longlong2* moves = s_move[values];
         constexpr int kBatch = 4;
         for (int i = 0; i < here; i += kBatch) {
           uint4 x[kBatch];
-          int4 move[kBatch];
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            move[k] = i + k < here ? s_move[i + k] : make_int4(0, 0, 0, 0);
-            if (move[k].x != move[k].z || move[k].y != move[k].w)
-              x[k] = *reinterpret_cast<const uint4*>(at + paged_offset(move[k].x, stride, head, move[k].y, kv.page_shift, kShift));
-          }
 #pragma unroll
           for (int k = 0; k < kBatch; ++k)
-            if (move[k].x != move[k].z || move[k].y != move[k].w)
-              *reinterpret_cast<uint4*>(at + paged_offset(move[k].z, stride, head, move[k].w, kv.page_shift, kShift)) = x[k];
+            if (i + k < here && moves[i + k].x >= 0) x[k] = *reinterpret_cast<const uint4*>(at + moves[i + k].x);
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k)
+            if (i + k < here && moves[i + k].x >= 0) *reinterpret_cast<uint4*>(at + moves[i + k].y) = x[k];
         }
       }
     }

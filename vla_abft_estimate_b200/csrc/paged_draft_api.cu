@@ -3,6 +3,7 @@
 // and fork. Declarations are in include/abft_b200.h.
 #include "paged_draft.cuh"
 #include "paged_launch.cuh"
+#include "paged_tree.cuh"
 
 using namespace abft;
 
@@ -13,6 +14,110 @@ int check_layers(const abft_paged_kv& kv, const void* const* pools, int32_t laye
   if (layers > 4096) return ABFT_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(pools) & 7u) != 0) return ABFT_ERR_ALIGNMENT;
   return check_kv(kv);
+}
+
+// How a tree call is cut: segments of a tile of query rows and one kv head, dealt by
+// the list or to clusters.
+struct TreePlan {
+  int tile_tokens;
+  int cluster;  // CTAs of a segment, or 0: the list
+  int grid;
+};
+
+// Short caches get a cluster of up to 8 CTAs per segment, as long as all clusters
+// run at once (two CTAs an SM; 8 x 30 and 4 x 65 fit the device's groups of SMs) and a
+// CTA has no more than 12 steps, or 16 where the list would cut each segment into
+// more than 24 pieces. Measured (28/4 heads of 128; cluster / list): 1 tree of 16 tokens
+// on 1,000 slots 11.7 / 13.7 us, 4,000 15.6 / 21.9, 8,000 (16 steps) 21.9 / 26.5; 1 of
+// 64 on 2,000 15.5 / 18.2, on 8,000 (16 steps, 18 pieces) 26.8 / 23.9; 16 of 16 on
+// 500 15.7 / 19.7; 32 of 8 on 600 20.5 / 23.1, on 1,200 (20 steps) 29.1 / 29.3. (The
+// lengths are on the device: what is known here, and decides, is the width of the
+// table.)
+int tree_plan(const abft_paged_attn_args* a, int sms, TreePlan* r) {
+  r->tile_tokens = kTreeRows / (a->heads / a->kv.kv_heads);
+  // Segments at most (the boundaries are on the device), and steps of one.
+  const int64_t segments = a->kv.kv_heads * (a->kv.batch == 1 ? (a->tokens + r->tile_tokens - 1) / r->tile_tokens
+                                                              : a->tokens / r->tile_tokens + a->kv.batch);
+  const int64_t slots = static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size;
+  const int64_t steps = slots > kTreeKeys ? (slots + kTreeKeys - 1) / kTreeKeys : 1;
+  if (segments * (steps + kTreeCost) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;  // the list is counted in 32 bits
+  const int ctas = 2 * sms;
+  r->cluster = 0;
+  if (segments <= ctas) {
+    int c = 8 * segments <= ctas * 13 / 16 ? 8 : 4 * segments <= ctas * 7 / 8 ? 4 : 2 * segments <= ctas ? 2 : 1;
+    while (c > 1 && c / 2 >= steps) c /= 2;
+    if (steps <= (24 * segments <= ctas ? 16 : 12) * c) {
+      r->cluster = c;
+      r->grid = static_cast<int>(segments) * c;
+      return ABFT_OK;
+    }
+  }
+  r->grid = static_cast<int>(segments * steps < ctas ? segments * steps : ctas);
+  return ABFT_OK;
+}
+
+size_t tree_bytes(const abft_paged_attn_args* a, const TreePlan& plan) {
+  if (plan.cluster > 0) return 0;
+  const size_t rows = static_cast<size_t>(plan.grid) * 2 * kTreeRows;
+  return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2)) + plan.grid * (sizeof(int2) + sizeof(int32_t));
+}
+
+template <int D, bool F16>
+int launch_tree(int dev, int slot, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const TreeParams& p, const TreePlan& plan,
+                int sms, cudaStream_t s) {
+  using Cfg = TreeCfg<D>;
+  int rc = raise_smem(dev, slot, paged_tree_kernel<D, F16>, Cfg::kSmemBytes);
+  if (rc != ABFT_OK) return rc;
+  rc = launch_clusters(p.work.cluster, paged_tree_kernel<D, F16>, dim3(plan.grid), dim3(kTreeThreads), Cfg::kSmemBytes, s, tm_k,
+                       tm_v, p);
+  if (rc != ABFT_OK || p.work.cluster > 0) return rc;
+  return launch(paged_tree_join_kernel<D, F16>, dim3(4 * sms), dim3(kTreeJoinThreads), 0, s, p, plan.grid);
+}
+
+int tree_call(const abft_paged_tree_args* t, void* stream) {
+  const abft_paged_attn_args* a = &t->attn;
+  int rc = attn_check(a, false);
+  if (rc != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return rc;
+  if (t->parents == nullptr) return ABFT_ERR_INVALID_ARG;
+  int dev = 0, sms = 0;
+  if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
+  if (a->num_sms > 0) sms = a->num_sms;
+  TreePlan plan;
+  if ((rc = tree_plan(a, sms, &plan)) != ABFT_OK) return rc;
+  const size_t need = tree_bytes(a, plan);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
+  if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
+  TreeParams p = {};
+  p.kv = view_of(a->kv);
+  p.q = a->q, p.out = a->out;
+  p.qt = a->q_token_stride, p.qh = a->q_head_stride;
+  p.ot = a->o_token_stride, p.oh = a->o_head_stride;
+  p.cu = a->cu_seqlens;
+  p.tokens = static_cast<int32_t>(a->tokens);
+  p.group = a->heads / a->kv.kv_heads;
+  p.tile_tokens = plan.tile_tokens;
+  const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
+  p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
+  p.negate = a->scale < 0.f;
+  p.group_inv = (65536u + p.group - 1) / p.group;
+  p.work.parents = t->parents;
+  p.work.cluster = plan.cluster;
+  while (1 << (p.work.cluster_shift + 1) <= plan.cluster) ++p.work.cluster_shift;
+  const size_t rows = static_cast<size_t>(plan.grid) * 2 * kTreeRows;
+  p.work.part = static_cast<float4*>(a->workspace);
+  p.work.part_ml = reinterpret_cast<float2*>(p.work.part + rows * (a->kv.head_dim / 4));
+  p.work.spill = reinterpret_cast<int2*>(p.work.part_ml + rows);
+  p.work.pieces = reinterpret_cast<int32_t*>(p.work.spill + plan.grid);
+  CUtensorMap tm_k, tm_v;
+  if ((rc = page_map(&tm_k, a->kv, a->kv.k_pages, a->kv.k_page_stride, kTreeKeys)) != ABFT_OK) return rc;
+  if ((rc = page_map(&tm_v, a->kv, a->kv.v_pages, a->kv.v_page_stride, kTreeKeys)) != ABFT_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
+  if (a->kv.head_dim == 128)
+    return f16 ? launch_tree<128, true>(dev, 19, tm_k, tm_v, p, plan, sms, s)
+               : launch_tree<128, false>(dev, 18, tm_k, tm_v, p, plan, sms, s);
+  return f16 ? launch_tree<64, true>(dev, 17, tm_k, tm_v, p, plan, sms, s)
+             : launch_tree<64, false>(dev, 16, tm_k, tm_v, p, plan, sms, s);
 }
 
 bool overlap(const void* a, const void* b, size_t bytes) {
@@ -52,12 +157,18 @@ int abft_kv_append_at(const abft_kv_append_at_args* a, void* stream) {
   return append_call<true>(p, a->append.kv, sms, stream);
 }
 
-size_t abft_paged_tree_workspace_bytes(const abft_paged_tree_args* a) {
-  return a == nullptr ? 0 : abft_paged_prefill_workspace_bytes(&a->attn);
+size_t abft_paged_tree_workspace_bytes(const abft_paged_tree_args* t) {
+  if (t == nullptr) return 0;
+  const abft_paged_attn_args* a = &t->attn;
+  if (attn_check(a, false) != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return 0;
+  int dev = 0, sms = a->num_sms;
+  if (sms == 0 && paged_device(&dev, &sms) != ABFT_OK) sms = 148;
+  TreePlan plan;
+  return tree_plan(a, sms, &plan) == ABFT_OK ? tree_bytes(a, plan) : 0;
 }
 
-int abft_paged_tree(const abft_paged_tree_args* a, void* stream) {
-  return a == nullptr ? ABFT_ERR_INVALID_ARG : prefill_call<true>(&a->attn, a->parents, stream);
+int abft_paged_tree(const abft_paged_tree_args* t, void* stream) {
+  return t == nullptr ? ABFT_ERR_INVALID_ARG : tree_call(t, stream);
 }
 
 int abft_draft_accept(const abft_draft_accept_args* a, void* stream) {
@@ -111,10 +222,12 @@ int abft_kv_keep(const abft_kv_keep_args* a, void* stream) {
   p.cu = a->cu_seqlens, p.kept = a->kept, p.counts = a->counts;
   p.lens_out = a->lens_out;
   p.tokens = static_cast<int32_t>(a->tokens);
-  // A thread for each 16 bytes of a slot in all layers, as far as a cluster has them.
+  // A thread for each 16 bytes of a slot in all layers, as far as a cluster has them;
+  // half as many where that makes more CTAs than run at once (28 layers, CTAs of 512 /
+  // 256 threads: 1 sequence 3.4 / 3.9 us, 64 sequences 7.4 / 5.6).
   const int64_t columns = int64_t{2} * a->layers * a->kv.kv_heads * a->kv.head_dim / 8;
   for (p.cluster = 1; p.cluster < kKeepCluster && int64_t{p.cluster} * kKeepThreads < columns;) p.cluster *= 2;
-  const dim3 grid(a->kv.batch * p.cluster), block(kKeepThreads);
+  const dim3 grid(a->kv.batch * p.cluster), block(int64_t{a->kv.batch} * p.cluster > 3 * sms ? kKeepThreads / 2 : kKeepThreads);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return a->kv.head_dim == 128 ? launch_clusters(p.cluster, kv_keep_kernel<128>, grid, block, 0, s, p)
                                : launch_clusters(p.cluster, kv_keep_kernel<64>, grid, block, 0, s, p);

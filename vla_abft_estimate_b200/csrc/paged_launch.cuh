@@ -11,6 +11,7 @@
 #include "paged_append.cuh"
 #include "paged_decode.cuh"
 #include "paged_prefill.cuh"
+#include "paged_tree.cuh"
 
 namespace abft {
 
@@ -18,7 +19,7 @@ constexpr int kMaxDevices = 64;
 struct DeviceInfo {
   bool init, ok;
   int sms;
-  bool smem_set[24];  // decode instances 0-7, prefill 8-15, trees 16-23
+  bool smem_set[20];  // decode instances 0-7, prefill 8-15, trees 16-19
 };
 inline DeviceInfo g_paged_dev[kMaxDevices];
 inline std::mutex g_paged_mu;
@@ -300,9 +301,9 @@ inline EncodeTiledFn tile_encoder() {
 }
 
 // Map of a page pool: [page][group of 8 slots of a head][64-column block][slot
-// of the group][64 columns]; a box is one page's slots of one head, whole rows,
-// 128-byte swizzled.
-inline int page_map(CUtensorMap* m, const abft_paged_kv& c, const void* pages, int64_t stride) {
+// of the group][64 columns]; a box is one page's slots of one head (`most` of them
+// at most), whole rows, 128-byte swizzled.
+inline int page_map(CUtensorMap* m, const abft_paged_kv& c, const void* pages, int64_t stride, int most = 128) {
   EncodeTiledFn enc = tile_encoder();
   if (enc == nullptr) return ABFT_ERR_DRIVER;
   const int64_t dense = static_cast<int64_t>(c.kv_heads) * c.page_size * c.head_dim;
@@ -311,7 +312,7 @@ inline int page_map(CUtensorMap* m, const abft_paged_kv& c, const void* pages, i
   cuuint64_t dims[5] = {64, 8, static_cast<cuuint64_t>(c.head_dim / 64),
                         static_cast<cuuint64_t>(c.kv_heads) * c.page_size / 8, static_cast<cuuint64_t>(c.num_pages)};
   cuuint64_t strides[4] = {row, 128, 8 * row, static_cast<cuuint64_t>(stride) * 2};
-  cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(c.head_dim / 64), static_cast<cuuint32_t>(c.page_size / 8), 1};
+  cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(c.head_dim / 64), static_cast<cuuint32_t>((c.page_size < most ? c.page_size : most) / 8), 1};
   cuuint32_t es[5] = {1, 1, 1, 1, 1};
   const CUtensorMapDataType type =
       c.dtype == ABFT_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -371,13 +372,13 @@ inline size_t prefill_bytes(const abft_paged_attn_args* a, const PrefillPlan& pl
   return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2)) + (plan.choose ? 16 : 0);
 }
 
-template <int D, bool F16, bool kShared, bool kTree = false>
+template <int D, bool F16, bool kShared>
 int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                    const PrefillParams& p, int64_t items, cudaStream_t s) {
   using Cfg = PrefillCfg<D>;
-  int rc = raise_smem(dev, slot, paged_prefill_kernel<D, F16, kShared, kTree>, Cfg::kSmemBytes);
+  int rc = raise_smem(dev, slot, paged_prefill_kernel<D, F16, kShared>, Cfg::kSmemBytes);
   if (rc != ABFT_OK) return rc;
-  rc = launch(paged_prefill_kernel<D, F16, kShared, kTree>, dim3(static_cast<unsigned>(items)), dim3(kPreThreads), Cfg::kSmemBytes, s,
+  rc = launch(paged_prefill_kernel<D, F16, kShared>, dim3(static_cast<unsigned>(items)), dim3(kPreThreads), Cfg::kSmemBytes, s,
               tm_k, tm_v, p);
   if (rc != ABFT_OK || p.splits == 1) return rc;
   PrefillJoinParams j;
@@ -397,64 +398,6 @@ int launch_prefill(int dev, int slot, const abft_paged_attn_args* a, const CUten
   const unsigned rows = static_cast<unsigned>(p.tokens) * a->heads;
   return launch(paged_prefill_join_kernel<D, F16>, dim3((rows + kPreJoinWarps - 1) / kPreJoinWarps),
                 dim3(32 * kPreJoinWarps), 0, s, j);
-}
-
-// The causal call, or that of trees (`parents`: each row's).
-template <bool kTree>
-int prefill_call(const abft_paged_attn_args* a, const int32_t* parents, void* stream) {
-  int rc = attn_check(a, false);
-  if (rc != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return rc;
-  if (kTree && parents == nullptr) return ABFT_ERR_INVALID_ARG;
-  int dev = 0, sms = 0;
-  if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
-  if (a->num_sms > 0) sms = a->num_sms;
-  PrefillParams p;
-  p.kv = view_of(a->kv);
-  p.q = a->q, p.out = a->out;
-  p.qt = a->q_token_stride, p.qh = a->q_head_stride;
-  p.ot = a->o_token_stride, p.oh = a->o_head_stride;
-  p.cu = a->cu_seqlens;
-  p.parents = parents;
-  p.tokens = static_cast<int32_t>(a->tokens);
-  p.group = a->heads / a->kv.kv_heads;
-  const PrefillPlan plan = prefill_plan(a, sms);
-  if (plan.items >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
-  p.tile_tokens = plan.tile_tokens;
-  p.block_tokens = plan.block_tokens;
-  p.splits = plan.splits;
-  p.piece = plan.choose ? 0 : plan.piece;
-  p.sms = sms;
-  const float s2 = fabsf(a->scale) * 1.44269504088896340736f;
-  p.scale_log2 = s2 > 1e-30f ? s2 : 1e-30f;  // scale 0: every visible weight 2^0, masked scores still -inf
-  p.negate = a->scale < 0.f;
-  p.group_inv = (65536u + p.group - 1) / p.group;
-  const size_t need = prefill_bytes(a, plan);
-  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ABFT_ERR_WORKSPACE;
-  if (need > 0 && off16(a->workspace)) return ABFT_ERR_ALIGNMENT;
-  p.part_o = static_cast<float*>(a->workspace);
-  p.part_ml = reinterpret_cast<float2*>(
-      p.part_o + static_cast<size_t>(a->tokens) * a->heads * p.splits * a->kv.head_dim);
-  p.chosen = plan.choose ? reinterpret_cast<int32_t*>(p.part_ml + static_cast<size_t>(a->tokens) * a->heads * p.splits)
-                         : nullptr;
-  CUtensorMap tm_k, tm_v;
-  if ((rc = page_map(&tm_k, a->kv, a->kv.k_pages, a->kv.k_page_stride)) != ABFT_OK) return rc;
-  if ((rc = page_map(&tm_v, a->kv, a->kv.v_pages, a->kv.v_page_stride)) != ABFT_OK) return rc;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
-  const bool shared = plan.block_tokens == plan.tile_tokens;
-  const int slot = (a->kv.head_dim == 128 ? 4 : 0) + (f16 ? 2 : 0) + (shared ? 1 : 0);
-  const int64_t items = plan.items;
-  const int at = slot + (kTree ? 16 : 8);
-  switch (slot) {
-    case 0: return launch_prefill<64, false, false, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-    case 1: return launch_prefill<64, false, true, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-    case 2: return launch_prefill<64, true, false, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-    case 3: return launch_prefill<64, true, true, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-    case 4: return launch_prefill<128, false, false, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-    case 5: return launch_prefill<128, false, true, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-    case 6: return launch_prefill<128, true, false, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-    default: return launch_prefill<128, true, true, kTree>(dev, at, a, tm_k, tm_v, p, items, s);
-  }
 }
 
 }  // namespace abft

@@ -117,7 +117,6 @@ struct PrefillParams {
   float scale_log2;        // |scale| * log2(e), never 0
   int32_t negate;          // scale < 0
   uint32_t group_inv;      // ceil(2^16 / group): row_token()
-  const int32_t* parents;  // trees: [tokens], each row's parent among its sequence's rows, or -1
   float* part_o;           // [tokens * heads][splits][head_dim]
   float2* part_ml;         // [tokens * heads][splits]
 };
@@ -414,34 +413,9 @@ __device__ __forceinline__ int work_answer(const void* answer) {
   return ok ? static_cast<int>(x) : -1;
 }
 
-// What a tree's row sees of a step's 128 slots, 32 to a word: every slot before
-// the drafted ones (`base` of them from the step's first on, may be negative or
-// beyond), and of those the row's own and its ancestors'. The walk up ends at the
-// root, at a parent that does not come before its child, or before the step.
-__device__ __forceinline__ void tree_words(const int32_t* parents, int own, int base, uint32_t (&w)[4]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int below = base - c * 32;
-    w[c] = below >= 32 ? 0xFFFFFFFFu : below > 0 ? (1u << below) - 1u : 0u;
-  }
-  int row = own;
-  while (row >= 0 && base + row >= 0) {
-    const int key = base + row;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (key >> 5 == c) w[c] |= 1u << (key & 31);
-    const int up = __ldg(parents + row);
-    row = up < row ? up : -1;
-  }
-}
-
-// kTree: query rows are a tree's (each sequence's new tokens): row i sees the
-// slots before the new ones, its own and its ancestors'. Parents come before
-// their children, so what a causal row sees bounds what this one does.
-//
 // kShared: one tile an item, its steps shared by both groups of row warps. (A
 // template argument: asked at run time it cost the two-tile form 2.5%.)
-template <int D, bool F16, bool kShared, bool kTree = false>
+template <int D, bool F16, bool kShared>
 __global__ void __launch_bounds__(kPreThreads, 1)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                          const PrefillParams p) {
@@ -609,25 +583,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
             for (int k = 0; k < 32; ++k) s[c][k] ^= 0x80000000u;
         }
-        if constexpr (kTree) {
-          const int base = x.len - x.n - j * kPreKeys;  // the step's slots before the drafted ones
-          if (base < kPreKeys) {
-            const int first = x.tok0 + tile * p.tile_tokens, own = first + row_token(row_of_thread(), p.group_inv);
-            const int32_t* parents = p.parents + x.row0;
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-            if (vis > 0) tree_words(parents, own, base, w);
-            // A row's own slot is in one step and one piece: there its parent is looked at.
-            if (vis > 0 && base + own >= 0 && base + own < kPreKeys) {
-              const int up = parents[own];
-              if ((up < -1 || up >= own) && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_DRAFT);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (!(w[c] >> k & 1u)) s[c][k] = 0xFF800000u;  // -inf
-          }
-        } else if (vis_min < (j + 1) * kPreKeys) {
+        if (vis_min < (j + 1) * kPreKeys) {
           const int lim = vis - j * kPreKeys;
 #pragma unroll
           for (int c = 0; c < 4; ++c)

@@ -426,14 +426,15 @@ class PagedKVCache:
         return self._attention(True, q, cu_seqlens, scale, out, num_splits, 0)
 
     def tree(self, q: torch.Tensor, cu_seqlens: torch.Tensor, parents: torch.Tensor, *, scale: Optional[float] = None,
-             out: Optional[torch.Tensor] = None, num_splits: int = 0) -> torch.Tensor:
+             out: Optional[torch.Tensor] = None, num_sms: int = 0) -> torch.Tensor:
         """Attention of a tree of drafted tokens for each sequence: rows as in
         ``prefill``, but row i of n sees the slots before the n new ones, its
         own and its ancestors'. ``parents`` int32 [tokens]: the place of row
         i's parent among its sequence's new rows, below i, or -1 for none (a row
         that follows the cached tokens directly; there may be several). Trees of
-        any size, one row included. Everything else is as in ``prefill``."""
-        return self._attention(True, q, cu_seqlens, scale, out, num_splits, 0, parents, True)
+        any size, one row included. Everything else is as in ``prefill``;
+        ``num_sms`` as in ``decode``."""
+        return self._attention(True, q, cu_seqlens, scale, out, 0, num_sms, parents, True)
 
     def _attention(self, prefill, q, cu, scale, out, num_splits, num_sms, parents=None, tree=False):
         if tree:
