@@ -545,7 +545,8 @@ int abft_kv_append_at(const abft_kv_append_at_args* args, void* stream);
 /* Tree attention: query row i of the n new tokens of sequence b sees the slots
  * before the new ones (j < seq_lens[b] - n), its own and its ancestors'.
  * Everything else is as for abft_paged_prefill, but for num_splits, which is not
- * used (the call's work is shared out to num_sms SMs). A parent that is below -1 or
+ * used (the call's work is shared out to num_sms SMs), and q's strides, which are
+ * above 0 where there is more than one row or head. A parent that is below -1 or
  * does not come before its child sets ABFT_PAGED_BAD_DRAFT; the way up ends
  * there. */
 typedef struct abft_paged_tree_args {

@@ -46,6 +46,7 @@ def _tree(kv):
     a = N.PagedTreeArgs()
     x = a.attn
     x.kv, x.q, x.out, x.tokens, x.heads, x.scale, x.cu_seqlens, x.num_sms = kv, 0x50000, 0x60000, 2, 28, 0.1, 0x70000, 148
+    x.q_token_stride, x.q_head_stride, x.o_token_stride, x.o_head_stride = 28 * 128, 128, 28 * 128, 128
     a.parents = 0x80000
     return a
 
@@ -128,7 +129,8 @@ def test_append_refusals():
 def test_tree_refusals():
     for over, code in [({"parents": None}, -1), ({"attn.cu_seqlens": None}, -1), ({"attn.tokens": -1}, -1),
                        ({"attn.num_splits": -1}, -1), ({"attn.num_sms": 5000}, -3), ({"attn.scale": float("nan")}, -1),
-                       ({"attn.heads": 4 * 65}, -3), ({"attn.q": 0x50008}, -2), ({"attn.o_head_stride": 2}, -2),
+                       ({"attn.heads": 4 * 65}, -3), ({"attn.q": 0x50008}, -2), ({"attn.q_head_stride": 0}, -1),
+                       ({"attn.q_token_stride": 0}, -1), ({"attn.q_token_stride": -8}, -1), ({"attn.o_head_stride": 2}, -2),
                        ({"attn.tokens": 1 << 30}, -3)]:
         assert _call("abft_paged_tree", _set(_tree(_kv()), over)) == code, over
     assert _call("abft_paged_tree", _set(_tree(_kv()), {"attn.tokens": 0})) == 0

@@ -231,6 +231,25 @@ def test_large_pools_and_rows(cuda_device):
     close(got, *attention_over(pool, q, [(0, visible_slots(tree, i, 50)) for i in range(21)]))
 
 
+def test_repeated_and_transposed_query_rows(cuda_device):
+    """One row for all heads or tokens, heads before tokens: the same as their dense copies."""
+    dev = cuda_device
+    cache = Pool([90, 40], 2, 16, 64, BF16).device_cache(dev, PagedKVCache)
+    cu, parents = packed([random_tree(20, 1), random_tree(7, 2)])
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(27, 6, 64, generator=g).to(BF16).to(dev)
+    for q in (x[:, :1].expand(27, 6, 64), x[:1].expand(27, 6, 64), x.transpose(0, 1).contiguous().transpose(0, 1),
+              torch.nn.functional.pad(x, (0, 8))[..., :64], x.flip(0), x.new_zeros(27 * 6 * 64 + 1)[1:].view(27, 6, 64).copy_(x)):
+        got = cache.tree(q, i32(cu, dev), i32(parents, dev))
+        assert torch.equal(got, cache.tree(q.clone(memory_format=torch.contiguous_format), i32(cu, dev), i32(parents, dev)))
+    cache.check_status()
+
+
+@pytest.mark.parametrize("n", [511, 512, 513, 700])
+def test_trees_around_the_parents_that_are_held(cuda_device, n):
+    run_tree(cuda_device, [random_tree(n, 1), chain(n), random_tree(3, 2)], [n + 130, n, 70], 2, 1, 64, 16, BF16)
+
+
 def test_refusals(cuda_device):
     dev = cuda_device
     cache = Pool([40], 2, 16, 64, BF16).device_cache(dev, PagedKVCache)

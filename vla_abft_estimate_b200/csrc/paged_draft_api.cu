@@ -62,14 +62,34 @@ size_t tree_bytes(const abft_paged_attn_args* a, const TreePlan& plan) {
   return rows * (a->kv.head_dim * sizeof(float) + sizeof(float2)) + plan.grid * (sizeof(int2) + sizeof(int32_t));
 }
 
+// Map of the query rows: [token][head][head_dim]; a box is the (token, head) rows of a
+// tile and 64 columns, 128-byte swizzled.
+int query_map(CUtensorMap* m, const abft_paged_attn_args* a, int tile_tokens) {
+  EncodeTiledFn enc = tile_encoder();
+  if (enc == nullptr) return ABFT_ERR_DRIVER;
+  const cuuint64_t row = static_cast<cuuint64_t>(a->kv.head_dim) * 2;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(a->kv.head_dim), static_cast<cuuint64_t>(a->heads),
+                        static_cast<cuuint64_t>(a->tokens)};
+  // (The stride of a dimension of one is not used, but has to be a valid one.)
+  cuuint64_t strides[2] = {a->heads > 1 ? static_cast<cuuint64_t>(a->q_head_stride) * 2 : row,
+                           a->tokens > 1 ? static_cast<cuuint64_t>(a->q_token_stride) * 2 : row};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a->heads / a->kv.kv_heads), static_cast<cuuint32_t>(tile_tokens)};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUtensorMapDataType type =
+      a->kv.dtype == ABFT_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = enc(m, type, 3, const_cast<void*>(a->q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ABFT_OK : ABFT_ERR_ALIGNMENT;
+}
+
 template <int D, bool F16>
-int launch_tree(int dev, int slot, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const TreeParams& p, const TreePlan& plan,
-                int sms, cudaStream_t s) {
+int launch_tree(int dev, int slot, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const CUtensorMap& tm_q,
+                const TreeParams& p, const TreePlan& plan, int sms, cudaStream_t s) {
   using Cfg = TreeCfg<D>;
   int rc = raise_smem(dev, slot, paged_tree_kernel<D, F16>, Cfg::kSmemBytes);
   if (rc != ABFT_OK) return rc;
   rc = launch_clusters(p.work.cluster, paged_tree_kernel<D, F16>, dim3(plan.grid), dim3(kTreeThreads), Cfg::kSmemBytes, s, tm_k,
-                       tm_v, p);
+                       tm_v, tm_q, p);
   if (rc != ABFT_OK || p.work.cluster > 0) return rc;
   return launch(paged_tree_join_kernel<D, F16>, dim3(4 * sms), dim3(kTreeJoinThreads), 0, s, p, plan.grid);
 }
@@ -79,6 +99,8 @@ int tree_call(const abft_paged_tree_args* t, void* stream) {
   int rc = attn_check(a, false);
   if (rc != ABFT_OK || a->kv.batch == 0 || a->tokens == 0) return rc;
   if (t->parents == nullptr) return ABFT_ERR_INVALID_ARG;
+  // Query rows come as boxes of a tensor, whose strides are above 0.
+  if ((a->heads > 1 && a->q_head_stride <= 0) || (a->tokens > 1 && a->q_token_stride <= 0)) return ABFT_ERR_INVALID_ARG;
   int dev = 0, sms = 0;
   if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
   if (a->num_sms > 0) sms = a->num_sms;
@@ -108,16 +130,17 @@ int tree_call(const abft_paged_tree_args* t, void* stream) {
   p.work.part_ml = reinterpret_cast<float2*>(p.work.part + rows * (a->kv.head_dim / 4));
   p.work.spill = reinterpret_cast<int2*>(p.work.part_ml + rows);
   p.work.pieces = reinterpret_cast<int32_t*>(p.work.spill + plan.grid);
-  CUtensorMap tm_k, tm_v;
+  CUtensorMap tm_k, tm_v, tm_q;
+  if ((rc = query_map(&tm_q, a, plan.tile_tokens)) != ABFT_OK) return rc;
   if ((rc = page_map(&tm_k, a->kv, a->kv.k_pages, a->kv.k_page_stride, kTreeKeys)) != ABFT_OK) return rc;
   if ((rc = page_map(&tm_v, a->kv, a->kv.v_pages, a->kv.v_page_stride, kTreeKeys)) != ABFT_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = a->kv.dtype == ABFT_DTYPE_F16;
   if (a->kv.head_dim == 128)
-    return f16 ? launch_tree<128, true>(dev, 19, tm_k, tm_v, p, plan, sms, s)
-               : launch_tree<128, false>(dev, 18, tm_k, tm_v, p, plan, sms, s);
-  return f16 ? launch_tree<64, true>(dev, 17, tm_k, tm_v, p, plan, sms, s)
-             : launch_tree<64, false>(dev, 16, tm_k, tm_v, p, plan, sms, s);
+    return f16 ? launch_tree<128, true>(dev, 19, tm_k, tm_v, tm_q, p, plan, sms, s)
+               : launch_tree<128, false>(dev, 18, tm_k, tm_v, tm_q, p, plan, sms, s);
+  return f16 ? launch_tree<64, true>(dev, 17, tm_k, tm_v, tm_q, p, plan, sms, s)
+             : launch_tree<64, false>(dev, 16, tm_k, tm_v, tm_q, p, plan, sms, s);
 }
 
 bool overlap(const void* a, const void* b, size_t bytes) {

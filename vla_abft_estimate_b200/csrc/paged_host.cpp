@@ -200,7 +200,7 @@ PyObject* attend(const Calls* c, int which, PyObject* q_, PyObject* cu_, PyObjec
   }
   if (which == 2) {
     const at::Tensor* parents = tensor_of(parents_);
-    if (c->tree == nullptr || !list_of(c->device, parents, q->size(0), at::kInt)) Py_RETURN_NONE;
+    if (c->tree == nullptr || repeats(q) || !list_of(c->device, parents, q->size(0), at::kInt)) Py_RETURN_NONE;
     tree.parents = static_cast<const int32_t*>(parents->const_data_ptr());
   }
   double scale = 1.0 / sqrt(static_cast<double>(c->kv.head_dim));

@@ -31,7 +31,7 @@
 // through shared memory in the one launch.
 //
 // Warps: 0-3 the rows (TMEM lane quadrant = warp), 4 TMA loads of pages into a ring
-// of tiles, 5 the MMA issuer, 6 finds the work, 7 brings the query rows.
+// of tiles, 5 the MMA issuer, 6 finds the work, 7 brings query rows and parents.
 #pragma once
 
 #include <cuda.h>
@@ -43,6 +43,9 @@ namespace abft {
 constexpr int kTreeRows = kPreRows;  // query rows of a tile
 constexpr int kTreeKeys = 64;        // keys of a step
 constexpr int kTreeThreads = 256;
+// Parents that are held in shared memory, where the walk up a tree takes a tenth of
+// the time; those of larger trees are read where they are.
+constexpr int kTreeHeld = 512;
 
 template <int D>
 struct TreeCfg {
@@ -53,11 +56,12 @@ struct TreeCfg {
   static constexpr int kSlots = D == 128 ? 4 : 8;
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffBar = kOffRing + kSlots * kTileBytes;
-  // full, empty, sfull, pfull, ofull, item full and empty, qfull, qempty, drain, one unused (an even number)
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 4 + 4;
+  // full, empty, sfull, pfull, ofull, item full and empty, upfull, qfull, qempty, drain, one unused (an even number)
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 4 + 2 + 4;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kOffItems = kOffMisc + 16;
-  static constexpr int kSmemBytes = kOffItems + 2 * 48 + 1024;
+  static constexpr int kOffUp = kOffItems + 2 * 48;  // parents of the items in the two slots
+  static constexpr int kSmemBytes = kOffUp + 2 * kTreeHeld * 4 + 1024;
   // A cluster's pieces take the ring's place: O as [D / 4][rows] float4, then (m, l).
   static_assert(kTreeRows * (D * 4 + 8) <= kQBytes + kSlots * kTileBytes, "a piece's place");
   static_assert(kSmemBytes <= 115 * 1024, "two CTAs per SM");
@@ -115,7 +119,7 @@ __device__ __forceinline__ void tree_words(const int32_t* parents, int own, int 
     const int key = base + row;
     if (key < 32) w[0] |= 1u << key;
     if (key >= 32 && key < 64) w[1] |= 1u << (key & 31);
-    const int up = __ldg(parents + row);
+    const int up = parents[row];
     row = up < row ? up : -1;
   }
 }
@@ -249,6 +253,12 @@ __device__ __forceinline__ void tree_locate(const TreeParams& p, int lane, TreeS
   }
 }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint64_t* bar, int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -369,17 +379,22 @@ __device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const Tre
     uint16_t* dst = tree_out(p, x.row0 + x.tok0, x.hk, r, token);
 #pragma unroll 1
     for (int col = rank * kSides + threadIdx.x / kTreeRows; col < D / 8; col += p.work.cluster * kSides) {
+      float4 v[kDecCluster][2];  // all asked for before the first is used
+#pragma unroll
+      for (int c = 0; c < kDecCluster; ++c)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (c < p.work.cluster) v[c][k] = ld_cluster_f4(map_rank(area + ((col * 2 + k) * kTreeRows + r) * 16, c));
       float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < kDecCluster; ++c) {
-        if (c >= p.work.cluster || ml[c].x == 0.f) continue;
+        if (c >= p.work.cluster || ml[c].x == 0.f) continue;  // not written
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float4 v = ld_cluster_f4(map_rank(area + ((col * 2 + k) * kTreeRows + r) * 16, c));
-          o[k].x += v.x * ml[c].x;
-          o[k].y += v.y * ml[c].x;
-          o[k].z += v.z * ml[c].x;
-          o[k].w += v.w * ml[c].x;
+          o[k].x += v[c][k].x * ml[c].x;
+          o[k].y += v[c][k].y * ml[c].x;
+          o[k].z += v[c][k].z * ml[c].x;
+          o[k].w += v[c][k].w * ml[c].x;
         }
       }
       tree_store8<F16>(dst + col * 8, o[0], o[1], inv);
@@ -390,7 +405,8 @@ __device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const Tre
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(kTreeThreads, 2)
-    paged_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TreeParams p) {
+    paged_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const __grid_constant__ CUtensorMap tm_q, const TreeParams p) {
   using Cfg = TreeCfg<D>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -401,12 +417,14 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
   uint64_t* ofull = pfull + 2;
   uint64_t* item_full = ofull + 2;
   uint64_t* item_empty = item_full + 2;
-  uint64_t* qfull = item_empty + 2;
+  uint64_t* upfull = item_empty + 2;
+  uint64_t* qfull = upfull + 2;
   uint64_t* qempty = qfull + 1;
   uint64_t* drain = qempty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   TreeItem* items = reinterpret_cast<TreeItem*>(smem + Cfg::kOffItems);
+  int32_t* held = reinterpret_cast<int32_t*>(smem + Cfg::kOffUp);  // [2][kTreeHeld]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedView& kv = p.kv;
@@ -421,14 +439,16 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
       mbar_init(&ofull[t], 1);
       mbar_init(&item_full[t], 1);
       mbar_init(&item_empty[t], 7);  // a lane of each row warp, the loader's, the issuer's and that of the query rows
+      mbar_init(&upfull[t], 1);
     }
-    mbar_init(qfull, 32);
+    mbar_init(qfull, 1);
     mbar_init(qempty, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_q);
   }
   if (warp == 5) {
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
@@ -441,7 +461,12 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
   griddep_wait();
   griddep_launch();
 
-  // The i-th item of this CTA, copied out of its slot.
+  // The i-th item of this CTA, copied out of its slot. (The rows give the slot free
+  // when they are done: its parents stay until then.)
+  auto free_slot = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[i & 1]);
+  };
   auto get_item = [&](int i, TreeItem* x) {
     const bool got = __all_sync(0xFFFFFFFFu, mbar_wait(&item_full[i & 1], (i >> 1) & 1, abort_flag));
     if (!got) {
@@ -449,8 +474,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
       return false;
     }
     *x = items[i & 1];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&item_empty[i & 1]);
+    if (warp >= 4) free_slot(i);
     return x->valid != 0;
   };
 
@@ -477,6 +501,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
       // A warp without rows only keeps step: what the products make of its lanes nobody
       // reads (exponentials are a step's longest part, and a tile may have few rows).
       const bool used = __any_sync(0xFFFFFFFFu, live);
+      bool parents_there = false;
       float m = -INFINITY, l = 0.f;  // m: maximum that P refers to (raw scores)
       for (int j = x.j0; j < x.j1; ++j, ++count) {
         const uint32_t ts = lanes + (count & 1) * 64;
@@ -501,12 +526,16 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
         const int base = x.len - x.n - j * kTreeKeys;  // of the step's slots those before the drafted ones
         if (base < kTreeKeys) {
           uint32_t w[2] = {0u, 0u};
+          if (!parents_there) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&upfull[i & 1], (i >> 1) & 1, abort_flag)) && ok;
+            parents_there = true;
+          }
           if (live && own >= x.n - x.len) {  // of more rows than tokens the first have no slots and see none
-            const int32_t* parents = p.work.parents + x.row0;
+            const int32_t* parents = x.n <= kTreeHeld ? held + (i & 1) * kTreeHeld : p.work.parents + x.row0;
             tree_words(parents, own, base, w);
             // A row's own slot is in one step and one piece: there its parent is looked at.
             if (base + own >= 0 && base + own < kTreeKeys) {
-              const int up = __ldg(parents + own);
+              const int up = parents[own];
               if ((up < -1 || up >= own) && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_DRAFT);
             }
           }
@@ -576,7 +605,10 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
         ok = summed(count - 1);
         if (!ok) break;
       }
-      if (!used) continue;
+      if (!used) {
+        free_slot(i);
+        continue;
+      }
       // Sums of a piece go to its place, or, for the cluster, to that of the ring (which
       // nothing is loaded into any more).
       const int64_t place = static_cast<int64_t>(blockIdx.x) * 2 + max(x.place, 0);
@@ -614,6 +646,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
         }
       }
       tc_fence_before();  // O is read before the next item's first P is announced
+      free_slot(i);
     }
     tc_fence_before();
   } else if (warp == 4) {
@@ -765,34 +798,33 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
   } else if (warp == 6) {
     list_tree(p, items, item_full, item_empty, abort_flag, lane);
   } else {
-    // ------------------------------------------------------------ query rows
-    // Into shared memory, in the swizzled layout of a TMA box, once the last item's
-    // scores have all been computed.
-    constexpr int kCpr = D / 8, kRowsAtOnce = 32 / kCpr;
-    const int c = lane % kCpr;
+    // ------------------------------------------------------------ query rows and parents
+    // Query rows by one box for each 64 columns, (token, head) rows of the tile, once
+    // the last item's scores have all been computed; rows behind the sequence's are
+    // another's, which nobody reads the sums of.
     int brought = 0;
     bool ok = true;
     TreeItem x;
     for (int i = 0; ok && get_item(i, &x); ++i) {
-      if (x.j0 >= x.j1) continue;
-      if (brought > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(qempty, (brought - 1) & 1, abort_flag));
-      if (!ok) break;
-      ++brought;
-      const int here = min(p.tile_tokens, x.n - x.tok0) * p.group;
-      const uint32_t dst = smem_u32(smem);
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (x.row0 + static_cast<int64_t>(x.tok0)) * p.qt +
-                            x.hk * p.group * p.qh + c * 8;
-#pragma unroll 4
-      for (int row = lane / kCpr; row < here; row += kRowsAtOnce) {
-        const int token = row_token(row, p.group_inv);
-        cp_async16(dst + (c >> 3) * Cfg::kBlockBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
-                   src + token * p.qt + (row - token * p.group) * p.qh, 16u);
+      if (x.j0 < x.j1) {
+        if (brought > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(qempty, (brought - 1) & 1, abort_flag));
+        if (!ok) break;
+        ++brought;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(qfull, static_cast<uint32_t>(p.tile_tokens * p.group * D * 2));
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_3d(smem_u32(smem) + c * Cfg::kBlockBytes, &tm_q, qfull, c * 64, x.hk * p.group, x.row0 + x.tok0);
+        }
+        __syncwarp();
+        if (x.n <= kTreeHeld && x.j1 * kTreeKeys > x.len - x.n)
+          for (int k = lane; k < x.n; k += 32) held[(i & 1) * kTreeHeld + k] = p.work.parents[x.row0 + k];
       }
-      cp_async_commit();
-      cp_async_wait<0>();
-      fence_proxy_async_smem();
-      mbar_arrive(qfull);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&upfull[i & 1]);
     }
+    // The last copy has landed before shared memory goes (it has, but after an abort).
+    if (brought > 0) mbar_wait_bounded(qfull, (brought - 1) & 1);
   }
   __syncthreads();
   if (p.work.cluster > 0 && items[0].valid) join_tree_cluster<D, F16>(p, items[0], smem_u32(smem));

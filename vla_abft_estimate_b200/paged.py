@@ -463,6 +463,8 @@ class PagedKVCache:
             if parents.shape[0] != q.shape[0]:
                 raise ValueError(f"parents must have an entry for each of the {q.shape[0]} rows, got {parents.shape[0]}")
             call.parents = parents.data_ptr()
+            if any(st == 0 and size > 1 for st, size in zip(q.stride(), q.shape)):
+                q = q.clone(memory_format=torch.contiguous_format)  # read as boxes of a tensor that does not repeat itself
         out = self._result("out", out, q)
         args.q, args.out, args.tokens, args.heads = q.data_ptr(), out.data_ptr(), q.shape[0], q.shape[1]
         args.q_token_stride, args.q_head_stride, _ = q.stride()
