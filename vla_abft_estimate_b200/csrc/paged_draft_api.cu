@@ -24,15 +24,17 @@ struct TreePlan {
   int grid;
 };
 
-// Short caches get a cluster of up to 8 CTAs per segment, as long as all clusters
-// run at once (two CTAs an SM; 8 x 30 and 4 x 65 fit the device's groups of SMs) and a
-// CTA has no more than 12 steps, or 16 where the list would cut each segment into
-// more than 24 pieces. Measured (28/4 heads of 128; cluster / list): 1 tree of 16 tokens
-// on 1,000 slots 11.7 / 13.7 us, 4,000 15.6 / 21.9, 8,000 (16 steps) 21.9 / 26.5; 1 of
-// 64 on 2,000 15.5 / 18.2, on 8,000 (16 steps, 18 pieces) 26.8 / 23.9; 16 of 16 on
-// 500 15.7 / 19.7; 32 of 8 on 600 20.5 / 23.1, on 1,200 (20 steps) 29.1 / 29.3. (The
-// lengths are on the device: what is known here, and decides, is the width of the
-// table.)
+// Short caches get a CTA per segment, or a cluster of up to 8 as long as all clusters
+// run at once (two CTAs an SM; 8 x 30 and 4 x 65 fit the device's groups of SMs). A
+// step takes 0.75 us, the join of a cluster 2.2, a second launch with its join 6 and
+// more the more pieces a segment has: one CTA up to 4 steps, or 16 where there are
+// segments for half of the CTAs; 12 steps for each CTA of a cluster, 16 where the list
+// would cut each segment into more than 24 pieces. Measured (28/4 heads of 128; one CTA
+// / cluster / list): 1 tree of 16 tokens on 112 slots 7.7 / 9.2 / - us, on 512
+// 12.7 / 9.6 / -, on 1,000 - / 10.3 / 13.7, on 4,000 - / 14.4 / 21.9, on 8,000 (16
+// steps a CTA) - / 20.8 / 26.5; 1 of 64 on 8,000 (16 steps, 18 pieces) - / 26.8 / 22.9;
+// 32 of 8 on 300 slots 10.9 / - / 18.8, on 1,000 21.6 / - / 27. (The lengths are on
+// the device: what is known here, and decides, is the width of the table.)
 int tree_plan(const abft_paged_attn_args* a, int sms, TreePlan* r) {
   r->tile_tokens = kTreeRows / (a->heads / a->kv.kv_heads);
   // Segments at most (the boundaries are on the device), and steps of one.
@@ -46,7 +48,8 @@ int tree_plan(const abft_paged_attn_args* a, int sms, TreePlan* r) {
   if (segments <= ctas) {
     int c = 8 * segments <= ctas * 13 / 16 ? 8 : 4 * segments <= ctas * 7 / 8 ? 4 : 2 * segments <= ctas ? 2 : 1;
     while (c > 1 && c / 2 >= steps) c /= 2;
-    if (steps <= (24 * segments <= ctas ? 16 : 12) * c) {
+    if (steps <= 4) c = 1;
+    if (steps <= (c == 1 || 24 * segments <= ctas ? 16 : 12) * c) {
       r->cluster = c;
       r->grid = static_cast<int>(segments) * c;
       return ABFT_OK;

@@ -76,7 +76,7 @@ constexpr int kTreeCost = 4;
 
 struct TreeWork {
   const int32_t* parents;  // [tokens]
-  int32_t cluster;         // CTAs of a segment (a cluster), no pieces in memory, no second kernel; 0: the list
+  int32_t cluster;         // CTAs of a segment (a cluster, or one), no pieces in memory, no second kernel; 0: the list
   int32_t cluster_shift;   // log2 of it
   // Pieces of segments that cross CTAs: each CTA has place 0 for one that began
   // earlier, place 1 for one that goes on. Rows are the fastest index: a thread has
@@ -295,7 +295,7 @@ __device__ __forceinline__ void list_tree(const TreeParams& p, TreeItem* items, 
     if (x.valid) {
       const int end = min(at.seq.steps, at.step + (at.u1 - at.u));
       x.hk = at.seq.tiles == 1 ? at.y : at.y / at.seq.tiles;
-      x.place = single || at.step > 0 ? 0 : end < at.seq.steps ? 1 : -1;
+      x.place = p.work.cluster > 1 || at.step > 0 ? 0 : end < at.seq.steps ? 1 : -1;
       x.seq = at.b;
       x.len = at.seq.len;
       x.row0 = at.seq.row0;
@@ -352,55 +352,53 @@ __device__ __forceinline__ void tree_store8(uint16_t* dst, const float4& a, cons
 }
 
 // The pieces of a cluster's CTAs, in their order; each CTA joins every cluster-th
-// pair of 8 columns, a thread a row.
+// pair of 8 columns, a thread a row. (The second barrier orders nothing but the end of
+// the reads: with the release of the results' stores in it, it took 1.5 us.)
 template <int D, bool F16>
 __device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const TreeItem& x, uint32_t area) {
   cluster_barrier();
   constexpr int kSides = kTreeThreads / kTreeRows;
   const int r = threadIdx.x & (kTreeRows - 1), rank = static_cast<int>(blockIdx.x) & (p.work.cluster - 1);
   const int token = row_token(r, p.group_inv);
-  if (token < min(p.tile_tokens, x.n - x.tok0)) {
-    float2 ml[kDecCluster];
-    float top = -INFINITY;
+  const bool live = token < min(p.tile_tokens, x.n - x.tok0);
+  float4 v[kDecCluster][2];
+  float2 ml[kDecCluster];
+  uint16_t* dst = tree_out(p, x.row0 + x.tok0, x.hk, r, token);
+#pragma unroll 1
+  for (int col = rank * kSides + threadIdx.x / kTreeRows; col < D / 8; col += p.work.cluster * kSides) {
+    if (!live) break;
+    // All asked for before the first is used.
 #pragma unroll
     for (int c = 0; c < kDecCluster; ++c) {
       ml[c] = make_float2(-INFINITY, 0.f);
-      if (c < p.work.cluster) ml[c] = ld_cluster_f2(map_rank(area + kTreeRows * D * 4 + r * 8, c));
-      top = fmaxf(top, ml[c].x);
+      if (c < p.work.cluster) {
+        ml[c] = ld_cluster_f2(map_rank(area + kTreeRows * D * 4 + r * 8, c));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[c][k] = ld_cluster_f4(map_rank(area + ((col * 2 + k) * kTreeRows + r) * 16, c));
+      }
     }
+    float top = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int c = 0; c < kDecCluster; ++c) top = fmaxf(top, ml[c].x);
     const float ms = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
+    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll
     for (int c = 0; c < kDecCluster; ++c) {
-      ml[c].x = ml[c].y == 0.f ? 0.f : exp2_approx(ml[c].x - ms);  // 0: no piece, or the row saw nothing of it
-      l += ml[c].y * ml[c].x;
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    uint16_t* dst = tree_out(p, x.row0 + x.tok0, x.hk, r, token);
-#pragma unroll 1
-    for (int col = rank * kSides + threadIdx.x / kTreeRows; col < D / 8; col += p.work.cluster * kSides) {
-      float4 v[kDecCluster][2];  // all asked for before the first is used
+      if (ml[c].y == 0.f) continue;  // no piece, or the row saw nothing of it: not written
+      const float f = exp2_approx(ml[c].x - ms);
+      l += ml[c].y * f;
 #pragma unroll
-      for (int c = 0; c < kDecCluster; ++c)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (c < p.work.cluster) v[c][k] = ld_cluster_f4(map_rank(area + ((col * 2 + k) * kTreeRows + r) * 16, c));
-      float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll
-      for (int c = 0; c < kDecCluster; ++c) {
-        if (c >= p.work.cluster || ml[c].x == 0.f) continue;  // not written
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          o[k].x += v[c][k].x * ml[c].x;
-          o[k].y += v[c][k].y * ml[c].x;
-          o[k].z += v[c][k].z * ml[c].x;
-          o[k].w += v[c][k].w * ml[c].x;
-        }
+      for (int k = 0; k < 2; ++k) {
+        o[k].x += v[c][k].x * f;
+        o[k].y += v[c][k].y * f;
+        o[k].z += v[c][k].z * f;
+        o[k].w += v[c][k].w * f;
       }
-      tree_store8<F16>(dst + col * 8, o[0], o[1], inv);
     }
+    tree_store8<F16>(dst + col * 8, o[0], o[1], l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
   }
-  cluster_barrier();  // shared memory stays until it has been read
+  // Shared memory stays until it has been read.
+  asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
 }
 
 template <int D, bool F16>
@@ -827,7 +825,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     if (brought > 0) mbar_wait_bounded(qfull, (brought - 1) & 1);
   }
   __syncthreads();
-  if (p.work.cluster > 0 && items[0].valid) join_tree_cluster<D, F16>(p, items[0], smem_u32(smem));
+  if (p.work.cluster > 1 && items[0].valid) join_tree_cluster<D, F16>(p, items[0], smem_u32(smem));
   if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   tc_fence_after();
   if (warp == 5) tmem_dealloc(tmem, Cfg::kTmemCols);
