@@ -9,7 +9,7 @@ import torch
 from vla_abft_estimate_b200 import _build
 from vla_abft_estimate_b200 import _native as N
 
-from .test_paged_host import BAD_KV, _kv
+from .test_paged_host import BAD_KV, _have_nvcc, _kv
 
 STRUCTS = {"abft_kv_append_at_args": (N.KvAppendAtArgs, ("positions", "axes", "sections")),
            "abft_paged_tree_args": (N.PagedTreeArgs, ("parents",)),
@@ -31,6 +31,62 @@ def test_struct_layouts_match_c(tmp_path):
         want += [ctypes.sizeof(t)] + [getattr(t, f).offset for f in fields]
     want += [N.MOST_AXES, N.PAGED_BAD_DRAFT, N.PAGED_BAD_FORK]
     assert [int(x) for x in subprocess.check_output([str(exe)]).split()] == want
+
+
+WORDS_PROGRAM = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "paged_tree.cuh"
+using namespace abft;
+int main() {
+  long checks = 0;
+  unsigned seed = 1;
+  auto rnd = [&]() { return (seed = seed * 1664525u + 1013904223u) >> 8; };
+  const int sizes[] = {1, 2, 31, 32, 33, 63, 64, 65, 150, 400};
+  for (int n : sizes)
+    for (int kind = 0; kind < 4; ++kind) {
+      int up[400];
+      for (int i = 0; i < n; ++i) {
+        up[i] = kind == 0 ? i - 1 : kind == 1 ? (i ? 0 : -1) : i ? static_cast<int>(rnd() % (i + 1)) - 1 : -1;
+        if (kind == 3 && rnd() % 8 == 0) up[i] = static_cast<int>(rnd()) - (1 << 23);  // bad ones among them
+        if (kind == 3 && rnd() % 8 == 0) up[i] = i;
+      }
+      for (int before = -n; before < 200; before += 7)  // slots before the drafted ones (below 0: more rows than tokens)
+        for (int step = 0; step * 64 < before + n; ++step)
+          for (int own = before < 0 ? -before : 0; own < n; ++own) {
+            uint32_t w[2];
+            tree_words(up, own, before - step * 64, w);
+            unsigned char see[700] = {0};
+            for (int i = 0; i < before; ++i) see[i] = 1;
+            for (int i = own; i >= 0;) {
+              if (before + i >= 0) see[before + i] = 1;
+              i = up[i] < i ? up[i] : -1;
+            }
+            for (int k = 0; k < 64; ++k) {
+              if ((w[k / 32] >> (k % 32) & 1u) != see[step * 64 + k]) {
+                std::printf("n %d kind %d before %d step %d own %d key %d\n", n, kind, before, step, own, k);
+                return 1;
+              }
+              ++checks;
+            }
+          }
+    }
+  std::printf("%ld\n", checks);
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(not _have_nvcc(), reason="needs nvcc")
+def test_what_a_row_of_a_tree_sees(tmp_path):
+    """The mask words on the host, against the way up row by row."""
+    src, exe = tmp_path / "words.cu", tmp_path / "words"
+    src.write_text(WORDS_PROGRAM)
+    subprocess.check_call([_build._nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O2",
+                           f"-I{_build.CSRC_DIR}", f"-I{_build.INCLUDE_DIR}", str(src), "-o", str(exe)])
+    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+    assert int(out.stdout) > 10_000_000
 
 
 def _append(kv):

@@ -108,7 +108,7 @@ struct TreeParams {
 // drafted ones (`base` of them from the step's first on, may be negative), and of
 // those the row's own and its ancestors'. The walk up ends at the root, at a parent
 // that does not come before its child, or before the step.
-__device__ __forceinline__ void tree_words(const int32_t* parents, int own, int base, uint32_t (&w)[2]) {
+__host__ __device__ __forceinline__ void tree_words(const int32_t* parents, int own, int base, uint32_t (&w)[2]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int below = base - c * 32;

@@ -30,10 +30,14 @@ class PagedCaches:
     page table and one array of lengths for all of them, and the rotation
     table. ``layers``: a ``paged.PagedKVCache`` per layer; ``table`` int32
     [batch, pages]; ``lens`` int32 [batch], the tokens of each sequence
-    including the ones of the next call."""
+    including the ones of the next call. ``together``: the ``paged.PagedLayers``
+    of all, for what a step with drafted tokens or a fork does in every layer."""
 
     def __init__(self, layers, table, lens, rope):
+        from .paged import PagedLayers
+
         self.layers, self.table, self.lens, self.rope = layers, table, lens, rope
+        self.together = PagedLayers(layers)
 
     @classmethod
     def allocate(cls, layers, batch, t_max, page_size, kv_heads, head_dim, theta, dtype, device):
@@ -67,6 +71,11 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
     of any length; rows behind the last sequence attend to nothing), or is
     None for one token per sequence.
     ``caches.lens`` counts the new tokens already: advance it first.
+    ``parents`` (int32, one for each row): the new tokens are trees of drafted
+    ones, attended to as such; ``positions`` (int32, [tokens] or [axes, tokens])
+    is what each token is rotated by in place of its slot's place: a drafted
+    token's depth, or the time, height and width of ``cfg["rope_sections"]``.
+    ``caches.together`` accepts, keeps and forks.
     ``dtype``: bfloat16 (default) or float16, the reference driver's
     ``--dtype`` (qwen_abft_benchmark.py:26)."""
     import torch
@@ -122,13 +131,20 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
             g, u = self.gate_up(self.ln2(x)).chunk(2, dim=-1)
             return x + self.down(F.silu(g) * u)
 
-        def forward_paged(self, x, rope, cache, cu_seqlens):
+        def forward_paged(self, x, rope, cache, cu_seqlens, parents, positions):
             nh, nkv, hd = cfg["heads"], cfg["kv_heads"], cfg["head_dim"]
             t = x.shape[0]
             q, k, v = self.qkv(self.ln1(x)).split([nh * hd, nkv * hd, nkv * hd], dim=-1)
-            q = cache.append(q.view(t, nh, hd), k.view(t, nkv, hd), v.view(t, nkv, hd), rope, cu_seqlens=cu_seqlens)
+            sections = None if positions is None else cfg.get("rope_sections")
+            q = cache.append(q.view(t, nh, hd), k.view(t, nkv, hd), v.view(t, nkv, hd), rope, cu_seqlens=cu_seqlens,
+                             positions=positions, sections=sections)
             # Rows of no sequence go on through the checked linears: zeros, not what memory held.
-            a = cache.decode(q) if cu_seqlens is None else cache.prefill(q, cu_seqlens, out=torch.zeros_like(q))
+            if cu_seqlens is None:
+                a = cache.decode(q)
+            elif parents is None:
+                a = cache.prefill(q, cu_seqlens, out=torch.zeros_like(q))
+            else:
+                a = cache.tree(q, cu_seqlens, parents, out=torch.zeros_like(q))
             x = x + self.o(a.view(t, nh * hd))
             g, u = self.gate_up(self.ln2(x)).chunk(2, dim=-1)
             return x + self.down(F.silu(g) * u)
@@ -159,10 +175,12 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
             return [torch.zeros(2, cfg["kv_heads"], t_max, cfg["head_dim"], dtype=dt,
                                 device=self.embed.weight.device) for _ in range(cfg["layers"])]
 
-        def forward_paged(self, ids, caches, cu_seqlens=None):
+        def forward_paged(self, ids, caches, cu_seqlens=None, parents=None, positions=None):
+            if parents is not None and cu_seqlens is None:
+                raise ValueError("trees of drafted tokens need cu_seqlens")
             x = self.embed(ids)
             for layer, cache in zip(self.layers, caches.layers):
-                x = layer.forward_paged(x, caches.rope, cache, cu_seqlens)
+                x = layer.forward_paged(x, caches.rope, cache, cu_seqlens, parents, positions)
             return self.lm_head(self.norm(x))
 
         def new_paged_caches(self, batch, t_max, page_size=16):
