@@ -100,9 +100,11 @@ constexpr int kAppendThreads = 32 * kAppendWarps;
 // kAxes: the rotation goes by positions of the caller's, of several axes (images
 // and video: time, height, width) or one (a drafted token's depth), each for its
 // share of the pairs:  (c_j, s_j) = rope[positions[axis of j][t]][j]. They are
-// asked for before the chain (sequence, length, page) begins.
+// asked for before the chain (sequence, length, page) begins. (Bound by HBM in large
+// calls: 10,400 tokens of 36 heads on three axes 34.9 us, 5.6 TB/s, with four CTAs an
+// SM; 35.6 with three.)
 template <int D, bool F16, bool kAxes = false>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, kAxes ? 4 : 1) kv_append_kernel(const AppendParams p) {
   constexpr int kChunks = D / 16;  // threads per row
   griddep_wait();
   constexpr int kRows = 32 / kChunks;  // rows a warp covers at once

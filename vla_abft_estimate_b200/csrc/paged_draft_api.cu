@@ -276,7 +276,10 @@ int abft_kv_fork(const abft_kv_fork_args* a, void* stream) {
   p.src = a->src, p.dst = a->dst, p.pages = a->pages;
   p.pairs = a->pairs;
   const int64_t items = int64_t{2} * a->layers * a->kv.kv_heads;
-  p.per_pair = static_cast<int32_t>((items + kForkWarps - 1) / kForkWarps);
+  // 1, 2 or 4 warps to a head, so that each has work when the page is full (32 forks,
+  // pages of 128: 35.4 us with 1, 32.2 with 2, 30.5 with 4, 33.3 with 8).
+  p.shift = a->kv.page_size == 16 ? 0 : a->kv.page_size == 32 ? 1 : 2;
+  p.per_pair = static_cast<int32_t>(((items << p.shift) + kForkWarps - 1) / kForkWarps);
   const int64_t blocks = int64_t{p.per_pair} * a->pairs;
   if (blocks >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks)), block(32 * kForkWarps);
