@@ -104,7 +104,7 @@ constexpr int kAppendThreads = 32 * kAppendWarps;
 // calls: 10,400 tokens of 36 heads on three axes 34.9 us, 5.6 TB/s, with four CTAs an
 // SM; 35.6 with three.)
 template <int D, bool F16, bool kAxes = false>
-__global__ void __launch_bounds__(kAppendThreads, kAxes ? 4 : 1) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, kAxes ? 4 : 3) kv_append_kernel(const AppendParams p) {
   constexpr int kChunks = D / 16;  // threads per row
   griddep_wait();
   constexpr int kRows = 32 / kChunks;  // rows a warp covers at once
