@@ -582,20 +582,21 @@ int abft_draft_accept(const abft_draft_accept_args* args, void* stream);
  * counts[b], rising, move to the slots of rows 0, 1, ... in every layer, and
  * lens_out[b] = seq_lens[b] - n + counts[b] (lens_out may be kv.seq_lens itself).
  * The layers share kv's geometry, strides, table and lengths; their pools are
- * pools[2 * layer] (keys) and pools[2 * layer + 1] (values), device memory of
- * 16-byte aligned addresses, or, with pools NULL and one layer, kv's. A sequence
+ * pools[2 * layer] (keys) and pools[2 * layer + 1] (values), a host array (read
+ * during the call) of distinct, 16-byte aligned device addresses, or, with pools
+ * NULL and one layer, kv's. A sequence
  * with bad boundaries, count or rows (ABFT_PAGED_BAD_ROWS, ABFT_PAGED_BAD_DRAFT), a
  * length below n or beyond the table, or a bad page under one of those slots is
  * left as it was, its length too. */
 typedef struct abft_kv_keep_args {
   abft_paged_kv kv;
-  const void* const* pools;
+  void* const* pools;          /* [layers][2]                                            */
   const int32_t* cu_seqlens;   /* [batch + 1]                                            */
   const int32_t* kept;         /* [tokens]                                               */
   const int32_t* counts;       /* [batch]                                                */
   int32_t* lens_out;           /* [batch]                                                */
   int64_t tokens;
-  int32_t layers;              /* 1 to 4096                                              */
+  int32_t layers;              /* 1 to 512                                               */
   int32_t reserved;
 } abft_kv_keep_args;
 int abft_kv_keep(const abft_kv_keep_args* args, void* stream);
@@ -612,7 +613,7 @@ int abft_kv_keep(const abft_kv_keep_args* args, void* stream);
  * source's length or either page is bad or both pages are the same. */
 typedef struct abft_kv_fork_args {
   abft_paged_kv kv;
-  const void* const* pools;    /* as for abft_kv_keep                                    */
+  void* const* pools;          /* as for abft_kv_keep                                    */
   const int32_t* src;          /* [pairs]                                                */
   const int32_t* dst;
   const int32_t* pages;

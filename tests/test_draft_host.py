@@ -107,16 +107,20 @@ def _tree(kv):
     return a
 
 
+POOLS = (ctypes.c_void_p * 1024)(*range(0x100000, 0x100000 + 1024 * 64, 64))  # addresses that nobody follows
+
+
 def _keep(kv):
     a = N.KvKeepArgs()
     a.kv, a.pools, a.cu_seqlens, a.kept, a.counts, a.lens_out, a.tokens, a.layers = \
-        kv, 0x50000, 0x60000, 0x70000, 0x80000, kv.seq_lens, 8, 28
+        kv, ctypes.addressof(POOLS), 0x60000, 0x70000, 0x80000, kv.seq_lens, 8, 28
     return a
 
 
 def _fork(kv):
     a = N.KvForkArgs()
-    a.kv, a.pools, a.src, a.dst, a.pages, a.pairs, a.layers = kv, 0x50000, 0x60000, 0x70000, 0x80000, 3, 28
+    a.kv, a.pools, a.src, a.dst, a.pages, a.pairs, a.layers = \
+        kv, ctypes.addressof(POOLS), 0x60000, 0x70000, 0x80000, 3, 28
     return a
 
 
@@ -202,16 +206,22 @@ def test_accept_refusals():
     assert _call("abft_draft_accept", _set(_accept(), {"batch": 0, "tokens": 0})) == 0
 
 
+OFF, NONE = (ctypes.c_void_p * 56)(*POOLS[:56]), (ctypes.c_void_p * 56)(*POOLS[:56])
+OFF[55], NONE[55] = 0x100008, None
+
+
 def test_keep_refusals():
     lens = _kv().seq_lens
-    for over, code in [({"layers": 0}, -1), ({"layers": 5000}, -3), ({"pools": None}, -1), ({"pools": 0x50004}, -2),
+    for over, code in [({"layers": 0}, -1), ({"layers": 513}, -3), ({"pools": None}, -1), ({"pools": ctypes.addressof(OFF)}, -2),
+                       ({"pools": ctypes.addressof(NONE)}, -1),
                        ({"tokens": -1}, -1), ({"tokens": 1 << 30}, -3), ({"cu_seqlens": None}, -1), ({"counts": None}, -1),
                        ({"lens_out": None}, -1), ({"kept": None}, -1), ({"lens_out": lens + 4}, -1), ({"lens_out": lens - 4}, -1)]:
         assert _call("abft_kv_keep", _set(_keep(_kv()), over)) == code, over
 
 
 def test_fork_refusals():
-    for over, code in [({"layers": 0}, -1), ({"layers": 5000}, -3), ({"pools": None}, -1), ({"pools": 0x50001}, -2),
+    for over, code in [({"layers": 0}, -1), ({"layers": 513}, -3), ({"pools": None}, -1), ({"pools": ctypes.addressof(OFF)}, -2),
+                       ({"pools": ctypes.addressof(NONE)}, -1),
                        ({"pairs": -1}, -1), ({"pairs": 70000}, -3), ({"src": None}, -1), ({"dst": None}, -1),
                        ({"pages": None}, -1)]:
         assert _call("abft_kv_fork", _set(_fork(_kv()), over)) == code, over
@@ -234,11 +244,13 @@ def test_the_extension_takes_only_its_structs_and_passes_on_the_rest():
     assert c.tree(t) is None
     x = torch.zeros(3)
     with pytest.raises(ValueError):
-        host.Layers(b"short", 0, 1, 0, 0, 0, 0, (x, x), x, x)
+        host.Layers(b"short", 0, bytes(16), 0, 0, 0, (x, x), x, x)
     with pytest.raises(ValueError):
-        host.Layers(bytes(_kv()), 0, 1, 0, 0, 0, 0, (x, 3), x, x)
+        host.Layers(bytes(_kv()), 0, bytes(16), 0, 0, 0, (x, 3), x, x)
+    with pytest.raises(ValueError):
+        host.Layers(bytes(_kv()), 0, bytes(24), 0, 0, 0, (x, x), x, x)
     with pytest.raises(TypeError):
         host.Layers(bytes(_kv()), 0, 1)
-    many = host.Layers(bytes(_kv()), 0, 1, 0, 0, 0, 0, (x, x), x, x)
+    many = host.Layers(bytes(_kv()), 0, bytes(16), 0, 0, 0, (x, x), x, x)
     assert many.accept(cu, up, up, up) is None and many.keep(cu, up, up, up) is None and many.fork(up, up, up) is None
     assert many.accept() is None and many.keep(1) is None and many.fork(1, 2, 3, 4) is None

@@ -385,3 +385,40 @@ def test_fork_refusals_and_layers_that_do_not_match(cuda_device):
         PagedLayers([one, one])
     with pytest.raises(ValueError, match="own"):
         PagedLayers([PagedKVCache(one.k_pages, one.k_pages, one.page_table, one.seq_lens)])
+
+
+@pytest.mark.parametrize("layers", [64, 65, 512])
+def test_many_layers(cuda_device, layers):
+    check_keep(cuda_device, [30, 2], [40, 20], [[0, 3, 4, 29], [1]], layers=layers, kv_heads=1)
+    check_fork(cuda_device, [21, 30, 0, 0], [(0, 2), (1, 3)], layers=layers, kv_heads=1)
+
+
+def test_more_layers_are_refused(cuda_device):
+    with pytest.raises(ValueError, match="512"):
+        PagedLayers(layers_of(cuda_device, [3], layers=1).layers * 513)
+
+
+def test_the_object_may_go_while_its_calls_run(cuda_device):
+    """Nothing of the object's is read by the GPU."""
+    dev = cuda_device
+    layers = layers_of(dev, [400] * 8, layers=28, d=128, kv_heads=4)
+    caches = layers.layers
+    path = list(range(1, 200))
+    before = contents(layers)
+    stream = torch.cuda.Stream()
+    cu, kept, counts = i32([200 * i for i in range(9)], dev), i32((path + [-1]) * 8, dev), i32([199] * 8, dev)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(2_000_000)
+        layers.keep(cu, kept, counts)
+    del layers
+    junk = [torch.full((1 << 16,), -1, dtype=torch.int64, device=dev) for _ in range(64)]
+    torch.cuda.synchronize()
+    del junk
+    layers = PagedLayers(caches)
+    table, want = layers.page_table.cpu(), before.clone()
+    for b in range(8):
+        for i, k in enumerate(path):
+            (p0, s0), (p1, s1) = divmod(200 + k, 16), divmod(200 + i, 16)
+            want[:, :, table[b, p1], :, s1] = before[:, :, table[b, p0], :, s0]
+    assert torch.equal(contents(layers), want) and layers.seq_lens.tolist() == [399] * 8

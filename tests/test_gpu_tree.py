@@ -53,7 +53,7 @@ def test_lengths(cuda_device, n, total, page):
     run_tree(cuda_device, [random_tree(n, n + total)], [total], 7, 1, 128, page, BF16)
 
 
-@pytest.mark.parametrize("sms", [0, 1, 2, 5, 37])
+@pytest.mark.parametrize("sms", [0, 1, 2, 5, 37, 600])
 @pytest.mark.parametrize("d", [64, 128])
 def test_long_caches_in_pieces(cuda_device, d, sms):
     trees = [random_tree(26, 5), random_tree(3, 6), [], random_tree(61, 7)]

@@ -93,6 +93,7 @@ PAGED_BAD_DRAFT = 32
 PAGED_BAD_FORK = 64
 
 MOST_AXES = 4  # of the positions of abft_kv_append_at
+MOST_LAYERS = 512  # of abft_kv_keep and abft_kv_fork
 
 
 class AbftError(RuntimeError):

@@ -123,16 +123,15 @@ __global__ void __launch_bounds__(kAcceptThreads) draft_accept_kernel(const Acce
 }
 
 // ---- keep -----------------------------------------------------------------------
-// A model's pools: [layers][2] base addresses of keys and values, which share
+// A model's pools: [layers][2] base addresses of keys and values (in the launch's
+// parameters: nothing in memory has to outlive the call), which share
 // one page table, one array of lengths and one geometry; or one layer's, in kv.
+constexpr int kFewLayers = 64, kMostLayers = 512;  // of the two instances of each kernel
+template <int kLayers>
 struct LayerPools {
-  const void* const* pools;
+  uint16_t* pools[2 * kLayers];
   int32_t layers;
 };
-__device__ __forceinline__ uint16_t* pool_of(const PagedView& kv, const LayerPools& l, int layer, int values) {
-  if (l.pools == nullptr) return static_cast<uint16_t*>(values ? kv.v_pages : kv.k_pages);
-  return static_cast<uint16_t*>(const_cast<void*>(l.pools[2 * layer + values]));
-}
 
 // Of sequence b's n new tokens (its last slots) the rows kept[0] < kept[1] < ...
 // < kept[m - 1] move to the slots of rows 0 to m - 1, and its length becomes
@@ -145,9 +144,10 @@ __device__ __forceinline__ uint16_t* pool_of(const PagedView& kv, const LayerPoo
 //
 // A sequence with anything wrong (boundaries, count, rows that do not rise,
 // length, pages) is left as it was.
+template <int kLayers>
 struct KeepParams {
   PagedView kv;
-  LayerPools layers;
+  LayerPools<kLayers> layers;
   const int32_t *cu, *kept, *counts;
   int32_t* lens_out;
   int32_t tokens;
@@ -157,8 +157,8 @@ constexpr int kKeepThreads = 512;  // at most
 constexpr int kKeepHeld = 256;  // rows whose places are in shared memory at a time
 constexpr int kKeepCluster = 8;
 
-template <int D>
-__global__ void __launch_bounds__(kKeepThreads, 3) kv_keep_kernel(const KeepParams p) {
+template <int D, int kLayers>
+__global__ void __launch_bounds__(kKeepThreads, 3) kv_keep_kernel(const __grid_constant__ KeepParams<kLayers> p) {
   // Where a row comes from (-1: it stays) and goes, in elements of head 0: in the
   // key pools, in the value pools.
   __shared__ longlong2 s_move[2][kKeepHeld];
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kKeepThreads, 3) kv_keep_kernel(const KeepPara
       for (int column = rank * threads + threadIdx.x; column < columns; column += p.cluster * threads) {
         const int c = column % kChunks, row = column / kChunks;
         const int head = row % kv.kv_heads, pool = row / kv.kv_heads, values = pool & 1;
-        uint16_t* at = pool_of(kv, p.layers, pool >> 1, values) + (static_cast<int64_t>(head) << kv.page_shift << kShift) + c * 8;
+        uint16_t* at = p.layers.pools[pool] + (static_cast<int64_t>(head) << kv.page_shift << kShift) + c * 8;
         const longlong2* moves = s_move[values];
         constexpr int kBatch = 4;
         for (int i = 0; i < here; i += kBatch) {
@@ -249,9 +249,10 @@ __global__ void __launch_bounds__(kKeepThreads, 3) kv_keep_kernel(const KeepPara
 // Bound: HBM, by rest slots of 2 * layers * heads rows in and out; slots of a head lie
 // one after another, and its warps take them in turn, eight 16-byte pieces a lane in
 // flight (32 forks of 64 slots on average, 28 layers of 4 heads: 30.5 us, 6.7 TB/s).
+template <int kLayers>
 struct ForkParams {
   PagedView kv;
-  LayerPools layers;
+  LayerPools<kLayers> layers;
   const int32_t *src, *dst, *pages;
   int32_t pairs;
   int32_t per_pair;  // CTAs of a pair: 2^shift warps for each head of each pool
@@ -259,8 +260,8 @@ struct ForkParams {
 };
 constexpr int kForkWarps = 8;
 
-template <int D>
-__global__ void __launch_bounds__(32 * kForkWarps) kv_fork_kernel(const ForkParams p) {
+template <int D, int kLayers>
+__global__ void __launch_bounds__(32 * kForkWarps) kv_fork_kernel(const __grid_constant__ ForkParams<kLayers> p) {
   constexpr int kShift = D == 128 ? 7 : 6;
   griddep_wait();
   const PagedView& kv = p.kv;
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(32 * kForkWarps) kv_fork_kernel(const ForkPara
   const int w = part * kForkWarps + (threadIdx.x >> 5), item = w >> p.shift, share = w & ((1 << p.shift) - 1);
   if (item >= items) return;
   const int head = item % kv.kv_heads, pool = item / kv.kv_heads, values = pool & 1;
-  uint16_t* at = pool_of(kv, p.layers, pool >> 1, values);
+  uint16_t* at = p.layers.pools[pool];
   const int64_t stride = values ? kv.v_page_stride : kv.k_page_stride;
   const uint4* from = reinterpret_cast<const uint4*>(at + paged_offset(old, stride, head, 0, kv.page_shift, kShift));
   uint4* to = reinterpret_cast<uint4*>(at + paged_offset(fresh, stride, head, 0, kv.page_shift, kShift));

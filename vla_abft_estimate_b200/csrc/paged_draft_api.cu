@@ -9,11 +9,25 @@ using namespace abft;
 
 namespace {
 
-int check_layers(const abft_paged_kv& kv, const void* const* pools, int32_t layers) {
+int check_layers(const abft_paged_kv& kv, void* const* pools, int32_t layers) {
   if (layers < 1 || (pools == nullptr && layers != 1)) return ABFT_ERR_INVALID_ARG;
-  if (layers > 4096) return ABFT_ERR_UNSUPPORTED;
-  if ((reinterpret_cast<uintptr_t>(pools) & 7u) != 0) return ABFT_ERR_ALIGNMENT;
-  return check_kv(kv);
+  if (layers > kMostLayers) return ABFT_ERR_UNSUPPORTED;
+  const int rc = check_kv(kv);
+  if (rc != ABFT_OK || pools == nullptr || kv.batch == 0) return rc;
+  for (int i = 0; i < 2 * layers; ++i) {
+    if (pools[i] == nullptr) return ABFT_ERR_INVALID_ARG;
+    if (off16(pools[i])) return ABFT_ERR_ALIGNMENT;
+  }
+  return ABFT_OK;
+}
+
+template <int kLayers>
+LayerPools<kLayers> layer_pools(const abft_paged_kv& kv, void* const* pools, int32_t layers) {
+  LayerPools<kLayers> r;
+  r.layers = layers;
+  for (int i = 0; i < 2 * layers; ++i)
+    r.pools[i] = static_cast<uint16_t*>(pools != nullptr ? pools[i] : i == 0 ? kv.k_pages : kv.v_pages);
+  return r;
 }
 
 // How a tree call is cut: segments of a tile of query rows and one kv head, dealt by
@@ -151,6 +165,43 @@ bool overlap(const void* a, const void* b, size_t bytes) {
   return x < y + bytes && y < x + bytes;
 }
 
+template <int kLayers>
+int keep_call(const abft_kv_keep_args* a, int sms, cudaStream_t s) {
+  KeepParams<kLayers> p;
+  p.kv = view_of(a->kv);
+  p.layers = layer_pools<kLayers>(a->kv, a->pools, a->layers);
+  p.cu = a->cu_seqlens, p.kept = a->kept, p.counts = a->counts;
+  p.lens_out = a->lens_out;
+  p.tokens = static_cast<int32_t>(a->tokens);
+  // A thread for each 16 bytes of a slot in all layers, as far as a cluster has them;
+  // half as many where that makes more CTAs than run at once (28 layers, CTAs of 512 /
+  // 256 threads: 1 sequence 3.4 / 3.9 us, 64 sequences 7.4 / 5.6).
+  const int64_t columns = int64_t{2} * a->layers * a->kv.kv_heads * a->kv.head_dim / 8;
+  for (p.cluster = 1; p.cluster < kKeepCluster && int64_t{p.cluster} * kKeepThreads < columns;) p.cluster *= 2;
+  const dim3 grid(a->kv.batch * p.cluster), block(int64_t{a->kv.batch} * p.cluster > 3 * sms ? kKeepThreads / 2 : kKeepThreads);
+  return a->kv.head_dim == 128 ? launch_clusters(p.cluster, kv_keep_kernel<128, kLayers>, grid, block, 0, s, p)
+                               : launch_clusters(p.cluster, kv_keep_kernel<64, kLayers>, grid, block, 0, s, p);
+}
+
+template <int kLayers>
+int fork_call(const abft_kv_fork_args* a, cudaStream_t s) {
+  ForkParams<kLayers> p;
+  p.kv = view_of(a->kv);
+  p.layers = layer_pools<kLayers>(a->kv, a->pools, a->layers);
+  p.src = a->src, p.dst = a->dst, p.pages = a->pages;
+  p.pairs = a->pairs;
+  const int64_t items = int64_t{2} * a->layers * a->kv.kv_heads;
+  // 1, 2 or 4 warps to a head, so that each has work when the page is full (32 forks,
+  // pages of 128: 35.4 us with 1, 32.2 with 2, 30.5 with 4, 33.3 with 8).
+  p.shift = a->kv.page_size == 16 ? 0 : a->kv.page_size == 32 ? 1 : 2;
+  p.per_pair = static_cast<int32_t>(((items << p.shift) + kForkWarps - 1) / kForkWarps);
+  const int64_t blocks = int64_t{p.per_pair} * a->pairs;
+  if (blocks >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(blocks)), block(32 * kForkWarps);
+  return a->kv.head_dim == 128 ? launch(kv_fork_kernel<128, kLayers>, grid, block, 0, s, p)
+                               : launch(kv_fork_kernel<64, kLayers>, grid, block, 0, s, p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -241,22 +292,8 @@ int abft_kv_keep(const abft_kv_keep_args* a, void* stream) {
     return ABFT_ERR_INVALID_ARG;
   int dev = 0, sms = 0;
   if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
-  KeepParams p;
-  p.kv = view_of(a->kv);
-  p.layers.pools = a->pools;
-  p.layers.layers = a->layers;
-  p.cu = a->cu_seqlens, p.kept = a->kept, p.counts = a->counts;
-  p.lens_out = a->lens_out;
-  p.tokens = static_cast<int32_t>(a->tokens);
-  // A thread for each 16 bytes of a slot in all layers, as far as a cluster has them;
-  // half as many where that makes more CTAs than run at once (28 layers, CTAs of 512 /
-  // 256 threads: 1 sequence 3.4 / 3.9 us, 64 sequences 7.4 / 5.6).
-  const int64_t columns = int64_t{2} * a->layers * a->kv.kv_heads * a->kv.head_dim / 8;
-  for (p.cluster = 1; p.cluster < kKeepCluster && int64_t{p.cluster} * kKeepThreads < columns;) p.cluster *= 2;
-  const dim3 grid(a->kv.batch * p.cluster), block(int64_t{a->kv.batch} * p.cluster > 3 * sms ? kKeepThreads / 2 : kKeepThreads);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a->kv.head_dim == 128 ? launch_clusters(p.cluster, kv_keep_kernel<128>, grid, block, 0, s, p)
-                               : launch_clusters(p.cluster, kv_keep_kernel<64>, grid, block, 0, s, p);
+  return a->layers <= kFewLayers ? keep_call<kFewLayers>(a, sms, s) : keep_call<kMostLayers>(a, sms, s);
 }
 
 int abft_kv_fork(const abft_kv_fork_args* a, void* stream) {
@@ -269,23 +306,8 @@ int abft_kv_fork(const abft_kv_fork_args* a, void* stream) {
   if (a->src == nullptr || a->dst == nullptr || a->pages == nullptr) return ABFT_ERR_INVALID_ARG;
   int dev = 0, sms = 0;
   if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
-  ForkParams p;
-  p.kv = view_of(a->kv);
-  p.layers.pools = a->pools;
-  p.layers.layers = a->layers;
-  p.src = a->src, p.dst = a->dst, p.pages = a->pages;
-  p.pairs = a->pairs;
-  const int64_t items = int64_t{2} * a->layers * a->kv.kv_heads;
-  // 1, 2 or 4 warps to a head, so that each has work when the page is full (32 forks,
-  // pages of 128: 35.4 us with 1, 32.2 with 2, 30.5 with 4, 33.3 with 8).
-  p.shift = a->kv.page_size == 16 ? 0 : a->kv.page_size == 32 ? 1 : 2;
-  p.per_pair = static_cast<int32_t>(((items << p.shift) + kForkWarps - 1) / kForkWarps);
-  const int64_t blocks = int64_t{p.per_pair} * a->pairs;
-  if (blocks >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>(blocks)), block(32 * kForkWarps);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a->kv.head_dim == 128 ? launch(kv_fork_kernel<128>, grid, block, 0, s, p)
-                               : launch(kv_fork_kernel<64>, grid, block, 0, s, p);
+  return a->layers <= kFewLayers ? fork_call<kFewLayers>(a, s) : fork_call<kMostLayers>(a, s);
 }
 
 }  // extern "C"

@@ -360,7 +360,7 @@ struct Layers {
   abft_paged_kv kv;
   int device;
   int32_t layers;
-  const void* const* pools;
+  PyObject* pools;   // bytes: the pools' addresses
   AcceptFn accept;
   KeepFn keep;
   ForkFn fork;
@@ -438,7 +438,7 @@ PyObject* layers_keep(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   abft_kv_keep_args args;
   memset(&args, 0, sizeof args);
   args.kv = c->kv;
-  args.pools = c->pools;
+  args.pools = reinterpret_cast<void* const*>(PyBytes_AS_STRING(c->pools));
   args.layers = c->layers;
   args.cu_seqlens = int_ptr(cu), args.kept = int_ptr(kept), args.counts = int_ptr(counts);
   args.lens_out = static_cast<int32_t*>(out->data_ptr());
@@ -464,7 +464,7 @@ PyObject* layers_fork(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   abft_kv_fork_args args;
   memset(&args, 0, sizeof args);
   args.kv = c->kv;
-  args.pools = c->pools;
+  args.pools = reinterpret_cast<void* const*>(PyBytes_AS_STRING(c->pools));
   args.layers = c->layers;
   args.src = int_ptr(src), args.dst = int_ptr(dst), args.pages = int_ptr(pages);
   args.pairs = static_cast<int32_t>(src->size(0));
@@ -481,31 +481,35 @@ PyObject* layers_fork(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 
 void layers_dealloc(PyObject* self) {
   Layers* c = reinterpret_cast<Layers*>(self);
+  Py_CLEAR(c->pools);
   Py_CLEAR(c->pages);
   Py_CLEAR(c->table);
   Py_CLEAR(c->lens);
   Py_TYPE(self)->tp_free(self);
 }
 
-// Layers(kv bytes, device, layers, address of the pools, addresses of accept,
-// keep, fork, tuple of page tensors, page table, lengths).
+// Layers(kv bytes, device, bytes of the pools' addresses, addresses of accept, keep,
+// fork, tuple of page tensors, page table, lengths).
 int layers_init(PyObject* self, PyObject* args, PyObject*) {
   Layers* c = reinterpret_cast<Layers*>(self);
   const char* kv;
   Py_ssize_t size;
-  unsigned long long pools, fn[3];
-  PyObject *pages, *table, *lens;
-  if (!PyArg_ParseTuple(args, "y#iiKKKKO!OO", &kv, &size, &c->device, &c->layers, &pools, fn, fn + 1, fn + 2, &PyTuple_Type,
+  unsigned long long fn[3];
+  PyObject *pools, *pages, *table, *lens;
+  if (!PyArg_ParseTuple(args, "y#iO!KKKO!OO", &kv, &size, &c->device, &PyBytes_Type, &pools, fn, fn + 1, fn + 2, &PyTuple_Type,
                         &pages, &table, &lens))
     return -1;
   bool tensors = THPVariable_Check(table) && THPVariable_Check(lens);
+  tensors = tensors && PyBytes_GET_SIZE(pools) == static_cast<Py_ssize_t>(sizeof(void*)) * PyTuple_GET_SIZE(pages);
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(pages); ++i) tensors = tensors && THPVariable_Check(PyTuple_GET_ITEM(pages, i));
   if (size != static_cast<Py_ssize_t>(sizeof c->kv) || !tensors) {
     PyErr_SetString(PyExc_ValueError, "the cache struct has another size, or no tensors follow");
     return -1;
   }
   memcpy(&c->kv, kv, sizeof c->kv);
-  c->pools = reinterpret_cast<const void* const*>(pools);
+  c->layers = static_cast<int32_t>(PyTuple_GET_SIZE(pages) / 2);
+  Py_INCREF(pools);
+  Py_XSETREF(c->pools, pools);
   Py_INCREF(pages);
   Py_XSETREF(c->pages, pages);
   Py_INCREF(table);

@@ -121,8 +121,8 @@ def _host():
             spec = importlib.util.spec_from_file_location("_paged_host", path)
             _HOST = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(_HOST)
-        else:
-            warnings.warn(f"{path} is missing: calls of the paged cache take longer on the host; build it with "
+        if not hasattr(_HOST, "Layers"):
+            warnings.warn(f"{path} is missing or of another build: calls of the paged cache take longer on the host; build it with "
                           "`python -m vla_abft_estimate_b200._build`")
             _HOST = _LongWay
     return _HOST
@@ -178,7 +178,7 @@ class PagedKVCache:
     call must go to distinct slots. Slots at or behind a sequence's length
     may hold anything; keys and values below it are taken as finite numbers
     (a non-finite value of a slot may reach every query of its sequence that
-    ``prefill`` answers in the same call).
+    ``prefill`` or ``tree`` answers in the same call).
     """
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -497,16 +497,17 @@ class PagedKVCache:
 class PagedLayers:
     """The caches of a model's layers, for what is done in all of them at once.
 
-    ``layers``: a ``PagedKVCache`` for each, with one page table, one array of
-    lengths, one type and one geometry, and pools of their own. Make it outside
-    of a graph capture; the calls may be captured. What the status tells of these
-    calls is in the first layer's.
+    ``layers``: a ``PagedKVCache`` for each (512 at most), with one page table, one
+    array of lengths, one type and one geometry, and pools of their own. What the
+    status tells of these calls is in the first layer's.
     """
 
     def __init__(self, layers: Sequence[PagedKVCache]):
         layers = tuple(layers)
         if not layers or not all(isinstance(c, PagedKVCache) for c in layers):
             raise TypeError("layers must be PagedKVCache objects, one at least")
+        if len(layers) > N.MOST_LAYERS:
+            raise ValueError(f"{len(layers)} layers: at most {N.MOST_LAYERS}")
         first = layers[0]
 
         def shared(c):
@@ -521,9 +522,9 @@ class PagedLayers:
             raise ValueError("layers must have pools of their own, for keys and for values")
         self.layers, self.batch, self.device = layers, first.batch, first.device
         self._kv, self._index = first._kv, first._index
-        self._pools = torch.tensor(pools, dtype=torch.int64, device=self.device)
+        self._pools = (ctypes.c_void_p * len(pools))(*pools)
         self._pages = tuple(x for c in layers for x in (c.k_pages, c.v_pages))
-        self._fast = _host().Layers(bytes(self._kv), self._index, len(layers), self._pools.data_ptr(),
+        self._fast = _host().Layers(bytes(self._kv), self._index, bytes(self._pools),
                                     *_addresses("abft_draft_accept", "abft_kv_keep", "abft_kv_fork"),
                                     self._pages, first.page_table, first.seq_lens)
 
@@ -605,7 +606,7 @@ class PagedLayers:
         self._list("counts", counts, self.batch)
         self._list("lens_out", out, self.batch)
         args = N.KvKeepArgs()
-        args.kv, args.pools, args.layers = self._kv, self._pools.data_ptr(), len(self.layers)
+        args.kv, args.pools, args.layers = self._kv, ctypes.addressof(self._pools), len(self.layers)
         args.cu_seqlens, args.kept, args.counts = cu_seqlens.data_ptr(), kept.data_ptr(), counts.data_ptr()
         args.lens_out, args.tokens = out.data_ptr(), kept.shape[0]
         self._call("abft_kv_keep", args)
@@ -634,7 +635,7 @@ class PagedLayers:
         self._list("dst", dst, src.shape[0])
         self._list("pages", pages, src.shape[0])
         args = N.KvForkArgs()
-        args.kv, args.pools, args.layers = self._kv, self._pools.data_ptr(), len(self.layers)
+        args.kv, args.pools, args.layers = self._kv, ctypes.addressof(self._pools), len(self.layers)
         args.src, args.dst, args.pages, args.pairs = src.data_ptr(), dst.data_ptr(), pages.data_ptr(), src.shape[0]
         self._call("abft_kv_fork", args)
         _mark_written(*self._pages, self.page_table, self.seq_lens)

@@ -34,10 +34,16 @@ class PagedCaches:
     of all, for what a step with drafted tokens or a fork does in every layer."""
 
     def __init__(self, layers, table, lens, rope):
-        from .paged import PagedLayers
-
         self.layers, self.table, self.lens, self.rope = layers, table, lens, rope
-        self.together = PagedLayers(layers)
+        self._together = None
+
+    @property
+    def together(self):
+        if self._together is None:
+            from .paged import PagedLayers
+
+            self._together = PagedLayers(self.layers)
+        return self._together
 
     @classmethod
     def allocate(cls, layers, batch, t_max, page_size, kv_heads, head_dim, theta, dtype, device):
