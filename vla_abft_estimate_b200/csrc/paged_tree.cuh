@@ -836,70 +836,89 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
 // segment, several where there are few pieces, and asks for 16 sums at once,
 // by asynchronous copies into its own column of shared memory: what counts is the
 // number of round trips. (In registers, three or six at once, the join of 18 pieces
-// took 14 us.) Units of 128 threads' work of all segments are one list, dealt to
-// the blocks in turn.
+// took 14 us.) Of more pieces than that each warp takes every fourth. Units of a
+// block's work of all segments are one list, dealt to the blocks in turn.
 constexpr int kTreeJoinThreads = 128;
 constexpr int kTreeJoinSlots = 16;
 
-// (row, 4 columns) of a thread, so that its first round has all pieces of up to 16.
-__device__ __forceinline__ int tree_join_columns(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 2 : 1; }
+// log2 of a unit's (row, 4 columns): a round has all pieces of up to 16.
+__device__ __forceinline__ int tree_join_shift(int pieces) { return pieces <= 4 ? 9 : pieces <= 8 ? 8 : pieces <= 16 ? 7 : 5; }
 
-template <int D, bool F16, int kIdx>
+template <int D, bool F16, int kParts, int kIdx>
 __device__ __forceinline__ void join_tree_unit(const TreeParams& p, int c, int pieces, int rows, int unit, float4* s_o, float2* s_ml) {
-  const int i0 = unit * (kTreeJoinThreads * kIdx) + threadIdx.x, all = rows * (D / 4);
+  constexpr int kLane = kTreeJoinThreads / kParts;  // threads of a part
+  const int part = kParts == 1 ? 0 : threadIdx.x / kLane;
+  const int i0 = unit * (kLane * kIdx) + threadIdx.x - part * kLane, all = rows * (D / 4);
   const int2 spill = p.work.spill[c];
+  const uint32_t rows_inv = ((1u << 20) + rows - 1) / rows;
   const uint32_t to = smem_u32(s_o + threadIdx.x), to_ml = smem_u32(s_ml + threadIdx.x);
   int row[kIdx], col[kIdx];
   float m[kIdx], l[kIdx];
   float4 o[kIdx];
 #pragma unroll
   for (int i = 0; i < kIdx; ++i) {
-    const int index = min(i0 + i * kTreeJoinThreads, all - 1);  // behind the end the last one again, which is not written
-    col[i] = index / rows;
+    const int index = min(i0 + i * kLane, all - 1);  // behind the end the last one again, which is not written
+    // index / rows: exact, since the product overshoots by less than index / 2^20 < 1 / rows.
+    col[i] = static_cast<int>(static_cast<uint32_t>(index) * rows_inv >> 20);
     row[i] = index - col[i] * rows;
     m[i] = -INFINITY;
     l[i] = 0.f;
     o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  auto add = [&](int i, const float2 ml, const float4 v) {
+    const float top = fmaxf(m[i], ml.x), ms = top == -INFINITY ? 0.f : top;
+    const float f = exp2_approx(m[i] - ms), f2 = exp2_approx(ml.x - ms);
+    const bool any = ml.y != 0.f;  // what a row saw nothing of was not written
+    m[i] = top;
+    l[i] = l[i] * f + ml.y * f2;
+    o[i].x = o[i].x * f + (any ? v.x * f2 : 0.f);
+    o[i].y = o[i].y * f + (any ? v.y * f2 : 0.f);
+    o[i].z = o[i].z * f + (any ? v.z * f2 : 0.f);
+    o[i].w = o[i].w * f + (any ? v.w * f2 : 0.f);
+  };
   constexpr int kAtOnce = kTreeJoinSlots / kIdx;  // pieces
 #pragma unroll 1
-  for (int s0 = 0; s0 < pieces; s0 += kAtOnce) {
+  for (int s0 = part; s0 < pieces; s0 += kParts * kAtOnce) {
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      if (s0 + k >= pieces) break;
-      const int64_t at = static_cast<int64_t>(c + s0 + k) * 2 + (s0 + k == 0 ? 1 : 0);
+      const int piece = s0 + k * kParts;
+      if (piece >= pieces) break;
+      // (Places stay below 2^14, sums below 2^26 float4.)
+      const int at = (c + piece) * 2 + (piece == 0 ? 1 : 0);
 #pragma unroll
       for (int i = 0; i < kIdx; ++i) {
         const int slot = (k * kIdx + i) * kTreeJoinThreads;
-        cp_async16(to + slot * 16, p.work.part + (at * (D / 4) + col[i]) * kTreeRows + row[i], 16u);
-        cp_async8(to_ml + slot * 8, p.work.part_ml + at * kTreeRows + row[i]);
+        cp_async16(to + slot * 16, p.work.part + ((at * (D / 4) + col[i]) * kTreeRows + row[i]), 16u);
+        cp_async8(to_ml + slot * 8, p.work.part_ml + (at * kTreeRows + row[i]));
       }
     }
     cp_async_commit();
     cp_async_wait<0>();
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      if (s0 + k >= pieces) break;
+      if (s0 + k * kParts >= pieces) break;
 #pragma unroll
       for (int i = 0; i < kIdx; ++i) {
         const int slot = (k * kIdx + i) * kTreeJoinThreads + threadIdx.x;
-        const float2 ml = s_ml[slot];
-        const float4 v = s_o[slot];
-        const float top = fmaxf(m[i], ml.x), ms = top == -INFINITY ? 0.f : top;
-        const float f = exp2_approx(m[i] - ms), f2 = exp2_approx(ml.x - ms);
-        const bool any = ml.y != 0.f;  // what a row saw nothing of was not written
-        m[i] = top;
-        l[i] = l[i] * f + ml.y * f2;
-        o[i].x = o[i].x * f + (any ? v.x * f2 : 0.f);
-        o[i].y = o[i].y * f + (any ? v.y * f2 : 0.f);
-        o[i].z = o[i].z * f + (any ? v.z * f2 : 0.f);
-        o[i].w = o[i].w * f + (any ? v.w * f2 : 0.f);
+        add(i, s_ml[slot], s_o[slot]);
       }
     }
   }
+  if constexpr (kParts > 1) {
+    static_assert(kIdx == 1, "one place for a thread's sums");
+    __syncthreads();
+    s_ml[threadIdx.x] = make_float2(m[0], l[0]);
+    s_o[threadIdx.x] = o[0];
+    __syncthreads();
+    if (part == 0)
+#pragma unroll
+      for (int k = 1; k < kParts; ++k) add(0, s_ml[k * kLane + threadIdx.x], s_o[k * kLane + threadIdx.x]);
+    __syncthreads();  // read before the next unit's sums come
+    if (part > 0) return;
+  }
 #pragma unroll
   for (int i = 0; i < kIdx; ++i) {
-    if (i0 + i * kTreeJoinThreads >= all) continue;
+    if (i0 + i * kLane >= all) continue;
     const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
     uint16_t* dst = tree_out(p, spill.y, spill.x, row[i], row_token(row[i], p.group_inv)) + col[i] * 4;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<F16>(o[i].x * inv, o[i].y * inv), pack2<F16>(o[i].z * inv, o[i].w * inv));
@@ -923,8 +942,9 @@ __global__ void __launch_bounds__(kTreeJoinThreads, 4) paged_tree_join_kernel(co
       n[k] = c < grid ? p.work.pieces[c] : 0;
     }
     auto units_of = [](int x) {
-      const int of = kTreeJoinThreads * tree_join_columns(x & 0xFFFF);
-      return ((x >> 16) * (D / 4) + of - 1) / of;
+      const int shift = tree_join_shift(x & 0xFFFF);
+      static_assert(kTreeJoinThreads == 1 << 7, "a unit's size");
+      return ((x >> 16) * (D / 4) + (1 << shift) - 1) >> shift;
     };
 #pragma unroll
     for (int k = 0; k < kLook; ++k) units += units_of(n[k]);
@@ -944,10 +964,11 @@ __global__ void __launch_bounds__(kTreeJoinThreads, 4) paged_tree_join_kernel(co
       c = __shfl_sync(0xFFFFFFFFu, c, src);
       x = __shfl_sync(0xFFFFFFFFu, x, src);
       const int pieces = x & 0xFFFF, rows = x >> 16;
-      switch (tree_join_columns(pieces)) {
-        case 4: join_tree_unit<D, F16, 4>(p, c, pieces, rows, at, s_o, s_ml); break;
-        case 2: join_tree_unit<D, F16, 2>(p, c, pieces, rows, at, s_o, s_ml); break;
-        default: join_tree_unit<D, F16, 1>(p, c, pieces, rows, at, s_o, s_ml); break;
+      switch (tree_join_shift(pieces)) {
+        case 9: join_tree_unit<D, F16, 1, 4>(p, c, pieces, rows, at, s_o, s_ml); break;
+        case 8: join_tree_unit<D, F16, 1, 2>(p, c, pieces, rows, at, s_o, s_ml); break;
+        case 7: join_tree_unit<D, F16, 1, 1>(p, c, pieces, rows, at, s_o, s_ml); break;
+        default: join_tree_unit<D, F16, 4, 1>(p, c, pieces, rows, at, s_o, s_ml); break;
       }
     }
     before += here;
