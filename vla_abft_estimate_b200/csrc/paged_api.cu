@@ -36,7 +36,9 @@ int abft_kv_append(const abft_kv_append_args* a, void* stream) {
   if (rc != ABFT_OK || a->tokens == 0 || a->kv.batch == 0) return rc;
   int dev = 0, sms = 0;
   if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
-  return append_call<false>(append_params(a), a->kv, sms, stream);
+  AppendParams p;
+  append_params(a, &p);
+  return append_call(p, a->kv, sms, stream);
 }
 
 size_t abft_paged_decode_workspace_bytes(const abft_paged_attn_args* a) {

@@ -46,6 +46,9 @@ struct AppendParams {
   int64_t tokens;
   int32_t heads;
   int32_t warps_shift;  // log2 of the warps that share a token
+};
+// With positions of the caller's.
+struct AppendAtParams : AppendParams {
   const int32_t* positions;  // [axes][position_stride]: what a token is rotated by, where that is not its slot's place
   int64_t position_stride;
   int32_t axes;
@@ -97,14 +100,16 @@ constexpr int kAppendWarps = 8;
 constexpr int kAppendThreads = 32 * kAppendWarps;
 
 //
-// kAxes: the rotation goes by positions of the caller's, of several axes (images
+// AppendAtParams: the rotation goes by positions of the caller's, of several axes (images
 // and video: time, height, width) or one (a drafted token's depth), each for its
 // share of the pairs:  (c_j, s_j) = rope[positions[axis of j][t]][j]. They are
 // asked for before the chain (sequence, length, page) begins. (Bound by HBM in large
 // calls: 10,400 tokens of 36 heads on three axes 34.9 us, 5.6 TB/s, with four CTAs an
 // SM; 35.6 with three.)
-template <int D, bool F16, bool kAxes = false>
-__global__ void __launch_bounds__(kAppendThreads, kAxes ? 4 : 3) kv_append_kernel(const AppendParams p) {
+template <int D, bool F16, typename Params>
+__global__ void __launch_bounds__(kAppendThreads, sizeof(Params) > sizeof(AppendParams) ? 4 : 3)
+    kv_append_kernel(const Params p) {
+  constexpr bool kAxes = sizeof(Params) > sizeof(AppendParams);
   constexpr int kChunks = D / 16;  // threads per row
   griddep_wait();
   constexpr int kRows = 32 / kChunks;  // rows a warp covers at once

@@ -223,7 +223,8 @@ int abft_kv_append_at(const abft_kv_append_at_args* a, void* stream) {
   if ((reinterpret_cast<uintptr_t>(a->positions) & 3u) != 0) return ABFT_ERR_ALIGNMENT;
   int dev = 0, sms = 0;
   if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
-  AppendParams p = append_params(&a->append);
+  AppendAtParams p;
+  append_params(&a->append, &p);
   p.positions = a->positions;
   p.position_stride = a->position_stride;
   p.axes = a->axes;
@@ -231,7 +232,7 @@ int abft_kv_append_at(const abft_kv_append_at_args* a, void* stream) {
     if (i < a->axes) end += a->sections[i];
     p.axis_end[i] = end;
   }
-  return append_call<true>(p, a->append.kv, sms, stream);
+  return append_call(p, a->append.kv, sms, stream);
 }
 
 size_t abft_paged_tree_workspace_bytes(const abft_paged_tree_args* t) {

@@ -163,8 +163,8 @@ inline int append_check(const abft_kv_append_args* a) {
   return ABFT_OK;
 }
 
-inline AppendParams append_params(const abft_kv_append_args* a) {
-  AppendParams p = {};
+inline void append_params(const abft_kv_append_args* a, AppendParams* to) {
+  AppendParams& p = *to;
   p.kv = view_of(a->kv);
   p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out;
   p.qt = a->q_token_stride, p.qh = a->q_head_stride;
@@ -176,24 +176,23 @@ inline AppendParams append_params(const abft_kv_append_args* a) {
   p.max_positions = a->max_positions;
   p.tokens = a->tokens;
   p.heads = a->heads;
-  return p;
 }
 
-template <int D, bool F16, bool kAxes>
-int launch_append(AppendParams p, int sms, cudaStream_t s) {
+template <int D, bool F16, typename Params>
+int launch_append(Params& p, int sms, cudaStream_t s) {
   // Halve the warps of a token while a full set of the SMs' blocks is left.
   p.warps_shift = 3;
   while (p.warps_shift > 0 && (p.tokens << (p.warps_shift - 1)) >= int64_t{16} * sms) --p.warps_shift;
   const int64_t blocks = ((p.tokens << p.warps_shift) + kAppendWarps - 1) / kAppendWarps + (p.cu != nullptr);
-  return launch(kv_append_kernel<D, F16, kAxes>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, s, p);
+  return launch(kv_append_kernel<D, F16, Params>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, s, p);
 }
 
-template <bool kAxes>
-int append_call(const AppendParams& p, const abft_paged_kv& kv, int sms, void* stream) {
+template <typename Params>
+int append_call(Params& p, const abft_paged_kv& kv, int sms, void* stream) {
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = kv.dtype == ABFT_DTYPE_F16;
-  if (kv.head_dim == 128) return f16 ? launch_append<128, true, kAxes>(p, sms, s) : launch_append<128, false, kAxes>(p, sms, s);
-  return f16 ? launch_append<64, true, kAxes>(p, sms, s) : launch_append<64, false, kAxes>(p, sms, s);
+  if (kv.head_dim == 128) return f16 ? launch_append<128, true>(p, sms, s) : launch_append<128, false>(p, sms, s);
+  return f16 ? launch_append<64, true>(p, sms, s) : launch_append<64, false>(p, sms, s);
 }
 
 // ---- decode -------------------------------------------------------------------

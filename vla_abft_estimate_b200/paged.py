@@ -331,17 +331,17 @@ class PagedKVCache:
         time, height and width. With several axes ``sections`` says how many
         pairs turn by each, in their order, head_dim / 2 in all.
         """
-        name = "abft_kv_append"
-        if positions is None:
-            if sections is not None:
-                raise ValueError("sections without positions")
+        if positions is None and sections is None:
             done = self._fast.append(q, k, v, rope, cu_seqlens, q_out)
+            if done is not None:
+                return done if type(done) is not int else N.check("abft_kv_append", done)
+        elif positions is None:
+            raise ValueError("sections without positions")
         else:
-            name = "abft_kv_append_at"
             positions, sections = self._axes(positions, sections)
             done = self._fast.append(q, k, v, rope, cu_seqlens, q_out, positions, sections)
-        if done is not None:
-            return done if type(done) is not int else N.check(name, done)
+            if done is not None:
+                return done if type(done) is not int else N.check("abft_kv_append_at", done)
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
                 return self.append(q, k, v, rope, cu_seqlens=cu_seqlens, q_out=q_out, positions=positions, sections=sections)
@@ -390,7 +390,9 @@ class PagedKVCache:
             by.positions, by.position_stride, by.axes = positions.data_ptr(), positions.stride(0), len(sections)
             for i, x in enumerate(sections):
                 by.sections[i] = x
-        self._call(name, args if positions is None else by)
+            self._call("abft_kv_append_at", by)
+        else:
+            self._call("abft_kv_append", args)
         self._written(self.k_pages, self.v_pages, q_out)
         return q_out
 
