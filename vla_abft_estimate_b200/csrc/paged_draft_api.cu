@@ -38,38 +38,56 @@ struct TreePlan {
   int grid;
 };
 
-// Short caches get a CTA per segment, or a cluster of up to 8 as long as all clusters
-// run at once (two CTAs an SM; 8 x 30 and 4 x 65 fit the device's groups of SMs). A
-// step takes 0.75 us, the join of a cluster 2.2, a second launch with its join 6 and
-// more the more pieces a segment has: one CTA up to 4 steps, or 16 where there are
-// segments for half of the CTAs; 12 steps for each CTA of a cluster, 16 where the list
-// would cut each segment into more than 24 pieces. Measured (28/4 heads of 128; one CTA
-// / cluster / list): 1 tree of 16 tokens on 112 slots 7.7 / 9.2 / - us, on 512
-// 12.7 / 9.6 / -, on 1,000 - / 10.3 / 13.7, on 4,000 - / 14.4 / 21.9, on 8,000 (16
-// steps a CTA) - / 20.8 / 26.5; 1 of 64 on 8,000 (16 steps, 18 pieces) - / 26.8 / 22.9;
-// 32 of 8 on 300 slots 10.9 / - / 18.8, on 1,000 21.6 / - / 27. (The lengths are on
-// the device: what is known here, and decides, is the width of the table.)
+// The list, or a CTA per segment, or a cluster of up to 8 as long as all clusters run
+// at once (two CTAs an SM; 8 x 30 and 4 x 65 fit the device's groups of SMs): whichever
+// takes least, counted in steps (0.85 us). The list evens out what sequences of unlike
+// length take, but its second launch and the pieces' way through memory cost 13; a
+// cluster's pieces go through the SMs' network, which is slow (25 GB/s an SM): 1 step
+// while 64 CTAs use it at once (one cluster of 8 in each group of SMs), above that 6, or
+// 3 with heads of 64. No more than 16 steps for a CTA: the lengths are on the device, what
+// is known here is the width of the table, and it is the longest sequence that the
+// others then wait for. Measured (us; 1, 2, 4, 8 CTAs / list; 28/4 heads of 128):
+//   1 tree of 16 tokens on 1,000 slots  18.7 14.4 11.0 10.0 / 11.9, 8,000  105 58 32.3 20.5 / 16.7
+//   4 of 16 on 1,000  18.9 14.6 11.5 14.2 / 14.8, 2,000  31.5 20.9 14.5 16.1 / 15.5, 4,000  57 34 21.2 19.2 / 21.8
+//   16 of 16 on 500  14.1 16.4 15.4 30.3 / 18.2, 2,000  34.1 28.0 21.8 37 / 26.8
+//   32 of 8 on 300  11.2 12.3 21.3 - / 17.9, 1,250  26.1 22.7 30.2 - / 29.2, on up to 1,200  20.9 16.6 19.2 - / 16.1
+//   8 of 16, heads of 64, on 500  11.7 10.3 12.5 13.7 / 13.9, 2,000  29.1 18.7 16.6 15.5 / 16.7
+constexpr int kTreeListSteps = 13, kTreeQuiet = 64, kTreeMostSteps = 16;
+
 int tree_plan(const abft_paged_attn_args* a, int sms, TreePlan* r) {
   r->tile_tokens = kTreeRows / (a->heads / a->kv.kv_heads);
-  // Segments at most (the boundaries are on the device), and steps of one.
-  const int64_t segments = a->kv.kv_heads * (a->kv.batch == 1 ? (a->tokens + r->tile_tokens - 1) / r->tile_tokens
-                                                              : a->tokens / r->tile_tokens + a->kv.batch);
+  // Segments at most (the boundaries are on the device), and as many as they are when
+  // all sequences have equally many rows.
+  const int64_t mean = a->kv.batch > 0 ? (a->tokens + a->kv.batch - 1) / a->kv.batch : 0;
+  auto most = [&](int tile) { return a->kv.kv_heads * (a->kv.batch == 1 ? (a->tokens + tile - 1) / tile : a->tokens / tile + a->kv.batch); };
+  auto likely = [&](int tile) { return a->kv.kv_heads * a->kv.batch * ((mean + tile - 1) / tile); };
+  const int64_t segments = likely(r->tile_tokens);
   const int64_t slots = static_cast<int64_t>(a->kv.max_pages) * a->kv.page_size;
   const int64_t steps = slots > kTreeKeys ? (slots + kTreeKeys - 1) / kTreeKeys : 1;
-  if (segments * (steps + kTreeCost) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;  // the list is counted in 32 bits
+  if (most(r->tile_tokens) * (steps + kTreeCost) >= (int64_t{1} << 31)) return ABFT_ERR_UNSUPPORTED;  // the list is counted in 32 bits
   const int ctas = 2 * sms;
   r->cluster = 0;
-  if (segments <= ctas) {
-    int c = 8 * segments <= ctas * 13 / 16 ? 8 : 4 * segments <= ctas * 7 / 8 ? 4 : 2 * segments <= ctas ? 2 : 1;
-    while (c > 1 && c / 2 >= steps) c /= 2;
-    if (steps <= 4) c = 1;
-    if (steps <= (c == 1 || 24 * segments <= ctas ? 16 : 12) * c) {
+  int64_t least = kTreeListSteps + segments * steps / ctas;
+  for (int c = 1; c <= 8 && c * segments <= ctas * (c == 8 ? 13 : c == 4 ? 14 : 16) / 16 && (c == 1 || c / 2 < steps); c *= 2) {
+    const int64_t per = (steps + c - 1) / c;
+    const int64_t time = per + (c == 1 ? 0 : c * segments <= kTreeQuiet ? 1 : a->kv.head_dim == 128 ? 6 : 3);
+    if (per <= kTreeMostSteps && time < least) {
+      least = time;
       r->cluster = c;
-      r->grid = static_cast<int>(segments) * c;
-      return ABFT_OK;
     }
   }
-  r->grid = static_cast<int>(segments * steps < ctas ? segments * steps : ctas);
+  if (r->cluster == 0) {
+    const int64_t places = most(r->tile_tokens) * steps;
+    r->grid = static_cast<int>(places < ctas ? places : ctas);
+    return ABFT_OK;
+  }
+  // Clusters of 8 with CTAs to spare take smaller tiles, of which less goes to and fro
+  // (1 tree of 16 tokens on 1,000 slots: 10.0 -> 9.0 us).
+  for (int half; r->cluster == 8 && r->tile_tokens > 1; r->tile_tokens = half) {
+    half = (r->tile_tokens + 1) / 2;
+    if (8 * likely(half) > kTreeQuiet) break;
+  }
+  r->grid = static_cast<int>(most(r->tile_tokens)) * r->cluster;  // those without a segment end at once
   return ABFT_OK;
 }
 

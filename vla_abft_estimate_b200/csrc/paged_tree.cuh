@@ -62,8 +62,8 @@ struct TreeCfg {
   static constexpr int kOffItems = kOffMisc + 16;
   static constexpr int kOffUp = kOffItems + 2 * 48;  // parents of the items in the two slots
   static constexpr int kSmemBytes = kOffUp + 2 * kTreeHeld * 4 + 1024;
-  // A cluster's pieces take the ring's place: O as [D / 4][rows] float4, then (m, l).
-  static_assert(kTreeRows * (D * 4 + 8) <= kQBytes + kSlots * kTileBytes, "a piece's place");
+  // A cluster's pieces take the tiles' place: D / 4 quads of sums a row, then (m, l) of each piece.
+  static_assert(kTreeRows * (D * 4 + kDecCluster * 8) <= kQBytes + kSlots * kTileBytes, "the pieces' place");
   static_assert(kSmemBytes <= 115 * 1024, "two CTAs per SM");
   // TMEM columns: two S (P over the first half of each), then O.
   static constexpr int kTmemCols = 256, kColO = 128;
@@ -345,60 +345,76 @@ __device__ __forceinline__ void list_tree(const TreeParams& p, TreeItem* items, 
 __device__ __forceinline__ uint16_t* tree_out(const TreeParams& p, int64_t first, int hk, int r, int token) {
   return static_cast<uint16_t*>(p.out) + (first + token) * p.ot + (hk * p.group + (r - token * p.group)) * p.oh;
 }
-template <bool F16>
-__device__ __forceinline__ void tree_store8(uint16_t* dst, const float4& a, const float4& b, float f) {
-  *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<F16>(a.x * f, a.y * f), pack2<F16>(a.z * f, a.w * f),
-                                              pack2<F16>(b.x * f, b.y * f), pack2<F16>(b.z * f, b.w * f));
-}
 
-// The pieces of a cluster's CTAs, in their order; each CTA joins every cluster-th
-// pair of 8 columns, a thread a row. (The second barrier orders nothing but the end of
-// the reads: with the release of the results' stores in it, it took 1.5 us.)
+// The pieces of a cluster's CTAs: each CTA joins D / cluster columns. The rows of each
+// send every CTA its part of their sums, from TMEM into its shared memory, where all
+// pieces then lie, in their order. (Each CTA reading its part out of the others' took
+// 2.6 us, and one more barrier.) All threads of the cluster come here; `m` and `l` are
+// those of the row, -infinity and 0 where it saw nothing.
 template <int D, bool F16>
-__device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const TreeItem& x, uint32_t area) {
-  cluster_barrier();
-  constexpr int kSides = kTreeThreads / kTreeRows;
-  const int r = threadIdx.x & (kTreeRows - 1), rank = static_cast<int>(blockIdx.x) & (p.work.cluster - 1);
-  const int token = row_token(r, p.group_inv);
+__device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const TreeItem& x, uint8_t* smem, uint32_t row_tmem, float m,
+                                                  float l) {
+  constexpr int kQuads = D / 4;
+  const int cluster = p.work.cluster, shift = p.work.cluster_shift, rank = static_cast<int>(blockIdx.x) & (cluster - 1);
+  const int per = kQuads >> shift;  // a CTA's columns, by four
+  const int per_shift = (D == 128 ? 5 : 4) - shift;
+  const int r = threadIdx.x & (kTreeRows - 1), token = row_token(r, p.group_inv);
   const bool live = token < min(p.tile_tokens, x.n - x.tok0);
-  float4 v[kDecCluster][2];
-  float2 ml[kDecCluster];
-  uint16_t* dst = tree_out(p, x.row0 + x.tok0, x.hk, r, token);
+  float4* sums = reinterpret_cast<float4*>(smem);                                // [piece][per][row]
+  float2* sums_ml = reinterpret_cast<float2*>(smem + kQuads * kTreeRows * 16);   // [piece][row]
+  cluster_barrier();  // nobody's products read the tiles any more
+  tc_fence_after();
+  if (__any_sync(0xFFFFFFFFu, live)) {
+    if (x.j0 < x.j1) {
 #pragma unroll 1
-  for (int col = rank * kSides + threadIdx.x / kTreeRows; col < D / 8; col += p.work.cluster * kSides) {
-    if (!live) break;
-    // All asked for before the first is used.
+      for (int c = threadIdx.x / kTreeRows * 32; c < D; c += kTreeThreads / kTreeRows * 32) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(row_tmem + c, o);
+        tmem_ld_wait();
 #pragma unroll
-    for (int c = 0; c < kDecCluster; ++c) {
-      ml[c] = make_float2(-INFINITY, 0.f);
-      if (c < p.work.cluster) {
-        ml[c] = ld_cluster_f2(map_rank(area + kTreeRows * D * 4 + r * 8, c));
-#pragma unroll
-        for (int k = 0; k < 2; ++k) v[c][k] = ld_cluster_f4(map_rank(area + ((col * 2 + k) * kTreeRows + r) * 16, c));
+        for (int k = 0; k < 8; ++k) {
+          const int quad = c / 4 + k, to = quad >> per_shift;
+          if (live)
+            st_cluster_f4(map_rank(smem_u32(sums + (rank * per + (quad & (per - 1))) * kTreeRows + r), to),
+                          make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
+                                      __uint_as_float(o[4 * k + 3])));
+        }
       }
     }
-    float top = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int c = 0; c < kDecCluster; ++c) top = fmaxf(top, ml[c].x);
-    const float ms = top == -INFINITY ? 0.f : top;
-    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll
-    for (int c = 0; c < kDecCluster; ++c) {
-      if (ml[c].y == 0.f) continue;  // no piece, or the row saw nothing of it: not written
-      const float f = exp2_approx(ml[c].x - ms);
-      l += ml[c].y * f;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        o[k].x += v[c][k].x * f;
-        o[k].y += v[c][k].y * f;
-        o[k].z += v[c][k].z * f;
-        o[k].w += v[c][k].w * f;
-      }
-    }
-    tree_store8<F16>(dst + col * 8, o[0], o[1], l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
+    if (live && threadIdx.x < kTreeRows)
+      for (int to = 0; to < cluster; ++to) st_cluster_f2(map_rank(smem_u32(sums_ml + rank * kTreeRows + r), to), make_float2(m, l));
   }
-  // Shared memory stays until it has been read.
-  asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
+  cluster_barrier();
+  if (!live) return;
+  float2 ml[kDecCluster];
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < kDecCluster; ++c) {
+    ml[c] = c < cluster ? sums_ml[c * kTreeRows + r] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[c].x);
+  }
+  if (top == -INFINITY) top = 0.f;
+#pragma unroll
+  for (int c = 0; c < kDecCluster; ++c) {
+    ml[c].x = exp2_approx(ml[c].x - top);
+    if (ml[c].y != 0.f) sum += ml[c].x * ml[c].y;
+  }
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  uint16_t* dst = tree_out(p, x.row0 + x.tok0, x.hk, r, token);
+  for (int quad = threadIdx.x / kTreeRows; quad < per; quad += kTreeThreads / kTreeRows) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kDecCluster; ++c) {
+      if (ml[c].y == 0.f) continue;  // its sums may not have been written
+      const float4 v = sums[(c * per + quad) * kTreeRows + r];
+      o.x += v.x * ml[c].x;
+      o.y += v.y * ml[c].x;
+      o.z += v.z * ml[c].x;
+      o.w += v.w * ml[c].x;
+    }
+    *reinterpret_cast<uint2*>(dst + (rank * per + quad) * 4) =
+        make_uint2(pack2<F16>(o.x * inv, o.y * inv), pack2<F16>(o.z * inv, o.w * inv));
+  }
 }
 
 template <int D, bool F16>
@@ -476,6 +492,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     return x->valid != 0;
   };
 
+  float row_m = -INFINITY, row_l = 0.f;  // of a cluster's one item
   if (warp < 4) {
     // ------------------------------------------------------------ softmax rows
     const int r = threadIdx.x;
@@ -607,11 +624,15 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
         free_slot(i);
         continue;
       }
-      // Sums of a piece go to its place, or, for the cluster, to that of the ring (which
-      // nothing is loaded into any more).
+      if (p.work.cluster > 1) {  // joined below
+        row_m = any ? m * p.scale_log2 : -INFINITY;
+        row_l = any ? l : 0.f;
+        break;
+      }
+      // Sums of a piece go to its place.
       const int64_t place = static_cast<int64_t>(blockIdx.x) * 2 + max(x.place, 0);
-      float4* sums = p.work.cluster > 0 ? reinterpret_cast<float4*>(smem) : p.work.part + place * (D / 4) * kTreeRows;
-      float2* sums_ml = p.work.cluster > 0 ? reinterpret_cast<float2*>(smem + kTreeRows * D * 4) : p.work.part_ml + place * kTreeRows;
+      float4* sums = p.work.part + place * (D / 4) * kTreeRows;
+      float2* sums_ml = p.work.part_ml + place * kTreeRows;
       uint16_t* dst = tree_out(p, x.row0 + x.tok0, x.hk, r, token);
       if (live && x.place >= 0) sums_ml[r] = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
       if (!any) {  // no keys
@@ -825,7 +846,8 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     if (brought > 0) mbar_wait_bounded(qfull, (brought - 1) & 1);
   }
   __syncthreads();
-  if (p.work.cluster > 1 && items[0].valid) join_tree_cluster<D, F16>(p, items[0], smem_u32(smem));
+  if (p.work.cluster > 1 && items[0].valid)
+    join_tree_cluster<D, F16>(p, items[0], smem, tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Cfg::kColO, row_m, row_l);
   if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   tc_fence_after();
   if (warp == 5) tmem_dealloc(tmem, Cfg::kTmemCols);
