@@ -9,7 +9,11 @@
 // tokens of a group of 7) and caches long: every key and value is read once for a
 // tile's rows, which the tensor cores take in faster than HBM gives it (32 KB of 64
 // keys: 0.74 us of an SM's share of HBM, 0.4 us of products). What counts is that
-// all SMs read all the time, and, for short caches, the chain of latencies.
+// all SMs read all the time, and, for short caches, the chain of latencies. (Rows of
+// small tiles spread over idle warps, a part of the keys each, so that a step's
+// exponentials take a quarter of the time: steps came no faster, being bound by the
+// reads, and the warps' sums had to be added up: 12 trees of up to 13 tokens, 32 heads,
+// 25.4 -> 30.5 us.)
 //
 // A CTA takes one tile of 128 rows of one kv head, in steps of 64 keys:
 //   S = Q K^T   tcgen05.mma, S in TMEM, two of them: the next one is computed
@@ -20,15 +24,17 @@
 // half of an SM's registers, shared memory and TMEM: two CTAs an SM, of which one
 // reads while the other begins, ends or changes its segment. (One CTA with two row
 // groups on steps of 128 keys of the same segment, the causal kernel's form for few
-// rows: 32 trees of 4 tokens of 32 heads on 512 slots 80 us, 55 so; up to 26 tokens on
-// up to 4,122 slots 29, 24; 64 trees of 8 on 8,188 slots 198, 174, where HBM's time is
-// 165.)
+// rows: 32 trees of 4 tokens of 32 heads on 512 slots 80 us, 54 so; up to 26 tokens on
+// up to 4,122 slots 29, 22.7; 64 trees of 8 on 8,188 slots 198, 175, where HBM's time is
+// 165.) One tree of 64 tokens on 131,008 slots takes 140 us where 73 are HBM's and the
+// products' time: each of its four tiles takes in all keys and values by itself, 1.07 GB
+// at the 62 GB/s that an SM takes in.
 //
 // Work: a call's steps over all (sequence, kv head, block of rows) segments are one
 // list, cut into equal shares for two CTAs per SM. A segment inside a share is
 // finished by its CTA; pieces of one that crosses CTAs are joined by a second, small
-// kernel, in a fixed order. Short caches get a cluster of CTAs per segment, joined
-// through shared memory in the one launch.
+// kernel, in a fixed order. Short caches get a CTA or a cluster of CTAs per segment,
+// whose sums meet in shared memory, in the one launch.
 //
 // Warps: 0-3 the rows (TMEM lane quadrant = warp), 4 TMA loads of pages into a ring
 // of tiles, 5 the MMA issuer, 6 finds the work, 7 brings query rows and parents.
@@ -70,9 +76,10 @@ struct TreeCfg {
 };
 
 // Places in the list that a segment takes before its first step, for its start and
-// end (trees of up to 26 tokens on up to 4,122 slots: 26.1 us with 1, 25.1 with 2,
-// 24.4 with 4, 24.6 with 6).
-constexpr int kTreeCost = 4;
+// end (1, 2, 3, 4 of them: 24 trees of up to 26 tokens on up to 4,122 slots 23.9, 22.8,
+// 22.7, 22.8 us; 96 of up to 8 on up to 2,000  29.6, 28.6, 27.6, 29.1; 8 of up to 4, 32
+// heads, on up to 1,200  15.0, 17.1, 19.2, 19.3).
+constexpr int kTreeCost = 3;
 
 struct TreeWork {
   const int32_t* parents;  // [tokens]
