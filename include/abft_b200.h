@@ -548,7 +548,8 @@ int abft_kv_append_at(const abft_kv_append_at_args* args, void* stream);
  * used (the call's work is shared out to num_sms SMs), and q's strides, which are
  * above 0 where there is more than one row or head. A parent that is below -1 or
  * does not come before its child sets ABFT_PAGED_BAD_DRAFT; the way up ends
- * there. */
+ * there. A call of 2^31 places or more (tiles of rows * kv heads * steps of 64
+ * slots of the table's width) is ABFT_ERR_UNSUPPORTED. */
 typedef struct abft_paged_tree_args {
   abft_paged_attn_args attn;
   const int32_t* parents;      /* [tokens]                                               */
