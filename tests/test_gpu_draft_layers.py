@@ -125,6 +125,31 @@ def test_accept_bad_boundaries(cuda_device):
             layers.check_status()
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("n", [1, 2, 7])
+def test_accept_results_are_tensors_of_their_own(cuda_device, dtype, n):
+    dev = cuda_device
+    trees = [chain(n)] * 3
+    layers = layers_of(dev, [1] * 3, layers=1)
+    cu, parents = packed(trees)
+    ids = torch.ones(3 * n, dtype=dtype, device=dev)
+    for inference in (False, True):
+        with torch.inference_mode(inference):
+            got = layers.accept(i32(cu, dev), i32(parents, dev), ids, ids)
+            want = [list(range(n)) * 3, [n] * 3, [1] * 3]
+            assert [x.tolist() for x in got] == want
+            assert all(x.is_contiguous() and not x._is_view() and x.is_inference() == inference for x in got)
+            before = [0 if inference else x._version for x in got]
+            for k, x in enumerate(got):  # a write reaches one of them only
+                x.fill_(-9)
+                want[k] = [-9] * len(want[k])
+                assert [y.tolist() for y in got] == want
+                assert inference or [y._version - v for y, v in zip(got, before)] == [int(j <= k) for j in range(3)]
+        kept = got[0].clone()
+        del got
+        assert kept.tolist() == [-9] * (3 * n)
+
+
 def test_accept_refusals(cuda_device):
     dev = cuda_device
     layers = layers_of(dev, [9, 9], layers=1)

@@ -1,5 +1,6 @@
 """Tree attention over the paged cache against the plain 64-bit form."""
 import math
+import random
 
 import pytest
 import torch
@@ -295,6 +296,20 @@ def test_uneven_small_trees(cuda_device, columns):
         total = [1, 900, 0, 40, 0, 33, 700, 64, 0, 300, 2, 129]
         run_tree(cuda_device, [random_tree(n, seed + n) for n in sizes], total, 12, 2, 128, 16, BF16, seed=seed, pad=5,
                  extra_columns=columns)
+
+
+# By the number of segments and the table's width one to eight CTAs share a segment,
+# with tiles of 128 rows or less.
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("batch,n,slots,d", [(1, 16, 1000, 128), (1, 5, 1000, 64), (1, 64, 1000, 128), (4, 16, 1000, 128),
+                                             (4, 16, 3900, 128), (8, 16, 500, 64), (8, 16, 1000, 64), (8, 16, 2000, 64),
+                                             (16, 16, 500, 128), (16, 16, 1000, 128), (32, 8, 1200, 128), (9, 30, 700, 128)])
+def test_segments_shared_by_some_ctas(cuda_device, batch, n, slots, d, ragged):
+    r = random.Random(batch * slots)
+    sizes = [r.choice([0, 1, n // 2, n, n]) if ragged else n for _ in range(batch - 1)] + [n]
+    total = [r.randrange(x, slots) if ragged else slots - b for b, x in enumerate(sizes)]
+    run_tree(cuda_device, [random_tree(x, 5 + i) for i, x in enumerate(sizes)], total, 28, 4, d, 16, F16 if ragged else BF16,
+             seed=batch, pad=3 * ragged)
 
 
 def test_long_caches_of_small_trees(cuda_device):

@@ -356,8 +356,9 @@ __device__ __forceinline__ uint16_t* tree_out(const TreeParams& p, int64_t first
 // The pieces of a cluster's CTAs: each CTA joins D / cluster columns. The rows of each
 // send every CTA its part of their sums, from TMEM into its shared memory, where all
 // pieces then lie, in their order. (Each CTA reading its part out of the others' took
-// 2.6 us, and one more barrier.) All threads of the cluster come here; `m` and `l` are
-// those of the row, -infinity and 0 where it saw nothing.
+// 2.6 us, and one more barrier.) All threads of the cluster come here, with or without
+// an item, so that no CTA has ended when another sends to it; `m` and `l` are those of
+// the row, -infinity and 0 where it saw nothing.
 template <int D, bool F16>
 __device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const TreeItem& x, uint8_t* smem, uint32_t row_tmem, float m,
                                                   float l) {
@@ -366,7 +367,7 @@ __device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const Tre
   const int per = kQuads >> shift;  // a CTA's columns, by four
   const int per_shift = (D == 128 ? 5 : 4) - shift;
   const int r = threadIdx.x & (kTreeRows - 1), token = row_token(r, p.group_inv);
-  const bool live = token < min(p.tile_tokens, x.n - x.tok0);
+  const bool live = x.valid && token < min(p.tile_tokens, x.n - x.tok0);
   float4* sums = reinterpret_cast<float4*>(smem);                                // [piece][per][row]
   float2* sums_ml = reinterpret_cast<float2*>(smem + kQuads * kTreeRows * 16);   // [piece][row]
   cluster_barrier();  // nobody's products read the tiles any more
@@ -853,7 +854,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     if (brought > 0) mbar_wait_bounded(qfull, (brought - 1) & 1);
   }
   __syncthreads();
-  if (p.work.cluster > 1 && items[0].valid)
+  if (p.work.cluster > 1)
     join_tree_cluster<D, F16>(p, items[0], smem, tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Cfg::kColO, row_m, row_l);
   if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   tc_fence_after();
