@@ -9,11 +9,13 @@
 // tokens of a group of 7) and caches long: every key and value is read once for a
 // tile's rows, which the tensor cores take in faster than HBM gives it (32 KB of 64
 // keys: 0.74 us of an SM's share of HBM, 0.4 us of products). What counts is that
-// all SMs read all the time, and, for short caches, the chain of latencies. (Rows of
-// small tiles spread over idle warps, a part of the keys each, so that a step's
-// exponentials take a quarter of the time: steps came no faster, being bound by the
-// reads, and the warps' sums had to be added up: 12 trees of up to 13 tokens, 32 heads,
-// 25.4 -> 30.5 us.)
+// all SMs read all the time, and, for short caches, the chain of latencies. A step
+// takes the issuing warp 1,400 cycles (heads of 64) to 1,700, and the row warps 1,370,
+// which is what small tiles are bound by, with one CTA on an SM or two. (Shorter
+// alone was either, and the whole no faster: rows of small tiles spread over idle warps,
+// a part of the keys each, 770 cycles, but the warps' sums had to be added up, 12
+// trees of up to 13 tokens of 32 heads 25.4 -> 30.7 us; a step's waits first and its
+// products in one go, 800 cycles, 25.4 -> 25.6, 24 of up to 26 22.8 -> 23.2.)
 //
 // A CTA takes one tile of 128 rows of one kv head, in steps of 64 keys:
 //   S = Q K^T   tcgen05.mma, S in TMEM, two of them: the next one is computed
