@@ -251,8 +251,9 @@ __device__ __forceinline__ void tree_locate(const TreeParams& p, int lane, TreeS
   out->seq.bad = false;
   if (work.cluster > 0) {
     out->y = at - before;
-    out->u = out->step = share_start(out->seq.steps, work.cluster, rank);
-    out->u1 = share_start(out->seq.steps, work.cluster, rank + 1);
+    const int base = out->seq.steps >> work.cluster_shift, rest = out->seq.steps & (work.cluster - 1);  // share_start()
+    out->u = out->step = rank * base + min(rank, rest);
+    out->u1 = out->u + base + (rank < rest);
   } else {
     const int per = out->seq.steps + kTreeCost, in = at - before;
     out->y = in / per;
@@ -372,7 +373,8 @@ __device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const Tre
   const bool live = x.valid && token < min(p.tile_tokens, x.n - x.tok0);
   float4* sums = reinterpret_cast<float4*>(smem);                                // [piece][per][row]
   float2* sums_ml = reinterpret_cast<float2*>(smem + kQuads * kTreeRows * 16);   // [piece][row]
-  cluster_barrier();  // nobody's products read the tiles any more
+  // Nobody's products read the tiles any more (they have ended: no write is to be seen).
+  asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
   tc_fence_after();
   if (__any_sync(0xFFFFFFFFu, live)) {
     if (x.j0 < x.j1) {
