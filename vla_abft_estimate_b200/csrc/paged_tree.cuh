@@ -379,7 +379,8 @@ __device__ __forceinline__ void join_tree_cluster(const TreeParams& p, const Tre
   if (__any_sync(0xFFFFFFFFu, live)) {
     if (x.j0 < x.j1) {
 #pragma unroll 1
-      for (int c = threadIdx.x / kTreeRows * 32; c < D; c += kTreeThreads / kTreeRows * 32) {
+      for (int i = threadIdx.x / kTreeRows; i < D / 32; i += kTreeThreads / kTreeRows) {
+        const int c = ((i + (rank >> 1)) & (D / 32 - 1)) * 32;  // not all to the same CTA at once
         uint32_t o[32];
         tmem_ld_32x32b_x32(row_tmem + c, o);
         tmem_ld_wait();
