@@ -966,6 +966,7 @@ __global__ void __launch_bounds__(kTreeJoinThreads, 4) paged_tree_join_kernel(co
   __shared__ float2 s_ml[kTreeJoinSlots * kTreeJoinThreads];
   const int lane = threadIdx.x & 31;
   griddep_wait();
+  griddep_launch();
   int before = 0, unit = blockIdx.x;
   constexpr int kLook = 10;  // CTAs that a lane looks at
 #pragma unroll 1
