@@ -47,11 +47,11 @@ struct TreePlan {
 // 3 with heads of 64. No more than 16 steps for a CTA: the lengths are on the device, what
 // is known here is the width of the table, and it is the longest sequence that the
 // others then wait for. Measured (us; 1, 2, 4, 8 CTAs / list; 28/4 heads of 128):
-//   1 tree of 16 tokens on 1,000 slots  18.7 14.4 11.0 10.0 / 11.9, 8,000  105 58 32.3 20.5 / 16.7
-//   4 of 16 on 1,000  18.9 14.6 11.5 14.2 / 14.8, 2,000  31.5 20.9 14.5 16.1 / 15.5, 4,000  57 34 21.2 19.2 / 21.8
-//   16 of 16 on 500  14.1 16.4 15.4 30.3 / 18.2, 2,000  34.1 28.0 21.8 37 / 26.8
-//   32 of 8 on 300  11.2 12.3 21.3 - / 17.9, 1,250  26.1 22.7 30.2 - / 29.2, on up to 1,200  20.9 16.6 19.2 - / 16.1
-//   8 of 16, heads of 64, on 500  11.7 10.3 12.5 13.7 / 13.9, 2,000  29.1 18.7 16.6 15.5 / 16.7
+//   1 tree of 16 tokens on 1,000 slots  18.3 13.9 10.6 9.2 / 10.9, 8,000  104 57 31.9 19.8 / 16.6
+//   4 of 16 on 1,000  18.4 14.2 11.1 13.1 / 14.3, 2,000  31.0 20.6 14.1 14.7 / 16.8, 4,000  57 33.7 20.9 18.4 / 21.8
+//   16 of 16 on 500  14.0 15.8 15.8 - / 17.5, 2,000  34.1 27.4 22.4 - / 28.3
+//   32 of 8 on 300  10.9 11.6 - - / 17.1, 1,250  26.1 21.8 - - / 28.4, on up to 1,200  20.8 16.0 - - / 15.3
+//   8 of 16, heads of 64, on 500  11.7 10.1 10.8 12.7 / 13.2, 2,000  29.0 18.4 15.2 15.3 / 15.2
 constexpr int kTreeListSteps = 13, kTreeQuiet = 64, kTreeMostSteps = 16;
 
 int tree_plan(const abft_paged_attn_args* a, int sms, TreePlan* r) {
@@ -82,7 +82,7 @@ int tree_plan(const abft_paged_attn_args* a, int sms, TreePlan* r) {
     return ABFT_OK;
   }
   // Clusters of 8 with CTAs to spare take smaller tiles, of which less goes to and fro
-  // (1 tree of 16 tokens on 1,000 slots: 10.0 -> 9.0 us).
+  // (1 tree of 16 tokens on 1,000 slots: 9.2 -> 8.3 us).
   for (int half; r->cluster == 8 && r->tile_tokens > 1; r->tile_tokens = half) {
     half = (r->tile_tokens + 1) / 2;
     if (8 * likely(half) > kTreeQuiet) break;
