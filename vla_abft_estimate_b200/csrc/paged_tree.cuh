@@ -879,39 +879,37 @@ constexpr int kTreeJoinSlots = 16;
 // log2 of a unit's (row, 4 columns): a round has all pieces of up to 16.
 __device__ __forceinline__ int tree_join_shift(int pieces) { return pieces <= 4 ? 9 : pieces <= 8 ? 8 : pieces <= 16 ? 7 : 5; }
 
-template <int D, bool F16, int kParts, int kIdx>
+template <int D, bool F16, int kParts, int kQuads>
 __device__ __forceinline__ void join_tree_unit(const TreeParams& p, int c, int pieces, int rows, int unit, float4* s_o, float2* s_ml) {
   constexpr int kLane = kTreeJoinThreads / kParts;  // threads of a part
   const int part = kParts == 1 ? 0 : threadIdx.x / kLane;
-  const int i0 = unit * (kLane * kIdx) + threadIdx.x - part * kLane, all = rows * (D / 4);
+  const int mine = unit * kLane + threadIdx.x - part * kLane, all = rows * (D / 4 / kQuads);
+  const int index = min(mine, all - 1);  // behind the end the last one again, which is not written
   const int2 spill = p.work.spill[c];
   const uint32_t rows_inv = ((1u << 20) + rows - 1) / rows;
   const uint32_t to = smem_u32(s_o + threadIdx.x), to_ml = smem_u32(s_ml + threadIdx.x);
-  int row[kIdx], col[kIdx];
-  float m[kIdx], l[kIdx];
-  float4 o[kIdx];
+  // index / rows: exact, since the product overshoots by less than index / 2^20 < 1 / rows.
+  const int group = static_cast<int>(static_cast<uint32_t>(index) * rows_inv >> 20), row = index - group * rows;
+  float m = -INFINITY, l = 0.f;
+  float4 o[kQuads];
 #pragma unroll
-  for (int i = 0; i < kIdx; ++i) {
-    const int index = min(i0 + i * kLane, all - 1);  // behind the end the last one again, which is not written
-    // index / rows: exact, since the product overshoots by less than index / 2^20 < 1 / rows.
-    col[i] = static_cast<int>(static_cast<uint32_t>(index) * rows_inv >> 20);
-    row[i] = index - col[i] * rows;
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  auto add = [&](int i, const float2 ml, const float4 v) {
-    const float top = fmaxf(m[i], ml.x), ms = top == -INFINITY ? 0.f : top;
-    const float f = exp2_approx(m[i] - ms), f2 = exp2_approx(ml.x - ms);
+  for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float2 ml, const float4* v, int stride) {
+    const float top = fmaxf(m, ml.x), ms = top == -INFINITY ? 0.f : top;
+    const float f = exp2_approx(m - ms), f2 = exp2_approx(ml.x - ms);
     const bool any = ml.y != 0.f;  // what a row saw nothing of was not written
-    m[i] = top;
-    l[i] = l[i] * f + ml.y * f2;
-    o[i].x = o[i].x * f + (any ? v.x * f2 : 0.f);
-    o[i].y = o[i].y * f + (any ? v.y * f2 : 0.f);
-    o[i].z = o[i].z * f + (any ? v.z * f2 : 0.f);
-    o[i].w = o[i].w * f + (any ? v.w * f2 : 0.f);
+    m = top;
+    l = l * f + ml.y * f2;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const float4 x = v[i * stride];
+      o[i].x = o[i].x * f + (any ? x.x * f2 : 0.f);
+      o[i].y = o[i].y * f + (any ? x.y * f2 : 0.f);
+      o[i].z = o[i].z * f + (any ? x.z * f2 : 0.f);
+      o[i].w = o[i].w * f + (any ? x.w * f2 : 0.f);
+    }
   };
-  constexpr int kAtOnce = kTreeJoinSlots / kIdx;  // pieces
+  constexpr int kAtOnce = kTreeJoinSlots / kQuads;  // pieces
 #pragma unroll 1
   for (int s0 = part; s0 < pieces; s0 += kParts * kAtOnce) {
 #pragma unroll
@@ -920,44 +918,37 @@ __device__ __forceinline__ void join_tree_unit(const TreeParams& p, int c, int p
       if (piece >= pieces) break;
       // (Places stay below 2^14, sums below 2^26 float4.)
       const int at = (c + piece) * 2 + (piece == 0 ? 1 : 0);
+      const float4* from = p.work.part + ((at * (D / 4) + group * kQuads) * kTreeRows + row);
 #pragma unroll
-      for (int i = 0; i < kIdx; ++i) {
-        const int slot = (k * kIdx + i) * kTreeJoinThreads;
-        cp_async16(to + slot * 16, p.work.part + ((at * (D / 4) + col[i]) * kTreeRows + row[i]), 16u);
-        cp_async8(to_ml + slot * 8, p.work.part_ml + (at * kTreeRows + row[i]));
-      }
+      for (int i = 0; i < kQuads; ++i) cp_async16(to + (k * kQuads + i) * kTreeJoinThreads * 16, from + i * kTreeRows, 16u);
+      cp_async8(to_ml + k * kTreeJoinThreads * 8, p.work.part_ml + (at * kTreeRows + row));
     }
     cp_async_commit();
     cp_async_wait<0>();
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
       if (s0 + k * kParts >= pieces) break;
-#pragma unroll
-      for (int i = 0; i < kIdx; ++i) {
-        const int slot = (k * kIdx + i) * kTreeJoinThreads + threadIdx.x;
-        add(i, s_ml[slot], s_o[slot]);
-      }
+      add(s_ml[k * kTreeJoinThreads + threadIdx.x], s_o + k * kQuads * kTreeJoinThreads + threadIdx.x, kTreeJoinThreads);
     }
   }
   if constexpr (kParts > 1) {
-    static_assert(kIdx == 1, "one place for a thread's sums");
+    static_assert(kQuads == 1, "one place for a thread's sums");
     __syncthreads();
-    s_ml[threadIdx.x] = make_float2(m[0], l[0]);
+    s_ml[threadIdx.x] = make_float2(m, l);
     s_o[threadIdx.x] = o[0];
     __syncthreads();
     if (part == 0)
 #pragma unroll
-      for (int k = 1; k < kParts; ++k) add(0, s_ml[k * kLane + threadIdx.x], s_o[k * kLane + threadIdx.x]);
+      for (int k = 1; k < kParts; ++k) add(s_ml[k * kLane + threadIdx.x], s_o + k * kLane + threadIdx.x, 0);
     __syncthreads();  // read before the next unit's sums come
     if (part > 0) return;
   }
+  if (mine >= all) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  uint16_t* dst = tree_out(p, spill.y, spill.x, row, row_token(row, p.group_inv)) + group * kQuads * 4;
 #pragma unroll
-  for (int i = 0; i < kIdx; ++i) {
-    if (i0 + i * kLane >= all) continue;
-    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
-    uint16_t* dst = tree_out(p, spill.y, spill.x, row[i], row_token(row[i], p.group_inv)) + col[i] * 4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<F16>(o[i].x * inv, o[i].y * inv), pack2<F16>(o[i].z * inv, o[i].w * inv));
-  }
+  for (int i = 0; i < kQuads; ++i)
+    *reinterpret_cast<uint2*>(dst + i * 4) = make_uint2(pack2<F16>(o[i].x * inv, o[i].y * inv), pack2<F16>(o[i].z * inv, o[i].w * inv));
 }
 
 template <int D, bool F16>
