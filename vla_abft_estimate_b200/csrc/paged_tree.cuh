@@ -93,7 +93,7 @@ struct TreeWork {
   float4* part;            // [grid][2][head_dim / 4][128]
   float2* part_ml;         // [grid][2][128] (m, l)
   // The segment that begins in this CTA and ends in a later one: its pieces (0: there
-  // is none) + rows << 16, and (kv head, first packed row).
+  // is none) + rows << 14 + units of its join << 22, and (kv head, first packed row).
   int32_t* pieces;         // [grid]
   int2* spill;             // [grid]
 };
@@ -285,8 +285,12 @@ struct __align__(16) TreeItem {
 };
 static_assert(sizeof(TreeItem) == 48, "items' place in shared memory");
 
+// log2 of a unit's (row, 4 columns): a round has all pieces of up to 16.
+__device__ __forceinline__ int tree_join_shift(int pieces) { return pieces <= 4 ? 9 : pieces <= 8 ? 8 : pieces <= 16 ? 7 : 5; }
+
 // The work warp: this CTA's share of the list (or of its cluster's segment), item by
 // item into the two slots.
+template <int D>
 __device__ __forceinline__ void list_tree(const TreeParams& p, TreeItem* items, uint64_t* item_full, uint64_t* item_empty,
                                           volatile int* abort_flag, int lane) {
   const PagedView& kv = p.kv;
@@ -318,7 +322,8 @@ __device__ __forceinline__ void list_tree(const TreeParams& p, TreeItem* items, 
       x.j1 = min(end, most);
       if (!single && at.step == 0 && end < at.seq.steps) {
         pieces = share_of(at.total, at.shares, at.u + at.seq.steps - 1) - static_cast<int>(blockIdx.x) + 1;
-        pieces |= (last + 1 - x.tok0) * p.group << 16;
+        const int rows = (last + 1 - x.tok0) * p.group, shift = tree_join_shift(pieces);
+        pieces |= rows << 14 | (rows * (D / 4) + (1 << shift) - 1) >> shift << 22;
         spill = make_int2(x.hk, x.row0 + x.tok0);
       }
     }
@@ -828,7 +833,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     __syncwarp();
     mbar_wait_bounded(drain, 0);
   } else if (warp == 6) {
-    list_tree(p, items, item_full, item_empty, abort_flag, lane);
+    list_tree<D>(p, items, item_full, item_empty, abort_flag, lane);
   } else {
     // ------------------------------------------------------------ query rows and parents
     // Query rows by one box for each 64 columns, (token, head) rows of the tile, once
@@ -875,9 +880,6 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
 // block's work of all segments are one list, dealt to the blocks in turn.
 constexpr int kTreeJoinThreads = 128;
 constexpr int kTreeJoinSlots = 16;
-
-// log2 of a unit's (row, 4 columns): a round has all pieces of up to 16.
-__device__ __forceinline__ int tree_join_shift(int pieces) { return pieces <= 4 ? 9 : pieces <= 8 ? 8 : pieces <= 16 ? 7 : 5; }
 
 template <int D, bool F16, int kParts, int kQuads>
 __device__ __forceinline__ void join_tree_unit(const TreeParams& p, int c, int pieces, int rows, int unit, float4* s_o, float2* s_ml) {
@@ -968,13 +970,8 @@ __global__ void __launch_bounds__(kTreeJoinThreads, 4) paged_tree_join_kernel(co
       const int c = c0 + lane * kLook + k;
       n[k] = c < grid ? p.work.pieces[c] : 0;
     }
-    auto units_of = [](int x) {
-      const int shift = tree_join_shift(x & 0xFFFF);
-      static_assert(kTreeJoinThreads == 1 << 7, "a unit's size");
-      return ((x >> 16) * (D / 4) + (1 << shift) - 1) >> shift;
-    };
 #pragma unroll
-    for (int k = 0; k < kLook; ++k) units += units_of(n[k]);
+    for (int k = 0; k < kLook; ++k) units += n[k] >> 22;
     const int upto = warp_scan(units, lane);
     const int here = __shfl_sync(0xFFFFFFFFu, upto, 31);
 #pragma unroll 1
@@ -983,14 +980,14 @@ __global__ void __launch_bounds__(kTreeJoinThreads, 4) paged_tree_join_kernel(co
       int at = unit - before - (upto - units), c = 0, x = 0;  // of the lane that has it: the unit among a CTA's
 #pragma unroll
       for (int k = 0; k < kLook; ++k) {
-        const int mine = units_of(n[k]);
+        const int mine = n[k] >> 22;
         if (x == 0 && at < mine) c = c0 + lane * kLook + k, x = n[k];
         if (x == 0) at -= mine;
       }
       at = __shfl_sync(0xFFFFFFFFu, at, src);
       c = __shfl_sync(0xFFFFFFFFu, c, src);
       x = __shfl_sync(0xFFFFFFFFu, x, src);
-      const int pieces = x & 0xFFFF, rows = x >> 16;
+      const int pieces = x & 0x3FFF, rows = x >> 14 & 0xFF;
       switch (tree_join_shift(pieces)) {
         case 9: join_tree_unit<D, F16, 1, 4>(p, c, pieces, rows, at, s_o, s_ml); break;
         case 8: join_tree_unit<D, F16, 1, 2>(p, c, pieces, rows, at, s_o, s_ml); break;
