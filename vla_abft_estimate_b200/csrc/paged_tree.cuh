@@ -285,8 +285,15 @@ struct __align__(16) TreeItem {
 };
 static_assert(sizeof(TreeItem) == 48, "items' place in shared memory");
 
-// log2 of a unit's (row, 4 columns): a round has all pieces of up to 16.
-__device__ __forceinline__ int tree_join_shift(int pieces) { return pieces <= 4 ? 9 : pieces <= 8 ? 8 : pieces <= 16 ? 7 : 5; }
+// log2 of a unit's (row, 4 columns), of which a thread has one or, where that still
+// asks for all pieces in one round, several of a row, which share the pieces' weights:
+// what the join of many rows is bound by are its instructions (96 trees of 56 rows on
+// 300 slots: 25.0 us, with one each 26.9), that of few rows by round trips, and it is
+// spread as far as it goes (12 trees of up to 13 rows, 32 heads: 22.6 with several, 21.6
+// with one). Of more than 16 pieces four threads share one.
+__device__ __forceinline__ int tree_join_shift(int pieces, int rows) {
+  return pieces > 16 ? 5 : pieces > 8 || rows <= 32 ? 7 : pieces > 2 ? 8 : 9;
+}
 
 // The work warp: this CTA's share of the list (or of its cluster's segment), item by
 // item into the two slots.
@@ -322,7 +329,7 @@ __device__ __forceinline__ void list_tree(const TreeParams& p, TreeItem* items, 
       x.j1 = min(end, most);
       if (!single && at.step == 0 && end < at.seq.steps) {
         pieces = share_of(at.total, at.shares, at.u + at.seq.steps - 1) - static_cast<int>(blockIdx.x) + 1;
-        const int rows = (last + 1 - x.tok0) * p.group, shift = tree_join_shift(pieces);
+        const int rows = (last + 1 - x.tok0) * p.group, shift = tree_join_shift(pieces, rows);
         pieces |= rows << 14 | (rows * (D / 4) + (1 << shift) - 1) >> shift << 22;
         spill = make_int2(x.hk, x.row0 + x.tok0);
       }
@@ -873,7 +880,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
 
 // Joins the segments that cross CTAs: of one that begins in CTA c the pieces are CTA
 // c's place 1 and the following CTAs' place 0. A thread has (row, 4 columns) of a
-// segment, several where there are few pieces, and asks for 16 sums at once,
+// segment, or several of a row, and asks for up to 16 sums at once,
 // by asynchronous copies into its own column of shared memory: what counts is the
 // number of round trips. (In registers, three or six at once, the join of 18 pieces
 // took 14 us.) Of more pieces than that each warp takes every fourth. Units of a
@@ -988,7 +995,7 @@ __global__ void __launch_bounds__(kTreeJoinThreads, 4) paged_tree_join_kernel(co
       c = __shfl_sync(0xFFFFFFFFu, c, src);
       x = __shfl_sync(0xFFFFFFFFu, x, src);
       const int pieces = x & 0x3FFF, rows = x >> 14 & 0xFF;
-      switch (tree_join_shift(pieces)) {
+      switch (tree_join_shift(pieces, rows)) {
         case 9: join_tree_unit<D, F16, 1, 4>(p, c, pieces, rows, at, s_o, s_ml); break;
         case 8: join_tree_unit<D, F16, 1, 2>(p, c, pieces, rows, at, s_o, s_ml); break;
         case 7: join_tree_unit<D, F16, 1, 1>(p, c, pieces, rows, at, s_o, s_ml); break;
