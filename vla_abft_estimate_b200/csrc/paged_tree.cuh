@@ -15,7 +15,8 @@
 // alone was either, and the whole no faster: rows of small tiles spread over idle warps,
 // a part of the keys each, 770 cycles, but the warps' sums had to be added up, 12
 // trees of up to 13 tokens of 32 heads 25.4 -> 30.7 us; a step's waits first and its
-// products in one go, 800 cycles, 25.4 -> 25.6, 24 of up to 26 22.8 -> 23.2.)
+// products in one go, 800 cycles, 25.4 -> 25.6, 24 of up to 26 22.8 -> 23.2 with the
+// join as it was then.)
 //
 // A CTA takes one tile of 128 rows of one kv head, in steps of 64 keys:
 //   S = Q K^T   tcgen05.mma, S in TMEM, two of them: the next one is computed
@@ -27,7 +28,7 @@
 // reads while the other begins, ends or changes its segment. (One CTA with two row
 // groups on steps of 128 keys of the same segment, the causal kernel's form for few
 // rows: 32 trees of 4 tokens of 32 heads on 512 slots 80 us, 54 so; up to 26 tokens on
-// up to 4,122 slots 29, 22.7; 64 trees of 8 on 8,188 slots 198, 175, where HBM's time is
+// up to 4,122 slots 29, 20.9; 64 trees of 8 on 8,188 slots 198, 175, where HBM's time is
 // 165.) One tree of 64 tokens on 131,008 slots takes 140 us where 73 are HBM's and the
 // products' time: each of its four tiles takes in all keys and values by itself, 1.07 GB
 // at the 62 GB/s that an SM takes in.
@@ -78,9 +79,9 @@ struct TreeCfg {
 };
 
 // Places in the list that a segment takes before its first step, for its start and
-// end (1, 2, 3, 4 of them: 24 trees of up to 26 tokens on up to 4,122 slots 23.9, 22.8,
-// 22.7, 22.8 us; 96 of up to 8 on up to 2,000  29.6, 28.6, 27.6, 29.1; 8 of up to 4, 32
-// heads, on up to 1,200  15.0, 17.1, 19.2, 19.3).
+// end (1, 2, 3, 4 of them: 24 trees of up to 26 tokens on up to 4,122 slots 22.9, 21.9,
+// 20.8, 21.3 us; 96 of 8 on 300  27.1, 26.8, 25.0, 25.3; 8 of up to 4, 32 heads, on up
+// to 1,200  13.5, 13.7, 14.3, 14.9).
 constexpr int kTreeCost = 3;
 
 struct TreeWork {
