@@ -99,7 +99,6 @@ __device__ __forceinline__ void check_boundaries(const int32_t* cu, int batch, i
 constexpr int kAppendWarps = 8;
 constexpr int kAppendThreads = 32 * kAppendWarps;
 
-//
 // AppendAtParams: the rotation goes by positions of the caller's, of several axes (images
 // and video: time, height, width) or one (a drafted token's depth), each for its
 // share of the pairs:  (c_j, s_j) = rope[positions[axis of j][t]][j]. They are
