@@ -124,6 +124,22 @@ def test_hidden_rows_do_not_count_however_large(cuda_device):
     close(got[odd], want[odd], tol[odd])
 
 
+@pytest.mark.parametrize("columns", [0, 1000])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_a_key_that_is_no_number_reaches_the_rows_that_see_it(cuda_device, value, columns):
+    tree, total, at_row = [-1, 0, 0, 1, 2, 3, 4], 200, 2  # rows 2, 4 and 6 are one branch
+    pool = Pool([total], 2, 16, 64, BF16, extra_columns=columns)
+    q = torch.randn(len(tree), 4, 64, generator=torch.Generator().manual_seed(6)).to(BF16).to(cuda_device)
+    cu, up = i32([0, len(tree)], cuda_device), i32(tree, cuda_device)
+    want = pool.device_cache(cuda_device, PagedKVCache).tree(q, cu, up)
+    at = total - len(tree) + at_row
+    pool.k[pool.table[0, at // 16].long(), :, at % 16] = value
+    got = pool.device_cache(cuda_device, PagedKVCache).tree(q, cu, up)
+    others = [0, 1, 3, 5]
+    assert torch.equal(bits(got[others]), bits(want[others]))
+    assert got[[2, 4, 6]].isnan().all()
+
+
 @pytest.mark.parametrize("sms", [0, 1, 3])
 def test_bad_parents_end_the_way_up(cuda_device, sms):
     dev = cuda_device
