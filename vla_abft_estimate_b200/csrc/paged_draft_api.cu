@@ -44,15 +44,16 @@ struct TreePlan {
 // length take, but its second launch and the pieces' way through memory cost 13; a
 // cluster's pieces go through the SMs' network, which is slow (25 GB/s an SM): 1 step
 // while 64 CTAs use it at once (one cluster of 8 in each group of SMs), above that 6, or
-// 3 with heads of 64. No more than 16 steps for a CTA: the lengths are on the device, what
+// 3 with heads of 64. No more than 12 steps for a CTA: the lengths are on the device, what
 // is known here is the width of the table, and it is the longest sequence that the
-// others then wait for. Measured (us; 1, 2, 4, 8 CTAs / list; 28/4 heads of 128):
+// others then wait for (16 steps: 32 trees of 8 on 2,000 slots each 30 us, by the list 37,
+// but on up to 2,000, most far below, 21 and 14). Measured (us; 1, 2, 4, 8 CTAs / list; 28/4 heads of 128):
 //   1 tree of 16 tokens on 1,000 slots  18.3 13.9 10.6 9.2 / 10.7, 8,000  104 57 31.9 19.8 / 16.0
 //   4 of 16 on 1,000  18.4 14.2 11.1 13.1 / 14.0, 2,000  31.0 20.6 14.1 14.7 / 16.3, 4,000  57 33.7 20.9 18.4 / 21.2
 //   16 of 16 on 500  14.0 15.8 15.8 - / 16.9, 2,000  34.1 27.4 22.4 - / 25.3
 //   32 of 8 on 300  10.9 11.6 - - / 16.3, 1,250  26.1 21.8 - - / 28.4, on up to 1,200  20.8 16.0 - - / 14.0
 //   8 of 16, heads of 64, on 500  11.7 10.1 10.8 12.7 / 13.8, 2,000  29.0 18.4 15.2 15.3 / 15.2
-constexpr int kTreeListSteps = 13, kTreeQuiet = 64, kTreeMostSteps = 16;
+constexpr int kTreeListSteps = 13, kTreeQuiet = 64, kTreeMostSteps = 12;
 
 int tree_plan(const abft_paged_attn_args* a, int sms, TreePlan* r) {
   r->tile_tokens = kTreeRows / (a->heads / a->kv.kv_heads);

@@ -73,7 +73,7 @@ struct TreeCfg {
   static constexpr int kSmemBytes = kOffUp + 2 * kTreeHeld * 4 + 1024;
   // A cluster's pieces take the tiles' place: D / 4 quads of sums a row, then (m, l) of each piece.
   static_assert(kTreeRows * (D * 4 + kDecCluster * 8) <= kQBytes + kSlots * kTileBytes, "the pieces' place");
-  static_assert(kSmemBytes <= 115 * 1024, "two CTAs per SM");
+  static_assert(kSmemBytes <= 113 * 1024, "two CTAs per SM");
   // TMEM columns: two S (P over the first half of each), then O.
   static constexpr int kTmemCols = 256, kColO = 128;
 };
