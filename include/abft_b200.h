@@ -610,7 +610,7 @@ int abft_kv_keep(const abft_kv_keep_args* args, void* stream);
  * looked at where the length ends with a page. -1 for src[i] or dst[i]: no pair.
  * A pair is left undone, with ABFT_PAGED_BAD_FORK, when src or dst is outside the
  * batch, dst is also a source or named by another pair, or the page it needs is
- * named by another pair; with ABFT_PAGED_BAD_LEN or ABFT_PAGED_BAD_PAGE when the
+ * named by another pair or the last page of another pair's source; with ABFT_PAGED_BAD_LEN or ABFT_PAGED_BAD_PAGE when the
  * source's length or either page is bad or both pages are the same. */
 typedef struct abft_kv_fork_args {
   abft_paged_kv kv;

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kKeepThreads, 3) kv_keep_kernel(const __grid_c
 //
 // Pairs work side by side, so none may write what another reads or writes: a
 // destination that is also a source or named twice, or a page named twice, is
-// refused with all that name it.
+// refused with all that name it, and so is a page that another pair copies from.
 //
 // Bound: HBM, by rest slots of 2 * layers * heads rows in and out; slots of a head lie
 // one after another, and its warps take them in turn, eight 16-byte pieces a lane in
@@ -273,27 +273,30 @@ __global__ void __launch_bounds__(32 * kForkWarps) kv_fork_kernel(const __grid_c
   const int i = blockIdx.x / p.per_pair, part = blockIdx.x - i * p.per_pair;
   const int s = p.src[i], d = p.dst[i], fresh = p.pages[i];
   if (s == -1 || d == -1) return;
+  // Where a source's length ends: its full pages, and the slots behind them.
+  auto ends = [&](int sequence, int* full, int* rest) {
+    const int len = kv.seq_lens[sequence];
+    *full = len >> kv.page_shift;
+    *rest = len & ((1 << kv.page_shift) - 1);
+    return len >= 0 && len <= static_cast<int64_t>(kv.max_pages) << kv.page_shift;
+  };
   bool clash = false, same_page = false;
   for (int j = threadIdx.x; j < p.pairs; j += 32 * kForkWarps) {
     const int sj = p.src[j], dj = p.dst[j];
     if (sj == -1 || dj == -1) continue;
     clash = clash || sj == d || (j != i && dj == d);
     same_page = same_page || (j != i && p.pages[j] == fresh);
+    int full, rest;  // (a page of the own source: below)
+    if (sj != s && sj >= 0 && sj < kv.batch && ends(sj, &full, &rest) && rest > 0)
+      same_page = same_page || kv.page_table[sj * kv.table_stride + full] == fresh;
   }
   uint32_t bad = 0;
   if (s < 0 || s >= kv.batch || d < 0 || d >= kv.batch) bad = ABFT_PAGED_BAD_FORK;
-  int len = 0, full = 0, rest = 0, old = 0;
-  if (bad == 0) {
-    len = kv.seq_lens[s];
-    if (len < 0 || len > static_cast<int64_t>(kv.max_pages) << kv.page_shift) bad = ABFT_PAGED_BAD_LEN;
-  }
-  if (bad == 0) {
-    full = len >> kv.page_shift;
-    rest = len & ((1 << kv.page_shift) - 1);
-    if (rest > 0) {
-      old = kv.page_table[s * kv.table_stride + full];
-      if (old < 0 || old >= kv.num_pages || fresh < 0 || fresh >= kv.num_pages || fresh == old) bad = ABFT_PAGED_BAD_PAGE;
-    }
+  int full = 0, rest = 0, old = 0;
+  if (bad == 0 && !ends(s, &full, &rest)) bad = ABFT_PAGED_BAD_LEN;
+  if (bad == 0 && rest > 0) {
+    old = kv.page_table[s * kv.table_stride + full];
+    if (old < 0 || old >= kv.num_pages || fresh < 0 || fresh >= kv.num_pages || fresh == old) bad = ABFT_PAGED_BAD_PAGE;
   }
   if (clash || (same_page && rest > 0)) bad |= ABFT_PAGED_BAD_FORK;
   const bool wrong = __syncthreads_or(bad != 0);
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(32 * kForkWarps) kv_fork_kernel(const __grid_c
     for (int j = threadIdx.x; j < full; j += 32 * kForkWarps) to[j] = from[j];
     if (threadIdx.x == 0) {
       if (rest > 0) to[full] = fresh;
-      const_cast<int32_t*>(kv.seq_lens)[d] = len;
+      const_cast<int32_t*>(kv.seq_lens)[d] = (full << kv.page_shift) + rest;
     }
   }
   const int lane = threadIdx.x & 31;

@@ -624,8 +624,8 @@ class PagedLayers:
         table names then (not looked at where the length ends with a page). -1
         in ``src`` or ``dst``: no pair. Sources may be named by several pairs;
         a destination that is also a source or named twice, or a page that
-        another pair names too, is refused: the pair is left undone, and the
-        status tells."""
+        another pair names too or that is another source's last, is refused: the
+        pair is left undone, and the status tells."""
         done = self._fast.fork(src, dst, pages)
         if done is not None:
             return N.check("abft_kv_fork", done)
