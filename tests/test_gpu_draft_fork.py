@@ -32,3 +32,13 @@ def test_a_page_that_no_pair_copies_from(cuda_device):
     dev, lens = cuda_device, [20, 48, 30, 0, 0, 0]
     check_fork(dev, lens, [(0, 3), (-1, 4), (2, -1)], pages=lambda free, table: [free[0], free[1], free[2]], undone=(1, 2))
     check_fork(dev, lens, [(1, 3), (0, 4)], pages=lambda free, table: [int(table[0, 1]), free[0]])
+
+
+@pytest.mark.parametrize("layers", [1, 28])
+def test_a_page_that_only_one_pair_needs(cuda_device, layers):
+    """Sources that end with a page need none: what stands in their places, the same page as another's, is not looked at."""
+    dev, lens = cuda_device, [20, 48, 30, 0, 0, 0, 0]
+    check_fork(dev, lens, [(0, 4), (1, 5)], pages=lambda free, table: [free[0], free[0]], layers=layers)
+    check_fork(dev, lens, [(1, 4), (3, 5), (2, 6)], pages=lambda free, table: [free[0]] * 3, layers=layers)
+    check_fork(dev, lens, [(1, 4), (0, 5), (2, 6)], pages=lambda free, table: [free[0]] * 3, bad="fork", undone=(1, 2),
+               layers=layers)

@@ -285,10 +285,10 @@ __global__ void __launch_bounds__(32 * kForkWarps) kv_fork_kernel(const __grid_c
     const int sj = p.src[j], dj = p.dst[j];
     if (sj == -1 || dj == -1) continue;
     clash = clash || sj == d || (j != i && dj == d);
-    same_page = same_page || (j != i && p.pages[j] == fresh);
-    int full, rest;  // (a page of the own source: below)
-    if (sj != s && sj >= 0 && sj < kv.batch && ends(sj, &full, &rest) && rest > 0)
-      same_page = same_page || kv.page_table[sj * kv.table_stride + full] == fresh;
+    int full, rest;
+    if (j == i || sj < 0 || sj >= kv.batch || !ends(sj, &full, &rest) || rest == 0) continue;  // needs no page
+    same_page = same_page || p.pages[j] == fresh;
+    if (sj != s) same_page = same_page || kv.page_table[sj * kv.table_stride + full] == fresh;  // (the own source's: below)
   }
   uint32_t bad = 0;
   if (s < 0 || s >= kv.batch || d < 0 || d >= kv.batch) bad = ABFT_PAGED_BAD_FORK;
