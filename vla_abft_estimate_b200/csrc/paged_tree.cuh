@@ -153,6 +153,22 @@ __device__ __forceinline__ TreeSeq tree_sequence(const PagedView& kv, const int3
   return s;
 }
 
+// Places of the list, counted up to kNoMore. The host keeps those of sequences that
+// follow one another below it, but boundaries that fall may give each of many sequences
+// all rows; such a list is not worked on, whatever its sum would be.
+__host__ __device__ __forceinline__ int add_places(int a, int b) {
+  const uint32_t sum = static_cast<uint32_t>(a) + static_cast<uint32_t>(b);  // both at most kNoMore
+  return sum < static_cast<uint32_t>(kNoMore) ? static_cast<int>(sum) : kNoMore;
+}
+__device__ __forceinline__ int scan_places(int x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    if (lane >= o) x = add_places(x, up);
+  }
+  return x;
+}
+
 // A CTA's share of the list, found and walked by one warp: segment y = (kv head,
 // tile) of sequence b, from `step` on.
 struct TreeShare {
@@ -185,7 +201,7 @@ __device__ __forceinline__ void tree_locate(const TreeParams& p, int lane, TreeS
 #pragma unroll 2
   for (int b = lane * part; b < min(kv.batch, (lane + 1) * part); ++b) {
     last = places_of(b);
-    sum += last;
+    sum = add_places(sum, last);
     *bad = *bad || mine.bad;
     if (mine.tiles > 0) {
       segments += mine.tiles * kv.kv_heads;
@@ -193,16 +209,17 @@ __device__ __forceinline__ void tree_locate(const TreeParams& p, int lane, TreeS
       most = max(most, mine.steps);
     }
   }
-  const int upto_all = warp_scan(sum, lane);
-  const int total = __shfl_sync(0xFFFFFFFFu, upto_all, 31);  // the host keeps it below 2^31
+  const int upto_all = scan_places(sum, lane);
+  const int total = __shfl_sync(0xFFFFFFFFu, upto_all, 31);
   const int rank = work.cluster > 0 ? static_cast<int>(blockIdx.x) & (work.cluster - 1) : 0;
   int at;
   out->total = total;
   out->shares = gridDim.x;
   out->seq.tiles = 0;  // none
+  out->u = out->u1 = 0;
+  if (total == kNoMore) return;  // (the boundaries are told of by list_tree)
   if (work.cluster > 0) {
     at = static_cast<int>(blockIdx.x) >> work.cluster_shift;
-    out->u = out->u1 = 0;
     if (at >= total) return;
   } else {
     if (__reduce_min_sync(0xFFFFFFFFu, least) == static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, most))) {
