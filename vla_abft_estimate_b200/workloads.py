@@ -80,7 +80,8 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
     ``parents`` (int32, one for each row): the new tokens are trees of drafted
     ones, attended to as such; ``positions`` (int32, [tokens] or [axes, tokens])
     is what each token is rotated by in place of its slot's place: a drafted
-    token's depth, or the time, height and width of ``cfg["rope_sections"]``.
+    token's depth (of a model with several axes, on all of them), or the time,
+    height and width of ``cfg["rope_sections"]``.
     ``caches.together`` accepts, keeps and forks.
     ``dtype``: bfloat16 (default) or float16, the reference driver's
     ``--dtype`` (qwen_abft_benchmark.py:26)."""
@@ -141,7 +142,9 @@ def build_qwen2(cfg, device, seed=0, dtype=None):
             nh, nkv, hd = cfg["heads"], cfg["kv_heads"], cfg["head_dim"]
             t = x.shape[0]
             q, k, v = self.qkv(self.ln1(x)).split([nh * hd, nkv * hd, nkv * hd], dim=-1)
-            sections = None if positions is None else cfg.get("rope_sections")
+            # One row of positions is all axes'.
+            axes = positions.shape[0] if torch.is_tensor(positions) and positions.dim() == 2 else 1
+            sections = cfg.get("rope_sections") if axes > 1 else None
             q = cache.append(q.view(t, nh, hd), k.view(t, nkv, hd), v.view(t, nkv, hd), rope, cu_seqlens=cu_seqlens,
                              positions=positions, sections=sections)
             # Rows of no sequence go on through the checked linears: zeros, not what memory held.
