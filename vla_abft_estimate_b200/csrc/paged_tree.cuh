@@ -52,8 +52,14 @@ namespace abft {
 constexpr int kTreeRows = kPreRows;  // query rows of a tile
 constexpr int kTreeKeys = 64;        // keys of a step
 constexpr int kTreeThreads = 256;
-// Parents that are held in shared memory, where the walk up a tree takes a tenth of
-// the time; those of larger trees are read where they are.
+// Parents of a tree that are held in shared memory, where a hop of the walk up takes a
+// tenth of the time. A larger tree takes its steps from the last to the first, as the walk
+// goes: each row goes on from where it was, so that a step costs 64 hops at most, and its
+// warp brings the parents of a step's rows to shared memory, if one of its walks is there.
+// (Each step from the row itself takes a time that grows with the square of the depth: a
+// chain of 4,000 rows 17.8 ms, of 8,000 141, where prefill takes 0.13 and 0.39; so 0.96
+// and 3.4. Random trees of 8,000 rows 1.02 -> 0.95, where each step of larger trees is
+// brought 1.08. A chain of 512 on 3,000 slots, as it is held: 163 us, prefill 47.)
 constexpr int kTreeHeld = 512;
 
 template <int D>
@@ -70,7 +76,8 @@ struct TreeCfg {
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kOffItems = kOffMisc + 16;
   static constexpr int kOffUp = kOffItems + 2 * 48;  // parents of the items in the two slots
-  static constexpr int kSmemBytes = kOffUp + 2 * kTreeHeld * 4 + 1024;
+  static constexpr int kOffWindow = kOffUp + 2 * kTreeHeld * 4;  // [4][kTreeKeys]: of each row warp's step, in larger trees
+  static constexpr int kSmemBytes = kOffWindow + 4 * kTreeKeys * 4 + 1024;
   // A cluster's pieces take the tiles' place: D / 4 quads of sums a row, then (m, l) of each piece.
   static_assert(kTreeRows * (D * 4 + kDecCluster * 8) <= kQBytes + kSlots * kTileBytes, "the pieces' place");
   static_assert(kSmemBytes <= 113 * 1024, "two CTAs per SM");
@@ -114,17 +121,26 @@ struct TreeParams {
   TreeWork work;
 };
 
+// Parents of a tree's rows from `first` on.
+struct TreeParents {
+  const int32_t* at;
+  int first;
+  __host__ __device__ __forceinline__ int operator[](int row) const { return at[row - first]; }
+};
+
 // What a row sees of a step's 64 slots, 32 to a word: every slot before the
 // drafted ones (`base` of them from the step's first on, may be negative), and of
-// those the row's own and its ancestors'. The walk up ends at the root, at a parent
-// that does not come before its child, or before the step.
-__host__ __device__ __forceinline__ void tree_words(const int32_t* parents, int own, int base, uint32_t (&w)[2]) {
+// those the row's own and its ancestors'. The walk up goes from `row`, the row itself
+// or the first of its ancestors that no later step holds, to the first before this
+// step, which is returned, -1 behind the root or a parent that does not come before its
+// child.
+template <typename Parents>
+__host__ __device__ __forceinline__ int tree_words(Parents parents, int row, int base, uint32_t (&w)[2]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int below = base - c * 32;
     w[c] = below >= 32 ? 0xFFFFFFFFu : below > 0 ? (1u << below) - 1u : 0u;
   }
-  int row = own;
   while (row >= 0 && base + row >= 0) {
     const int key = base + row;
     if (key < 32) w[0] |= 1u << key;
@@ -132,6 +148,7 @@ __host__ __device__ __forceinline__ void tree_words(const int32_t* parents, int 
     const int up = parents[row];
     row = up < row ? up : -1;
   }
+  return row;
 }
 
 // A sequence in the list: its rows, its length, tiles of rows, and steps
@@ -300,6 +317,9 @@ struct __align__(16) TreeItem {
   int32_t row0, n;  // its first packed row and its rows
   int32_t tok0;     // first token of the tile within them
   int32_t j0, j1;   // steps
+  // The step that is taken first, and the way to the next (kTreeHeld).
+  __device__ __forceinline__ int first() const { return n > kTreeHeld ? j1 - 1 : j0; }
+  __device__ __forceinline__ int way() const { return n > kTreeHeld ? -1 : 1; }
 };
 static_assert(sizeof(TreeItem) == 48, "items' place in shared memory");
 
@@ -485,7 +505,8 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   TreeItem* items = reinterpret_cast<TreeItem*>(smem + Cfg::kOffItems);
-  int32_t* held = reinterpret_cast<int32_t*>(smem + Cfg::kOffUp);  // [2][kTreeHeld]
+  int32_t* held = reinterpret_cast<int32_t*>(smem + Cfg::kOffUp);        // [2][kTreeHeld]
+  int32_t* window = reinterpret_cast<int32_t*>(smem + Cfg::kOffWindow);  // [4][kTreeKeys]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedView& kv = p.kv;
@@ -563,9 +584,13 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
       // A warp without rows only keeps step: what the products make of its lanes nobody
       // reads (exponentials are a step's longest part, and a tile may have few rows).
       const bool used = __any_sync(0xFFFFFFFFu, live);
+      int up_to = own;  // where the walk up has come to
       bool parents_there = false;
       float m = -INFINITY, l = 0.f;  // m: maximum that P refers to (raw scores)
-      for (int j = x.j0; j < x.j1; ++j, ++count) {
+      bool first = true;
+      int left = x.j1 - x.j0;
+      int base = x.len - x.n - x.first() * kTreeKeys;  // of the step's slots those before the drafted ones
+      for (; left > 0; --left, first = false, ++count, base += x.n > kTreeHeld ? kTreeKeys : -kTreeKeys) {
         const uint32_t ts = lanes + (count & 1) * 64;
         ok = mbar_wait(&sfull[count & 1], (count >> 1) & 1, abort_flag);
         tc_fence_after();
@@ -585,21 +610,40 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
 #pragma unroll
             for (int k = 0; k < 32; ++k) s[c][k] ^= 0x80000000u;
         }
-        const int base = x.len - x.n - j * kTreeKeys;  // of the step's slots those before the drafted ones
         if (base < kTreeKeys) {
           uint32_t w[2] = {0u, 0u};
           if (!parents_there) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(&upfull[i & 1], (i >> 1) & 1, abort_flag)) && ok;
             parents_there = true;
           }
-          if (live && own >= x.n - x.len) {  // of more rows than tokens the first have no slots and see none
-            const int32_t* parents = x.n <= kTreeHeld ? held + (i & 1) * kTreeHeld : p.work.parents + x.row0;
-            tree_words(parents, own, base, w);
-            // A row's own slot is in one step and one piece: there its parent is looked at.
-            if (base + own >= 0 && base + own < kTreeKeys) {
-              const int up = parents[own];
-              if ((up < -1 || up >= own) && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_DRAFT);
+          const bool sees = live && own >= x.n - x.len;  // of more rows than tokens the first have no slots and see none
+          TreeParents parents = {held + (i & 1) * kTreeHeld, 0};
+          if (x.n <= kTreeHeld) {
+            if (sees) tree_words(parents, own, base, w);
+          } else {
+            // This step's rows, and on the way to it those that the piece does not hold.
+            int32_t* mine = window + warp * kTreeKeys;
+            parents.at = mine;
+            int row = -base;
+            if (first) row += (min(x.tok0 + p.tile_tokens, x.n) - 1 - row) / kTreeKeys * kTreeKeys;
+            for (; row >= -base; row -= kTreeKeys) {
+              parents.first = row;
+              __syncwarp();
+              if (__any_sync(0xFFFFFFFFu, sees && up_to >= row)) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const int at = row + c * 32 + lane;
+                  if (at >= 0 && at < x.n) mine[c * 32 + lane] = p.work.parents[x.row0 + at];
+                }
+              }
+              __syncwarp();
+              if (sees) up_to = tree_words(parents, up_to, -row, w);
             }
+          }
+          // A row's own slot is in one step and one piece: there its parent is looked at.
+          if (sees && base + own >= 0 && base + own < kTreeKeys) {
+            const int up = parents[own];
+            if ((up < -1 || up >= own) && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_BAD_DRAFT);
           }
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -618,13 +662,13 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
         // Also true from m = -inf and for NaN, but not while all is -inf. Rows that
         // are none have what memory held as scores, and nobody reads their sums.
         const bool raise = live && !((mn - m) * p.scale_log2 <= kPreLag<F16>) && mn != -INFINITY;
-        if (j == x.j0 || __any_sync(0xFFFFFFFFu, raise || !ok)) {
+        if (first || __any_sync(0xFFFFFFFFu, raise || !ok)) {
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           if (mn == INFINITY) mn = __int_as_float(0x7FC00000);  // inf - inf: the row is NaN
           const float f = m == -INFINITY ? 0.f : exp2_approx((m - mn) * p.scale_log2);
           m = mn;
-          if (j > x.j0) {
+          if (!first) {
             ok = summed(count - 1);
             if (!ok) break;
             l *= f;
@@ -725,16 +769,18 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     for (int i = 0; ok && get_item(i, &x); ++i) {
       const int32_t* table = kv.page_table + x.seq * kv.table_stride;
       const int held = (x.len + box - 1) >> box_shift;  // boxes of the sequence
-      auto entry = [&](int j) {  // a lane per box of the step
-        const int at = j * per_step + lane;
-        return j < x.j1 && lane < per_step && at < held ? table[at >> (kv.page_shift - box_shift)] : 0;
+      const int steps = x.j1 - x.j0, way = x.way(), first = x.first();
+      auto entry = [&](int k) {  // a lane per box of the step
+        const int at = (first + k * way) * per_step + lane;
+        return k < steps && lane < per_step && at < held ? table[at >> (kv.page_shift - box_shift)] : 0;
       };
       // Keys come two steps before the values: K of the first two steps, then V and the
       // next K in turn, as the issuer uses them.
-      int ids[4];  // table entries of steps j to j + 3
+      int ids[4];  // table entries of the steps k to k + 3
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ids[k] = entry(x.j0 + k);
-      auto load = [&](int j, int id, bool values) {
+      for (int k = 0; k < 4; ++k) ids[k] = entry(k);
+      auto load = [&](int k, int id, bool values) {
+        const int j = first + k * way;
         const int boxes = min(per_step, held - j * per_step);
         const bool mine = lane < boxes;
         if (!values && mine && (id < 0 || id >= kv.num_pages) && kv.status != nullptr)
@@ -748,20 +794,20 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
         if (mine) {
           // A bad id lies outside the map's page dimension and loads zeros.
           const uint32_t dst = smem_u32(smem + Cfg::kOffRing + slot * Cfg::kTileBytes) + lane * box * D * 2;
-          const int first = ((j * per_step + lane) << box_shift) & ((1 << kv.page_shift) - 1);  // of the page's slots
-          tma_load_5d(dst, values ? &tm_v : &tm_k, &full[slot], 0, 0, 0, ((x.hk << kv.page_shift) + first) >> 3, id);
+          const int slot0 = ((j * per_step + lane) << box_shift) & ((1 << kv.page_shift) - 1);  // of the page's slots
+          tma_load_5d(dst, values ? &tm_v : &tm_k, &full[slot], 0, 0, 0, ((x.hk << kv.page_shift) + slot0) >> 3, id);
         }
         ++issued;
       };
-      if (x.j0 < x.j1) load(x.j0, ids[0], false);
-      if (x.j0 + 1 < x.j1 && ok) load(x.j0 + 1, ids[1], false);
-      for (int j = x.j0; j < x.j1 && ok; ++j) {
-        load(j, ids[0], true);
-        if (j + 2 < x.j1 && ok) load(j + 2, ids[2], false);
+      if (steps > 0) load(0, ids[0], false);
+      if (steps > 1 && ok) load(1, ids[1], false);
+      for (int k = 0; k < steps && ok; ++k) {
+        load(k, ids[0], true);
+        if (k + 2 < steps && ok) load(k + 2, ids[2], false);
         ids[0] = ids[1];
         ids[1] = ids[2];
         ids[2] = ids[3];
-        ids[3] = entry(j + 4);
+        ids[3] = entry(k + 4);
       }
     }
     // Copies in flight have landed before shared memory goes (all have, but after an
@@ -814,27 +860,28 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     };
     TreeItem x;
     for (int i = 0; ok && get_item(i, &x); ++i) {
-      const int first_j = __shfl_sync(0xFFFFFFFFu, x.j0, 0), last_j = __shfl_sync(0xFFFFFFFFu, x.j1, 0);
-      const int length = __shfl_sync(0xFFFFFFFFu, x.len, 0);
+      // `keys` of the sequence from the step's first on.
+      const int steps = __shfl_sync(0xFFFFFFFFu, x.j1 - x.j0, 0), way = __shfl_sync(0xFFFFFFFFu, x.way() * kTreeKeys, 0);
+      int keys = __shfl_sync(0xFFFFFFFFu, x.len - x.first() * kTreeKeys, 0);
       // (The query rows of an item without steps are not brought.)
-      if (first_j >= last_j) continue;
+      if (steps <= 0) continue;
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(qfull, begun & 1, abort_flag));
       ++begun;
       tc_fence_after();
       if (!ok) break;
-      scores(first_j + 1 >= last_j);
-      if (first_j + 1 < last_j && ok) scores(first_j + 2 >= last_j);
-      for (int j = first_j; j < last_j && ok; ++j) {
+      scores(steps == 1);
+      if (steps > 1 && ok) scores(steps == 2);
+      for (int k = 0; k < steps && ok; ++k, keys -= way) {
         if (!ready()) break;
         // Weights of slots behind the length are 0, but the slots may hold anything (a
         // page's last owner, NaN): only whole groups of 16 keys that the sequence
         // reaches are multiplied, the rest of the last group is cleared.
-        const int valid = min(kTreeKeys, length - j * kTreeKeys);
+        const int valid = min(kTreeKeys, keys);
         const int groups = (valid + 15) / 16;
         if (valid & 15) {
           uint8_t* v = smem + Cfg::kOffRing + slot * Cfg::kTileBytes;
-          for (int k = valid * (D / 8) + lane; k < groups * 16 * (D / 8); k += 32) {
-            const int row = k / (D / 8), c = k % (D / 8);  // every piece of the row: its order does not matter
+          for (int at = valid * (D / 8) + lane; at < groups * 16 * (D / 8); at += 32) {
+            const int row = at / (D / 8), c = at % (D / 8);  // every piece of the row: its order does not matter
             *reinterpret_cast<uint4*>(v + (row >> 3) * Cfg::kGroupBytes + (c >> 3) * 1024 + (row & 7) * 128 + ((c & 7) << 4)) =
                 make_uint4(0u, 0u, 0u, 0u);
           }
@@ -843,21 +890,21 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
         }
         // All tiles have been written and seen here: before another CTA's sums come over
         // them (join_tree_cluster). The rows' weights are waited for meanwhile.
-        if (p.work.cluster > 1 && j + 1 == last_j) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        if (p.work.cluster > 1 && k + 1 == steps) asm volatile("fence.acq_rel.cluster;" ::: "memory");
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&pfull[summed & 1], (summed >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t dv = desc_v + slot * (Cfg::kTileBytes >> 4);
           const uint32_t a = tm + (summed & 1) * 64, d = tm + Cfg::kColO;
-          umma_f16_ts(d, a, dv, idesc_o, j > first_j);
-          for (int k = 1; k < groups; ++k) umma_f16_ts(d, a + k * 8, dv + k * (2 * Cfg::kGroupBytes >> 4), idesc_o, 1);
+          umma_f16_ts(d, a, dv, idesc_o, k > 0);
+          for (int g = 1; g < groups; ++g) umma_f16_ts(d, a + g * 8, dv + g * (2 * Cfg::kGroupBytes >> 4), idesc_o, 1);
           umma_commit(&ofull[summed & 1]);
         }
         __syncwarp();
         ++summed;
         release();
-        if (j + 2 < last_j) scores(j + 3 >= last_j);
+        if (k + 2 < steps) scores(k + 3 == steps);
       }
     }
     // Nothing still writes TMEM when it is freed.
