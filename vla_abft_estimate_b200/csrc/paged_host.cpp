@@ -387,16 +387,6 @@ void* layers_stream(const Layers* c) {
 
 const int32_t* int_ptr(const at::Tensor* t) { return static_cast<const int32_t*>(t->const_data_ptr()); }
 
-// int32 [size] in t's memory, from its 4-byte word `offset` on. No view: it has
-// a version of its own, as a tensor allocated by itself would (three allocations:
-// 5.7 us a call, one: 4.2).
-at::Tensor behind(const at::Tensor& t, int64_t offset, int64_t size) {
-  at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), caffe2::TypeMeta::Make<int32_t>());
-  r.unsafeGetTensorImpl()->set_storage_offset(offset);
-  r.unsafeGetTensorImpl()->set_sizes_contiguous({size});
-  return r;
-}
-
 // accept(cu_seqlens, parents, ids, answers): (kept, counts, next); None; a status
 // code.
 PyObject* layers_accept(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -408,12 +398,11 @@ PyObject* layers_accept(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   if (!list_of(c->device, ids, -1, type) || !list_of(c->device, answers, ids->size(0), type) ||
       !list_of(c->device, parents, ids->size(0), at::kInt) || !list_of(c->device, cu, c->kv.batch + 1, at::kInt))
     Py_RETURN_NONE;
-  const int64_t batch = c->kv.batch, id_bytes = type == at::kLong ? 8 : 4;
-  at::Tensor next = at::empty({batch + ((batch + ids->size(0)) * 4 + id_bytes - 1) / id_bytes},
-                              at::TensorOptions().dtype(type).device(at::kCUDA, static_cast<c10::DeviceIndex>(c->device)));
-  at::Tensor counts = behind(next, batch * id_bytes / 4, batch);
-  at::Tensor kept = behind(next, batch * id_bytes / 4 + batch, ids->size(0));
-  next.unsafeGetTensorImpl()->set_sizes_contiguous({batch});
+  const at::TensorOptions on = at::TensorOptions().device(at::kCUDA, static_cast<c10::DeviceIndex>(c->device));
+  // A memory of its own for each, which the caller may resize, hand to a stream or free.
+  at::Tensor kept = at::empty({ids->size(0)}, on.dtype(at::kInt));
+  at::Tensor counts = at::empty({c->kv.batch}, on.dtype(at::kInt));
+  at::Tensor next = at::empty({c->kv.batch}, on.dtype(type));
   abft_draft_accept_args args;
   memset(&args, 0, sizeof args);
   args.cu_seqlens = int_ptr(cu), args.parents = int_ptr(parents);
@@ -424,7 +413,7 @@ PyObject* layers_accept(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   args.status = c->kv.status;
   args.tokens = ids->size(0);
   args.batch = c->kv.batch;
-  args.id_bytes = static_cast<int32_t>(id_bytes);
+  args.id_bytes = type == at::kLong ? 8 : 4;
   void* stream = layers_stream(c);
   int rc;
   Py_BEGIN_ALLOW_THREADS rc = c->accept(&args, stream);
