@@ -563,7 +563,8 @@ int abft_paged_tree(const abft_paged_tree_args* args, void* stream);
  * ends at the deepest confirmed row, the lowest of equals. kept[cu[b] + k]: its
  * rows from the top, then -1; rows behind cu[batch] -1; counts[b]: their
  * number; next[b]: the last one's answer, or -1 where there is none. A bad parent
- * (as above) sets ABFT_PAGED_BAD_DRAFT and confirms nothing. */
+ * (as above) sets ABFT_PAGED_BAD_DRAFT and confirms nothing. The results overlap
+ * neither each other nor what is read. */
 typedef struct abft_draft_accept_args {
   const int32_t* cu_seqlens;   /* [batch + 1]                                            */
   const int32_t* parents;      /* [tokens]                                               */
@@ -581,7 +582,8 @@ int abft_draft_accept(const abft_draft_accept_args* args, void* stream);
 
 /* Keep: of the n new tokens of sequence b the rows kept[cu[b] + i], i <
  * counts[b], rising, move to the slots of rows 0, 1, ... in every layer, and
- * lens_out[b] = seq_lens[b] - n + counts[b] (lens_out may be kv.seq_lens itself).
+ * lens_out[b] = seq_lens[b] - n + counts[b] (lens_out may be kv.seq_lens itself, or
+ * counts, but overlaps nothing that is read otherwise).
  * The layers share kv's geometry, strides, table and lengths; their pools are
  * pools[2 * layer] (keys) and pools[2 * layer + 1] (values), a host array (read
  * during the call) of distinct, 16-byte aligned device addresses, or, with pools
@@ -604,7 +606,7 @@ int abft_kv_keep(const abft_kv_keep_args* args, void* stream);
 
 /* Fork: for each pair i sequence dst[i] gets the cache of sequence src[i]: its
  * row of kv.page_table the source's full pages, kv.seq_lens[dst[i]] the source's
- * length (both arrays are written), and where the length ends inside a page,
+ * length (both arrays are written, and overlap no list of the pairs), and where the length ends inside a page,
  * page pages[i], which no sequence may hold, a copy of the slots in use of the
  * source's last page in every layer, and its place in the row. pages[i] is not
  * looked at where the length ends with a page. -1 for src[i] or dst[i]: no pair.

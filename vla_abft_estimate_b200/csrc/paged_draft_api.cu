@@ -179,9 +179,25 @@ int tree_call(const abft_paged_tree_args* t, void* stream) {
              : launch_tree<64, false>(dev, 16, tm_k, tm_v, tm_q, p, plan, sms, s);
 }
 
-bool overlap(const void* a, const void* b, size_t bytes) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + bytes && y < x + bytes;
+// An array of a call, as memory: what one sequence's or pair's CTAs write must not be
+// what another's read.
+struct Span {
+  uintptr_t at;
+  size_t bytes;
+  Span(const void* p, int64_t items, size_t size = sizeof(int32_t))
+      : at(reinterpret_cast<uintptr_t>(p)), bytes(static_cast<size_t>(items) * size) {}
+  bool meets(const Span& o) const { return bytes > 0 && o.bytes > 0 && at < o.at + o.bytes && o.at < at + bytes; }
+};
+
+// Some row of the table (what lies between its rows is not its own).
+bool meets_table(const Span& x, const abft_paged_kv& kv) {
+  const Span whole(kv.page_table, (kv.batch - 1) * kv.table_stride + kv.max_pages);
+  if (!x.meets(whole)) return false;
+  if (kv.batch == 1 || x.at <= whole.at) return true;
+  // The first row that ends behind x's start.
+  const int64_t pitch = kv.table_stride * 4, row = kv.max_pages * int64_t{4}, from = static_cast<int64_t>(x.at - whole.at);
+  const int64_t first = from < row ? 0 : (from - row) / pitch + 1;
+  return first * pitch < from + static_cast<int64_t>(x.bytes);
 }
 
 template <int kLayers>
@@ -279,6 +295,13 @@ int abft_draft_accept(const abft_draft_accept_args* a, void* stream) {
   const uintptr_t ids = reinterpret_cast<uintptr_t>(a->ids) | reinterpret_cast<uintptr_t>(a->answers) |
                         reinterpret_cast<uintptr_t>(a->next);
   if ((ids & static_cast<uintptr_t>(a->id_bytes - 1)) != 0) return ABFT_ERR_ALIGNMENT;
+  // What is read is read by any thread at any time.
+  const Span kept(a->kept, a->tokens), counts(a->counts, a->batch), next(a->next, a->batch, a->id_bytes);
+  const Span read[] = {Span(a->cu_seqlens, int64_t{a->batch} + 1), Span(a->parents, a->tokens), Span(a->ids, a->tokens, a->id_bytes),
+                       Span(a->answers, a->tokens, a->id_bytes)};
+  for (const Span& x : read)
+    if (kept.meets(x) || counts.meets(x) || next.meets(x)) return ABFT_ERR_INVALID_ARG;
+  if (kept.meets(counts) || kept.meets(next) || counts.meets(next)) return ABFT_ERR_INVALID_ARG;
   int dev = 0, sms = 0;
   const int rc = paged_device(&dev, &sms);
   if (rc != ABFT_OK) return rc;
@@ -307,8 +330,11 @@ int abft_kv_keep(const abft_kv_keep_args* a, void* stream) {
   if (a->kv.batch == 0) return ABFT_OK;
   if (a->cu_seqlens == nullptr || a->counts == nullptr || a->lens_out == nullptr || (a->tokens > 0 && a->kept == nullptr))
     return ABFT_ERR_INVALID_ARG;
-  // The lengths themselves, or an array of its own: not a part of them.
-  if (a->lens_out != a->kv.seq_lens && overlap(a->lens_out, a->kv.seq_lens, a->kv.batch * sizeof(int32_t)))
+  // The lengths themselves, or an array of its own: not a part of them, nor of what other
+  // sequences still read. (A sequence's count is read before its length is written.)
+  const Span out(a->lens_out, a->kv.batch), lens(a->kv.seq_lens, a->kv.batch), counts(a->counts, a->kv.batch);
+  if ((out.at != lens.at && out.meets(lens)) || (out.at != counts.at && out.meets(counts)) ||
+      out.meets(Span(a->cu_seqlens, a->kv.batch + 1)) || out.meets(Span(a->kept, a->tokens)) || meets_table(out, a->kv))
     return ABFT_ERR_INVALID_ARG;
   int dev = 0, sms = 0;
   if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
@@ -324,6 +350,11 @@ int abft_kv_fork(const abft_kv_fork_args* a, void* stream) {
   if (a->pairs > 65535) return ABFT_ERR_UNSUPPORTED;
   if (a->pairs == 0 || a->kv.batch == 0) return ABFT_OK;
   if (a->src == nullptr || a->dst == nullptr || a->pages == nullptr) return ABFT_ERR_INVALID_ARG;
+  // Table and lengths are written: not the lists of the pairs.
+  for (const int32_t* list : {a->src, a->dst, a->pages}) {
+    const Span pairs(list, a->pairs);
+    if (meets_table(pairs, a->kv) || pairs.meets(Span(a->kv.seq_lens, a->kv.batch))) return ABFT_ERR_INVALID_ARG;
+  }
   int dev = 0, sms = 0;
   if ((rc = paged_device(&dev, &sms)) != ABFT_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -590,8 +590,8 @@ class PagedLayers:
         keeps the rows ``kept[cu[b]]`` to ``kept[cu[b] + counts[b] - 1]``, rising
         places among them: their keys and values move up to the slots behind
         the cache, in all layers, and ``seq_lens[b]`` falls by ``n - counts[b]``.
-        ``lens_out``: int32 [batch] that gets the lengths instead, ``seq_lens``
-        stays. Pages behind the new lengths stay in the table, for the caller to
+        ``lens_out``: int32 [batch] that gets the lengths instead (and overlaps
+        none of the arrays, but may be ``counts``), ``seq_lens`` stays. Pages behind the new lengths stay in the table, for the caller to
         use again. A sequence with bad rows, boundaries, length or pages is left
         as it was, and the status tells. Returns the array of lengths written."""
         out = self.seq_lens if lens_out is None else lens_out
@@ -622,7 +622,8 @@ class PagedLayers:
         inside a page, a copy of that page's slots in use, in all layers, in
         page ``pages[i]``, which no sequence may hold and which its row of the
         table names then (not looked at where the length ends with a page). -1
-        in ``src`` or ``dst``: no pair. Sources may be named by several pairs;
+        in ``src`` or ``dst``: no pair. The lists are no part of the table or the
+        lengths, which are written. Sources may be named by several pairs;
         a destination that is also a source or named twice, or a page that
         another pair names too or that is another source's last, is refused: the
         pair is left undone, and the status tells."""
