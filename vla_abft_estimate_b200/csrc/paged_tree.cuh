@@ -947,6 +947,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     join_tree_cluster<D, F16>(p, items[0], smem, tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Cfg::kColO, row_m, row_l);
   if (threadIdx.x == 0 && *abort_flag && kv.status != nullptr) atomicOr(kv.status, ABFT_PAGED_TIMEOUT);
   tc_fence_after();
+  __syncwarp();  // lanes without rows come from the join before the others
   if (warp == 5) tmem_dealloc(tmem, Cfg::kTmemCols);
 }
 
