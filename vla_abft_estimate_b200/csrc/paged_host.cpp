@@ -10,10 +10,12 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/EmptyTensor.h>
 #include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <math.h>
@@ -398,11 +400,13 @@ PyObject* layers_accept(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   if (!list_of(c->device, ids, -1, type) || !list_of(c->device, answers, ids->size(0), type) ||
       !list_of(c->device, parents, ids->size(0), at::kInt) || !list_of(c->device, cu, c->kv.batch + 1, at::kInt))
     Py_RETURN_NONE;
-  const at::TensorOptions on = at::TensorOptions().device(at::kCUDA, static_cast<c10::DeviceIndex>(c->device));
-  // A memory of its own for each, which the caller may resize, hand to a stream or free.
-  at::Tensor kept = at::empty({ids->size(0)}, on.dtype(at::kInt));
-  at::Tensor counts = at::empty({c->kv.batch}, on.dtype(at::kInt));
-  at::Tensor next = at::empty({c->kv.batch}, on.dtype(type));
+  // A memory of its own for each, which the caller may resize, hand to a stream or free;
+  // asked for on the current device, which is the layers', without a dispatcher's way each.
+  auto list = [](int64_t size, at::ScalarType type) {
+    return at::Tensor(at::detail::empty_generic({size}, c10::cuda::CUDACachingAllocator::get(),
+                                                c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
+  };
+  at::Tensor kept = list(ids->size(0), at::kInt), counts = list(c->kv.batch, at::kInt), next = list(c->kv.batch, type);
   abft_draft_accept_args args;
   memset(&args, 0, sizeof args);
   args.cu_seqlens = int_ptr(cu), args.parents = int_ptr(parents);
