@@ -22,8 +22,8 @@ namespace abft {
 // One CTA per sequence: all threads fetch rows (parent, id, the parent's
 // answer: independent loads), the first warp resolves depths 32 rows at a time,
 // parents of the same 32 by shuffles. Bound: a launch and four loads in a row
-// (boundaries, parent, its answer, the last row's answer): 1 tree of 16 rows 2.2 us,
-// 256 of up to 61 2.6 from a graph.
+// (boundaries, parent, its answer, the last row's answer): 1 tree of 16 rows 2.1-2.5 us,
+// 256 of up to 61 2.5-2.9 from a graph.
 struct AcceptParams {
   const int32_t* cu;
   const int32_t* parents;
@@ -253,7 +253,9 @@ __global__ void __launch_bounds__(kKeepThreads, 3) kv_keep_kernel(const __grid_c
 //
 // Bound: HBM, by rest slots of 2 * layers * heads rows in and out; slots of a head lie
 // one after another, and its warps take them in turn, eight 16-byte pieces a lane in
-// flight (32 forks of 64 slots on average, 28 layers of 4 heads: 30.4 us, 6.8 TB/s).
+// flight (32 forks of 64 slots on average, 28 layers of 4 heads: 30.8 us, 6.7 TB/s).
+// What the other pairs name and copy from is looked up beside the own chain of loads (3
+// forks 2.7 us).
 template <int kLayers>
 struct ForkParams {
   PagedView kv;

@@ -29,9 +29,13 @@
 // groups on steps of 128 keys of the same segment, the causal kernel's form for few
 // rows: 32 trees of 4 tokens of 32 heads on 512 slots 80 us, 54 so; up to 26 tokens on
 // up to 4,122 slots 29, 20.9; 64 trees of 8 on 8,188 slots 198, 175, where HBM's time is
-// 165.) One tree of 64 tokens on 131,008 slots takes 140 us where 73 are HBM's and the
-// products' time: each of its four tiles takes in all keys and values by itself, 1.07 GB
-// at the 62 GB/s that an SM takes in.
+// 165.) One tree of 64 tokens on 131,008 slots takes 135-155 us (163 in a loop, at the
+// power cap) where 73 are HBM's and the products' time: each of its four tiles takes in
+// all keys and values by itself, 1.07 GB at the 62 GB/s that an SM takes in.
+//
+// Rounding: P has the 16 bits that the product takes, l sums it unrounded, O, m, l and
+// the pieces have 32 (why: paged_prefill.cuh). Relative error against 64 bits 1.8-2.3e-3
+// bf16 and 2.2e-4 fp16, of which the output's rounding alone is 1.6-1.7e-3 and 2.0e-4.
 //
 // Work: a call's steps over all (sequence, kv head, block of rows) segments are one
 // list, cut into equal shares for two CTAs per SM. A segment inside a share is
@@ -114,7 +118,7 @@ struct TreeParams {
   const int32_t* cu;
   int32_t tokens;          // rows of q
   int32_t group;           // query heads per kv head
-  int32_t tile_tokens;     // tokens of a tile: 128 / group
+  int32_t tile_tokens;     // tokens of a tile: 128 / group, or fewer (tree_plan)
   float scale_log2;        // |scale| * log2(e), never 0
   int32_t negate;          // scale < 0
   uint32_t group_inv;      // ceil(2^16 / group): row_token()
